@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from contextlib import nullcontext
 from pathlib import Path
 
 import torch
@@ -109,6 +110,16 @@ SIGNATURES = {
                                       _c_int, _c_int, _vp]),
     "vdnh3_swiglu": (_c_int, [_vp, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp]),
     "vdnh3_swiglu_quant_rows": (_c_int, [_c_int, _vp, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp, _vp]),
+    "vdnh3_residual_rmsnorm_quant_rows": (_c_int, [_c_int, _vp, _c_i64, _vp, _c_i64, _vp, _c_float, _c_int, _c_int, _vp,
+                                                   _c_i64, _vp, _vp, _c_i64, _vp]),
+    "vdnh3_qk_rotary_axes": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_float, _vp, _c_i64, _c_i64, _c_int,
+                                      _vp, _c_i64, _c_i64, _vp, _c_float, _vp, _c_i64, _c_i64, _c_int,
+                                      _vp, _c_int, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    "vdnh3_causal_attn_packed": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64,
+                                          _c_i64, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _vp]),
+    "vdnh3_causal_attn_cached": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                                          _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int, _c_int, _c_int, _c_int,
+                                          _c_int, _c_int, _c_float, _vp]),
     "vdnh3_head_gate": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int, _vp]),
     "vdnh3_mfma_peak": (_c_int, [_c_int, _vp, _vp, _c_int, _c_int, _vp, _vp]),
     "vdnh3_mfma_peak_ops": (ctypes.c_double, [_c_int, _c_int, _c_int]),
@@ -175,6 +186,29 @@ def stream_handle(device: torch.device) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def strides(t) -> list[int]:
+    """The strides of every dim but the last; one of size 1 has none (torch may report anything for it)."""
+    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())]
+
+
+def in_place(t) -> bool:
+    """Whether a kernel can take a bf16 tensor where it lies: 16-byte aligned rows of contiguous channels."""
+    return (t.stride(-1) == 1 or t.shape[-1] == 1) and not any(s % 8 for s in strides(t)) and t.data_ptr() % 16 == 0
+
+
+def operand(t):
+    """``t`` where a kernel can read it in place, else a contiguous copy (also of a contiguous tensor off 16 bytes)."""
+    return t if in_place(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one: a launch on a stream of another device than the current one fails."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(index)
 
 
 def forward_only(what: str, *tensors) -> None:

@@ -235,6 +235,53 @@ def swiglu_quantize_rows(hidden: torch.Tensor, kind: int):
     return q, scale
 
 
+def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, kind: int,
+                              *, sum_out: torch.Tensor | None = None):
+    """``t = x + residual`` and the RMSNorm of ``t`` as a projection takes it: ``(codes, scale[rows, 1] fp32, t bf16)``.
+
+    ``kind`` (``linear.KIND_I8`` / ``KIND_F8``): the row-wise int8 / e4m3 codes and scales of ``rms_norm(t, weight, eps)``,
+    as ``quantize_rows`` gives them for ``gemm_w8a8``; ``KIND_BF16``: the norm itself in bf16, and no scale. The sum, the
+    norm and the codes are computed in fp32 from the bf16 inputs, each output rounded once: the norm is that of the
+    unrounded sum. ``residual=None`` (a model's first layer) norms ``x`` and returns it as ``t``. ``sum_out`` takes ``t``;
+    it may be ``x`` or ``residual``, otherwise it must not overlap them. A row with an infinity or a NaN in its norm gets
+    the scale NaN (``KIND_BF16``: the NaNs that arise).
+    """
+    if x.ndim != 2 or x.dtype != torch.bfloat16:
+        raise ValueError("residual_rmsnorm_quantize expects bf16 [rows, hidden]")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != torch.bfloat16):
+        raise ValueError("the residual must be bf16 and of x's shape")
+    if kind not in (_linear.KIND_BF16, _linear.KIND_I8, _linear.KIND_F8):
+        raise ValueError(f"unknown kind {kind!r}; expected KIND_BF16, KIND_I8 or KIND_F8")
+    rows, width = x.shape
+    if weight.numel() != width or width == 0 or width % 8:
+        raise ValueError(f"the width must be a positive multiple of 8 and the weight's, got {width} and {weight.numel()}")
+    if sum_out is not None and (residual is None or sum_out.shape != x.shape or sum_out.dtype != torch.bfloat16
+                                or not _lib.in_place(sum_out) or (rows > 1 and sum_out.stride(0) < width)):
+        raise ValueError("sum_out needs a residual, x's shape, bf16 and 16-byte rows")
+
+    def stride(t):  # of rows; one row's may be anything
+        return 0 if t is None else t.stride(0) if rows > 1 else width
+
+    _lib.forward_only("residual_rmsnorm_quantize", x, residual, weight)
+    device = _lib.require_device(x, residual, weight, sum_out)
+    xr, rr = _lib.operand(x), None if residual is None else _lib.operand(residual)
+    w = _lib.operand(weight.reshape(-1).to(torch.bfloat16))
+    total = x
+    if residual is not None:
+        total = torch.empty((rows, width), dtype=torch.bfloat16, device=device) if sum_out is None else sum_out
+    dtype = {_linear.KIND_BF16: torch.bfloat16, _linear.KIND_I8: torch.int8, _linear.KIND_F8: torch.float8_e4m3fn}[kind]
+    out = torch.empty((rows, width), dtype=dtype, device=device)
+    scale = None if kind == _linear.KIND_BF16 else torch.empty((rows, 1), dtype=torch.float32, device=device)
+    if rows == 0:
+        return out, scale, total
+    with _lib.on_device(device):
+        rc = _lib.lib().vdnh3_residual_rmsnorm_quant_rows(
+            kind, _lib.ptr(xr), stride(xr), _lib.ptr(rr), stride(rr), _lib.ptr(w), float(eps), rows, width, _lib.ptr(out), width,
+            _lib.ptr(scale), None if rr is None else _lib.ptr(total), stride(total), _lib.stream_handle(device))
+    _lib.check(rc, "vdnh3_residual_rmsnorm_quant_rows")
+    return out, scale, total
+
+
 def _mlp_forward(block: Any, h: torch.Tensor) -> torch.Tensor:
     """The H3 MLP (``vdn_h3/block_kernels.py:119-146``): ``fc2(swiglu(fc1(h)))``.
 
@@ -341,4 +388,5 @@ def release_block_fusions(state: Any) -> None:
 
 
 __all__ = ["BlockPointwiseCache", "SegmentIndex", "build_segment_index", "gated_residual", "install_block_fusions",
-           "make_fast_block_forward", "release_block_fusions", "rmsnorm_modulate", "swiglu", "swiglu_quantize_rows"]
+           "make_fast_block_forward", "release_block_fusions", "residual_rmsnorm_quantize", "rmsnorm_modulate", "swiglu",
+           "swiglu_quantize_rows"]

@@ -511,6 +511,48 @@ int vdnh3_swiglu_quant_rows(int kind, const uint16_t *h, int64_t h_row, int rows
 int vdnh3_fill_rows_bf16(uint16_t *p, int64_t ld, int rows, int cols, float value, void *stream);
 
 /* ------------------------------------------------------------------------------
+ * Operators of the language model that encodes the prompts (not in the reference). Strides in
+ * elements; bf16 operands 16-byte aligned with strides that are multiples of 8 elements.
+ * ------------------------------------------------------------------------------ */
+
+/* t = x + residual; y = t / sqrt(mean(t^2) + eps) * weight, in fp32. kind 0: out = bf16(y) (uint16_t, 16-byte
+ * rows). kind 1 / 2: out = the int8 / e4m3fn codes of y / scale (8-byte rows), scale[row] = max(max|y| / 127 or
+ * 448, 1e-12), NaN (with zero codes) for a row whose y is not finite. sum = bf16(t); it may be x or residual.
+ * residual and sum may be null; row strides of x and residual may be 0 (one row for all). hidden is a multiple
+ * of 8. */
+int vdnh3_residual_rmsnorm_quant_rows(int kind, const uint16_t *x, int64_t x_row, const uint16_t *residual,
+                                      int64_t residual_row, const uint16_t *weight, float eps, int rows, int hidden,
+                                      void *out, int64_t out_row, float *scale, uint16_t *sum, int64_t sum_row,
+                                      void *stream);
+
+/* q and k ([rows, q_heads / k_heads, head_dim]): RMSNorm over the head where a weight is given (null: none), then
+ * pair i < rot_dim / 2 (channels i and i + rot_dim / 2) turned by 2 pi positions[axis_of_pair[i]][row] turns[i].
+ * position_type 0 int32, 1 int64, 2 fp32; p_axis / p_row are its strides. head_dim is a multiple of 8 up to 128,
+ * rot_dim a multiple of 16 up to head_dim. axis_of_pair is not checked: it must index an axis of `positions`. */
+int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_head, const uint16_t *q_weight, float q_eps,
+                         uint16_t *q_out, int64_t qo_row, int64_t qo_head, int q_heads, const uint16_t *k, int64_t k_row,
+                         int64_t k_head, const uint16_t *k_weight, float k_eps, uint16_t *k_out, int64_t ko_row,
+                         int64_t ko_head, int k_heads, const void *positions, int position_type, int64_t p_axis,
+                         int64_t p_row, const double *turns, const int32_t *axis_of_pair, int rot_dim, int rows,
+                         int head_dim, void *stream);
+
+/* Causal softmax attention of packed sequences, query head h on key / value head h / (heads / kv_heads): sequence b
+ * is the rows [cu_seqlens[b], cu_seqlens[b + 1]) (device, sequences + 1 values, cut to [0, rows]) of q, k, v and
+ * out; its row i sees its rows 0 .. i. Rows of no sequence are not written. head_dim 64 or 128, scale > 0. */
+int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_t q_head, const uint16_t *k, int64_t k_row,
+                             int64_t k_head, const uint16_t *v, int64_t v_row, int64_t v_head, uint16_t *out,
+                             int64_t o_row, int64_t o_head, const int32_t *cu_seqlens, int sequences, int rows, int heads,
+                             int kv_heads, int head_dim, float scale, void *stream);
+
+/* The same for new_tokens queries of each of `batch` sequences over caches of `room` rows: sequence b has
+ * lengths[b] (device, cut to [0, room]) keys, and token i sees keys 0 .. lengths[b] - new_tokens + i (none: zeros). */
+int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
+                             int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch,
+                             int64_t v_row, int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row, int64_t o_head,
+                             const int32_t *lengths, int batch, int new_tokens, int room, int heads, int kv_heads,
+                             int head_dim, float scale, void *stream);
+
+/* ------------------------------------------------------------------------------
  * Calibration (no counterpart in the reference): the sustained MFMA rate of the part on
  * caller-supplied operand bits, the ceiling the kernels' rates are read against besides the
  * datasheet peak (the part is power-limited, so the rate depends on how many bits toggle).

@@ -1,0 +1,251 @@
+"""Causal attention of packed prompts and of new tokens over caches against float64 (GPU).
+
+Bar, from the arithmetic: a score is a sum of D products in fp32, off by at most (D + 8) 2^-24 of scale sum |q_d k_d| (`score`
+below), and an exponential by 2^-20 of itself with its argument's rounding, so each probability by e = (D + 8) 2^-24 score
++ 2^-20 (1 + score). Probabilities are rounded to bf16 for the products with the values (2^-8 each), in the sum of the
+values and in the row's sum alike: with A = sum p |v| the result is off by at most 2 (2^-8 + e) A, and 2^-8 of itself for
+its own rounding.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import prompt_oracle as po
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def _qkv(rows, heads, kv, dim, seed, loud=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return ((loud * torch.randn(rows, heads, dim, generator=g)).to(BF), torch.randn(rows, kv, dim, generator=g).to(BF),
+            torch.randn(rows, kv, dim, generator=g).to(BF))
+
+
+def _check(got, want, dim):
+    out, size, score = want
+    e = ((dim + 8) * 2.0 ** -24 * score + 2.0 ** -20 * (1 + score))[..., None]
+    bar = 2 * (2.0 ** -8 + e) * size + 2.0 ** -8 * out.abs()
+    g = got.double().cpu()
+    live = ~out.isnan()
+    d = (g - out).abs()[live]
+    assert (d <= bar[live]).all(), (d / bar[live].clamp_min(1e-30)).max()
+
+
+PACKED = [  # lengths, heads, kv heads, dim
+    ([1], 1, 1, 64), ([2], 5, 1, 128), ([5, 1, 33], 4, 4, 64), ([0, 3, 0, 1, 64, 0], 8, 2, 128), ([95, 96, 97], 5, 1, 128),
+    ([255, 256, 257], 2, 2, 128), ([51, 52, 103], 10, 2, 128), ([640], 40, 8, 128), ([1, 500, 63], 14, 2, 64),
+    ([700], 3, 3, 64), ([130, 31], 7, 1, 128), ([600], 32, 1, 64), ([200], 6, 2, 80), ([90, 7], 4, 4, 24),
+    ([1] * 40, 8, 1, 128), ([17, 1, 1, 300] * 3, 20, 20, 64)]
+
+
+@pytest.mark.parametrize("lengths,heads,kv,dim", PACKED)
+def test_packed_against_float64(device, lengths, heads, kv, dim):
+    from vdn_h3_amd.causal import causal_softmax_packed
+
+    print(f"case packed {lengths} {heads}/{kv}x{dim}", flush=True)
+    bounds = [0]
+    for n in lengths:
+        bounds.append(bounds[-1] + n)
+    rows = bounds[-1]
+    q, k, v = _qkv(rows, heads, kv, dim, rows + dim, loud=2.0)
+    scale = dim ** -0.5
+    cu = torch.tensor(bounds, dtype=torch.int32, device=device)
+    got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), cu, scale)
+    want = po.packed(q, k, v, bounds, scale)
+    _check(got, want, dim)
+    if dim % 8 == 0:  # views of one projection, and heads in front of rows
+        fused = torch.cat([q, k, v], 1).to(device).split((heads, kv, kv), 1)
+        first = [t.to(device).transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+        assert torch.equal(causal_softmax_packed(*fused, bounds, scale), got)
+        assert torch.equal(causal_softmax_packed(*first, cu.long(), scale), got)
+
+
+def test_rows_outside_every_sequence_stay(device):
+    from vdn_h3_amd.causal import causal_softmax_packed
+
+    for dim in (128, 80):
+        q, k, v = _qkv(300, 4, 2, dim, 1)
+        for bounds in ([20, 130, 130, 260], [0, 0], [300, 300], [299, 300], [7, 8]):
+            out = torch.full((300, 4, dim), 3.0, dtype=BF, device=device)
+            # what lies outside a sequence takes no part, whatever it holds
+            a, b = bounds[0], bounds[-1]
+            dk, dv = k.clone(), v.clone()
+            dk[:a], dk[b:], dv[:a], dv[b:] = torch.nan, torch.inf, torch.inf, torch.nan
+            got = causal_softmax_packed(q.to(device), dk.to(device), dv.to(device),
+                                        torch.tensor(bounds, dtype=torch.int32, device=device), 0.1, out=out)
+            assert got is out and (out[:a] == 3).all() and (out[b:] == 3).all()
+            _check(got, po.packed(q, k, v, bounds, 0.1), dim)
+
+
+def test_bounds_on_the_device_are_cut(device):
+    from vdn_h3_amd.causal import causal_softmax_packed
+
+    q, k, v = _qkv(100, 2, 1, 64, 2)
+    cu = torch.tensor([-7, 40, 2000000000], dtype=torch.int32, device=device)
+    got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), cu, 0.125)
+    _check(got, po.packed(q, k, v, [0, 40, 100], 0.125), 64)
+
+
+@pytest.mark.parametrize("dim,kv", [(128, 1), (64, 4)])
+def test_infinities_and_nans_where_a_row_does_not_look(device, dim, kv):
+    """Keys and values behind a row, or of another sequence, are not a number: the row does not change. Rows that see one
+    hold what the softmax gives."""
+    from vdn_h3_amd.causal import causal_softmax_packed
+
+    print(f"case non-finite {dim} {kv}", flush=True)
+    bounds, heads = [0, 150, 340], 4
+    q, k, v = _qkv(340, heads, kv, dim, 11)
+    k[100], v[120] = torch.nan, torch.inf
+    v[120, :, 1::2] = torch.nan
+    k[150 + 96], v[150 + 97] = -torch.inf, torch.nan
+    k[339], v[339] = torch.inf, torch.nan
+    got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), bounds, dim ** -0.5).cpu()
+    seen = [i for i in range(340) if i < 100 or 150 <= i < 150 + 96]
+    want = [t[seen] for t in po.packed(q, k, v, bounds, dim ** -0.5)]
+    assert not want[0].isnan().any()
+    _check(got[seen], want, dim)
+    assert got[100:150].isnan().all()  # a key that is no number
+    assert got[150 + 97:].isnan().all()  # a value that is none, or a key of infinities
+
+
+def test_scores_at_the_ends_of_the_range(device):
+    """One key far above the rest, all keys equal, scores in the thousands either way."""
+    from vdn_h3_amd.causal import causal_softmax_packed
+
+    q, k, v = _qkv(400, 2, 1, 64, 12, loud=40.0)
+    got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), [0, 400], 4.0)
+    _check(got, po.packed(q, k, v, [0, 400], 4.0), 64)
+    same = k[:1].expand(400, 1, 64).contiguous()
+    got = causal_softmax_packed(q.to(device), same.to(device), v.to(device), [0, 400], 4.0)
+    _check(got, po.packed(q, same, v, [0, 400], 4.0), 64)
+    down = (-q.float().abs().mean((0, 1)))[None, None].expand(400, 1, 64).to(BF).contiguous()
+    up = q.abs()
+    got = causal_softmax_packed(up.to(device), down.to(device), v.to(device), [0, 400], 1.0)
+    _check(got, po.packed(up, down, v, [0, 400], 1.0), 64)
+
+
+CACHED = [  # new, room, lengths, heads, kv heads, dim
+    (1, 1, [1], 1, 1, 64), (1, 70, [0, 1, 2, 63, 64, 65, 70], 5, 1, 128), (1, 1000, [1000, 31, 999], 40, 8, 128),
+    (1, 257, [256, 257, 5], 16, 16, 64), (2, 300, [0, 1, 2, 3, 299], 8, 2, 128), (5, 400, [3, 5, 128, 400], 28, 4, 128),
+    (1, 500, [500, 77], 32, 1, 128), (9, 130, [130, 9, 100], 14, 2, 64), (70, 200, [200, 70, 10, 0], 6, 2, 128),
+    (300, 640, [640, 400, 257], 5, 1, 64), (1, 4100, [4100], 4, 1, 128), (4, 2500, [2500, 0, 1300], 6, 1, 64),
+    (40, 96, [96] * 3, 1, 1, 128), (1, 90, [45] * 70, 2, 1, 64)]
+
+
+@pytest.mark.parametrize("new,room,lengths,heads,kv,dim", CACHED)
+def test_cached_against_float64(device, new, room, lengths, heads, kv, dim):
+    from vdn_h3_amd.causal import causal_softmax_cached
+
+    print(f"case cached {new}/{room} {lengths} {heads}/{kv}x{dim}", flush=True)
+    batch = len(lengths)
+    q, k, v = _qkv(batch * max(new, room), heads, kv, dim, room + new, loud=2.0)
+    q = q[:batch * new].view(batch, new, heads, dim)
+    k, v = (t[:batch * room].view(batch, room, kv, dim) for t in (k, v))
+    scale = dim ** -0.5
+    want = po.cached(q, k, v, lengths, scale)
+    n = torch.tensor(lengths, dtype=torch.int32, device=device)
+    got = causal_softmax_cached(q.to(device), k.to(device), v.to(device), n, scale)
+    _check(got, want, dim)
+    # heads in front of rows in the caches, stale rows that are no numbers, a view of q, an output with a wider row
+    dk, dv = (t.transpose(1, 2).contiguous().to(device).transpose(1, 2) for t in (k, v))
+    for b, m in enumerate(lengths):
+        dk[b, m:], dv[b, m:] = torch.nan, torch.inf
+    wide = torch.full((batch, new, heads + 3, dim), 9.0, dtype=BF, device=device)
+    view = torch.cat([q, q], 2).to(device)[:, :, :heads]
+    got2 = causal_softmax_cached(view, dk, dv, n.long(), scale, out=wide[:, :, :heads])
+    assert torch.equal(got2, got) and (wide[:, :, heads:] == 9).all()
+
+
+def test_cached_infinities_behind_a_new_token(device):
+    from vdn_h3_amd.causal import causal_softmax_cached
+
+    for new in (4, 40):
+        q, k, v = _qkv(200, 4, 2, 64, 14)
+        q, k, v = q[None, :new], k[None], v[None]
+        v[0, 199], k[0, 198] = torch.nan, torch.nan  # what only the last two tokens see
+        n = torch.tensor([200], dtype=torch.int32, device=device)
+        got = causal_softmax_cached(q.to(device), k.to(device), v.to(device), n, 0.125).cpu()
+        want = po.cached(q, k, v, [200], 0.125)
+        _check(got[:, :-2], [t[:, :-2] for t in want], 64)
+        assert got[:, -2:].isnan().all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_past_32_bits(device, new):
+    """Caches whose rows lie more than 2^32 bytes, and 2^31 elements, behind their first."""
+    from vdn_h3_amd.causal import causal_softmax_cached
+
+    print(f"case cached far {new}", flush=True)
+    room, row = 1200, 1 << 21  # row 1199 starts at element 2.5e9
+    store = torch.empty(room * row, dtype=BF, device=device)
+    k, v = (torch.as_strided(store, (1, room, 2, 64), (8, row, 64, 1), off) for off in (0, 1 << 20))
+    q, hk, hv = _qkv(room, 4, 2, 64, 15)
+    k.copy_(hk[None]), v.copy_(hv[None])
+    q = q[None, :new]
+    n = torch.tensor([room - 1], dtype=torch.int32, device=device)
+    got = causal_softmax_cached(q.to(device), k, v, n, 0.125)
+    _check(got, po.cached(q, hk[None], hv[None], [room - 1], 0.125), 64)
+
+
+def test_cache_layout_and_lengths_are_checked(device):
+    from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
+
+    q, k = torch.zeros(2, 1, 4, 64, dtype=BF, device=device), torch.zeros(2, 9, 2, 72, dtype=BF, device=device)
+    n = torch.ones(2, dtype=torch.int32, device=device)
+    for bad in (k[..., 1:65], torch.zeros(2, 9, 64, 2, dtype=BF, device=device).transpose(2, 3)):
+        with pytest.raises(ValueError, match="in place|copied"):
+            causal_softmax_cached(q, bad, bad, n, 0.1)
+    good = k[..., :64]
+    with pytest.raises(ValueError, match="out"):
+        causal_softmax_cached(q, good, good, n, 0.1, out=torch.zeros(2, 1, 4, 64, device=device))
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            causal_softmax_cached(q, good, good, n, scale)
+        with pytest.raises(ValueError, match="scale"):
+            causal_softmax_packed(q[:, 0], good[:, 0], good[:, 0], [0, 2], scale)
+    with pytest.raises(RuntimeError, match="CPU"):
+        causal_softmax_cached(q, good, good, n.cpu(), 0.1)
+    empty = causal_softmax_cached(q, good[:, :0], good[:, :0], n, 0.1)
+    assert (empty == 0).all()
+    assert causal_softmax_packed(q[:0, 0], good[:0, 0], good[:0, 0], [0], 0.1).shape == (0, 4, 64)
+    assert causal_softmax_cached(q[:0], good[:0], good[:0], n[:0], 0.1).shape == (0, 1, 4, 64)
+
+
+def test_repeatable_on_streams_and_in_graphs(device):
+    """The same bits again; on another stream; and from a graph replayed with other lengths and other bounds."""
+    from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
+
+    q, k, v = (t.to(device) for t in _qkv(1500, 10, 2, 128, 16))
+    cu = torch.tensor([0, 700, 1500], dtype=torch.int32, device=device)
+    qc, kc, vc = q[:6].view(2, 3, 10, 128), k.view(2, 750, 2, 128), v.view(2, 750, 2, 128)
+    n = torch.tensor([750, 20], dtype=torch.int32, device=device)
+    q1 = q[:2].view(2, 1, 10, 128)
+
+    def calls():
+        return (causal_softmax_packed(q, k, v, cu, 0.1), causal_softmax_cached(qc, kc, vc, n, 0.1),
+                causal_softmax_cached(q1, kc, vc, n, 0.1))
+
+    want = calls()
+    assert all(torch.equal(a, b) for a, b in zip(calls(), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = calls()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for first, lengths in ((700, (750, 20)), (1, (1, 0)), (1499, (333, 749)), (0, (640, 2))):
+        cu.copy_(torch.tensor([0, first, 1500], dtype=torch.int32))
+        n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, calls())), (first, lengths)
+    assert math.isfinite(got[0].float().abs().max().item())

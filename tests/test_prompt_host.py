@@ -1,0 +1,128 @@
+"""Refusals of the prompt encoder's operators, which need no GPU: arguments are checked before any device work."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+def _z(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def test_norm_refusals(built_lib):
+    from vdn_h3_amd import linear
+    from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize as op
+
+    x, w = _z(4, 64), _z(64)
+    for bad in [lambda: op(_z(4, 64, dtype=torch.float32), x, w, 1e-6, 1), lambda: op(_z(64), None, w, 1e-6, 1),
+                lambda: op(x, _z(3, 64), w, 1e-6, 1), lambda: op(x, x.float(), w, 1e-6, 1),
+                lambda: op(x, x, _z(32), 1e-6, 1), lambda: op(_z(4, 60), None, _z(60), 1e-6, 1),
+                lambda: op(_z(4, 0), None, _z(0), 1e-6, 1), lambda: op(x, x, w, 1e-6, 3),
+                lambda: op(x, None, w, 1e-6, 1, sum_out=_z(4, 64)), lambda: op(x, x, w, 1e-6, 1, sum_out=_z(4, 128)[:, ::2]),
+                lambda: op(x, x, w, 1e-6, 1, sum_out=x[:1].expand(4, 64))]:
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        op(x, x, w, 1e-6, linear.KIND_I8)
+    with pytest.raises(RuntimeError, match="residual_rmsnorm_quantize is forward-only"):
+        op(x, x.clone().requires_grad_(), w, 1e-6, linear.KIND_I8)
+
+
+def test_rotary_refusals(built_lib):
+    from vdn_h3_amd.rotary import RotaryAxes, normalise_qk_axes as op
+
+    for bad in [lambda: RotaryAxes(()), lambda: RotaryAxes((0, 0)), lambda: RotaryAxes((9, -1)), lambda: RotaryAxes((3, 2)),
+                lambda: RotaryAxes((8,), theta=0.0), lambda: RotaryAxes((8,), theta=float("inf")),
+                lambda: RotaryAxes((8,), ladder="other")]:
+        with pytest.raises(ValueError):
+            bad()
+    axes = RotaryAxes((8, 12, 12))
+    assert axes.rot_dim == 64 and axes.axes == 3
+    q, k, pos = _z(5, 4, 64), _z(5, 2, 64), torch.zeros(3, 5, dtype=torch.int64)
+    for bad in [lambda: op(q, _z(4, 2, 64), pos, axes), lambda: op(q, _z(5, 2, 128), pos, axes),
+                lambda: op(q[0], k, pos, axes)]:
+        with pytest.raises(ValueError):
+            bad()
+    for bad in [lambda: op(q.float(), k, pos, axes)]:
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        op(q, k, pos, axes)
+    with pytest.raises(RuntimeError, match="normalise_qk_axes is forward-only"):
+        op(q.requires_grad_(), k, pos, axes)
+
+
+def test_attention_refusals(built_lib):
+    from vdn_h3_amd.causal import causal_softmax_cached as cached, causal_softmax_packed as packed
+
+    q, k = _z(6, 4, 64), _z(6, 2, 64)
+    for bad in [lambda: packed(q, _z(5, 2, 64), _z(5, 2, 64), [0, 6], 0.1), lambda: packed(q, k, _z(6, 4, 64), [0, 6], 0.1),
+                lambda: packed(q, _z(6, 3, 64), _z(6, 3, 64), [0, 6], 0.1), lambda: packed(q, k[..., :32], k[..., :32], [0, 6], 1),
+                lambda: packed(q, _z(6, 0, 64), _z(6, 0, 64), [0, 6], 0.1), lambda: packed(q[0], k, k, [0, 6], 0.1)]:
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        packed(q, k.float(), k.float(), [0, 6], 0.1)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        packed(q, k, k, [0, 6], 0.1)
+    with pytest.raises(RuntimeError, match="causal_softmax_packed is forward-only"):
+        packed(q.clone().requires_grad_(), k, k, [0, 6], 0.1)
+    q, k, n = _z(2, 1, 4, 64), _z(2, 9, 2, 64), torch.zeros(2, dtype=torch.int32)
+    for bad in [lambda: cached(q, k[:1], k[:1], n, 0.1), lambda: cached(q, k, _z(2, 8, 2, 64), n, 0.1),
+                lambda: cached(q, k, k, n[:1], 0.1), lambda: cached(q, k, k, n.float(), 0.1),
+                lambda: cached(_z(2, 1, 3, 64), k, k, n, 0.1), lambda: cached(_z(2, 1, 4, 80), _z(2, 9, 2, 80), _z(2, 9, 2, 80), n, 0.1)]:
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        cached(q, k, k, n, 0.1)
+    with pytest.raises(RuntimeError, match="causal_softmax_cached is forward-only"):
+        cached(q, k.clone().requires_grad_(), k, n, 0.1)
+
+
+def test_bounds_that_the_host_holds_are_checked():
+    from vdn_h3_amd.causal import _sequence_bounds
+
+    device = torch.device("cuda:0")
+    for bad in ([0, 7], [-1, 3], [0, 4, 3], [], torch.tensor([0.0, 3.0]), torch.tensor([[0, 3]]), torch.tensor([0, 9])):
+        with pytest.raises(ValueError):
+            _sequence_bounds(bad, 6, device)
+
+
+def test_c_entry_points_refuse_before_any_launch(built_lib):
+    """Null and misaligned operands, sizes that the kernels do not take: a status, never a launch."""
+    from vdn_h3_amd import _lib
+
+    lib, p = _lib.lib(), 1 << 20  # an address that is never read
+
+    def norm(kind=1, x=p, x_row=64, res=p, res_row=64, w=p, eps=1e-6, rows=4, hidden=64, out=p, out_row=64, scale=p, s=p,
+             s_row=64):
+        return lib.vdnh3_residual_rmsnorm_quant_rows(kind, x, x_row, res, res_row, w, eps, rows, hidden, out, out_row, scale, s,
+                                                     s_row, None)
+
+    for bad in [dict(kind=3), dict(kind=-1), dict(x=None), dict(x=p + 8), dict(x_row=60), dict(x_row=8), dict(res=p + 2),
+                dict(w=None), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(rows=0), dict(hidden=0),
+                dict(hidden=60), dict(out=None), dict(out=p + 4), dict(out_row=32), dict(scale=None), dict(s=p + 8),
+                dict(s_row=0), dict(kind=0, out=p + 8)]:
+        assert norm(**bad) == _lib.VDNH3_ERR_INVALID, bad
+        assert "residual_rmsnorm" in _lib.last_error()
+
+    def rotary(q=p, q_row=256, qh=4, out=p, kh=2, pos=p, kind=1, turns=p, axis=p, rot=64, rows=3, dim=64, w=None):
+        return lib.vdnh3_qk_rotary_axes(q, q_row, 64, w, 1e-6, out, 256, 64, qh, p, 128, 64, None, 1e-6, p, 128, 64, kh, pos,
+                                        kind, 3, 1, turns, axis, rot, rows, dim, None)
+
+    for bad in [dict(q=None), dict(q=p + 8), dict(q_row=100), dict(qh=0), dict(out=None), dict(kh=0), dict(pos=None),
+                dict(kind=3), dict(turns=None), dict(axis=None), dict(rot=0), dict(rot=24), dict(rot=80), dict(rows=0),
+                dict(dim=60), dict(dim=136), dict(w=p + 2)]:
+        assert rotary(**bad) == _lib.VDNH3_ERR_INVALID, bad
+
+    def packed(q=p, q_row=256, k=p, out=p, cu=p, n=1, rows=4, h=4, kh=2, dim=64, scale=0.1):
+        return lib.vdnh3_causal_attn_packed(q, q_row, 64, k, 128, 64, p, 128, 64, out, 256, 64, cu, n, rows, h, kh, dim, scale,
+                                            None)
+
+    for bad in [dict(q=None), dict(q=p + 8), dict(q_row=100), dict(k=None), dict(out=p + 8), dict(cu=None), dict(n=0),
+                dict(rows=0), dict(h=5), dict(kh=0), dict(h=0), dict(dim=80), dict(scale=0.0), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(scale=float("inf"))]:
+        assert packed(**bad) == _lib.VDNH3_ERR_INVALID, bad
