@@ -10,6 +10,7 @@
 // The sequences' bounds are read on the device, so no length is needed on the host and a captured call can be replayed
 // with other lengths. Bounds outside the buffers are cut to them.
 #include "common.h"
+#include "lane_groups.h"
 
 namespace vdnh3 {
 namespace {
@@ -81,34 +82,346 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
   for (int c = 0; c < C; ++c) out[C * lane + c] = f2bf(keys > 0 ? o[c] / l : 0.f);
 }
 
-// One wavefront per (query row, head), four per workgroup.
+// ---------------------------------------------------------------------------------
+// Whole prompts: one workgroup = 8 wavefronts = 256 rows of one key / value head x the key tiles that they see.
+// A row is a (token, query head) pair of the head's group, token-major: row r of a sequence is token r / group and head
+// r % group, so every query head of a group shares the workgroup's K and V tiles and a block's rows span few tokens
+// (256 rows of 5 heads: 51), which keeps the part of its last tiles that lies behind the diagonal small.
+//
+// Scores are computed transposed, S^T = K Q^T, on v_mfma_f32_16x16x32_bf16: a lane owns a query of each of its
+// wavefront's two 16-query blocks and 24 of a tile's 96 keys, and its probabilities are operands of O^T += V^T P^T as
+// they lie. V tiles are loaded as they are, key by key, and read transposed (ds_read_b64_tr_b16: 16 lanes get 4 keys of
+// 16 channels), so no pass writes a transposed copy first.
+constexpr int kBM = 256;       // rows per workgroup
+constexpr int kBN = 96;        // keys per tile
+constexpr int kThreads = 512;
+constexpr int kRing = 3;       // LDS slots per K and V ring (144 KB at D = 128): loads run kRing - 1 tiles ahead
+constexpr int kAhead = 4;      // fragments a wavefront's LDS reads run ahead of its MFMAs
+constexpr int kNQ = 2;         // 16-query blocks per wavefront
+constexpr float kLazy = 8.0f;  // log2 of the largest probability a stale running max allows
+constexpr float kNoMax = -3.402823466e38f;  // the running max before any score: finite, so a masked score gives exp2(-inf) = 0
+
+// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). K: the 16 rows of a fragment read hit 16 different
+// 16-byte bank groups. V: the 8 rows that half a wavefront reads 32 bytes of hit 8 different 32-byte ones.
 template <int D>
-__global__ __launch_bounds__(256) void causal_rows_kernel(Operand q, Operand k, Operand v, Operand out, Sequences seqs,
-                                                          int heads, int group, float scale_log2, int64_t total) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= total) return;
-  const int64_t at = w / heads;
-  const int head = (int)(w - at * heads), lane = threadIdx.x & 63;
-  int b, row;
+__device__ __forceinline__ int k_slot(int r, int c) {
+  if constexpr (D == 128) return c ^ (r & 15);
+  else return c ^ ((r >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int v_slot(int r, int c) {
+  if constexpr (D == 128) return c ^ (2 * (r & 7));
+  else return c ^ (2 * ((r >> 1) & 3));
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+// Four keys of one channel per lane: 16 lanes read 4 rows of 16 channels (lane i: channels 4 (i % 4) .. + 3 of row i / 4)
+// and get their transpose (lane i: channel i of the 4 rows).
+__device__ __forceinline__ u32x2_t lds_read_transposed(const uint16_t *p) {
+  typedef __attribute__((address_space(3))) s16x4_t *lds_ptr;
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)));
+}
+
+// The block of rows a workgroup takes: sequence b, rows [r0, r1) of its n x group. Blocks of packed sequences are numbered
+// without a count on the host: sequence b's begin at floor(cu[b] group / kBM) + b, which leaves room for those before.
+struct Block {
+  int b, r0, r1;
+  Sequence s;
+};
+__device__ __forceinline__ Block block_at(const Sequences &seqs, int block, int group) {
+  int b, first;
   if (seqs.cu) {
-    row = (int)at;
-    int lo = 0, hi = seqs.count;  // the last sequence that starts at or before the row
+    auto begin = [&](int i) __device__ { return (int)((int64_t)min(max(seqs.cu[i], 0), seqs.rows) * group / kBM) + i; };
+    int lo = 0, hi = seqs.count;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (seqs.cu[mid] <= row) lo = mid;
+      if (begin(mid) <= block) lo = mid;
       else hi = mid;
     }
     b = lo;
+    first = begin(lo);
   } else {
-    b = (int)(at / seqs.rows);
-    row = (int)(at - (int64_t)b * seqs.rows);
+    const int per = (int)(((int64_t)seqs.rows * group + kBM - 1) / kBM);
+    b = block / per;
+    first = b * per;
   }
   const Sequence s = sequence_at(seqs, b);
-  const int i = row - s.q0;
-  if (i < 0 || i >= s.n) return;  // no sequence's row
-  const int kvh = head / group, keys = min(max(s.keys - s.n + 1 + i, 0), s.keys);
-  attend_row<D>(q.at(b, row, head), k.at(b, s.k0, kvh), k.row, v.at(b, s.k0, kvh), v.row, keys, scale_log2,
-                const_cast<uint16_t *>(out.at(b, row, head)), lane);
+  const int64_t rows = (int64_t)s.n * group, r0 = (int64_t)(block - first) * kBM;
+  if (r0 < 0 || r0 >= rows) return Block{b, 0, 0, s};
+  return Block{b, (int)r0, (int)min(r0 + kBM, rows), s};
+}
+
+// Two-group ping-pong over the key tiles t = 0 .. T-1: wavefronts 0-3 (group A) and 4-7 (group B) each own 32 rows a
+// wavefront; w and w + 4 share a SIMD. In each of the barrier-separated phases p = 0 .. 2T+1 one group works on the matrix
+// cores and the other on the VALU:
+//   MFMA phase of tile t :  O^T += V(t-1)^T P(t-1)^T, l += 1^T P(t-1)^T, S(t)^T = K(t) Q^T
+//   VALU phase of tile t :  P(t) = exp2(scale S(t) - m), row max, O and l rescale
+// Group A runs tile t's MFMA phase in phase 2t and its VALU phase in 2t+1; group B one phase later. K(t) and V(t-1) are
+// read in phases 2t and 2t+1 only; group A loads K tiles and group B V tiles straight to LDS, each at the start of its VALU
+// phase, two tiles ahead. A wavefront leaves out tiles behind its own rows' diagonal.
+template <int D>
+__global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Operand k, Operand v, Operand out,
+                                                                  Sequences seqs, int blocks, int kv_heads, int group,
+                                                                  float scale_log2) {
+  constexpr int KC = D / 8;      // 16-byte chunks per row
+  constexpr int NS = D / 32;     // k-steps of the QK^T contraction
+  constexpr int NO = D / 16;     // 16-row blocks of O^T
+  constexpr int NKB = kBN / 16;  // 16-key blocks of S^T
+  constexpr int NT = kBN / 32;   // k-steps of the PV contraction
+  constexpr int TILE = kBN * D;  // elements per tile
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[kRing][TILE];
+  __shared__ __attribute__((aligned(16))) uint16_t Vs[kRing][TILE];
+
+  // the last blocks, which see the most keys, first; heads next to each other, so with 8 heads each XCD has its own
+  const int kvh = (int)blockIdx.x % kv_heads;
+  const Block blk = block_at(seqs, blocks - 1 - (int)blockIdx.x / kv_heads, group);
+  if (blk.r0 >= blk.r1) return;
+  const Sequence &sq = blk.s;
+  const int behind = sq.keys - sq.n;  // token i sees keys 0 .. behind + i
+  const int block_keys = min(behind + (blk.r1 - 1) / group + 1, sq.keys);
+  const int T = block_keys > 0 ? (block_keys + kBN - 1) / kBN : 0;
+
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int turn = wave >> 2;  // 0: group A, 1: group B
+  const int w0 = blk.r0 + wave * 16 * kNQ;  // the wavefront's first row
+  const bool rows_live = w0 < blk.r1;
+  // the wavefront's tiles, and those of its tiles that need no mask
+  const int w_keys = rows_live ? min(behind + (min(w0 + 16 * kNQ, blk.r1) - 1) / group + 1, sq.keys) : 0;
+  const int w_tiles = __builtin_amdgcn_readfirstlane(w_keys > 0 ? (w_keys + kBN - 1) / kBN : 0);
+  const int w_clear = __builtin_amdgcn_readfirstlane(rows_live ? max(behind + w0 / group + 1, 0) / kBN : 0);
+
+  int last[kNQ];
+  const uint16_t *qp[kNQ];
+  uint16_t *op[kNQ];
+#pragma unroll
+  for (int n = 0; n < kNQ; ++n) {
+    const int r = min(w0 + 16 * n + l16, blk.r1 - 1), token = r / group, head = kvh * group + (r - token * group);
+    last[n] = behind + token;
+    qp[n] = q.at(blk.b, sq.q0 + token, head);
+    op[n] = const_cast<uint16_t *>(out.at(blk.b, sq.q0 + token, head));
+  }
+
+  f32x4_t oacc[NO][kNQ], l_run[kNQ];
+  float m_run[kNQ];
+#pragma unroll
+  for (int n = 0; n < kNQ; ++n) {
+#pragma unroll
+    for (int m = 0; m < NO; ++m) oacc[m][n] = f32x4_t{};
+    m_run[n] = kNoMax;
+    l_run[n] = f32x4_t{};
+  }
+
+  if (T > 0) {
+    bf16x8_t qf[kNQ][NS];
+#pragma unroll
+    for (int n = 0; n < kNQ; ++n)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[n][s] = as_bf16x8(ld16(qp[n] + 32 * s + 8 * g));
+
+    // Tile loads, by one group of 256 threads: thread chunk i fills LDS position P = 256 i + gtid (16-byte units): row
+    // P / KC, slot P % KC, which holds chunk slot ^ swizzle(row) of that key; the swizzle is the same for every i. Rows
+    // past the sequence's keys read its last key (their scores are masked).
+    constexpr int CG = kBN * KC / 256;
+    const int gtid = tid & 255, kr0 = gtid / KC;
+    const int slot = (turn == 0 ? k_slot<D>(kr0, gtid % KC) : v_slot<D>(kr0, gtid % KC)) * 8;
+    const int64_t src_row = turn == 0 ? k.row : v.row;
+    const uint16_t *src = turn == 0 ? k.at(blk.b, sq.k0, kvh) : v.at(blk.b, sq.k0, kvh);
+    uint32_t doff[CG];
+#pragma unroll
+    for (int i = 0; i < CG; ++i) doff[i] = 2u * ((uint32_t)(kr0 + i * (256 / KC)) * (uint32_t)src_row + slot);
+    const uint32_t lds_dma = __builtin_amdgcn_readfirstlane(
+        (turn == 0 ? lds_address(&Ks[0][0]) : lds_address(&Vs[0][0])) + (wave & 3) * 64 * 16);
+    auto tile_dma = [&](int t, int ring) __device__ {
+      const int ks = t * kBN;
+      const uint16_t *base = src + (int64_t)ks * src_row;
+      uint32_t off[CG];
+#pragma unroll
+      for (int i = 0; i < CG; ++i) off[i] = doff[i];
+      if (ks + kBN > sq.keys) {  // uniform: the last tile only
+#pragma unroll
+        for (int i = 0; i < CG; ++i)
+          off[i] = 2u * ((uint32_t)(min(ks + kr0 + i * (256 / KC), sq.keys - 1) - ks) * (uint32_t)src_row + slot);
+      }
+#pragma unroll
+      for (int i = 0; i < CG; ++i)
+        global_to_lds16_sbase(base, off[i], lds_dma + (uint32_t)ring * (TILE * 2) + (uint32_t)(i * 256 * 16));
+    };
+
+    // Fragment offsets inside a tile (elements): K by k-step (16-key blocks differ by a constant), V by 16-channel block
+    // (its 4-row reads differ by constants: the rows of a lane are 16 a + 4 g + l16 / 4).
+    int kfo[NS], vfo[NO];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) kfo[st] = (l16 * KC + k_slot<D>(l16, 4 * st + g)) * 8;
+    const int vr = 4 * g + (l16 >> 2);
+#pragma unroll
+    for (int m = 0; m < NO; ++m) vfo[m] = vr * D + v_slot<D>(vr, 2 * m + ((l16 >> 1) & 1)) * 8 + 4 * (l16 & 1);
+
+    f32x4_t sacc[NKB][kNQ];
+    u32x4_t pb[NT][kNQ];  // P^T fragments: bf16 pairs
+    const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int n = 0; n < kNQ; ++n) pb[j][n] = u32x4_t{};
+
+    // K(t) and V(t) live in slot t % kRing. Past the end the tile index is clamped to T-1: such loads rewrite slots that no
+    // tile reads any more, and every VALU phase issues the same count, so each group's wait at the end of odd phases is
+    // exact. Prologue: K(0 .. kRing-2) by group A, V(0 .. kRing-3) by group B; V(-1), which the PV product of tile 0 reads
+    // with P(-1) = 0, is zeroed. Group B's first issue (phase 0) is V(kRing-2).
+#pragma unroll
+    for (int j = 0; j < kRing - 1; ++j)
+      if (j < kRing - 2 || turn == 0) tile_dma(min(j, T - 1), j);
+    for (int i = tid; i < TILE / 8; i += kThreads) st16(Vs[kRing - 1] + i * 8, u32x4_t{0, 0, 0, 0});
+    wait_vm_lds<0>();
+    bare_barrier();
+
+    const int phases = 2 * T + 2;
+    for (int p = 0; p < phases; ++p) {
+      const int t_mfma = p >> 1, t_valu = (p - 1) >> 1;
+      if (turn == (p & 1)) {
+        // t = w_tiles has no scores to make and t = 0 no product with values: those halves run on what is there
+        const int t = t_mfma;
+        if (t <= w_tiles && w_tiles > 0) {
+          const uint16_t *vtile = Vs[(t + kRing - 1) % kRing];
+          const uint16_t *ktile = Ks[t % kRing];
+          // fragment i < NP: V^T block m = i % NO, k-step i / NO; i >= NP: K block (i - NP) % NKB, k-step (i - NP) / NKB
+          constexpr int NP = NO * NT, NF = NP + NKB * NS;
+          auto frag = [&](int i) __device__ {
+            if (i < NP) {
+              const uint16_t *vp = vtile + (i / NO) * 32 * D + vfo[i % NO];
+              const u32x2_t a = lds_read_transposed(vp), b = lds_read_transposed(vp + 16 * D);
+              return u32x4_t{a[0], a[1], b[0], b[1]};
+            }
+            return ld16(ktile + ((i - NP) % NKB) * 16 * D + kfo[(i - NP) / NKB]);
+          };
+          __builtin_amdgcn_s_setprio(1);  // the MFMA wavefront of each SIMD issues ahead of the VALU wavefront beside it
+          u32x4_t fr[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) fr[i] = frag(i);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < NF; ++i) {
+            const u32x4_t a = fr[i % kAhead];
+#pragma unroll
+            for (int x = 0; x < kNQ; ++x) {
+              const int n = (i & 1) ? kNQ - 1 - x : x;
+              if (i < NP) {
+                oacc[i % NO][n] = mfma_bf16_16x16x32(as_bf16x8(a), as_bf16x8(pb[i / NO][n]), oacc[i % NO][n]);
+                if (i % NO == NO - 1)
+                  l_run[n] = mfma_bf16_16x16x32(as_bf16x8(ones), as_bf16x8(pb[i / NO][n]), l_run[n]);
+              } else {
+                const int kb = (i - NP) % NKB, st = (i - NP) / NKB;
+                if (st == 0) sacc[kb][n] = f32x4_t{};
+                sacc[kb][n] = mfma_bf16_16x16x32(as_bf16x8(a), qf[n][st], sacc[kb][n]);
+              }
+            }
+            if (i + kAhead < NF) fr[i % kAhead] = frag(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          __builtin_amdgcn_s_setprio(0);
+        }
+      } else {
+        tile_dma(min(t_valu + kRing - 1, T - 1), (t_valu + kRing - 1) % kRing);
+        if (p >= 1 + turn && t_valu < w_tiles) {
+          if (t_valu >= w_clear) {  // part of the tile lies behind a row
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int key = t_valu * kBN + 16 * kb + 4 * g + i;
+#pragma unroll
+                for (int n = 0; n < kNQ; ++n)
+                  if (key > last[n]) sacc[kb][n][i] = -INFINITY;
+              }
+          }
+          static_assert(NKB == 6 && kNQ == 2, "the max tree is written for 2 x 24 scores per lane");
+          float mt[kNQ];
+#pragma unroll
+          for (int n = 0; n < kNQ; ++n) {
+            float m1[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              m1[i] = fmaxf(fmaxf(sacc[0][n][i], sacc[1][n][i]), sacc[2][n][i]);
+              m1[4 + i] = fmaxf(fmaxf(sacc[3][n][i], sacc[4][n][i]), sacc[5][n][i]);
+            }
+            const float a = fmaxf(fmaxf(m1[0], m1[1]), m1[2]), b = fmaxf(fmaxf(m1[3], m1[4]), m1[5]);
+            mt[n] = fmaxf(fmaxf(a, b), fmaxf(m1[6], m1[7]));
+          }
+          group_max(mt[0], mt[1]);
+          bool grow = false;
+#pragma unroll
+          for (int n = 0; n < kNQ; ++n) {
+            mt[n] *= scale_log2;
+            grow = grow || mt[n] > m_run[n] + kLazy;
+          }
+          if (__any(grow)) {
+#pragma unroll
+            for (int n = 0; n < kNQ; ++n) {
+              const float m_new = mt[n] > m_run[n] + kLazy ? mt[n] : m_run[n];
+              const float corr = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+              m_run[n] = m_new;
+              l_run[n] *= corr;
+#pragma unroll
+              for (int m = 0; m < NO; ++m) oacc[m][n] *= corr;
+            }
+          }
+          // P in bf16 pairs (the values the PV product and the row sums use)
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+            for (int n = 0; n < kNQ; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sacc[kb][n][i], scale_log2, -m_run[n]));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sacc[kb][n][i + 1], scale_log2, -m_run[n]));
+                pb[kb >> 1][n][2 * (kb & 1) + (i >> 1)] = pack_bf2(p0, p1);
+              }
+        }
+      }
+      // before an even phase 2(t+1): K(t+1) and V(t) have landed; each group's latest issue may still be in flight
+      if (p & 1) wait_vm_lds<(kRing - 2) * CG>();
+      bare_barrier();
+    }
+    wait_vm_lds<0>();  // no tile load may land in LDS after the workgroup ends
+  }
+
+  bool again[kNQ];
+#pragma unroll
+  for (int n = 0; n < kNQ; ++n) {
+    const float inv = 1.f / l_run[n][0];
+    again[n] = false;
+    if (w0 + 16 * n + l16 < blk.r1) {
+      const bool any = last[n] >= 0;
+#pragma unroll
+      for (int m = 0; m < NO; ++m) {
+        float o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] = any ? oacc[m][n][i] * inv : 0.f;
+          again[n] = again[n] || !(fabsf(o[i]) < INFINITY);
+        }
+        *reinterpret_cast<uint2 *>(op[n] + 16 * m + 4 * g) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+      }
+    }
+  }
+  // A value that is not finite behind a row, in a tile that the row sees a part of, times the row's probability 0 is a NaN in
+  // its sum. Rows whose result is not finite are computed once more without the keys that they do not see: never for
+  // finite inputs whose result bf16 holds.
+#pragma unroll
+  for (int n = 0; n < kNQ; ++n) {
+    uint64_t todo = __ballot(again[n]);
+    todo |= todo >> 32;
+    todo |= todo >> 16;
+    if (todo) wait_vm_lds<0>();  // the stores above come first
+    for (uint32_t rows = (uint32_t)todo & 0xffffu; rows; rows &= rows - 1) {
+      const int r = w0 + 16 * n + __builtin_ctz(rows), token = r / group, head = kvh * group + (r - token * group);
+      attend_row<D>(q.at(blk.b, sq.q0 + token, head), k.at(blk.b, sq.k0, kvh), k.row, v.at(blk.b, sq.k0, kvh), v.row,
+                    min(behind + token + 1, sq.keys), scale_log2, const_cast<uint16_t *>(out.at(blk.b, sq.q0 + token, head)),
+                    lane);
+    }
+  }
 }
 
 int check_operand(const Operand &o, const char *name) {
@@ -131,23 +444,28 @@ int check_causal(const Operand &q, const Operand &k, const Operand &v, const Ope
   if (!rc) rc = check_operand(k, "k");
   if (!rc) rc = check_operand(v, "v");
   if (!rc) rc = check_operand(out, "out");
-  return rc;
+  if (rc) return rc;
+  // a lane's offset inside a tile is 32 bits of bytes: 95 rows and a row's channels
+  VDNH3_HOST_CHECK(k.row >= 0 && v.row >= 0 && k.row <= (1 << 24) && v.row <= (1 << 24), VDNH3_ERR_INVALID,
+                   "causal attention: rows of k and v may be at most %d elements apart", 1 << 24);
+  return VDNH3_OK;
 }
 
-int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs,
-                  int64_t rows, int heads, int kv_heads, int head_dim, float scale, hipStream_t s) {
-  const int64_t total = rows * heads;
+int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int heads,
+                  int kv_heads, int head_dim, float scale, hipStream_t s) {
+  const int group = heads / kv_heads;
+  const int64_t blocks = seqs.cu ? (int64_t)seqs.rows * group / kBM + seqs.count
+                                 : seqs.count * (((int64_t)seqs.rows * group + kBM - 1) / kBM);
+  VDNH3_HOST_CHECK((int64_t)seqs.rows * group <= INT32_MAX - kBM && blocks * kv_heads <= INT32_MAX, VDNH3_ERR_INVALID,
+                   "causal attention: %d rows of %d heads are too many for one launch", seqs.rows, heads);
   const float scale_log2 = scale * 1.4426950408889634f;
-  const int64_t groups = (total + 3) / 4;
-  VDNH3_HOST_CHECK(groups <= INT32_MAX, VDNH3_ERR_INVALID, "causal attention: %lld query rows are too many for one launch",
-                   (long long)rows);
-  const dim3 grid((unsigned)groups);
+  const dim3 grid((unsigned)(blocks * kv_heads));
   if (head_dim == 128)
-    hipLaunchKernelGGL(causal_rows_kernel<128>, grid, dim3(256), 0, s, q, k, v, out, seqs, heads, heads / kv_heads,
-                       scale_log2, total);
+    hipLaunchKernelGGL(causal_tile_kernel<128>, grid, dim3(kThreads), 0, s, q, k, v, out, seqs, (int)blocks, kv_heads, group,
+                       scale_log2);
   else
-    hipLaunchKernelGGL(causal_rows_kernel<64>, grid, dim3(256), 0, s, q, k, v, out, seqs, heads, heads / kv_heads,
-                       scale_log2, total);
+    hipLaunchKernelGGL(causal_tile_kernel<64>, grid, dim3(kThreads), 0, s, q, k, v, out, seqs, (int)blocks, kv_heads, group,
+                       scale_log2);
   return check_launch("causal attention");
 }
 
@@ -164,8 +482,8 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
   if (rc) return rc;
   VDNH3_HOST_CHECK(cu_seqlens && sequences > 0 && rows > 0, VDNH3_ERR_INVALID,
                    "causal attention: null sequence bounds, or no sequences or rows");
-  return launch_causal(qo, ko, vo, oo, Sequences{cu_seqlens, nullptr, sequences, rows, 0}, rows, heads, kv_heads, head_dim,
-                       scale, static_cast<hipStream_t>(stream));
+  return launch_causal(qo, ko, vo, oo, Sequences{cu_seqlens, nullptr, sequences, rows, 0}, heads, kv_heads, head_dim, scale,
+                       static_cast<hipStream_t>(stream));
 }
 
 extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head,
@@ -181,6 +499,6 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
   if (rc) return rc;
   VDNH3_HOST_CHECK(lengths && batch > 0 && new_tokens > 0 && room > 0, VDNH3_ERR_INVALID,
                    "causal attention: null lengths, or no sequences, new tokens or room in the cache");
-  return launch_causal(qo, ko, vo, oo, Sequences{nullptr, lengths, batch, new_tokens, room}, (int64_t)batch * new_tokens,
-                       heads, kv_heads, head_dim, scale, static_cast<hipStream_t>(stream));
+  return launch_causal(qo, ko, vo, oo, Sequences{nullptr, lengths, batch, new_tokens, room}, heads, kv_heads, head_dim,
+                       scale, static_cast<hipStream_t>(stream));
 }
