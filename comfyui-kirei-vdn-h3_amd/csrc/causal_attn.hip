@@ -427,22 +427,76 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
 }
 
 // ---------------------------------------------------------------------------------
-// Few rows over long caches (new tokens): what counts is to stream the keys and values once. The keys of a sequence are cut
-// into chunks, a workgroup taking one chunk of a key / value head for up to 16 NQ of its (token, head) rows. Its kW
-// wavefronts take the chunk's 32-key tiles in turn, each through two LDS slots of its own (one tile in flight while it works
-// on the other, no barrier), with a running softmax of its own; they are merged in LDS. A chunk's result is written
-// unnormalised in fp32 with its max and sum, and combined by a second launch; a sequence of one chunk is finished at once.
-constexpr int kFewKeys = 32;  // keys per tile: one k-step of the PV product
+// Few rows over long caches (new tokens): what counts is to stream the keys and values once. The 32-key tiles of all
+// sequences, one behind another, are cut into `ranges` equal ranges for each key / value head, one workgroup each and about
+// one workgroup per CU: whatever the lengths are, every CU streams the same number of tiles, in one round. A range crosses
+// from one sequence into the next; only the sequences at its two ends can be shared with other ranges. Such a part is
+// written unnormalised in fp32 with its max and sum and combined by a second launch; a sequence inside a range is
+// finished at once. The cut follows from the lengths on the device, in both kernels alike.
+// A workgroup takes up to 16 NQ of a head's (token, head) rows. Its wavefronts take the tiles in turn, each through two LDS
+// slots of its own (one tile in flight while it works on the other, no barrier), with a running softmax of its own; they
+// are merged in LDS at the end of a sequence.
+constexpr int kFewKeys = 32;      // keys per tile: one k-step of the PV product
 constexpr int kFewRing = 2;
+constexpr int kFewLeast = 8;      // tiles of a range, at least (two per wavefront): short caches take fewer ranges
+constexpr int kFewThreads = 256;  // of both kernels
 
-// Unnormalised results of the chunks: [sequence][kv head][chunk][row] of D floats, then the same of (max, sum).
-struct Chunks {
+// Unnormalised results of the ranges' ends: [kv head][range][end][row] of D floats, then the same of (max, sum).
+struct Parts {
   float *o;
   float2 *ml;
-  int size, count;  // keys of a chunk, chunks of a whole cache
+  int ranges;
+  __device__ __forceinline__ int64_t at(int kvh, int range, int end, int rows) const {
+    return (((int64_t)kvh * ranges + range) * 2 + end) * rows;
+  }
 };
-// The chunks that a sequence of `keys` keys has; one without keys still has one, which writes its rows.
-__device__ __forceinline__ int chunks_of(const Chunks &c, int keys) { return max(1, (keys + c.size - 1) / c.size); }
+
+// The tiles of a sequence; one without keys has one, which writes its rows.
+__device__ __forceinline__ int tiles_of(const Sequences &seqs, int b) {
+  const int keys = min(max(seqs.lengths[b], 0), seqs.room);
+  return max(1, (keys + kFewKeys - 1) / kFewKeys);
+}
+
+// How the tiles of all sequences are cut. Each of the workgroup's threads counts the tiles of `per` sequences; before[i] is
+// what the threads in front of i counted.
+struct Cut {
+  int64_t total;
+  int per, ranges;
+  const int64_t *before;
+  __device__ __forceinline__ int64_t start(int range) const { return range * total / ranges; }
+  // the range that holds tile u: the last that starts at or before it
+  __device__ __forceinline__ int range_of(int64_t u) const { return (int)(((u + 1) * ranges - 1) / total); }
+  // tiles in front of sequence b
+  __device__ __forceinline__ int64_t in_front(const Sequences &seqs, int b) const {
+    int64_t u = before[b / per];
+    for (int i = b / per * per; i < b; ++i) u += tiles_of(seqs, i);
+    return u;
+  }
+};
+__device__ __forceinline__ Cut make_cut(const Sequences &seqs, int ranges, int64_t (&before)[kFewThreads + 1]) {
+  __shared__ int64_t waves[kFewThreads / 64];
+  const int tid = threadIdx.x, per = (seqs.count + kFewThreads - 1) / kFewThreads;
+  int64_t own = 0;
+  for (int b = tid * per; b < min((tid + 1) * per, seqs.count); ++b) own += tiles_of(seqs, b);
+  int64_t sum = own;  // up to and with this lane's
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t x = __shfl_up(sum, o);
+    if ((tid & 63) >= o) sum += x;
+  }
+  if ((tid & 63) == 63) waves[tid >> 6] = sum;
+  __syncthreads();
+  int64_t front = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kFewThreads / 64; ++w) {
+    if (w < tid >> 6) front += waves[w];
+    total += waves[w];
+  }
+  before[tid] = front + sum - own;
+  if (tid == kFewThreads - 1) before[kFewThreads] = total;
+  __syncthreads();
+  return Cut{total, per, (int)min((int64_t)ranges, max(total / kFewLeast, (int64_t)1)), before};
+}
 
 // O / l of one row, two (one) channels per lane. Where new tokens stand behind one another (`masked`), a value that is not
 // finite behind the row, in a tile that it sees a part of, times the probability 0 is a NaN in its sum: such a row is
@@ -470,248 +524,278 @@ __device__ __forceinline__ void finish_row(const Operand &q, const Operand &k, c
   else op[lane] = f2bf(y[0]);
 }
 
-template <int D, int NQ, int W>
-__global__ __launch_bounds__(64 * W) void causal_few_kernel(Operand q, Operand k, Operand v, Operand out, Sequences seqs,
-                                                            int kv_heads, int group, int row_blocks, float scale_log2,
-                                                            Chunks chunks) {
-  constexpr int KC = D / 8, NS = D / 32, NO = D / 16, C = D / 64, ROWS = 16 * NQ;
+template <int D, int NQ>
+__global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Operand k, Operand v, Operand out, Sequences seqs,
+                                                                 int kv_heads, int group, int row_blocks, float scale_log2,
+                                                                 Parts parts) {
+  constexpr int KC = D / 8, NS = D / 32, NO = D / 16, C = D / 64, ROWS = 16 * NQ, W = kFewThreads / 64;
   constexpr int TILE = kFewKeys * D;  // elements
   static_assert(ROWS * D * 2 <= kFewRing * 2 * TILE, "a wavefront's sums fit its tiles' place");
   __shared__ __attribute__((aligned(16))) uint16_t tiles[W][kFewRing][2][TILE];
   __shared__ float2 stats[W][ROWS];
+  __shared__ int64_t before[kFewThreads + 1];
 
   // heads next to each other, whose rows lie side by side in a cache, then the row blocks, which read the same keys
-  int at = (int)blockIdx.x;
-  const int kvh = at % kv_heads;
-  at /= kv_heads;
-  const int rb = at % row_blocks;
-  at /= row_blocks;
-  const int chunk = at % chunks.count, b = at / chunks.count;
-  const Sequence s = sequence_at(seqs, b);
-  const int n_chunks = chunks_of(chunks, s.keys);
-  if (chunk >= n_chunks) return;
-  const int rows = s.n * group, r0 = rb * ROWS, r1 = min(r0 + ROWS, rows);
-  const int behind = s.keys - s.n;
-  const int k0 = chunk * chunks.size;
-  const int k1 = min(min(k0 + chunks.size, s.keys), behind + (r1 - 1) / group + 1);  // the last row sees keys below k1
-  const int n_tiles = k1 > k0 ? (k1 - k0 + kFewKeys - 1) / kFewKeys : 0;
-  const int clear = behind + r0 / group + 1;  // every row sees keys below it
+  const int kvh = (int)blockIdx.x % kv_heads, rb = (int)blockIdx.x / kv_heads % row_blocks;
+  const int range = (int)blockIdx.x / (kv_heads * row_blocks);
+  const Cut cut = make_cut(seqs, parts.ranges, before);
+  if (range >= cut.ranges) return;
+  int64_t u = cut.start(range);
+  const int64_t u1 = cut.start(range + 1);
+  const int rows = seqs.rows * group, r0 = rb * ROWS, r1 = min(r0 + ROWS, rows);
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int l16 = lane & 15, g = lane >> 4;
-  bf16x8_t qf[NQ][NS];
-  int last[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = min(r0 + 16 * n + l16, r1 - 1), token = r / group, head = kvh * group + (r - token * group);
-    last[n] = behind + token;
-    const uint16_t *qp = q.at(b, s.q0 + token, head) + 8 * g;
-#pragma unroll
-    for (int st = 0; st < NS; ++st) qf[n][st] = as_bf16x8(ld16(qp + 32 * st));
-  }
-
-  // A wavefront's load of a tile: instruction i brings rows i * 64 / KC + lane / KC, slot lane % KC (swizzled as in the
-  // kernel above). Rows past the chunk's keys read its last one (their scores are masked).
-  constexpr int LOADS = kFewKeys * KC / 64;
-  const int lr = lane / KC;
-  const uint16_t *kb = k.at(b, s.k0, kvh), *vb = v.at(b, s.k0, kvh);
-  const uint32_t lds0 = lds_address(&tiles[wave][0][0][0]);
-  auto load_tile = [&](int t, int ring) __device__ {
-    const int key = k0 + t * kFewKeys;
-    const uint16_t *kt = kb + (int64_t)key * k.row, *vt = vb + (int64_t)key * v.row;
-#pragma unroll
-    for (int which = 0; which < 2; ++which)
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = i * (64 / KC) + lr;
-        const int slot = which ? v_slot<D>(r, lane % KC) : k_slot<D>(r, lane % KC);
-        const uint32_t row = (uint32_t)(min(key + r, k1 - 1) - key);
-        global_to_lds16_sbase(which ? vt : kt, 2u * (row * (uint32_t)(which ? v.row : k.row) + slot * 8),
-                              lds0 + (uint32_t)((ring * 2 + which) * TILE * 2 + i * 1024));
-      }
-  };
-  int kfo[NS], vfo[NO];
-#pragma unroll
-  for (int st = 0; st < NS; ++st) kfo[st] = (l16 * KC + k_slot<D>(l16, 4 * st + g)) * 8;
-  const int vr = 4 * g + (l16 >> 2);
-#pragma unroll
-  for (int m = 0; m < NO; ++m) vfo[m] = vr * D + v_slot<D>(vr, 2 * m + ((l16 >> 1) & 1)) * 8 + 4 * (l16 & 1);
-
-  f32x4_t oacc[NO][NQ], l_run[NQ];
-  float m_run[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-    for (int m = 0; m < NO; ++m) oacc[m][n] = f32x4_t{};
-    m_run[n] = kNoMax;
-    l_run[n] = f32x4_t{};
-  }
-  const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
-
-  if (wave < n_tiles) load_tile(wave, 0);
-  int ring = 0;
-  for (int t = wave; t < n_tiles; t += W, ring ^= 1) {
-    // the reads of the slot that is loaded now ended with the products of the last tile
-    if (t + W < n_tiles) {
-      load_tile(t + W, ring ^ 1);
-      wait_vm_lds<2 * LOADS>();
-    } else {
-      wait_vm_lds<0>();
+  // the sequence that holds tile u, and the tiles in front of it
+  int b = 0;
+  {
+    int lo = 0, hi = kFewThreads;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= u) lo = mid;
+      else hi = mid;
     }
-    asm volatile("" ::: "memory");
-    const uint16_t *ktile = tiles[wave][ring][0], *vtile = tiles[wave][ring][1];
-    f32x4_t sacc[2][NQ];
+    b = lo * cut.per;
+  }
+  int64_t front = before[b / cut.per];
+  int here = tiles_of(seqs, b);
+  while (front + here <= u) {
+    front += here;
+    here = tiles_of(seqs, ++b);
+  }
+  for (bool first_part = true; u < u1; first_part = false) {
+    const Sequence s = sequence_at(seqs, b);
+    const int behind = s.keys - s.n;
+    const int k0 = (int)(u - front) * kFewKeys;
+    const int n_units = (int)(min(u1, front + here) - u);
+    const int k1 = min(k0 + n_units * kFewKeys, s.keys);
+    const int n_tiles = s.keys > 0 ? n_units : 0;
+    const int clear = behind + r0 / group + 1;  // every row sees keys below it
+    bf16x8_t qf[NQ][NS];
+    int last[NQ];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int n = 0; n < NQ; ++n) {
+      const int r = min(r0 + 16 * n + l16, r1 - 1), token = r / group, head = kvh * group + (r - token * group);
+      last[n] = behind + token;
+      const uint16_t *qp = q.at(b, s.q0 + token, head) + 8 * g;
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) sacc[h][n] = f32x4_t{};
-#pragma unroll
-      for (int st = 0; st < NS; ++st) {
-        const bf16x8_t a = as_bf16x8(ld16(ktile + h * 16 * D + kfo[st]));
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) sacc[h][n] = mfma_bf16_16x16x32(a, qf[n][st], sacc[h][n]);
-      }
+      for (int st = 0; st < NS; ++st) qf[n][st] = as_bf16x8(ld16(qp + 32 * st));
     }
-    const int key = k0 + t * kFewKeys;
-    if (key + kFewKeys > min(clear, k1)) {
+
+    // A wavefront's load of a tile: instruction i brings rows i * 64 / KC + lane / KC, slot lane % KC (swizzled as in the
+    // kernel above). Rows past the part's keys read its last one (their scores are masked).
+    constexpr int LOADS = kFewKeys * KC / 64;
+    const int lr = lane / KC;
+    const uint16_t *kb = k.at(b, s.k0, kvh), *vb = v.at(b, s.k0, kvh);
+    const uint32_t lds0 = lds_address(&tiles[wave][0][0][0]);
+    auto load_tile = [&](int t, int ring) __device__ {
+      const int key = k0 + t * kFewKeys;
+      const uint16_t *kt = kb + (int64_t)key * k.row, *vt = vb + (int64_t)key * v.row;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int which = 0; which < 2; ++which)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at_key = key + 16 * h + 4 * g + i;
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-            if (at_key > last[n] || at_key >= k1) sacc[h][n][i] = -INFINITY;
+        for (int i = 0; i < LOADS; ++i) {
+          const int r = i * (64 / KC) + lr;
+          const int slot = which ? v_slot<D>(r, lane % KC) : k_slot<D>(r, lane % KC);
+          const uint32_t row = (uint32_t)(min(key + r, k1 - 1) - key);
+          global_to_lds16_sbase(which ? vt : kt, 2u * (row * (uint32_t)(which ? v.row : k.row) + slot * 8),
+                                lds0 + (uint32_t)((ring * 2 + which) * TILE * 2 + i * 1024));
         }
-    }
-    u32x4_t pb[NQ];
-    float mt[NQ];
+    };
+    int kfo[NS], vfo[NO];
+#pragma unroll
+    for (int st = 0; st < NS; ++st) kfo[st] = (l16 * KC + k_slot<D>(l16, 4 * st + g)) * 8;
+    const int vr = 4 * g + (l16 >> 2);
+#pragma unroll
+    for (int m = 0; m < NO; ++m) vfo[m] = vr * D + v_slot<D>(vr, 2 * m + ((l16 >> 1) & 1)) * 8 + 4 * (l16 & 1);
+
+    f32x4_t oacc[NO][NQ], l_run[NQ];
+    float m_run[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const f32x4_t x = sacc[0][n], y = sacc[1][n];
-      mt[n] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
-    }
 #pragma unroll
-    for (int n = 0; n < NQ; n += 2) {
-      float other = mt[n];
-      group_max(mt[n], n + 1 < NQ ? mt[n + 1 < NQ ? n + 1 : n] : other);
+      for (int m = 0; m < NO; ++m) oacc[m][n] = f32x4_t{};
+      m_run[n] = kNoMax;
+      l_run[n] = f32x4_t{};
     }
-    bool grow = false;
+    const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
+
+    if (wave < n_tiles) load_tile(wave, 0);
+    int ring = 0;
+    for (int t = wave; t < n_tiles; t += W, ring ^= 1) {
+      // the reads of the slot that is loaded now ended with the products of the last tile
+      if (t + W < n_tiles) {
+        load_tile(t + W, ring ^ 1);
+        wait_vm_lds<2 * LOADS>();
+      } else {
+        wait_vm_lds<0>();
+      }
+      asm volatile("" ::: "memory");
+      const uint16_t *ktile = tiles[wave][ring][0], *vtile = tiles[wave][ring][1];
+      f32x4_t sacc[2][NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      mt[n] *= scale_log2;
-      grow = grow || mt[n] > m_run[n] + kLazy;
-    }
-    if (__any(grow)) {
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) sacc[h][n] = f32x4_t{};
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+          const bf16x8_t a = as_bf16x8(ld16(ktile + h * 16 * D + kfo[st]));
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) sacc[h][n] = mfma_bf16_16x16x32(a, qf[n][st], sacc[h][n]);
+        }
+      }
+      const int key = k0 + t * kFewKeys;
+      if (key + kFewKeys > min(clear, k1)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at_key = key + 16 * h + 4 * g + i;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+              if (at_key > last[n] || at_key >= k1) sacc[h][n][i] = -INFINITY;
+          }
+      }
+      u32x4_t pb[NQ];
+      float mt[NQ];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        const float m_new = mt[n] > m_run[n] + kLazy ? mt[n] : m_run[n];
-        const float corr = __builtin_amdgcn_exp2f(m_run[n] - m_new);
-        m_run[n] = m_new;
-        l_run[n] *= corr;
-#pragma unroll
-        for (int m = 0; m < NO; ++m) oacc[m][n] *= corr;
+        const f32x4_t x = sacc[0][n], y = sacc[1][n];
+        mt[n] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
       }
+#pragma unroll
+      for (int n = 0; n < NQ; n += 2) {
+        float other = mt[n];
+        group_max(mt[n], n + 1 < NQ ? mt[n + 1 < NQ ? n + 1 : n] : other);
+      }
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        mt[n] *= scale_log2;
+        grow = grow || mt[n] > m_run[n] + kLazy;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          const float m_new = mt[n] > m_run[n] + kLazy ? mt[n] : m_run[n];
+          const float corr = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+          m_run[n] = m_new;
+          l_run[n] *= corr;
+#pragma unroll
+          for (int m = 0; m < NO; ++m) oacc[m][n] *= corr;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(sacc[h][n][i], scale_log2, -m_run[n]));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(sacc[h][n][i + 1], scale_log2, -m_run[n]));
+            pb[n][2 * h + (i >> 1)] = pack_bf2(p0, p1);
+          }
+        l_run[n] = mfma_bf16_16x16x32(as_bf16x8(ones), as_bf16x8(pb[n]), l_run[n]);
+      }
+#pragma unroll
+      for (int m = 0; m < NO; ++m) {
+        const u32x2_t x = lds_read_transposed(vtile + vfo[m]), y = lds_read_transposed(vtile + 16 * D + vfo[m]);
+        const bf16x8_t a = as_bf16x8(u32x4_t{x[0], x[1], y[0], y[1]});
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) oacc[m][n] = mfma_bf16_16x16x32(a, as_bf16x8(pb[n]), oacc[m][n]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this tile is read: the next trip loads over it
     }
+
+    // Each wavefront's sums into its tiles' place: row 16 n + l16, 16-byte chunk 4 m + g at chunk ^ (row % 16).
+    float *mine = reinterpret_cast<float *>(&tiles[wave][0][0][0]);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
+      const int r = 16 * n + l16;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int m = 0; m < NO; ++m)
+        *reinterpret_cast<f32x4_t *>(mine + r * D + 4 * ((4 * m + g) ^ l16)) = oacc[m][n];
+      if (g == 0) stats[wave][r] = make_float2(m_run[n], l_run[n][0]);
+    }
+    __syncthreads();
+    for (int r = wave; r < r1 - r0; r += W) {
+      float top = kNoMax;
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sacc[h][n][i], scale_log2, -m_run[n]));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sacc[h][n][i + 1], scale_log2, -m_run[n]));
-          pb[n][2 * h + (i >> 1)] = pack_bf2(p0, p1);
+      for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w][r].x);
+      float o[C] = {}, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float2 ml = stats[w][r];
+        const float by = __builtin_amdgcn_exp2f(ml.x - top);
+        const float *from = reinterpret_cast<const float *>(&tiles[w][0][0][0]) + r * D;
+        l = fmaf(by, ml.y, l);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int d = C * lane + c;
+          o[c] = fmaf(by, from[4 * ((d >> 2) ^ (r & 15)) + (d & 3)], o[c]);
         }
-      l_run[n] = mfma_bf16_16x16x32(as_bf16x8(ones), as_bf16x8(pb[n]), l_run[n]);
-    }
+      }
+      if (n_units == here) {
+        finish_row<D>(q, k, v, out, s, b, kvh, group, r0 + r, o, l, scale_log2, lane);
+      } else {
+        const int64_t to = parts.at(kvh, range, first_part ? 0 : 1, rows) + r0 + r;
 #pragma unroll
-    for (int m = 0; m < NO; ++m) {
-      const u32x2_t x = lds_read_transposed(vtile + vfo[m]), y = lds_read_transposed(vtile + 16 * D + vfo[m]);
-      const bf16x8_t a = as_bf16x8(u32x4_t{x[0], x[1], y[0], y[1]});
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) oacc[m][n] = mfma_bf16_16x16x32(a, as_bf16x8(pb[n]), oacc[m][n]);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this tile is read: the next trip loads over it
-  }
-
-  // Each wavefront's sums into its tiles' place: row 16 n + l16, 16-byte chunk 4 m + g at chunk ^ (row % 16).
-  float *mine = reinterpret_cast<float *>(&tiles[wave][0][0][0]);
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = 16 * n + l16;
-#pragma unroll
-    for (int m = 0; m < NO; ++m)
-      *reinterpret_cast<f32x4_t *>(mine + r * D + 4 * ((4 * m + g) ^ l16)) = oacc[m][n];
-    if (g == 0) stats[wave][r] = make_float2(m_run[n], l_run[n][0]);
-  }
-  __syncthreads();
-  for (int r = wave; r < r1 - r0; r += W) {
-    float top = kNoMax;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w][r].x);
-    float o[C] = {}, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float2 ml = stats[w][r];
-      const float by = __builtin_amdgcn_exp2f(ml.x - top);
-      const float *from = reinterpret_cast<const float *>(&tiles[w][0][0][0]) + r * D;
-      l = fmaf(by, ml.y, l);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int d = C * lane + c;
-        o[c] = fmaf(by, from[4 * ((d >> 2) ^ (r & 15)) + (d & 3)], o[c]);
+        for (int c = 0; c < C; ++c) parts.o[to * D + C * lane + c] = o[c];
+        if (lane == 0) parts.ml[to] = make_float2(top, l);
       }
     }
-    if (n_chunks == 1) {
-      finish_row<D>(q, k, v, out, s, b, kvh, group, r0 + r, o, l, scale_log2, lane);
-    } else {
-      const int64_t to = (((int64_t)b * kv_heads + kvh) * chunks.count + chunk) * rows + r0 + r;
-#pragma unroll
-      for (int c = 0; c < C; ++c) chunks.o[to * D + C * lane + c] = o[c];
-      if (lane == 0) chunks.ml[to] = make_float2(top, l);
+    u += n_units;
+    if (u < u1) {
+      front += here;
+      here = tiles_of(seqs, ++b);
+      __syncthreads();  // the sums are read: the next sequence's tiles load over them
     }
   }
 }
 
-// One workgroup per row of a sequence with more than one chunk: its wavefronts take the chunks in turn.
+// One workgroup per row of a sequence that several ranges share: its wavefronts take the parts in turn.
 template <int D>
-__global__ __launch_bounds__(256) void causal_combine_kernel(Operand q, Operand k, Operand v, Operand out, Sequences seqs,
-                                                             int kv_heads, int group, float scale_log2, Chunks chunks) {
-  constexpr int C = D / 64;
-  __shared__ float sums[4][D];
-  __shared__ float2 stats[4];
+__global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, Operand k, Operand v, Operand out,
+                                                                     Sequences seqs, int kv_heads, int group,
+                                                                     float scale_log2, Parts parts) {
+  constexpr int C = D / 64, W = kFewThreads / 64;
+  __shared__ float sums[W][D];
+  __shared__ float totals[W];
+  __shared__ int64_t before[kFewThreads + 1];
   const int rows = seqs.rows * group;
   const int row = (int)blockIdx.x % rows, bh = (int)blockIdx.x / rows, b = bh / kv_heads, kvh = bh - b * kv_heads;
-  const Sequence s = sequence_at(seqs, b);
-  const int n_chunks = chunks_of(chunks, s.keys);
-  if (n_chunks == 1) return;
+  const Cut cut = make_cut(seqs, parts.ranges, before);
+  const int64_t u = cut.in_front(seqs, b);
+  const int first = cut.range_of(u), past = cut.range_of(u + tiles_of(seqs, b) - 1) + 1;
+  if (past - first == 1) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t first = (int64_t)bh * chunks.count * rows + row;
+  // a range's part of the sequence is its first one, but in a range that began in an earlier sequence
+  const int early = cut.start(first) < u ? first : -1;
   float top = kNoMax;
-  for (int c = lane; c < n_chunks; c += 64) top = fmaxf(top, chunks.ml[first + (int64_t)c * rows].x);
+  for (int i = first + lane; i < past; i += 64) top = fmaxf(top, parts.ml[parts.at(kvh, i, i == early, rows) + row].x);
   top = wave_max(top);
   float o[C] = {}, l = 0.f;
-  for (int c = wave; c < n_chunks; c += 4) {
-    const int64_t from = first + (int64_t)c * rows;
-    const float2 ml = chunks.ml[from];
+#pragma unroll 4
+  for (int i = first + wave; i < past; i += W) {
+    const int64_t from = parts.at(kvh, i, i == early, rows) + row;
+    const float2 ml = parts.ml[from];
     const float by = __builtin_amdgcn_exp2f(ml.x - top);
     l = fmaf(by, ml.y, l);
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = fmaf(by, chunks.o[from * D + C * lane + i], o[i]);
+    for (int c = 0; c < C; ++c) o[c] = fmaf(by, parts.o[from * D + C * lane + c], o[c]);
   }
 #pragma unroll
-  for (int i = 0; i < C; ++i) sums[wave][C * lane + i] = o[i];
-  if (lane == 0) stats[wave].y = l;
+  for (int c = 0; c < C; ++c) sums[wave][C * lane + c] = o[c];
+  if (lane == 0) totals[wave] = l;
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    l += stats[w].y;
+  for (int w = 1; w < W; ++w) {
+    l += totals[w];
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] += sums[w][C * lane + i];
+    for (int c = 0; c < C; ++c) o[c] += sums[w][C * lane + c];
   }
-  finish_row<D>(q, k, v, out, s, b, kvh, group, row, o, l, scale_log2, lane);
+  finish_row<D>(q, k, v, out, sequence_at(seqs, b), b, kvh, group, row, o, l, scale_log2, lane);
 }
 
 int check_operand(const Operand &o, const char *name) {
@@ -761,39 +845,32 @@ int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Op
 
 // Rows of a key / value head (new tokens x heads of a group) up to which a cached call takes the few-row kernel.
 constexpr int kFewRows = 128;
-constexpr int kFewWaves = 4;
+constexpr int kFewGroups = 256;  // workgroups: one per CU (128 KB of LDS at D = 128)
 
-int few_rows_of_block(int64_t rows) { return rows <= 16 ? 16 : 32; }
-
-// Keys of a chunk: a whole cache in one round of workgroups where that leaves them at most 1,024 keys each, else 1,024.
-int few_chunk(int batch, int64_t rows, int room, int kv_heads) {
-  const int64_t blocks = (rows + few_rows_of_block(rows) - 1) / few_rows_of_block(rows);
-  const int64_t keys = (int64_t)room * batch * kv_heads * blocks / 256;
-  return (int)std::min<int64_t>(std::max<int64_t>((keys + 127) / 128 * 128, 128), 1024);
-}
+int few_block(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
 template <int D, int NQ>
 int launch_few(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int kv_heads,
-               int group, float scale_log2, const Chunks &chunks, hipStream_t s) {
+               int group, float scale_log2, const Parts &parts, hipStream_t s) {
   const int rows = seqs.rows * group, row_blocks = (rows + 16 * NQ - 1) / (16 * NQ);
-  const int64_t blocks = (int64_t)seqs.count * row_blocks * chunks.count * kv_heads;
-  VDNH3_HOST_CHECK(blocks <= INT32_MAX, VDNH3_ERR_INVALID, "causal attention: %lld chunks are too many for one launch",
+  const int64_t blocks = (int64_t)kv_heads * row_blocks * parts.ranges;
+  VDNH3_HOST_CHECK(blocks <= INT32_MAX, VDNH3_ERR_INVALID, "causal attention: %lld ranges are too many for one launch",
                    (long long)blocks);
-  hipLaunchKernelGGL((causal_few_kernel<D, NQ, kFewWaves>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, s, q, k, v, out,
-                     seqs, kv_heads, group, row_blocks, scale_log2, chunks);
+  hipLaunchKernelGGL((causal_few_kernel<D, NQ>), dim3((unsigned)blocks), dim3(kFewThreads), 0, s, q, k, v, out, seqs, kv_heads,
+                     group, row_blocks, scale_log2, parts);
   int rc = check_launch("causal attention over caches");
-  if (rc || chunks.count == 1) return rc;
-  hipLaunchKernelGGL(causal_combine_kernel<D>, dim3((unsigned)(seqs.count * kv_heads * rows)), dim3(256), 0, s, q, k, v, out,
-                     seqs, kv_heads, group, scale_log2, chunks);
-  return check_launch("causal attention's chunks");
+  if (rc || parts.ranges == 1) return rc;
+  hipLaunchKernelGGL(causal_combine_kernel<D>, dim3((unsigned)(seqs.count * kv_heads * rows)), dim3(kFewThreads), 0, s, q, k,
+                     v, out, seqs, kv_heads, group, scale_log2, parts);
+  return check_launch("causal attention's ranges");
 }
 
 template <int D>
 int launch_few_rows(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs,
-                    int kv_heads, int group, float scale_log2, const Chunks &chunks, hipStream_t s) {
-  const int block = few_rows_of_block((int64_t)seqs.rows * group);
-  if (block == 16) return launch_few<D, 1>(q, k, v, out, seqs, kv_heads, group, scale_log2, chunks, s);
-  return launch_few<D, 2>(q, k, v, out, seqs, kv_heads, group, scale_log2, chunks, s);
+                    int kv_heads, int group, float scale_log2, const Parts &parts, hipStream_t s) {
+  if (few_block((int64_t)seqs.rows * group) == 16)
+    return launch_few<D, 1>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
+  return launch_few<D, 2>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
 }
 
 }  // namespace
@@ -813,16 +890,20 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
                        static_cast<hipStream_t>(stream));
 }
 
-extern "C" int vdnh3_causal_cached_chunk(int batch, int new_tokens, int room, int heads, int kv_heads) {
+extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads) {
+  using namespace vdnh3;
   if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
   const int64_t rows = (int64_t)new_tokens * (heads / kv_heads);
-  return rows > vdnh3::kFewRows ? 0 : vdnh3::few_chunk(batch, rows, room, kv_heads);
+  if (rows > kFewRows) return 0;
+  const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
+  // no more ranges than full caches have tiles for
+  const int64_t most = (int64_t)batch * ((room + kFewKeys - 1) / kFewKeys) / kFewLeast;
+  return (int)std::max<int64_t>(std::min<int64_t>(kFewGroups / blocks, most), 1);
 }
 
-extern "C" size_t vdnh3_causal_partial_bytes(int batch, int new_tokens, int room, int heads, int head_dim, int chunk) {
-  if (batch <= 0 || new_tokens <= 0 || room <= 0 || heads <= 0 || head_dim <= 0 || chunk <= 0 || room <= chunk) return 0;
-  const size_t count = ((size_t)room + chunk - 1) / chunk;
-  return count * batch * new_tokens * heads * (head_dim + 2) * sizeof(float);
+extern "C" size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges) {
+  if (new_tokens <= 0 || heads <= 0 || head_dim <= 0 || ranges <= 1) return 0;
+  return (size_t)ranges * 2 * new_tokens * heads * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head,
@@ -830,7 +911,7 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
                                         const uint16_t *v, int64_t v_batch, int64_t v_row, int64_t v_head, uint16_t *out,
                                         int64_t o_batch, int64_t o_row, int64_t o_head, const int32_t *lengths, int batch,
                                         int new_tokens, int room, int heads, int kv_heads, int head_dim, float scale,
-                                        int chunk, float *partial, size_t partial_bytes, void *stream) {
+                                        int ranges, float *partial, size_t partial_bytes, void *stream) {
   using namespace vdnh3;
   const Operand qo{q, q_batch, q_row, q_head}, ko{k, k_batch, k_row, k_head}, vo{v, v_batch, v_row, v_head},
       oo{out, o_batch, o_row, o_head};
@@ -840,21 +921,19 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
                    "causal attention: null lengths, or no sequences, new tokens or room in the cache");
   const Sequences seqs{nullptr, lengths, batch, new_tokens, room};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (chunk == 0) return launch_causal(qo, ko, vo, oo, seqs, heads, kv_heads, head_dim, scale, s);
+  if (ranges == 0) return launch_causal(qo, ko, vo, oo, seqs, heads, kv_heads, head_dim, scale, s);
   const int group = heads / kv_heads;
   const int64_t rows = (int64_t)new_tokens * group;
-  VDNH3_HOST_CHECK(chunk > 0 && chunk % kFewKeys == 0 && room <= INT32_MAX - chunk, VDNH3_ERR_INVALID,
-                   "causal attention: a chunk must be a positive multiple of %d keys, got %d", kFewKeys, chunk);
+  VDNH3_HOST_CHECK(ranges > 0 && room <= INT32_MAX - kFewKeys, VDNH3_ERR_INVALID,
+                   "causal attention: the ranges must not be negative, got %d", ranges);
   VDNH3_HOST_CHECK(rows * batch * kv_heads <= INT32_MAX, VDNH3_ERR_INVALID,
-                   "causal attention: %d x %d new tokens are too many for chunks of keys", batch, new_tokens);
-  const size_t need = vdnh3_causal_partial_bytes(batch, new_tokens, room, heads, head_dim, chunk);
+                   "causal attention: %d x %d new tokens are too many for ranges of keys", batch, new_tokens);
+  const size_t need = vdnh3_causal_partial_bytes(new_tokens, heads, head_dim, ranges);
   VDNH3_HOST_CHECK(need == 0 || (partial && reinterpret_cast<uintptr_t>(partial) % 16 == 0 && partial_bytes >= need),
-                   VDNH3_ERR_INVALID, "causal attention: the chunks' buffer must be 16-byte aligned and hold %zu bytes, got %zu",
+                   VDNH3_ERR_INVALID, "causal attention: the ranges' buffer must be 16-byte aligned and hold %zu bytes, got %zu",
                    need, partial_bytes);
-  const int count = (room + chunk - 1) / chunk;
-  const Chunks chunks{partial, reinterpret_cast<float2 *>(partial + (size_t)count * batch * kv_heads * rows * head_dim), chunk,
-                      count};
+  const Parts parts{partial, reinterpret_cast<float2 *>(partial + (size_t)ranges * 2 * new_tokens * heads * head_dim), ranges};
   const float scale_log2 = scale * 1.4426950408889634f;
-  return head_dim == 128 ? launch_few_rows<128>(qo, ko, vo, oo, seqs, kv_heads, group, scale_log2, chunks, s)
-                         : launch_few_rows<64>(qo, ko, vo, oo, seqs, kv_heads, group, scale_log2, chunks, s);
+  return head_dim == 128 ? launch_few_rows<128>(qo, ko, vo, oo, seqs, kv_heads, group, scale_log2, parts, s)
+                         : launch_few_rows<64>(qo, ko, vo, oo, seqs, kv_heads, group, scale_log2, parts, s);
 }

@@ -125,14 +125,14 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
         return out.zero_()
     lengths = lengths.to(torch.int32).contiguous()
     lib = _lib.lib()
-    chunk = lib.vdnh3_causal_cached_chunk(batch, new, room, heads, kv_heads)
-    size = lib.vdnh3_causal_partial_bytes(batch, new, room, heads, dim, chunk)
+    ranges = lib.vdnh3_causal_cached_ranges(batch, new, room, heads, kv_heads)
+    size = lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
     partial = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     with _lib.on_device(device):
         rc = lib.vdnh3_causal_attn_cached(
             _lib.ptr(q), *_lib.strides(q), _lib.ptr(key_cache), *_lib.strides(key_cache), _lib.ptr(value_cache),
             *_lib.strides(value_cache), _lib.ptr(out), *_lib.strides(out), _lib.ptr(lengths), batch, new, room, heads, kv_heads, dim,
-            float(scale), chunk, _lib.ptr(partial), size, _lib.stream_handle(device))
+            float(scale), ranges, _lib.ptr(partial), size, _lib.stream_handle(device))
     _lib.check(rc, "causal_softmax_cached")
     return out
 

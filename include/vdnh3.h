@@ -546,16 +546,17 @@ int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_t q_head, c
 
 /* The same for new_tokens queries of each of `batch` sequences over caches of `room` rows: sequence b has
  * lengths[b] (device, cut to [0, room]) keys, and token i sees keys 0 .. lengths[b] - new_tokens + i (none: zeros).
- * chunk 0 takes whole rows; a multiple of 32 cuts the keys into chunks of that many, whose results are kept in
- * `partial` (vdnh3_causal_partial_bytes, 16-byte aligned; 0 bytes where a cache is one chunk) and combined.
- * vdnh3_causal_cached_chunk gives the chunk that suits a call (0 for many new tokens). */
-int vdnh3_causal_cached_chunk(int batch, int new_tokens, int room, int heads, int kv_heads);
-size_t vdnh3_causal_partial_bytes(int batch, int new_tokens, int room, int heads, int head_dim, int chunk);
+ * ranges 0 takes whole rows; otherwise the keys of all sequences, one behind another, are cut into that many ranges,
+ * equal in length, and the results of sequences that ranges share are kept in `partial`
+ * (vdnh3_causal_partial_bytes, 16-byte aligned; 0 bytes for one range) and combined. vdnh3_causal_cached_ranges gives
+ * the number that suits a call (0 for many new tokens). */
+int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads);
+size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges);
 int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
                              int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch,
                              int64_t v_row, int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row, int64_t o_head,
                              const int32_t *lengths, int batch, int new_tokens, int room, int heads, int kv_heads,
-                             int head_dim, float scale, int chunk, float *partial, size_t partial_bytes, void *stream);
+                             int head_dim, float scale, int ranges, float *partial, size_t partial_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------
  * Calibration (no counterpart in the reference): the sustained MFMA rate of the part on
