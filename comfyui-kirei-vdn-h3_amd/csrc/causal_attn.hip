@@ -438,7 +438,10 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
 // are merged in LDS at the end of a sequence.
 constexpr int kFewKeys = 32;      // keys per tile: one k-step of the PV product
 constexpr int kFewRing = 2;
-constexpr int kFewLeast = 8;      // tiles of a range, at least (two per wavefront): short caches take fewer ranges
+// Tiles of a range, at least: one per wavefront (one request of 1,000 keys x 40 / 8 heads: 16 ranges 11.1 us, 8 11.3, 4 12.2).
+constexpr int kFewLeast = 4;
+// Tiles of all caches up to which one range takes them and no second launch is needed (600 keys 11.1 us against 11.2 to 12.9).
+constexpr int kFewOne = 18;
 constexpr int kFewThreads = 256;  // of both kernels
 
 // Unnormalised results of the ranges' ends: [kv head][range][end][row] of D floats, then the same of (max, sum).
@@ -457,45 +460,45 @@ __device__ __forceinline__ int tiles_of(const Sequences &seqs, int b) {
   return max(1, (keys + kFewKeys - 1) / kFewKeys);
 }
 
-// How the tiles of all sequences are cut. Each of the workgroup's threads counts the tiles of `per` sequences; before[i] is
-// what the threads in front of i counted.
+// How the tiles of all sequences are cut: `each` per range, the first `more` ranges one more. Each of the workgroup's threads
+// counts the tiles of `per` sequences; before[i] is what the threads in front of i counted.
 struct Cut {
-  int64_t total;
-  int per, ranges;
-  const int64_t *before;
-  __device__ __forceinline__ int64_t start(int range) const { return range * total / ranges; }
-  // the range that holds tile u: the last that starts at or before it
-  __device__ __forceinline__ int range_of(int64_t u) const { return (int)(((u + 1) * ranges - 1) / total); }
+  int total, per, ranges, each, more;
+  const int *before;
+  __device__ __forceinline__ int start(int range) const { return range * each + min(range, more); }
+  __device__ __forceinline__ int range_of(int u) const {
+    return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each;
+  }
   // tiles in front of sequence b
-  __device__ __forceinline__ int64_t in_front(const Sequences &seqs, int b) const {
-    int64_t u = before[b / per];
+  __device__ __forceinline__ int in_front(const Sequences &seqs, int b) const {
+    int u = before[b / per];
     for (int i = b / per * per; i < b; ++i) u += tiles_of(seqs, i);
     return u;
   }
 };
-__device__ __forceinline__ Cut make_cut(const Sequences &seqs, int ranges, int64_t (&before)[kFewThreads + 1]) {
-  __shared__ int64_t waves[kFewThreads / 64];
+__device__ __forceinline__ Cut make_cut(const Sequences &seqs, int ranges, int (&before)[kFewThreads]) {
+  __shared__ int waves[kFewThreads / 64];
   const int tid = threadIdx.x, per = (seqs.count + kFewThreads - 1) / kFewThreads;
-  int64_t own = 0;
+  int own = 0;
   for (int b = tid * per; b < min((tid + 1) * per, seqs.count); ++b) own += tiles_of(seqs, b);
-  int64_t sum = own;  // up to and with this lane's
+  int sum = own;  // up to and with this lane's
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t x = __shfl_up(sum, o);
+    const int x = __shfl_up(sum, o);
     if ((tid & 63) >= o) sum += x;
   }
   if ((tid & 63) == 63) waves[tid >> 6] = sum;
   __syncthreads();
-  int64_t front = 0, total = 0;
+  int front = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kFewThreads / 64; ++w) {
     if (w < tid >> 6) front += waves[w];
     total += waves[w];
   }
   before[tid] = front + sum - own;
-  if (tid == kFewThreads - 1) before[kFewThreads] = total;
   __syncthreads();
-  return Cut{total, per, (int)min((int64_t)ranges, max(total / kFewLeast, (int64_t)1)), before};
+  const int n = min(ranges, max(total / kFewLeast, 1)), each = total / n;
+  return Cut{total, per, n, each, total - n * each, before};
 }
 
 // O / l of one row, two (one) channels per lane. Where new tokens stand behind one another (`masked`), a value that is not
@@ -533,15 +536,15 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
   static_assert(ROWS * D * 2 <= kFewRing * 2 * TILE, "a wavefront's sums fit its tiles' place");
   __shared__ __attribute__((aligned(16))) uint16_t tiles[W][kFewRing][2][TILE];
   __shared__ float2 stats[W][ROWS];
-  __shared__ int64_t before[kFewThreads + 1];
+  __shared__ int before[kFewThreads];
 
   // heads next to each other, whose rows lie side by side in a cache, then the row blocks, which read the same keys
   const int kvh = (int)blockIdx.x % kv_heads, rb = (int)blockIdx.x / kv_heads % row_blocks;
   const int range = (int)blockIdx.x / (kv_heads * row_blocks);
   const Cut cut = make_cut(seqs, parts.ranges, before);
   if (range >= cut.ranges) return;
-  int64_t u = cut.start(range);
-  const int64_t u1 = cut.start(range + 1);
+  int u = cut.start(range);
+  const int u1 = cut.start(range + 1);
   const int rows = seqs.rows * group, r0 = rb * ROWS, r1 = min(r0 + ROWS, rows);
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -557,7 +560,7 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
     }
     b = lo * cut.per;
   }
-  int64_t front = before[b / cut.per];
+  int front = before[b / cut.per];
   int here = tiles_of(seqs, b);
   while (front + here <= u) {
     front += here;
@@ -566,8 +569,8 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
   for (bool first_part = true; u < u1; first_part = false) {
     const Sequence s = sequence_at(seqs, b);
     const int behind = s.keys - s.n;
-    const int k0 = (int)(u - front) * kFewKeys;
-    const int n_units = (int)(min(u1, front + here) - u);
+    const int k0 = (u - front) * kFewKeys;
+    const int n_units = min(u1, front + here) - u;
     const int k1 = min(k0 + n_units * kFewKeys, s.keys);
     const int n_tiles = s.keys > 0 ? n_units : 0;
     const int clear = behind + r0 / group + 1;  // every row sees keys below it
@@ -753,47 +756,72 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
   }
 }
 
-// One workgroup per row of a sequence that several ranges share: its wavefronts take the parts in turn.
+// One workgroup per row of a sequence that several ranges share: its wavefronts take the parts in turn, eight at once (their
+// loads do not wait for one another's maxima), and are merged in LDS.
 template <int D>
 __global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, Operand k, Operand v, Operand out,
                                                                      Sequences seqs, int kv_heads, int group,
                                                                      float scale_log2, Parts parts) {
-  constexpr int C = D / 64, W = kFewThreads / 64;
+  constexpr int C = D / 64, W = kFewThreads / 64, AT_ONCE = 8;
   __shared__ float sums[W][D];
-  __shared__ float totals[W];
-  __shared__ int64_t before[kFewThreads + 1];
+  __shared__ float2 stats[W];
+  __shared__ int before[kFewThreads];
   const int rows = seqs.rows * group;
   const int row = (int)blockIdx.x % rows, bh = (int)blockIdx.x / rows, b = bh / kv_heads, kvh = bh - b * kv_heads;
   const Cut cut = make_cut(seqs, parts.ranges, before);
-  const int64_t u = cut.in_front(seqs, b);
+  const int u = cut.in_front(seqs, b);
   const int first = cut.range_of(u), past = cut.range_of(u + tiles_of(seqs, b) - 1) + 1;
   if (past - first == 1) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // a range's part of the sequence is its first one, but in a range that began in an earlier sequence
   const int early = cut.start(first) < u ? first : -1;
-  float top = kNoMax;
-  for (int i = first + lane; i < past; i += 64) top = fmaxf(top, parts.ml[parts.at(kvh, i, i == early, rows) + row].x);
-  top = wave_max(top);
-  float o[C] = {}, l = 0.f;
-#pragma unroll 4
-  for (int i = first + wave; i < past; i += W) {
-    const int64_t from = parts.at(kvh, i, i == early, rows) + row;
-    const float2 ml = parts.ml[from];
-    const float by = __builtin_amdgcn_exp2f(ml.x - top);
-    l = fmaf(by, ml.y, l);
+  float o[C] = {}, l = 0.f, m = kNoMax;
+  for (int i0 = first + wave; i0 < past; i0 += W * AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float x[AT_ONCE][C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = fmaf(by, parts.o[from * D + C * lane + c], o[c]);
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int i = min(i0 + W * j, past - 1);
+      const int64_t from = parts.at(kvh, i, i == early, rows) + row;
+      ml[j] = parts.ml[from];
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[j][c] = parts.o[from * D + C * lane + c];
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      if (i0 + W * j < past) top = fmaxf(top, ml[j].x);
+    const float by = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= by;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] *= by;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (i0 + W * j >= past) break;
+      const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+      l = fmaf(f, ml[j].y, l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(f, x[j][c], o[c]);
+    }
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) sums[wave][C * lane + c] = o[c];
-  if (lane == 0) totals[wave] = l;
+  if (lane == 0) stats[wave] = make_float2(m, l);
   __syncthreads();
   if (wave) return;
+  float top = kNoMax;
 #pragma unroll
-  for (int w = 1; w < W; ++w) {
-    l += totals[w];
+  for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w].x);
+  l = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] += sums[w][C * lane + c];
+  for (int c = 0; c < C; ++c) o[c] = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float by = __builtin_amdgcn_exp2f(stats[w].x - top);
+    l = fmaf(by, stats[w].y, l);
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = fmaf(by, sums[w][C * lane + c], o[c]);
   }
   finish_row<D>(q, k, v, out, sequence_at(seqs, b), b, kvh, group, row, o, l, scale_log2, lane);
 }
@@ -896,9 +924,9 @@ extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, i
   const int64_t rows = (int64_t)new_tokens * (heads / kv_heads);
   if (rows > kFewRows) return 0;
   const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
-  // no more ranges than full caches have tiles for
-  const int64_t most = (int64_t)batch * ((room + kFewKeys - 1) / kFewKeys) / kFewLeast;
-  return (int)std::max<int64_t>(std::min<int64_t>(kFewGroups / blocks, most), 1);
+  const int64_t tiles = (int64_t)batch * ((room + kFewKeys - 1) / kFewKeys);
+  if (tiles > INT32_MAX) return 0;
+  return tiles <= kFewOne ? 1 : (int)std::max<int64_t>(std::min<int64_t>(kFewGroups / blocks, tiles / kFewLeast), 1);
 }
 
 extern "C" size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges) {
@@ -926,8 +954,9 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
   const int64_t rows = (int64_t)new_tokens * group;
   VDNH3_HOST_CHECK(ranges > 0 && room <= INT32_MAX - kFewKeys, VDNH3_ERR_INVALID,
                    "causal attention: the ranges must not be negative, got %d", ranges);
-  VDNH3_HOST_CHECK(rows * batch * kv_heads <= INT32_MAX, VDNH3_ERR_INVALID,
-                   "causal attention: %d x %d new tokens are too many for ranges of keys", batch, new_tokens);
+  VDNH3_HOST_CHECK(rows * batch * kv_heads <= INT32_MAX && (int64_t)batch * (room / kFewKeys + 1) <= INT32_MAX,
+                   VDNH3_ERR_INVALID, "causal attention: %d x %d new tokens or caches of %d rows are too many for ranges",
+                   batch, new_tokens, room);
   const size_t need = vdnh3_causal_partial_bytes(new_tokens, heads, head_dim, ranges);
   VDNH3_HOST_CHECK(need == 0 || (partial && reinterpret_cast<uintptr_t>(partial) % 16 == 0 && partial_bytes >= need),
                    VDNH3_ERR_INVALID, "causal attention: the ranges' buffer must be 16-byte aligned and hold %zu bytes, got %zu",
