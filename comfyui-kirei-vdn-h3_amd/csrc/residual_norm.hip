@@ -14,8 +14,6 @@
 namespace vdnh3 {
 namespace {
 
-constexpr int kNormThreads = 256;
-
 __device__ __forceinline__ void unpack8r(u32x4_t w, float *x) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -32,133 +30,254 @@ __device__ __forceinline__ u32x4_t pack8r(const float *y) {
 __device__ __forceinline__ uint32_t abs_bits(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 constexpr uint32_t kInfBits = 0x7f800000u;
 
-// Sum / largest over a workgroup of WAVES wavefronts; `red` is used by one reduction only.
-template <int WAVES>
-__device__ __forceinline__ float workgroup_sum(float v, float *red) {
+// The sum of v and the largest `top` over the THREADS threads of a row: a wavefront's lanes, or a workgroup of several
+// wavefronts through `red` (used once).
+struct Reduced {
+  float sum;
+  uint32_t top;
+};
+template <int THREADS>
+__device__ __forceinline__ Reduced reduce_row(float v, uint32_t top, uint2 *red) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = red[0];
+  for (int o = 32; o > 0; o >>= 1) {
+    v += __shfl_xor(v, o);
+    top = max(top, (uint32_t)__shfl_xor((int)top, o));
+  }
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_uint2(__float_as_uint(v), top);
+    __syncthreads();
+    v = __uint_as_float(red[0].x);
+    top = red[0].y;
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) s += red[w];
-  return s;
-}
-template <int WAVES>
-__device__ __forceinline__ uint32_t workgroup_max(uint32_t v, uint32_t *red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  uint32_t m = red[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) m = max(m, red[w]);
-  return m;
+    for (int w = 1; w < THREADS / 64; ++w) {
+      v += __uint_as_float(red[w].x);
+      top = max(top, red[w].y);
+    }
+  }
+  return Reduced{v, top};
 }
 
-// The quantisation of a row whose largest |y| has the bits `top`.
+// Eight int8 (KIND 1) or e4m3fn (KIND 2) codes of y * by, |y * by| at most the kind's largest number but for rounding.
 template <int KIND>
-struct RowScale {
-  float s, r;
-  bool fine;
-  __device__ __forceinline__ explicit RowScale(uint32_t top) {
-    fine = top < kInfBits;
-    s = fine ? fmaxf(__uint_as_float(top) / (KIND == 1 ? kI8Max : kF8Max), 1e-12f) : __builtin_nanf("");
-    r = fine ? 1.f / s : 0.f;
-  }
-  // quant_div: y / s to within its last place, by a product and one correction
-  __device__ __forceinline__ uint32_t code(float y) const {
-    if (!fine) return 0;
-    const float e = quant_div(y, s, r);
-    return KIND == 1 ? i8_code(e) : e4m3_code(fminf(fmaxf(e, -kF8Max), kF8Max));
-  }
-  __device__ __forceinline__ u32x2_t codes(const float *y) const {
+__device__ __forceinline__ u32x2_t codes8(const float *y, float by) {
+  float e[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = y[j] * by;
+  if constexpr (KIND == 1) {
+    // 1.5 * 2^23 + e rounds e to a whole number, ties to even, whose low byte is the code
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(e[j] + 12582912.f);
+    const uint32_t p0 = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), p1 = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
+    const uint32_t p2 = __builtin_amdgcn_perm(b[5], b[4], 0x0c0c0400), p3 = __builtin_amdgcn_perm(b[7], b[6], 0x04000c0c);
+    return u32x2_t{p0 | p1, p2 | p3};
+  } else {
+    // v_cvt_pk_fp8_f32 rounds to nearest even and keeps subnormals: for every fp32 up to 448 the code of e4m3_code
     u32x2_t w = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j >> 2] |= code(y[j]) << (8 * (j & 3));
+    for (int h = 0; h < 2; ++h) {
+      float c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = fminf(fmaxf(e[4 * h + j], -kF8Max), kF8Max);
+      int x = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+      w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], x, true);
+    }
     return w;
+  }
+}
+
+// What turns a row's t * w into y and into codes. With z = t w and r = 1 / sqrt(mean(t^2) + eps), y = z r, and
+// scale = max|z| r / q with q = 127 or 448: both reductions of a row are of its inputs alone and take one pass, and
+// y / scale = z (q / max|z|). Each is the row's by one more rounding than (t r) w would take.
+constexpr float kLeastMean = 0x1p-90f;  // below it the squares lose bits under fp32's smallest normal number
+template <int KIND>
+struct RowFactors {
+  float mean, y, code, scale;
+  bool plain;  // else the squares or the products pass fp32 either way, or are not numbers
+  __device__ __forceinline__ RowFactors(const Reduced &red, int hidden, float eps) {
+    constexpr float kMost = KIND == 1 ? kI8Max : kF8Max;
+    mean = red.sum / (float)hidden + eps;
+    plain = mean > kLeastMean && red.sum < INFINITY && red.top < kInfBits;
+    y = 1.f / sqrtf(mean);
+    if constexpr (KIND != 0) {
+      const float top = __uint_as_float(red.top), s = top * y / kMost;
+      scale = fmaxf(s, 1e-12f);
+      code = s > 1e-12f ? kMost / top : y / scale;
+      plain = plain && top * y < INFINITY && code < INFINITY;
+    }
   }
 };
 
-// 1 / sqrt(mean + eps) from a row's sum of squares. A sum past fp32 (values above 1e19) is taken again from values
-// scaled by 2^-64; `again` gives it.
-template <class Again>
-__device__ __forceinline__ float row_factor(float ss, int hidden, float eps, Again again) {
-  if (ss < INFINITY) return 1.f / sqrtf(ss / (float)hidden + eps);
-  constexpr float kDown = 5.421010862427522e-20f;  // 2^-64
-  return kDown / sqrtf(again(kDown) / (float)hidden + eps * kDown * kDown);
+// The rest of a row's outputs, where fp32 does not hold them that way: t scaled by a power of two for the squares, y =
+// (t r) w, and a row whose y is not finite gets the scale NaN and zero codes.
+template <int KIND>
+__device__ __forceinline__ float row_scale(uint32_t top) {
+  return top < kInfBits ? fmaxf(__uint_as_float(top) / (KIND == 1 ? kI8Max : kF8Max), 1e-12f) : __builtin_nanf("");
 }
 
-// One workgroup per row, any width: a sweep over the row for the sum of squares, one for the largest |y| (8-bit
-// kinds) and one for the outputs. The sum is written in the last sweep, each thread over what it alone read, so
-// `sum` may be x or the residual itself.
-template <int KIND>
-__global__ __launch_bounds__(kNormThreads) void residual_norm_sweep_kernel(
-    const uint16_t *x, int64_t x_row, const uint16_t *res, int64_t res_row, const uint16_t *__restrict__ w, float eps,
-    int hidden, void *__restrict__ out, int64_t out_row, float *__restrict__ scale, uint16_t *sum, int64_t sum_row) {
-  constexpr int WAVES = kNormThreads / 64;
-  __shared__ float red[2][WAVES];
-  __shared__ uint32_t top[WAVES];
-  const int64_t row = blockIdx.x;
-  const uint16_t *xr = x + row * x_row, *rr = res ? res + row * res_row : nullptr;
-  const int chunks = hidden / 8;
-  auto load = [&](int c, float *t) __device__ {
-    unpack8r(ld16(xr + 8 * c), t);
-    if (rr) {
+struct Rows {
+  const uint16_t *x, *res, *w;
+  int64_t x_row, res_row;
+  void *out;
+  float *scale;
+  uint16_t *sum;
+  int64_t out_row, sum_row;
+  int rows, hidden;
+  float eps;
+
+  __device__ __forceinline__ void load(int64_t row, int c, float *t) const {
+    unpack8r(ld16(x + row * x_row + 8 * c), t);
+    if (res) {
       float b[8];
-      unpack8r(ld16(rr + 8 * c), b);
+      unpack8r(ld16(res + row * res_row + 8 * c), b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) t[j] += b[j];
     }
-  };
-  auto squares = [&](float by, float *slot) __device__ {
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < chunks; c += kNormThreads) {
-      float t[8];
-      load(c, t);
+  }
+  __device__ __forceinline__ void weights(int c, float *wf) const { unpack8r(ld16(w + 8 * c), wf); }
+  // the outputs of chunk c: y * by is the norm (KIND 0) or the value that is coded
+  template <int KIND>
+  __device__ __forceinline__ void store(int64_t row, int c, const float *t, const float *y, float by) const {
+    if constexpr (KIND == 0) {
+      float n[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(t[j] * by, t[j] * by, ss);
+      for (int j = 0; j < 8; ++j) n[j] = y[j] * by;
+      st16(static_cast<uint16_t *>(out) + row * out_row + 8 * c, pack8r(n));
+    } else {
+      *reinterpret_cast<u32x2_t *>(static_cast<uint8_t *>(out) + row * out_row + 8 * c) = codes8<KIND>(y, by);
     }
-    return workgroup_sum<WAVES>(ss, slot);
-  };
-  const float r = row_factor(squares(1.f, red[0]), hidden, eps, [&](float by) __device__ { return squares(by, red[1]); });
-  auto normed = [&](int c, const float *t, float *y) __device__ {
+    // the next layer reads the sum, not the projection behind this kernel: it streams past the caches (253 -> 246 us below)
+    if (sum) st16_stream(sum + row * sum_row + 8 * c, pack8r(t));
+  }
+};
+
+// One row on THREADS threads: `each` calls a function with every chunk of the row that the thread has and its t. The outputs
+// are written after every read of the row, each thread's over what it alone read, so the sum may lie over x or the
+// residual.
+template <int KIND, int THREADS, class Each>
+__device__ __forceinline__ void norm_row(const Rows &p, int64_t row, bool leader, uint2 (*red)[THREADS / 64], Each each) {
+  float ss = 0.f;
+  uint32_t top = 0;
+  each([&](int c, const float *t) __device__ {
     float wf[8];
-    unpack8r(ld16(w + 8 * c), wf);
+    if constexpr (KIND != 0) p.weights(c, wf);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = t[j] * r * wf[j];
+    for (int j = 0; j < 8; ++j) {
+      ss = fmaf(t[j], t[j], ss);
+      if constexpr (KIND != 0) top = max(top, abs_bits(t[j] * wf[j]));
+    }
+  });
+  const RowFactors<KIND> f(reduce_row<THREADS>(ss, top, red[0]), p.hidden, p.eps);
+  if (f.plain) {
+    if (KIND != 0 && leader) p.scale[row] = f.scale;
+    each([&](int c, const float *t) __device__ {
+      float z[8];
+      p.weights(c, z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] *= t[j];
+      p.template store<KIND>(row, c, t, z, KIND == 0 ? f.y : f.code);
+    });
+    return;
+  }
+  const float shift = f.mean > 1.f || !(f.mean == f.mean) ? 0x1p-64f : 0x1p64f;
+  ss = 0.f;
+  each([&](int, const float *t) __device__ {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fmaf(t[j] * shift, t[j] * shift, ss);
+  });
+  const float r = shift / sqrtf(reduce_row<THREADS>(ss, 0, red[1]).sum / (float)p.hidden + p.eps * shift * shift);
+  auto normed = [&](int c, const float *t, float *y) __device__ {
+    p.weights(c, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] *= t[j] * r;
   };
-  uint32_t most = 0;
+  float by = 1.f;
   if constexpr (KIND != 0) {
-    for (int c = threadIdx.x; c < chunks; c += kNormThreads) {
-      float t[8], y[8];
-      load(c, t);
+    top = 0;
+    each([&](int c, const float *t) __device__ {
+      float y[8];
       normed(c, t, y);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, abs_bits(y[j]));
-    }
-    most = workgroup_max<WAVES>(most, top);
+      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(y[j]));
+    });
+    const float s = row_scale<KIND>(reduce_row<THREADS>(0.f, top, red[2]).top);
+    if (leader) p.scale[row] = s;
+    by = 1.f / s;
   }
-  const RowScale<KIND> q(most);
-  if (KIND != 0 && threadIdx.x == 0) scale[row] = q.s;
-  for (int c = threadIdx.x; c < chunks; c += kNormThreads) {
-    float t[8], y[8];
-    load(c, t);
+  each([&](int c, const float *t) __device__ {
+    float y[8];
     normed(c, t, y);
-    if constexpr (KIND == 0)
-      st16(static_cast<uint16_t *>(out) + row * out_row + 8 * c, pack8r(y));
-    else
-      *reinterpret_cast<u32x2_t *>(static_cast<uint8_t *>(out) + row * out_row + 8 * c) = q.codes(y);
-    if (sum) st16(sum + row * sum_row + 8 * c, pack8r(t));
-  }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (KIND != 0 && !(by > 0.f)) y[j] = 0.f;
+    p.template store<KIND>(row, c, t, y, KIND != 0 && !(by > 0.f) ? 0.f : by);
+  });
 }
 
+// Rows of up to 8 THREADS NCH channels: the row's sum stays in registers (fp32) from the loads, all in flight at once, to the
+// outputs. THREADS 64: a wavefront per row, four rows per workgroup, no barrier; 256: a workgroup per row.
+template <int KIND, int THREADS, int NCH>
+__global__ __launch_bounds__(256) void residual_norm_kernel(Rows p) {
+  __shared__ uint2 red[3][4];
+  const int64_t row = THREADS == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= p.rows) return;  // a whole wavefront (THREADS 64) or none
+  const int chunks = p.hidden / 8, tid = threadIdx.x % THREADS;
+  u32x4_t xv[NCH], rv[NCH];
+#pragma unroll
+  for (int u = 0; u < NCH; ++u) {
+    const int c = tid + THREADS * u;
+    if (c < chunks) {
+      xv[u] = ld16(p.x + row * p.x_row + 8 * c);
+      if (p.res) rv[u] = ld16(p.res + row * p.res_row + 8 * c);
+    }
+  }
+  float t[NCH][8];
+#pragma unroll
+  for (int u = 0; u < NCH; ++u) {
+    if (tid + THREADS * u < chunks) {
+      unpack8r(xv[u], t[u]);
+      if (p.res) {
+        float b[8];
+        unpack8r(rv[u], b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[u][j] += b[j];
+      }
+    }
+  }
+  norm_row<KIND, THREADS>(p, row, tid == 0, reinterpret_cast<uint2 (*)[THREADS / 64]>(red), [&](auto f) __device__ {
+#pragma unroll
+    for (int u = 0; u < NCH; ++u)
+      if (tid + THREADS * u < chunks) f(tid + THREADS * u, t[u]);
+  });
+}
+
+// Longer rows: a workgroup per row that reads it once for the sums and once more for the outputs.
 template <int KIND>
-void launch_residual_norm(const uint16_t *x, int64_t x_row, const uint16_t *res, int64_t res_row, const uint16_t *w,
-                          float eps, int rows, int hidden, void *out, int64_t out_row, float *scale, uint16_t *sum,
-                          int64_t sum_row, hipStream_t s) {
-  hipLaunchKernelGGL(residual_norm_sweep_kernel<KIND>, dim3(rows), dim3(kNormThreads), 0, s, x, x_row, res, res_row, w,
-                     eps, hidden, out, out_row, scale, sum, sum_row);
+__global__ __launch_bounds__(256) void residual_norm_sweep_kernel(Rows p) {
+  __shared__ uint2 red[3][4];
+  const int64_t row = blockIdx.x;
+  norm_row<KIND, 256>(p, row, threadIdx.x == 0, red, [&](auto f) __device__ {
+    for (int c = threadIdx.x; c < p.hidden / 8; c += 256) {
+      float t[8];
+      p.load(row, c, t);
+      f(c, t);
+    }
+  });
+}
+
+// A workgroup per row, but for many narrow rows in 8 bits, which leave its threads one chunk each or less: a wavefront per row.
+// 40,688 rows x 5,120 in int8: 253 us against 282 with a wavefront and ten chunks a lane; x 2,048: 113 against 106. HBM is
+// the bound: 246 us are 5.9 TB/s for the 7 bytes of an element, where a copy reaches 4.8.
+constexpr int kWaveWidth = 2048, kWaveRows = 4096;
+
+template <int KIND>
+void launch_residual_norm(const Rows &p, hipStream_t s) {
+  if (p.hidden > 8 * 256 * 4)
+    hipLaunchKernelGGL(residual_norm_sweep_kernel<KIND>, dim3(p.rows), dim3(256), 0, s, p);
+  else if (KIND != 0 && p.hidden <= kWaveWidth && p.rows >= kWaveRows)
+    hipLaunchKernelGGL((residual_norm_kernel<KIND, 64, 4>), dim3((p.rows + 3) / 4), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((residual_norm_kernel<KIND, 256, 4>), dim3(p.rows), dim3(256), 0, s, p);
 }
 
 // An operand that is only read may repeat one row (stride 0).
@@ -194,11 +313,9 @@ extern "C" int vdnh3_residual_rmsnorm_quant_rows(int kind, const uint16_t *x, in
                      VDNH3_ERR_INVALID,
                      "residual_rmsnorm: codes must be 8-byte aligned with a row stride of a multiple of 8, and have scales");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (kind == 0)
-    launch_residual_norm<0>(x, x_row, residual, residual_row, weight, eps, rows, hidden, out, out_row, scale, sum, sum_row, s);
-  else if (kind == 1)
-    launch_residual_norm<1>(x, x_row, residual, residual_row, weight, eps, rows, hidden, out, out_row, scale, sum, sum_row, s);
-  else
-    launch_residual_norm<2>(x, x_row, residual, residual_row, weight, eps, rows, hidden, out, out_row, scale, sum, sum_row, s);
+  const Rows p{x, residual, weight, x_row, residual_row, out, scale, sum, out_row, sum_row, rows, hidden, eps};
+  if (kind == 0) launch_residual_norm<0>(p, s);
+  else if (kind == 1) launch_residual_norm<1>(p, s);
+  else launch_residual_norm<2>(p, s);
   return check_launch("residual_rmsnorm");
 }

@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from contextlib import nullcontext
 from pathlib import Path
 
 import torch
@@ -190,14 +189,20 @@ def stream_handle(device: torch.device) -> int:
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
-def strides(t) -> list[int]:
+def strides(t) -> tuple[int, ...]:
     """The strides of every dim but the last; one of size 1 has none (torch may report anything for it)."""
-    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride())]
+    if 1 in t.shape:
+        return tuple(0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()))
+    return t.stride()[:-1]
 
 
 def in_place(t) -> bool:
     """Whether a kernel can take a bf16 tensor where it lies: 16-byte aligned rows of contiguous channels."""
-    return (t.stride(-1) == 1 or t.shape[-1] == 1) and not any(s % 8 for s in strides(t)) and t.data_ptr() % 16 == 0
+    if t.data_ptr() % 16:
+        return False
+    if t.shape[-1] % 8 == 0 and t.is_contiguous():
+        return True
+    return (t.stride(-1) == 1 or t.shape[-1] == 1) and not any(s % 8 for s in strides(t))
 
 
 def operand(t):
@@ -205,12 +210,16 @@ def operand(t):
     return t if in_place(t) else t.clone(memory_format=torch.contiguous_format)
 
 
-def on_device(device: torch.device):
-    """A context in which ``device`` is the current one: a launch on a stream of another device than the current one fails."""
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(index)
+def launch(what: str, fn, device: torch.device, *args) -> None:
+    """``fn(*args, stream)`` on torch's current stream of ``device``, with that device current (a launch on a stream of
+    another device than the current one fails); its status as ``check`` raises it."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_handle(device))
+    if rc:
+        check(rc, what)
 
 
 def forward_only(what: str, *tensors) -> None:

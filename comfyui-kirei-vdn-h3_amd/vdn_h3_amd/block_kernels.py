@@ -235,6 +235,9 @@ def swiglu_quantize_rows(hidden: torch.Tensor, kind: int):
     return q, scale
 
 
+_NORM_DTYPES = {_linear.KIND_BF16: torch.bfloat16, _linear.KIND_I8: torch.int8, _linear.KIND_F8: torch.float8_e4m3fn}
+
+
 def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, kind: int,
                               *, sum_out: torch.Tensor | None = None):
     """``t = x + residual`` and the RMSNorm of ``t`` as a projection takes it: ``(codes, scale[rows, 1] fp32, t bf16)``.
@@ -250,7 +253,7 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
         raise ValueError("residual_rmsnorm_quantize expects bf16 [rows, hidden]")
     if residual is not None and (residual.shape != x.shape or residual.dtype != torch.bfloat16):
         raise ValueError("the residual must be bf16 and of x's shape")
-    if kind not in (_linear.KIND_BF16, _linear.KIND_I8, _linear.KIND_F8):
+    if kind not in _NORM_DTYPES:
         raise ValueError(f"unknown kind {kind!r}; expected KIND_BF16, KIND_I8 or KIND_F8")
     rows, width = x.shape
     if weight.numel() != width or width == 0 or width % 8:
@@ -258,27 +261,26 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
     if sum_out is not None and (residual is None or sum_out.shape != x.shape or sum_out.dtype != torch.bfloat16
                                 or not _lib.in_place(sum_out) or (rows > 1 and sum_out.stride(0) < width)):
         raise ValueError("sum_out needs a residual, x's shape, bf16 and 16-byte rows")
-
-    def stride(t):  # of rows; one row's may be anything
-        return 0 if t is None else t.stride(0) if rows > 1 else width
-
     _lib.forward_only("residual_rmsnorm_quantize", x, residual, weight)
     device = _lib.require_device(x, residual, weight, sum_out)
-    xr, rr = _lib.operand(x), None if residual is None else _lib.operand(residual)
-    w = _lib.operand(weight.reshape(-1).to(torch.bfloat16))
-    total = x
-    if residual is not None:
-        total = torch.empty((rows, width), dtype=torch.bfloat16, device=device) if sum_out is None else sum_out
-    dtype = {_linear.KIND_BF16: torch.bfloat16, _linear.KIND_I8: torch.int8, _linear.KIND_F8: torch.float8_e4m3fn}[kind]
-    out = torch.empty((rows, width), dtype=dtype, device=device)
+    if weight.ndim != 1 or weight.dtype != torch.bfloat16:
+        weight = weight.reshape(-1).to(torch.bfloat16)
+    xr, w = _lib.operand(x), _lib.operand(weight)
+    out = torch.empty((rows, width), dtype=_NORM_DTYPES[kind], device=device)
     scale = None if kind == _linear.KIND_BF16 else torch.empty((rows, 1), dtype=torch.float32, device=device)
+    total, rr = x, None
+    if residual is not None:
+        rr = _lib.operand(residual)
+        total = torch.empty((rows, width), dtype=torch.bfloat16, device=device) if sum_out is None else sum_out
     if rows == 0:
         return out, scale, total
-    with _lib.on_device(device):
-        rc = _lib.lib().vdnh3_residual_rmsnorm_quant_rows(
-            kind, _lib.ptr(xr), stride(xr), _lib.ptr(rr), stride(rr), _lib.ptr(w), float(eps), rows, width, _lib.ptr(out), width,
-            _lib.ptr(scale), None if rr is None else _lib.ptr(total), stride(total), _lib.stream_handle(device))
-    _lib.check(rc, "vdnh3_residual_rmsnorm_quant_rows")
+
+    def operand(t):  # address and row stride; one row's stride may be anything
+        return (None, 0) if t is None else (t.data_ptr(), t.stride(0) if rows > 1 else width)
+
+    _lib.launch("vdnh3_residual_rmsnorm_quant_rows", _lib.lib().vdnh3_residual_rmsnorm_quant_rows, device, kind,
+                *operand(xr), *operand(rr), w.data_ptr(), eps, rows, width, out.data_ptr(), width, _lib.ptr(scale),
+                *operand(None if rr is None else total))
     return out, scale, total
 
 

@@ -38,6 +38,8 @@ def _sequence_bounds(cu_seqlens, rows: int, device) -> torch.Tensor:
         return cu_seqlens.to(torch.int32).to(device)
     if cu_seqlens.device != device:
         raise RuntimeError(f"tensors on different devices: {device} and {cu_seqlens.device}")
+    if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous():
+        return cu_seqlens
     return cu_seqlens.to(torch.int32).contiguous()
 
 
@@ -81,12 +83,10 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
     out = _output(out, query.shape, device)
     if rows == 0 or heads == 0 or cu.numel() == 1:
         return out
-    q, k, v = (_lib.operand(t) for t in (query, key, value))
-    with _lib.on_device(device):
-        rc = _lib.lib().vdnh3_causal_attn_packed(
-            _lib.ptr(q), *_lib.strides(q), _lib.ptr(k), *_lib.strides(k), _lib.ptr(v), *_lib.strides(v), _lib.ptr(out), *_lib.strides(out),
-            _lib.ptr(cu), cu.numel() - 1, rows, heads, key.shape[1], dim, float(scale), _lib.stream_handle(device))
-    _lib.check(rc, "causal_softmax_packed")
+    q, k, v = _lib.operand(query), _lib.operand(key), _lib.operand(value)
+    _lib.launch("causal_softmax_packed", _lib.lib().vdnh3_causal_attn_packed, device,
+                q.data_ptr(), *_lib.strides(q), k.data_ptr(), *_lib.strides(k), v.data_ptr(), *_lib.strides(v),
+                out.data_ptr(), *_lib.strides(out), cu.data_ptr(), cu.numel() - 1, rows, heads, key.shape[1], dim, scale)
     return out
 
 
@@ -123,17 +123,16 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
         return out
     if room == 0:
         return out.zero_()
-    lengths = lengths.to(torch.int32).contiguous()
+    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        lengths = lengths.to(torch.int32).contiguous()
     lib = _lib.lib()
     ranges = lib.vdnh3_causal_cached_ranges(batch, new, room, heads, kv_heads)
     size = lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
     partial = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    with _lib.on_device(device):
-        rc = lib.vdnh3_causal_attn_cached(
-            _lib.ptr(q), *_lib.strides(q), _lib.ptr(key_cache), *_lib.strides(key_cache), _lib.ptr(value_cache),
-            *_lib.strides(value_cache), _lib.ptr(out), *_lib.strides(out), _lib.ptr(lengths), batch, new, room, heads, kv_heads, dim,
-            float(scale), ranges, _lib.ptr(partial), size, _lib.stream_handle(device))
-    _lib.check(rc, "causal_softmax_cached")
+    _lib.launch("causal_softmax_cached", lib.vdnh3_causal_attn_cached, device,
+                q.data_ptr(), *_lib.strides(q), key_cache.data_ptr(), *_lib.strides(key_cache), value_cache.data_ptr(),
+                *_lib.strides(value_cache), out.data_ptr(), *_lib.strides(out), lengths.data_ptr(), batch, new, room, heads,
+                kv_heads, dim, scale, ranges, _lib.ptr(partial), size)
     return out
 
 

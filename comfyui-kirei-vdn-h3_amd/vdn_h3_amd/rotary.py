@@ -59,7 +59,6 @@ class RotaryAxes:
     def table(self, device) -> tuple[torch.Tensor, torch.Tensor]:
         """``(turns per position float64, axis int32)`` on ``device``, made once per device (a copy from the host, so a
         graph capture needs one call, or this method, before it)."""
-        device = torch.device(device)
         hit = self._tables.get(device)
         if hit is None:
             radians, axis = self.frequencies()
@@ -93,7 +92,8 @@ def normalise_qk_axes(q_raw: torch.Tensor, k_raw: torch.Tensor, positions: torch
     device = _lib.require_device(q_raw, k_raw, q_weight, k_weight, positions)
     seq, heads, dim = q_raw.shape
     kv_heads = k_raw.shape[1]
-    if positions.dtype not in _POSITION_CODES:
+    code = _POSITION_CODES.get(positions.dtype)
+    if code is None:
         raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
     if positions.ndim == 1:
         positions = positions.expand(axes.axes, positions.shape[0])
@@ -102,20 +102,17 @@ def normalise_qk_axes(q_raw: torch.Tensor, k_raw: torch.Tensor, positions: torch
     if axes.rot_dim > dim or dim % 8 or not 0 < dim <= 128:
         raise ValueError(f"head dim {dim} must be a multiple of 8 up to 128 and hold the {axes.rot_dim} rotated channels")
     wq, wk = _norm_weight(q_weight, dim, "q_weight"), _norm_weight(k_weight, dim, "k_weight")
-    q, k = (_lib.operand(t) for t in (q_raw, k_raw))
+    q, k = _lib.operand(q_raw), _lib.operand(k_raw)
     qn = torch.empty((seq, heads, dim), dtype=torch.bfloat16, device=device)
     kn = torch.empty((seq, kv_heads, dim), dtype=torch.bfloat16, device=device)
     if seq == 0:
         return qn, kn
     turns, axis = axes.table(device)
-    with _lib.on_device(device):
-        rc = _lib.lib().vdnh3_qk_rotary_axes(
-            _lib.ptr(q), *_lib.strides(q), _lib.ptr(wq), float(eps), _lib.ptr(qn), qn.stride(0), qn.stride(1), heads,
-            _lib.ptr(k), *_lib.strides(k), _lib.ptr(wk), float(eps if k_eps is None else k_eps), _lib.ptr(kn),
-            kn.stride(0), kn.stride(1), kv_heads, _lib.ptr(positions), _POSITION_CODES[positions.dtype],
-            positions.stride(0), positions.stride(1), _lib.ptr(turns), _lib.ptr(axis), axes.rot_dim, seq, dim,
-            _lib.stream_handle(device))
-    _lib.check(rc, "vdnh3_qk_rotary_axes")
+    _lib.launch("vdnh3_qk_rotary_axes", _lib.lib().vdnh3_qk_rotary_axes, device,
+                q.data_ptr(), *_lib.strides(q), _lib.ptr(wq), eps, qn.data_ptr(), heads * dim, dim, heads,
+                k.data_ptr(), *_lib.strides(k), _lib.ptr(wk), eps if k_eps is None else k_eps, kn.data_ptr(),
+                kv_heads * dim, dim, kv_heads, positions.data_ptr(), code, *positions.stride(), turns.data_ptr(),
+                axis.data_ptr(), axes.rot_dim, seq, dim)
     return qn, kn
 
 

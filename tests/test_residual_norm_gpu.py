@@ -51,7 +51,8 @@ def _check(got, kind, x, res, w, eps):
 # widths of one chunk, ragged ones, one at each edge of a lane's chunks, and one past what registers hold
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("rows,hidden", [(1, 8), (3, 72), (1, 5120), (2, 2048), (2, 2056), (5, 5128), (513, 5120), (7, 8192),
-                                         (3, 8200), (2, 16384), (2, 20008), (1030, 256), (2051, 1024)])
+                                         (3, 8200), (2, 16384), (2, 20008), (1030, 256), (2051, 1024), (4099, 2048),
+                                         (4098, 24)])
 def test_against_float64(device, kind, rows, hidden):
     from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
 
@@ -94,6 +95,18 @@ def test_strided_repeated_and_in_place(device, kind, hidden):
     assert (out[:, hidden:] == 5).all() and (wide[:, :8] == 7).all()
     one = residual_rmsnorm_quantize(x.to(device), res[:1].to(device).expand(9, hidden), w.to(device), 1e-5, KINDS[kind])
     _check(one, kind, x, res[:1].expand(9, hidden), w, 1e-5)
+
+
+def test_squares_under_the_smallest_numbers(device):
+    """With no epsilon the norm of a row does not depend on its size."""
+    from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
+
+    for hidden in (256, 5120, 9216):
+        x, res, w = _case(5, hidden, 30)
+        for kind in KINDS:
+            for by in (2.0 ** -70, 2.0 ** 60):
+                a, b = (x.float() * by).to(BF), (res.float() * by).to(BF)
+                _check(residual_rmsnorm_quantize(a.to(device), b.to(device), w.to(device), 0.0, KINDS[kind]), kind, a, b, w, 0.0)
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
