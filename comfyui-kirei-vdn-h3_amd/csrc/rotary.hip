@@ -43,51 +43,87 @@ struct Vectors {
   int heads;
 };
 
-// One group of LANES lanes per head vector, 8 channels a lane; dim <= 8 LANES, lanes past it idle.
-template <int LANES>
-__global__ __launch_bounds__(256) void rotary_kernel(Vectors q, Vectors k, Positions pos,
-                                                     const double *__restrict__ turns, const int32_t *__restrict__ axis,
-                                                     int rot, int dim, int64_t n_vec) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t vec = t / LANES;
-  const int c = (int)(t % LANES);
-  if (vec >= n_vec) return;  // a lane group is wholly in range or wholly out
-  const int nv = q.heads + k.heads;
-  const int64_t row = vec / nv;
-  const int v = (int)(vec - row * nv), which = v >= q.heads, head = which ? v - q.heads : v;
-  const Vectors &s = which ? k : q;
+// The vectors of one row's q or k that a lane group takes: heads j, j + step, ... (its 8 channels of each), RB of them in
+// flight. cs holds cos and sin of the lane's pairs, the second of a pair with the sine's sign turned.
+template <int LANES, int RB>
+__device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j, int step, int c, int dim, bool rotated,
+                                           bool row_turn, int partner, const float2 (&cs)[8]) {
   const bool live = 8 * c < dim;
-  float y[8] = {}, o[8];
-  if (live) {
-    const u32x4_t raw = ld16(s.x + row * s.row + head * s.head + 8 * c);
+  const uint16_t *x = s.x + row * s.row + 8 * c;
+  uint16_t *out = s.out + row * s.out_row + 8 * c;
+  float wf[8];
+  if (s.w && live) {
+    const u32x4_t w = ld16(s.w + 8 * c);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = __uint_as_float((j & 1) ? (raw[j >> 1] & 0xffff0000u) : (raw[j >> 1] << 16));
+    for (int i = 0; i < 8; ++i) wf[i] = __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
   }
-  if (s.w) {
-    const float r = rms_factor(group_tree_sum<LANES>(chunk_sumsq(y)), dim, s.eps);
-    if (live) {
-      const u32x4_t w = ld16(s.w + 8 * c);
+  for (int h0 = j; h0 < s.heads; h0 += RB * step) {
+    u32x4_t raw[RB];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        y[j] = y[j] * r * __uint_as_float((j & 1) ? (w[j >> 1] & 0xffff0000u) : (w[j >> 1] << 16));
+    for (int u = 0; u < RB; ++u) {
+      raw[u] = u32x4_t{0, 0, 0, 0};
+      if (live && h0 + u * step < s.heads) raw[u] = ld16(x + (h0 + u * step) * s.head);
+    }
+#pragma unroll
+    for (int u = 0; u < RB; ++u) {
+      if (h0 + u * step >= s.heads) break;  // a whole lane group
+      float y[8], o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[i] = __uint_as_float((i & 1) ? (raw[u][i >> 1] & 0xffff0000u) : (raw[u][i >> 1] << 16));
+      if (s.w) {
+        const float r = rms_factor(group_tree_sum<LANES>(chunk_sumsq(y)), dim, s.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * r * wf[i];
+      }
+      if (row_turn) {  // the partner is 8 lanes away in a 16-lane DPP row (row_ror:8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          o[i] = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y[i]), 0x128, 0xf, 0xf, false));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __shfl(y[i], partner);
+      }
+      if (rotated) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = fmaf(cs[i].x, y[i], cs[i].y * o[i]);
+      }
+      if (live)
+        st16(out + (h0 + u * step) * s.out_head,
+             u32x4_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7])});
     }
   }
-  const int half = rot >> 1, step = half >> 3, lane = __lane_id();
+}
+
+// A workgroup takes R rows: its threads compute the rows' cosines and sines once, one pair each (R rot / 2 <= 256 at the
+// widths that R is made for), and share them through LDS. LANES lanes hold a head vector, 8 channels each (dim <= 8 LANES,
+// lanes past it idle), 256 / LANES / R lane groups a row; a group keeps its row's pairs in registers and walks the heads.
+template <int LANES, int R>
+__global__ __launch_bounds__(256) void rotary_kernel(Vectors q, Vectors k, Positions pos, const double *__restrict__ turns,
+                                                     const int32_t *__restrict__ axis, int rot, int dim, int rows) {
+  constexpr int PAIRS = 4 * LANES, STEP = 256 / LANES / R;
+  __shared__ __attribute__((aligned(16))) float2 table[R][PAIRS];
+  const int half = rot >> 1, tid = threadIdx.x;
+  const int64_t row0 = (int64_t)blockIdx.x * R;
+  for (int i = tid; i < R * PAIRS; i += 256) {
+    const int r = i / PAIRS, pair = i % PAIRS;
+    if (pair < half && row0 + r < rows) table[r][pair] = turn(position_at(pos, axis[pair], row0 + r), turns[pair]);
+  }
+  __syncthreads();
+  const int c = tid % LANES, group = tid / LANES, r = group % R, j = group / R;
+  const int64_t row = row0 + r;
+  if (row >= rows) return;  // a whole lane group
   const bool first = 8 * c < half, rotated = 8 * c < rot;
-  const int partner = !rotated ? lane : first ? lane + step : lane - step;
+  const int lane = __lane_id(), partner = !rotated ? lane : first ? lane + (half >> 3) : lane - (half >> 3);
+  float2 cs[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = __shfl(y[j], partner);
-  if (!live) return;
-  if (rotated) {
-    const int i0 = first ? 8 * c : 8 * c - half;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 cs = turn(position_at(pos, axis[i0 + j], row), turns[i0 + j]);
-      y[j] = rope_rotate(y[j], o[j], f32x4_t{cs.x, -cs.y, cs.y, cs.x}, first);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = table[r][rotated ? (first ? 8 * c : 8 * c - half) + i : 0];
+    cs[i] = make_float2(f.x, first ? -f.y : f.y);
   }
-  st16(s.out + row * s.out_row + head * s.out_head + 8 * c,
-       u32x4_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7])});
+  const bool row_turn = LANES == 16 && rot == 128;
+  turn_heads<LANES, 4>(q, row, j, STEP, c, dim, rotated, row_turn, partner, cs);
+  turn_heads<LANES, 4>(k, row, j, STEP, c, dim, rotated, row_turn, partner, cs);
 }
 
 int check_vectors(const Vectors &s, const char *name) {
@@ -98,6 +134,20 @@ int check_vectors(const Vectors &s, const char *name) {
                    VDNH3_ERR_INVALID,
                    "rotary: %s, its output and its weight must be 16-byte aligned with strides that are multiples of 8", name);
   return VDNH3_OK;
+}
+
+// Rows up to which each has a workgroup of its own.
+constexpr int kSingleRows = 2048;
+
+template <int LANES>
+void launch_rotary(const Vectors &q, const Vectors &k, const Positions &pos, const double *turns, const int32_t *axis, int rot,
+                   int dim, int rows, hipStream_t s) {
+  constexpr int R = 64 / LANES;  // a pair per thread
+  if (rows <= kSingleRows)
+    hipLaunchKernelGGL((rotary_kernel<LANES, 1>), dim3(rows), dim3(256), 0, s, q, k, pos, turns, axis, rot, dim, rows);
+  else
+    hipLaunchKernelGGL((rotary_kernel<LANES, R>), dim3((rows + R - 1) / R), dim3(256), 0, s, q, k, pos, turns, axis, rot, dim,
+                       rows);
 }
 
 }  // namespace
@@ -123,17 +173,10 @@ extern "C" int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_
   if (!rc) rc = check_vectors(ks, "k");
   if (rc) return rc;
   const Positions pos{positions, p_axis, p_row, position_type};
-  const int64_t n_vec = (int64_t)rows * (q_heads + k_heads);
-  const int lanes = head_dim <= 64 ? 8 : 16;
-  const int64_t groups = (n_vec * lanes + 255) / 256;
-  VDNH3_HOST_CHECK(groups <= INT32_MAX, VDNH3_ERR_INVALID, "rotary: %lld head vectors are too many for one launch",
-                   (long long)n_vec);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (lanes == 8)
-    hipLaunchKernelGGL(rotary_kernel<8>, dim3((unsigned)groups), dim3(256), 0, s, qs, ks, pos, turns, axis_of_pair, rot_dim,
-                       head_dim, n_vec);
+  if (head_dim <= 64)
+    launch_rotary<8>(qs, ks, pos, turns, axis_of_pair, rot_dim, head_dim, rows, s);
   else
-    hipLaunchKernelGGL(rotary_kernel<16>, dim3((unsigned)groups), dim3(256), 0, s, qs, ks, pos, turns, axis_of_pair, rot_dim,
-                       head_dim, n_vec);
+    launch_rotary<16>(qs, ks, pos, turns, axis_of_pair, rot_dim, head_dim, rows, s);
   return check_launch("rotary");
 }
