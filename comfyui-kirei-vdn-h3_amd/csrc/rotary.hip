@@ -4,7 +4,8 @@
 //   pair i of rot / 2 turns by angle_i = 2 pi * position[axis_i][row] * turns_i:
 //   out_i = y_i cos - y_{i+h} sin,  out_{i+h} = y_i sin + y_{i+h} cos,  h = rot / 2; channels >= rot pass
 //
-// position * turns is taken in 64 bits and only its fraction rounded to fp32: at position 40,688 an fp32 angle would be
+// A table of rotations per row, as qk_rmsnorm_rope takes, would be 16 bytes a row and pair and is shared by the heads alone;
+// here a workgroup computes its rows' angles. position * turns is taken in 64 bits and only its fraction rounded to fp32: at position 40,688 an fp32 angle would be
 // off by 2e-3, a bf16 step. q and k have their own numbers of heads; one rounding to bf16 at the end.
 #include "common.h"
 #include "qk_norm.h"
@@ -136,7 +137,9 @@ int check_vectors(const Vectors &s, const char *name) {
   return VDNH3_OK;
 }
 
-// Rows up to which each has a workgroup of its own.
+// Rows up to which each has a workgroup of its own: with 40 + 8 heads of 128, 512 rows take 7.9 us against 12.4 with four rows a
+// workgroup, 2,048 15.1 against 15.5, 4,096 30.9 against 23.7. HBM is the bound of many rows: 40,688 x 80 heads x 128 take
+// 327 us with the norms, 5.1 TB/s; 2 or 8 vectors in flight instead of 4 and non-temporal loads are no faster.
 constexpr int kSingleRows = 2048;
 
 template <int LANES>
