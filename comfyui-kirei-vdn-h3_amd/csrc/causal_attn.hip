@@ -94,12 +94,10 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
 // wavefront's two 16-query blocks and 24 of a tile's 96 keys, and its probabilities are operands of O^T += V^T P^T as
 // they lie. V tiles are loaded as they are, key by key, and read transposed (ds_read_b64_tr_b16: 16 lanes get 4 keys of
 // 16 channels), so no pass writes a transposed copy first.
-constexpr int kBM = 256;       // rows per workgroup
 constexpr int kBN = 96;        // keys per tile
 constexpr int kThreads = 512;
 constexpr int kRing = 3;       // LDS slots per K and V ring (144 KB at D = 128): loads run kRing - 1 tiles ahead
 constexpr int kAhead = 4;      // fragments a wavefront's LDS reads run ahead of its MFMAs
-constexpr int kNQ = 2;         // 16-query blocks per wavefront
 constexpr float kLazy = 8.0f;  // log2 of the largest probability a stale running max allows
 constexpr float kNoMax = -3.402823466e38f;  // the running max before any score: finite, so a masked score gives exp2(-inf) = 0
 
@@ -125,33 +123,43 @@ __device__ __forceinline__ u32x2_t lds_read_transposed(const uint16_t *p) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)));
 }
 
-// The block of rows a workgroup takes: sequence b, rows [r0, r1) of its n x group. Blocks of packed sequences are numbered
-// without a count on the host: sequence b's begin at floor(cu[b] group / kBM) + b, which leaves room for those before.
+// The block of rows a workgroup takes: sequence b, rows [r0, r1) of its n x group.
 struct Block {
   int b, r0, r1;
   Sequence s;
 };
-__device__ __forceinline__ Block block_at(const Sequences &seqs, int block, int group) {
-  int b, first;
-  if (seqs.cu) {
-    auto begin = [&](int i) __device__ { return (int)((int64_t)min(max(seqs.cu[i], 0), seqs.rows) * group / kBM) + i; };
-    int lo = 0, hi = seqs.count;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (begin(mid) <= block) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-    first = begin(lo);
-  } else {
-    const int per = (int)(((int64_t)seqs.rows * group + kBM - 1) / kBM);
-    b = block / per;
-    first = b * per;
+
+// Blocks of packed sequences are numbered without a count on the host: sequence b's begin at floor(cu[b] group / BM) + b, which
+// leaves room for those before. Every wavefront looks for its own, a lane per sequence: one load, a ballot. Numbers that
+// are no block's give no rows.
+template <int BM>
+__device__ __forceinline__ Block packed_block(const Sequences &seqs, int block, int group) {
+  const int lane = threadIdx.x & 63;
+  int b = 0, a = 0, e = 0, first = 0;
+  for (int b0 = 0; b0 < seqs.count; b0 += 64) {
+    const int i = min(b0 + lane, seqs.count - 1);
+    const int from = min(max(seqs.cu[i], 0), seqs.rows), to = min(max(seqs.cu[i + 1], from), seqs.rows);
+    const int begin = (int)((int64_t)from * group / BM) + b0 + lane;
+    const uint64_t before = __ballot(b0 + lane < seqs.count && begin <= block);
+    if (before == 0) break;
+    const int l = 63 - __builtin_clzll(before);
+    b = b0 + l;
+    a = __builtin_amdgcn_readlane(from, l);
+    e = __builtin_amdgcn_readlane(to, l);
+    first = __builtin_amdgcn_readlane(begin, l);
+    if (l < 63) break;
   }
-  const Sequence s = sequence_at(seqs, b);
-  const int64_t rows = (int64_t)s.n * group, r0 = (int64_t)(block - first) * kBM;
+  const int64_t rows = (int64_t)(e - a) * group, r0 = (int64_t)(block - first) * BM;
+  const Sequence s{a, e - a, a, e - a};
   if (r0 < 0 || r0 >= rows) return Block{b, 0, 0, s};
-  return Block{b, (int)r0, (int)min(r0 + kBM, rows), s};
+  return Block{b, (int)r0, (int)min(r0 + BM, rows), s};
+}
+
+// Caches: every sequence has the same rows.
+template <int BM>
+__device__ __forceinline__ Block cached_block(const Sequences &seqs, int block, int group) {
+  const int rows = seqs.rows * group, per = (rows + BM - 1) / BM, b = block / per, r0 = (block - b * per) * BM;
+  return Block{b, r0, min(r0 + BM, rows), sequence_at(seqs, b)};
 }
 
 // Two-group ping-pong over the key tiles t = 0 .. T-1: wavefronts 0-3 (group A) and 4-7 (group B) each own 32 rows a
@@ -162,7 +170,7 @@ __device__ __forceinline__ Block block_at(const Sequences &seqs, int block, int 
 // Group A runs tile t's MFMA phase in phase 2t and its VALU phase in 2t+1; group B one phase later. K(t) and V(t-1) are
 // read in phases 2t and 2t+1 only; group A loads K tiles and group B V tiles straight to LDS, each at the start of its VALU
 // phase, two tiles ahead. A wavefront leaves out tiles behind its own rows' diagonal.
-template <int D>
+template <int D, int NQ>
 __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Operand k, Operand v, Operand out,
                                                                   Sequences seqs, int blocks, int kv_heads, int group,
                                                                   float scale_log2) {
@@ -175,9 +183,9 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   __shared__ __attribute__((aligned(16))) uint16_t Ks[kRing][TILE];
   __shared__ __attribute__((aligned(16))) uint16_t Vs[kRing][TILE];
 
-  // the last blocks, which see the most keys, first; heads next to each other, so with 8 heads each XCD has its own
-  const int kvh = (int)blockIdx.x % kv_heads;
-  const Block blk = block_at(seqs, blocks - 1 - (int)blockIdx.x / kv_heads, group);
+  // a sequence's last blocks, which see the most keys, first; heads next to each other, so with 8 heads each XCD has its own
+  const int kvh = (int)blockIdx.x % kv_heads, block = blocks - 1 - (int)blockIdx.x / kv_heads;
+  const Block blk = seqs.cu ? packed_block<128 * NQ>(seqs, block, group) : cached_block<128 * NQ>(seqs, block, group);
   if (blk.r0 >= blk.r1) return;
   const Sequence &sq = blk.s;
   const int behind = sq.keys - sq.n;  // token i sees keys 0 .. behind + i
@@ -187,28 +195,26 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int l16 = lane & 15, g = lane >> 4;
   const int turn = wave >> 2;  // 0: group A, 1: group B
-  const int w0 = blk.r0 + wave * 16 * kNQ;  // the wavefront's first row
+  const int w0 = blk.r0 + wave * 16 * NQ;  // the wavefront's first row
   const bool rows_live = w0 < blk.r1;
   // the wavefront's tiles, and those of its tiles that need no mask
-  const int w_keys = rows_live ? min(behind + (min(w0 + 16 * kNQ, blk.r1) - 1) / group + 1, sq.keys) : 0;
+  const int w_keys = rows_live ? min(behind + (min(w0 + 16 * NQ, blk.r1) - 1) / group + 1, sq.keys) : 0;
   const int w_tiles = __builtin_amdgcn_readfirstlane(w_keys > 0 ? (w_keys + kBN - 1) / kBN : 0);
   const int w_clear = __builtin_amdgcn_readfirstlane(rows_live ? max(behind + w0 / group + 1, 0) / kBN : 0);
 
-  int last[kNQ];
-  const uint16_t *qp[kNQ];
-  uint16_t *op[kNQ];
+  int last[NQ];
+  const uint16_t *qp[NQ];
 #pragma unroll
-  for (int n = 0; n < kNQ; ++n) {
+  for (int n = 0; n < NQ; ++n) {
     const int r = min(w0 + 16 * n + l16, blk.r1 - 1), token = r / group, head = kvh * group + (r - token * group);
     last[n] = behind + token;
     qp[n] = q.at(blk.b, sq.q0 + token, head);
-    op[n] = const_cast<uint16_t *>(out.at(blk.b, sq.q0 + token, head));
   }
 
-  f32x4_t oacc[NO][kNQ], l_run[kNQ];
-  float m_run[kNQ];
+  f32x4_t oacc[NO][NQ], l_run[NQ];
+  float m_run[NQ];
 #pragma unroll
-  for (int n = 0; n < kNQ; ++n) {
+  for (int n = 0; n < NQ; ++n) {
 #pragma unroll
     for (int m = 0; m < NO; ++m) oacc[m][n] = f32x4_t{};
     m_run[n] = kNoMax;
@@ -216,12 +222,6 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   }
 
   if (T > 0) {
-    bf16x8_t qf[kNQ][NS];
-#pragma unroll
-    for (int n = 0; n < kNQ; ++n)
-#pragma unroll
-      for (int s = 0; s < NS; ++s) qf[n][s] = as_bf16x8(ld16(qp[n] + 32 * s + 8 * g));
-
     // Tile loads, by one group of 256 threads: thread chunk i fills LDS position P = 256 i + gtid (16-byte units): row
     // P / KC, slot P % KC, which holds chunk slot ^ swizzle(row) of that key; the swizzle is the same for every i. Rows
     // past the sequence's keys read its last key (their scores are masked).
@@ -260,21 +260,24 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
 #pragma unroll
     for (int m = 0; m < NO; ++m) vfo[m] = vr * D + v_slot<D>(vr, 2 * m + ((l16 >> 1) & 1)) * 8 + 4 * (l16 & 1);
 
-    f32x4_t sacc[NKB][kNQ];
-    u32x4_t pb[NT][kNQ];  // P^T fragments: bf16 pairs
-    const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
+    f32x4_t sacc[NKB][NQ];
+    u32x4_t pb[NT][NQ];  // P^T fragments: bf16 pairs
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int n = 0; n < kNQ; ++n) pb[j][n] = u32x4_t{};
+      for (int n = 0; n < NQ; ++n) pb[j][n] = u32x4_t{};
+    const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
 
-    // K(t) and V(t) live in slot t % kRing. Past the end the tile index is clamped to T-1: such loads rewrite slots that no
-    // tile reads any more, and every VALU phase issues the same count, so each group's wait at the end of odd phases is
-    // exact. Prologue: K(0 .. kRing-2) by group A, V(0 .. kRing-3) by group B; V(-1), which the PV product of tile 0 reads
-    // with P(-1) = 0, is zeroed. Group B's first issue (phase 0) is V(kRing-2).
+    // K(t) and V(t) live in slot t % kRing. Prologue: K(0 .. kRing-2) by group A, V(0 .. kRing-3) by group B; V(-1), which the
+    // product of tile 0 reads with P(-1) = 0, is zeroed. Group B's first issue (phase 0) is V(kRing-2).
 #pragma unroll
     for (int j = 0; j < kRing - 1; ++j)
-      if (j < kRing - 2 || turn == 0) tile_dma(min(j, T - 1), j);
+      if (j < T && (j < kRing - 2 || turn == 0)) tile_dma(j, j);
+    bf16x8_t qf[NQ][NS];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[n][s] = as_bf16x8(ld16(qp[n] + 32 * s + 8 * g));
     for (int i = tid; i < TILE / 8; i += kThreads) st16(Vs[kRing - 1] + i * 8, u32x4_t{0, 0, 0, 0});
     wait_vm_lds<0>();
     bare_barrier();
@@ -283,7 +286,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
     for (int p = 0; p < phases; ++p) {
       const int t_mfma = p >> 1, t_valu = (p - 1) >> 1;
       if (turn == (p & 1)) {
-        // t = w_tiles has no scores to make and t = 0 no product with values: those halves run on what is there
+        // t = w_tiles has no scores to make and t = 0 no product with values: those halves run on what is there (leaving them out
+        // in code of their own carries both operands through the loop, which spills)
         const int t = t_mfma;
         if (t <= w_tiles && w_tiles > 0) {
           const uint16_t *vtile = Vs[(t + kRing - 1) % kRing];
@@ -307,8 +311,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
           for (int i = 0; i < NF; ++i) {
             const u32x4_t a = fr[i % kAhead];
 #pragma unroll
-            for (int x = 0; x < kNQ; ++x) {
-              const int n = (i & 1) ? kNQ - 1 - x : x;
+            for (int x = 0; x < NQ; ++x) {
+              const int n = (i & 1) ? NQ - 1 - x : x;
               if (i < NP) {
                 oacc[i % NO][n] = mfma_bf16_16x16x32(as_bf16x8(a), as_bf16x8(pb[i / NO][n]), oacc[i % NO][n]);
                 if (i % NO == NO - 1)
@@ -325,23 +329,22 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
           __builtin_amdgcn_s_setprio(0);
         }
       } else {
-        tile_dma(min(t_valu + kRing - 1, T - 1), (t_valu + kRing - 1) % kRing);
+        if (t_valu + kRing - 1 < T) tile_dma(t_valu + kRing - 1, (t_valu + kRing - 1) % kRing);
         if (p >= 1 + turn && t_valu < w_tiles) {
           if (t_valu >= w_clear) {  // part of the tile lies behind a row
 #pragma unroll
-            for (int kb = 0; kb < NKB; ++kb)
+            for (int n = 0; n < NQ; ++n) {
+              const int seen = last[n] - t_valu * kBN - 4 * g;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int key = t_valu * kBN + 16 * kb + 4 * g + i;
+              for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-                for (int n = 0; n < kNQ; ++n)
-                  if (key > last[n]) sacc[kb][n][i] = -INFINITY;
-              }
+                for (int i = 0; i < 4; ++i) sacc[kb][n][i] = 16 * kb + i > seen ? -INFINITY : sacc[kb][n][i];
+            }
           }
-          static_assert(NKB == 6 && kNQ == 2, "the max tree is written for 2 x 24 scores per lane");
-          float mt[kNQ];
+          static_assert(NKB == 6 && NQ <= 2, "the max tree is written for 24 scores per lane and query");
+          float mt[NQ];
 #pragma unroll
-          for (int n = 0; n < kNQ; ++n) {
+          for (int n = 0; n < NQ; ++n) {
             float m1[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -351,16 +354,16 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
             const float a = fmaxf(fmaxf(m1[0], m1[1]), m1[2]), b = fmaxf(fmaxf(m1[3], m1[4]), m1[5]);
             mt[n] = fmaxf(fmaxf(a, b), fmaxf(m1[6], m1[7]));
           }
-          group_max(mt[0], mt[1]);
+          group_max(mt[0], mt[NQ - 1]);
           bool grow = false;
 #pragma unroll
-          for (int n = 0; n < kNQ; ++n) {
+          for (int n = 0; n < NQ; ++n) {
             mt[n] *= scale_log2;
             grow = grow || mt[n] > m_run[n] + kLazy;
           }
           if (__any(grow)) {
 #pragma unroll
-            for (int n = 0; n < kNQ; ++n) {
+            for (int n = 0; n < NQ; ++n) {
               const float m_new = mt[n] > m_run[n] + kLazy ? mt[n] : m_run[n];
               const float corr = __builtin_amdgcn_exp2f(m_run[n] - m_new);
               m_run[n] = m_new;
@@ -373,7 +376,7 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
 #pragma unroll
           for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-            for (int n = 0; n < kNQ; ++n)
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
               for (int i = 0; i < 4; i += 2) {
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sacc[kb][n][i], scale_log2, -m_run[n]));
@@ -382,29 +385,54 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
               }
         }
       }
-      // before an even phase 2(t+1): K(t+1) and V(t) have landed; each group's latest issue may still be in flight
-      if (p & 1) wait_vm_lds<(kRing - 2) * CG>();
+      // before an even phase 2(t+1): K(t+1) and V(t) have landed. While there are tiles to load, each group's latest one, K(t+2)
+      // or V(t+1), may still be in flight; after that there is none later.
+      if (p & 1) {
+        if (t_valu + kRing - 1 < T) wait_vm_lds<(kRing - 2) * CG>();
+        else wait_vm_lds<0>();
+      }
       bare_barrier();
     }
-    wait_vm_lds<0>();  // no tile load may land in LDS after the workgroup ends
   }
 
-  bool again[kNQ];
+  // The rows leave through LDS, whole: a lane holds 4 channels of 16 blocks each, and stores of 8 bytes to 16 rows take
+  // longer than this. Row r's 16-byte chunk c lies at chunk c ^ (r % 16) of its wavefront's part of the K ring.
+  uint16_t *mine = &Ks[0][0] + wave * (16 * NQ * D);
+  bool again[NQ];
 #pragma unroll
-  for (int n = 0; n < kNQ; ++n) {
+  for (int n = 0; n < NQ; ++n) {
     const float inv = 1.f / l_run[n][0];
+    const bool any = last[n] >= 0;
     again[n] = false;
-    if (w0 + 16 * n + l16 < blk.r1) {
-      const bool any = last[n] >= 0;
 #pragma unroll
-      for (int m = 0; m < NO; ++m) {
-        float o[4];
+    for (int m = 0; m < NO; ++m) {
+      float o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[i] = any ? oacc[m][n][i] * inv : 0.f;
-          again[n] = again[n] || !(fabsf(o[i]) < INFINITY);
-        }
-        *reinterpret_cast<uint2 *>(op[n] + 16 * m + 4 * g) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+      for (int i = 0; i < 4; ++i) {
+        o[i] = any ? oacc[m][n][i] * inv : 0.f;
+        again[n] = again[n] || !(fabsf(o[i]) < INFINITY);
+      }
+      *reinterpret_cast<uint2 *>(mine + (16 * n + l16) * D + (((2 * m + (g >> 1)) ^ l16) & (KC - 1)) * 8 + 4 * (g & 1)) =
+          make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+    }
+    again[n] = again[n] && w0 + 16 * n + l16 < blk.r1;
+  }
+  {
+    constexpr int RPI = 64 / KC;  // rows per instruction
+    const int c = lane % KC;
+    int r = lane / KC, token = (w0 + r) / group, head = w0 + r - token * group;
+    const int tokens = RPI / group, heads = RPI - tokens * group;
+#pragma unroll
+    for (int i = 0; i < 16 * NQ / RPI; ++i) {
+      if (w0 + r < blk.r1)
+        st16(const_cast<uint16_t *>(out.at(blk.b, sq.q0 + token, kvh * group + head)) + 8 * c,
+             ld16(mine + r * D + ((c ^ r) & (KC - 1)) * 8));
+      r += RPI;
+      token += tokens;
+      head += heads;
+      if (head >= group) {
+        head -= group;
+        ++token;
       }
     }
   }
@@ -412,7 +440,7 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   // its sum. Rows whose result is not finite are computed once more without the keys that they do not see: never for
   // finite inputs whose result bf16 holds.
 #pragma unroll
-  for (int n = 0; n < kNQ; ++n) {
+  for (int n = 0; n < NQ; ++n) {
     uint64_t todo = __ballot(again[n]);
     todo |= todo >> 32;
     todo |= todo >> 16;
@@ -533,6 +561,7 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
                                                                  Parts parts) {
   constexpr int KC = D / 8, NS = D / 32, NO = D / 16, C = D / 64, ROWS = 16 * NQ, W = kFewThreads / 64;
   constexpr int TILE = kFewKeys * D;  // elements
+  static_assert(NQ <= 2, "one exchange reduces the maxima of two queries");
   static_assert(ROWS * D * 2 <= kFewRing * 2 * TILE, "a wavefront's sums fit its tiles' place");
   __shared__ __attribute__((aligned(16))) uint16_t tiles[W][kFewRing][2][TILE];
   __shared__ float2 stats[W][ROWS];
@@ -666,11 +695,7 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
         const f32x4_t x = sacc[0][n], y = sacc[1][n];
         mt[n] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
       }
-#pragma unroll
-      for (int n = 0; n < NQ; n += 2) {
-        float other = mt[n];
-        group_max(mt[n], n + 1 < NQ ? mt[n + 1 < NQ ? n + 1 : n] : other);
-      }
+      group_max(mt[0], mt[NQ - 1]);
       bool grow = false;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -853,22 +878,33 @@ int check_causal(const Operand &q, const Operand &k, const Operand &v, const Ope
   return VDNH3_OK;
 }
 
+template <int D, int NQ>
+int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int heads,
+                 int kv_heads, float scale, hipStream_t s) {
+  constexpr int BM = 128 * NQ;
+  const int group = heads / kv_heads;
+  const int64_t blocks = seqs.cu ? (int64_t)seqs.rows * group / BM + seqs.count
+                                 : seqs.count * (((int64_t)seqs.rows * group + BM - 1) / BM);
+  VDNH3_HOST_CHECK((int64_t)seqs.rows * group <= INT32_MAX - BM && blocks * kv_heads <= INT32_MAX, VDNH3_ERR_INVALID,
+                   "causal attention: %d rows of %d heads are too many for one launch", seqs.rows, heads);
+  hipLaunchKernelGGL((causal_tile_kernel<D, NQ>), dim3((unsigned)(blocks * kv_heads)), dim3(kThreads), 0, s, q, k, v, out, seqs,
+                     (int)blocks, kv_heads, group, scale * 1.4426950408889634f);
+  return check_launch("causal attention");
+}
+
+// Workgroups of 256 rows from which on they are taken; with fewer, workgroups of 128 leave fewer CUs without one and end closer
+// together.
+constexpr int kHighGroups128 = 288, kHighGroups64 = 512;
+
 int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int heads,
                   int kv_heads, int head_dim, float scale, hipStream_t s) {
-  const int group = heads / kv_heads;
-  const int64_t blocks = seqs.cu ? (int64_t)seqs.rows * group / kBM + seqs.count
-                                 : seqs.count * (((int64_t)seqs.rows * group + kBM - 1) / kBM);
-  VDNH3_HOST_CHECK((int64_t)seqs.rows * group <= INT32_MAX - kBM && blocks * kv_heads <= INT32_MAX, VDNH3_ERR_INVALID,
-                   "causal attention: %d rows of %d heads are too many for one launch", seqs.rows, heads);
-  const float scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid((unsigned)(blocks * kv_heads));
+  const bool high = (int64_t)seqs.rows * (seqs.cu ? 1 : seqs.count) * heads / 256 >=
+                    (head_dim == 128 ? kHighGroups128 : kHighGroups64);
   if (head_dim == 128)
-    hipLaunchKernelGGL(causal_tile_kernel<128>, grid, dim3(kThreads), 0, s, q, k, v, out, seqs, (int)blocks, kv_heads, group,
-                       scale_log2);
-  else
-    hipLaunchKernelGGL(causal_tile_kernel<64>, grid, dim3(kThreads), 0, s, q, k, v, out, seqs, (int)blocks, kv_heads, group,
-                       scale_log2);
-  return check_launch("causal attention");
+    return high ? launch_tiles<128, 2>(q, k, v, out, seqs, heads, kv_heads, scale, s)
+                : launch_tiles<128, 1>(q, k, v, out, seqs, heads, kv_heads, scale, s);
+  return high ? launch_tiles<64, 2>(q, k, v, out, seqs, heads, kv_heads, scale, s)
+              : launch_tiles<64, 1>(q, k, v, out, seqs, heads, kv_heads, scale, s);
 }
 
 // Rows of a key / value head (new tokens x heads of a group) up to which a cached call takes the few-row kernel.

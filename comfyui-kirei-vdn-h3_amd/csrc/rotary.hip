@@ -4,9 +4,9 @@
 //   pair i of rot / 2 turns by angle_i = 2 pi * position[axis_i][row] * turns_i:
 //   out_i = y_i cos - y_{i+h} sin,  out_{i+h} = y_i sin + y_{i+h} cos,  h = rot / 2; channels >= rot pass
 //
-// A table of rotations per row, as qk_rmsnorm_rope takes, would be 16 bytes a row and pair and is shared by the heads alone;
-// here a workgroup computes its rows' angles. position * turns is taken in 64 bits and only its fraction rounded to fp32: at position 40,688 an fp32 angle would be
-// off by 2e-3, a bf16 step. q and k have their own numbers of heads; one rounding to bf16 at the end.
+// A workgroup computes its rows' angles itself: a table of rotations would be 16 more bytes a row and pair to write and read.
+// position * turns is taken in 64 bits and only its fraction rounded to fp32: at position 40,688 an fp32 angle would be off
+// by 2e-3, a bf16 step. q and k have their own numbers of heads; one rounding to bf16 at the end.
 #include "common.h"
 #include "qk_norm.h"
 
