@@ -200,7 +200,7 @@ def in_place(t) -> bool:
     """Whether a kernel can take a bf16 tensor where it lies: 16-byte aligned rows of contiguous channels."""
     if t.data_ptr() % 16:
         return False
-    if t.shape[-1] % 8 == 0 and t.is_contiguous():
+    if t.is_contiguous() and t.shape[-1] % 8 == 0:
         return True
     return (t.stride(-1) == 1 or t.shape[-1] == 1) and not any(s % 8 for s in strides(t))
 
@@ -225,22 +225,26 @@ def launch(what: str, fn, device: torch.device, *args) -> None:
 def forward_only(what: str, *tensors) -> None:
     """The HIP ops have no backward: in gradient mode an input that requires grad is an error, since the
     result would silently carry no gradient."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} is forward-only (no backward) and an input requires grad; "
-                           "call it under torch.no_grad() or torch.inference_mode()")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            raise RuntimeError(f"{what} is forward-only (no backward) and an input requires grad; "
+                               "call it under torch.no_grad() or torch.inference_mode()")
 
 
 def require_device(*tensors) -> torch.device:
     """All tensors must live on one GPU; the HIP path has no CPU fallback."""
-    device = None
+    first = index = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()  # -1 for a CPU tensor; a number compares faster than a device
+        if i < 0 or not t.is_cuda:
             raise RuntimeError("vdn_h3_amd ops run on a ROCm GPU only (got a CPU tensor); "
                                "there is no CPU fallback")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"tensors on different devices: {device} and {t.device}")
-    return device
+        if first is None:
+            first, index = t, i
+        elif i != index:
+            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
+    return None if first is None else first.device

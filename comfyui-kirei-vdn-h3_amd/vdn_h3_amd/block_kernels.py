@@ -266,12 +266,12 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
     if weight.ndim != 1 or weight.dtype != torch.bfloat16:
         weight = weight.reshape(-1).to(torch.bfloat16)
     xr, w = _lib.operand(x), _lib.operand(weight)
-    out = torch.empty((rows, width), dtype=_NORM_DTYPES[kind], device=device)
-    scale = None if kind == _linear.KIND_BF16 else torch.empty((rows, 1), dtype=torch.float32, device=device)
+    out = torch.empty(rows, width, dtype=_NORM_DTYPES[kind], device=device)
+    scale = None if kind == _linear.KIND_BF16 else torch.empty(rows, 1, dtype=torch.float32, device=device)
     total, rr = x, None
     if residual is not None:
         rr = _lib.operand(residual)
-        total = torch.empty((rows, width), dtype=torch.bfloat16, device=device) if sum_out is None else sum_out
+        total = torch.empty(rows, width, dtype=torch.bfloat16, device=device) if sum_out is None else sum_out
     if rows == 0:
         return out, scale, total
 

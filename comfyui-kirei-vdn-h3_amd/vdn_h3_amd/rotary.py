@@ -103,8 +103,8 @@ def normalise_qk_axes(q_raw: torch.Tensor, k_raw: torch.Tensor, positions: torch
         raise ValueError(f"head dim {dim} must be a multiple of 8 up to 128 and hold the {axes.rot_dim} rotated channels")
     wq, wk = _norm_weight(q_weight, dim, "q_weight"), _norm_weight(k_weight, dim, "k_weight")
     q, k = _lib.operand(q_raw), _lib.operand(k_raw)
-    qn = torch.empty((seq, heads, dim), dtype=torch.bfloat16, device=device)
-    kn = torch.empty((seq, kv_heads, dim), dtype=torch.bfloat16, device=device)
+    qn = torch.empty(seq, heads, dim, dtype=torch.bfloat16, device=device)
+    kn = torch.empty(seq, kv_heads, dim, dtype=torch.bfloat16, device=device)
     if seq == 0:
         return qn, kn
     turns, axis = axes.table(device)
