@@ -688,7 +688,9 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
               if (at_key > last[n] || at_key >= k1) sacc[h][n][i] = -INFINITY;
           }
       }
-      u32x4_t pb[NQ];
+      // P as bf16 and what that leaves, again as bf16 (16 bits of each probability): the matrix cores are idle beside the loads,
+      // and the result is then as exact as its own rounding
+      u32x4_t pb[NQ], pl[NQ];
       float mt[NQ];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -721,16 +723,22 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
           for (int i = 0; i < 4; i += 2) {
             const float p0 = __builtin_amdgcn_exp2f(fmaf(sacc[h][n][i], scale_log2, -m_run[n]));
             const float p1 = __builtin_amdgcn_exp2f(fmaf(sacc[h][n][i + 1], scale_log2, -m_run[n]));
-            pb[n][2 * h + (i >> 1)] = pack_bf2(p0, p1);
+            const uint32_t w = pack_bf2(p0, p1);
+            pb[n][2 * h + (i >> 1)] = w;
+            pl[n][2 * h + (i >> 1)] = pack_bf2(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
           }
         l_run[n] = mfma_bf16_16x16x32(as_bf16x8(ones), as_bf16x8(pb[n]), l_run[n]);
+        l_run[n] = mfma_bf16_16x16x32(as_bf16x8(ones), as_bf16x8(pl[n]), l_run[n]);
       }
 #pragma unroll
       for (int m = 0; m < NO; ++m) {
         const u32x2_t x = lds_read_transposed(vtile + vfo[m]), y = lds_read_transposed(vtile + 16 * D + vfo[m]);
         const bf16x8_t a = as_bf16x8(u32x4_t{x[0], x[1], y[0], y[1]});
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) oacc[m][n] = mfma_bf16_16x16x32(a, as_bf16x8(pb[n]), oacc[m][n]);
+        for (int n = 0; n < NQ; ++n) {
+          oacc[m][n] = mfma_bf16_16x16x32(a, as_bf16x8(pb[n]), oacc[m][n]);
+          oacc[m][n] = mfma_bf16_16x16x32(a, as_bf16x8(pl[n]), oacc[m][n]);
+        }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this tile is read: the next trip loads over it
     }
