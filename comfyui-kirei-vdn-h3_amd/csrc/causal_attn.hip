@@ -268,11 +268,10 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
       for (int n = 0; n < NQ; ++n) pb[j][n] = u32x4_t{};
     const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
 
-    // K(t) and V(t) live in slot t % kRing. Prologue: K(0 .. kRing-2) by group A, V(0 .. kRing-3) by group B; V(-1), which the
-    // product of tile 0 reads with P(-1) = 0, is zeroed. Group B's first issue (phase 0) is V(kRing-2).
-#pragma unroll
-    for (int j = 0; j < kRing - 1; ++j)
-      if (j < T && (j < kRing - 2 || turn == 0)) tile_dma(j, j);
+    // K(t) and V(t) live in slot t % kRing. Phase 0 needs K(0), by group A, and the queries; K(1 .. kRing-2) by group A and
+    // V(0 .. kRing-3) by group B, which phase 2 needs, follow behind its barrier. V(-1), which the product of tile 0 reads with
+    // P(-1) = 0, is zeroed. Group B's first issue in its turn (phase 0) is V(kRing-2).
+    if (turn == 0) tile_dma(0, 0);
     bf16x8_t qf[NQ][NS];
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -281,6 +280,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
     for (int i = tid; i < TILE / 8; i += kThreads) st16(Vs[kRing - 1] + i * 8, u32x4_t{0, 0, 0, 0});
     wait_vm_lds<0>();
     bare_barrier();
+    static_assert(kRing == 3, "one tile of each ring is left to load here");
+    if (turn == 0 ? T > 1 : true) tile_dma(turn == 0 ? 1 : 0, turn == 0 ? 1 : 0);
 
     const int phases = 2 * T + 2;
     for (int p = 0; p < phases; ++p) {
@@ -401,21 +402,20 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   bool again[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const float inv = 1.f / l_run[n][0];
-    const bool any = last[n] >= 0;
-    again[n] = false;
+    const float inv = last[n] >= 0 ? 1.f / l_run[n][0] : 0.f;  // a row that sees nothing gives zeros
+    float odd = 0.f;  // 0 as long as every value is finite, then a NaN
 #pragma unroll
     for (int m = 0; m < NO; ++m) {
       float o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[i] = any ? oacc[m][n][i] * inv : 0.f;
-        again[n] = again[n] || !(fabsf(o[i]) < INFINITY);
+        o[i] = oacc[m][n][i] * inv;
+        odd = fmaf(o[i], 0.f, odd);
       }
       *reinterpret_cast<uint2 *>(mine + (16 * n + l16) * D + (((2 * m + (g >> 1)) ^ l16) & (KC - 1)) * 8 + 4 * (g & 1)) =
           make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
     }
-    again[n] = again[n] && w0 + 16 * n + l16 < blk.r1;
+    again[n] = !(odd == 0.f) && w0 + 16 * n + l16 < blk.r1;
   }
   {
     constexpr int RPI = 64 / KC;  // rows per instruction
