@@ -10,6 +10,7 @@
 // The sequences' bounds are read on the device, so no length is needed on the host and a captured call can be replayed
 // with other lengths. Bounds outside the buffers are cut to them.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "lane_groups.h"
@@ -915,10 +916,6 @@ int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Op
               : launch_tiles<64, 1>(q, k, v, out, seqs, heads, kv_heads, scale, s);
 }
 
-// Rows of a key / value head (new tokens x heads of a group) up to which a cached call takes the few-row kernel.
-constexpr int kFewRows = 128;
-constexpr int kFewGroups = 256;  // workgroups: one per CU (128 KB of LDS at D = 128)
-
 int few_block(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
 template <int D, int NQ>
@@ -962,15 +959,27 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
                        static_cast<hipStream_t>(stream));
 }
 
+// The ranges of a call, or 0 for the kernel above: what its caches take at full length either way, in us. The prompt kernel goes
+// through all keys of a block of 128 rows in one workgroup (1.3 us per 96 keys), which is little at a time where there are
+// few blocks. Here 256 workgroups are at work always, but on 32 rows each (1.9 us per 4 tiles of 32 keys). 40 / 8 heads x
+// 128, measured: 40,688 keys and 32 new tokens 139 us against 560, 128 tokens 399 against 563, 256 tokens 759 against 566; 16
+// requests of 2,000 keys and 16 tokens 93 against 38. With up to 16 rows it is the loads that count, and this kernel
+// always.
 extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads) {
   using namespace vdnh3;
   if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
-  const int64_t rows = (int64_t)new_tokens * (heads / kv_heads);
-  if (rows > kFewRows) return 0;
+  const int64_t rows = (int64_t)new_tokens * (heads / kv_heads), tiles = (int64_t)batch * ((room + kFewKeys - 1) / kFewKeys);
+  if (tiles > INT32_MAX || rows * batch * kv_heads > INT32_MAX) return 0;
   const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
-  const int64_t tiles = (int64_t)batch * ((room + kFewKeys - 1) / kFewKeys);
-  if (tiles > INT32_MAX) return 0;
-  return tiles <= kFewOne ? 1 : (int)std::max<int64_t>(std::min<int64_t>(kFewGroups / blocks, tiles / kFewLeast), 1);
+  if (rows > 16) {
+    const double groups = (double)((rows + 127) / 128) * batch * kv_heads;
+    const double whole = 8. + 1.3 * std::ceil(groups / 256) * ((room + kBN - 1) / kBN);
+    if (whole < 14. + 1.9 * (double)blocks * tiles / (256 * 4)) return 0;
+  }
+  if (tiles <= kFewOne) return 1;
+  // one round of workgroups, or several where one would leave CUs idle
+  const int64_t ranges = blocks <= 24 ? 256 / blocks : (1024 + blocks - 1) / blocks;
+  return (int)std::max<int64_t>(std::min<int64_t>(ranges, tiles / kFewLeast), 1);
 }
 
 extern "C" size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges) {

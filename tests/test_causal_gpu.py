@@ -41,7 +41,7 @@ PACKED = [  # lengths, heads, kv heads, dim
     ([1], 1, 1, 64), ([2], 5, 1, 128), ([5, 1, 33], 4, 4, 64), ([0, 3, 0, 1, 64, 0], 8, 2, 128), ([95, 96, 97], 5, 1, 128),
     ([255, 256, 257], 2, 2, 128), ([51, 52, 103], 10, 2, 128), ([640], 40, 8, 128), ([1, 500, 63], 14, 2, 64),
     ([700], 3, 3, 64), ([130, 31], 7, 1, 128), ([600], 32, 1, 64), ([200], 6, 2, 80), ([90, 7], 4, 4, 24),
-    ([1] * 40, 8, 1, 128), ([17, 1, 1, 300] * 3, 20, 20, 64)]
+    ([1] * 40, 8, 1, 128), ([1300, 900], 40, 8, 128), ([2100], 20, 20, 64), ([17, 1, 1, 300] * 3, 20, 20, 64)]
 
 
 @pytest.mark.parametrize("lengths,heads,kv,dim", PACKED)
@@ -160,6 +160,64 @@ def test_cached_against_float64(device, new, room, lengths, heads, kv, dim):
     view = torch.cat([q, q], 2).to(device)[:, :, :heads]
     got2 = causal_softmax_cached(view, dk, dv, n.long(), scale, out=wide[:, :, :heads])
     assert torch.equal(got2, got) and (wide[:, :, heads:] == 9).all()
+
+
+@pytest.mark.parametrize("new,heads,kv,dim", [(1, 5, 1, 128), (1, 4, 4, 64), (3, 12, 2, 64), (7, 10, 2, 128)])
+def test_cached_however_it_is_cut(device, new, heads, kv, dim):
+    """Whole rows and every number of ranges, more than there are tiles for among them; lengths of every kind at once."""
+    from vdn_h3_amd import _lib
+
+    lengths = [0, 1, 31, 32, 33, 700, 64, 0, 257, 128, 96, 1, 0]
+    batch, room = len(lengths), 704
+    q, k, v = _qkv(batch * room, heads, kv, dim, 40 + new, loud=2.0)
+    q, k, v = q[:batch * new].view(batch, new, heads, dim), k.view(batch, room, kv, dim), v.view(batch, room, kv, dim)
+    want = po.cached(q, k, v, lengths, 0.1)
+    n = torch.tensor(lengths, dtype=torch.int32, device=device)
+    dq, dk, dv = q.to(device), k.to(device), v.to(device)
+    lib = _lib.lib()
+    for ranges in (0, 1, 2, 3, 5, 8, 13, 17, 40, 256):
+        print(f"case {ranges} ranges, {new} new tokens {heads}/{kv}x{dim}", flush=True)
+        size = lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
+        partial = torch.full((max(size, 16),), 0xFF, dtype=torch.uint8, device=device)  # NaNs where nothing is written
+        out = torch.full_like(dq, 7.0)
+        rc = lib.vdnh3_causal_attn_cached(
+            dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(), *dv.stride()[:3], out.data_ptr(),
+            *out.stride()[:3], n.data_ptr(), batch, new, room, heads, kv, dim, 0.1, ranges, partial.data_ptr(), size,
+            _lib.stream_handle(device))
+        _lib.check(rc, "cached")
+        _check(out, want, dim)
+    assert lib.vdnh3_causal_attn_cached(
+        dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(), *dv.stride()[:3], out.data_ptr(),
+        *out.stride()[:3], n.data_ptr(), batch, new, room, heads, kv, dim, 0.1, 4, partial.data_ptr(), 64,
+        _lib.stream_handle(device)) == _lib.VDNH3_ERR_INVALID  # too small a buffer
+
+
+def test_many_requests(device):
+    """More requests than a workgroup has threads, some without keys."""
+    from vdn_h3_amd.causal import causal_softmax_cached
+
+    batch, room = 700, 40
+    g = torch.Generator().manual_seed(50)
+    lengths = torch.randint(0, room + 1, (batch,), generator=g)
+    q, k, v = _qkv(batch * room, 4, 2, 64, 51)
+    q, k, v = q[:batch * 2].view(batch, 2, 4, 64), k.view(batch, room, 2, 64), v.view(batch, room, 2, 64)
+    got = causal_softmax_cached(q.to(device), k.to(device), v.to(device), lengths.to(device), 0.125)
+    _check(got, po.cached(q, k, v, lengths.tolist(), 0.125), 64)
+
+
+def test_many_sequences(device):
+    """More packed sequences than a wavefront has lanes, empty ones among them."""
+    from vdn_h3_amd.causal import causal_softmax_packed
+
+    g = torch.Generator().manual_seed(52)
+    lengths = torch.randint(0, 40, (150,), generator=g)
+    lengths[:3], lengths[63:66], lengths[128], lengths[-2:] = 0, 0, 300, 0
+    bounds = [0] + lengths.cumsum(0).tolist()
+    for heads, kv, dim in ((5, 1, 64), (4, 4, 128)):
+        q, k, v = _qkv(bounds[-1], heads, kv, dim, 53)
+        cu = torch.tensor(bounds, dtype=torch.int32, device=device)
+        got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), cu, 0.125)
+        _check(got, po.packed(q, k, v, bounds, 0.125), dim)
 
 
 def test_cached_infinities_behind_a_new_token(device):
