@@ -31,6 +31,12 @@ int check_launch(const char *what) {
   return VDNH3_OK;
 }
 
+int check_grid(int64_t workgroups, int threads, const char *what) {
+  if (workgroups * threads > (int64_t)UINT32_MAX)
+    return set_error(VDNH3_ERR_INVALID, "%s: %lld workgroups are too many for one launch", what, (long long)workgroups);
+  return VDNH3_OK;
+}
+
 }  // namespace vdnh3
 
 extern "C" const char *vdnh3_last_error(void) { return g_last_error.c_str(); }

@@ -894,8 +894,9 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
   const int group = heads / kv_heads;
   const int64_t blocks = seqs.cu ? (int64_t)seqs.rows * group / BM + seqs.count
                                  : seqs.count * (((int64_t)seqs.rows * group + BM - 1) / BM);
-  VDNH3_HOST_CHECK((int64_t)seqs.rows * group <= INT32_MAX - BM && blocks * kv_heads <= INT32_MAX, VDNH3_ERR_INVALID,
-                   "causal attention: %d rows of %d heads are too many for one launch", seqs.rows, heads);
+  VDNH3_HOST_CHECK((int64_t)seqs.rows * group <= INT32_MAX - BM, VDNH3_ERR_INVALID,
+                   "causal attention: %d rows of %d heads are too many", seqs.rows, heads);
+  if (int rc = check_grid(blocks * kv_heads, kThreads, "causal attention")) return rc;
   hipLaunchKernelGGL((causal_tile_kernel<D, NQ>), dim3((unsigned)(blocks * kv_heads)), dim3(kThreads), 0, s, q, k, v, out, seqs,
                      (int)blocks, kv_heads, group, scale * 1.4426950408889634f);
   return check_launch("causal attention");
@@ -923,11 +924,12 @@ int launch_few(const Operand &q, const Operand &k, const Operand &v, const Opera
                int group, float scale_log2, const Parts &parts, hipStream_t s) {
   const int rows = seqs.rows * group, row_blocks = (rows + 16 * NQ - 1) / (16 * NQ);
   const int64_t blocks = (int64_t)kv_heads * row_blocks * parts.ranges;
-  VDNH3_HOST_CHECK(blocks <= INT32_MAX, VDNH3_ERR_INVALID, "causal attention: %lld ranges are too many for one launch",
-                   (long long)blocks);
+  int rc = check_grid(blocks, kFewThreads, "causal attention over caches");
+  if (!rc) rc = check_grid((int64_t)seqs.count * kv_heads * rows, kFewThreads, "causal attention over caches");
+  if (rc) return rc;
   hipLaunchKernelGGL((causal_few_kernel<D, NQ>), dim3((unsigned)blocks), dim3(kFewThreads), 0, s, q, k, v, out, seqs, kv_heads,
                      group, row_blocks, scale_log2, parts);
-  int rc = check_launch("causal attention over caches");
+  rc = check_launch("causal attention over caches");
   if (rc || parts.ranges == 1) return rc;
   hipLaunchKernelGGL(causal_combine_kernel<D>, dim3((unsigned)(seqs.count * kv_heads * rows)), dim3(kFewThreads), 0, s, q, k,
                      v, out, seqs, kv_heads, group, scale_log2, parts);

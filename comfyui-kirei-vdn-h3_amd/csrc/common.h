@@ -24,6 +24,8 @@ namespace vdnh3 {
 // ---- error channel (host) ---------------------------------------------------------
 int set_error(int code, const char *fmt, ...);
 int check_launch(const char *what);
+// A launch holds fewer than 2^32 threads; VDNH3_ERR_INVALID past it.
+int check_grid(int64_t workgroups, int threads, const char *what);
 
 // ---- bf16 <-> fp32 (device) ---------------------------------------------------------
 __device__ __forceinline__ float bf2f(uint16_t b) { return __uint_as_float(uint32_t(b) << 16); }

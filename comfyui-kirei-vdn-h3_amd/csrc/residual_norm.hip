@@ -307,6 +307,7 @@ extern "C" int vdnh3_residual_rmsnorm_quant_rows(int kind, const uint16_t *x, in
   if (!rc) rc = check_bf16_rows(weight, hidden, hidden, "the weight");
   if (!rc && sum) rc = check_bf16_rows(sum, sum_row, hidden, "the sum");
   if (!rc && kind == 0) rc = check_bf16_rows(out, out_row, hidden, "out");
+  if (!rc) rc = check_grid(rows, 256, "residual_rmsnorm");
   if (rc) return rc;
   if (kind != 0)
     VDNH3_HOST_CHECK(out && scale && out_row % 8 == 0 && out_row >= hidden && reinterpret_cast<uintptr_t>(out) % 8 == 0,

@@ -167,6 +167,8 @@ extern "C" int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_
                    "rotary: head_dim must be a multiple of 8 up to 128, got %d", head_dim);
   VDNH3_HOST_CHECK(rot_dim > 0 && rot_dim % 16 == 0 && rot_dim <= head_dim, VDNH3_ERR_INVALID,
                    "rotary: rot_dim must be a positive multiple of 16 and at most head_dim %d, got %d", head_dim, rot_dim);
+  VDNH3_HOST_CHECK(q_eps >= 0.f && k_eps >= 0.f && q_eps < INFINITY && k_eps < INFINITY, VDNH3_ERR_INVALID,
+                   "rotary: eps must be finite and not negative");
   VDNH3_HOST_CHECK(rows > 0 && q_heads > 0 && k_heads > 0, VDNH3_ERR_INVALID, "rotary: rows and heads must be positive");
   VDNH3_HOST_CHECK(positions && turns && axis_of_pair && position_type >= 0 && position_type <= 2, VDNH3_ERR_INVALID,
                    "rotary: null positions or frequencies, or a position type other than 0 (int32), 1 (int64), 2 (fp32)");
@@ -174,6 +176,7 @@ extern "C" int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_
   const Vectors ks{k, k_row, k_head, k_weight, k_eps, k_out, ko_row, ko_head, k_heads};
   int rc = check_vectors(qs, "q");
   if (!rc) rc = check_vectors(ks, "k");
+  if (!rc) rc = check_grid(rows, 64, "rotary");  // four rows a workgroup of 256, or fewer rows
   if (rc) return rc;
   const Positions pos{positions, p_axis, p_row, position_type};
   hipStream_t s = static_cast<hipStream_t>(stream);

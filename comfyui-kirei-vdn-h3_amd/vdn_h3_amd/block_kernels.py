@@ -245,7 +245,7 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
     ``kind`` (``linear.KIND_I8`` / ``KIND_F8``): the row-wise int8 / e4m3 codes and scales of ``rms_norm(t, weight, eps)``,
     as ``quantize_rows`` gives them for ``gemm_w8a8``; ``KIND_BF16``: the norm itself in bf16, and no scale. The sum, the
     norm and the codes are computed in fp32 from the bf16 inputs, each output rounded once: the norm is that of the
-    unrounded sum. ``residual=None`` (a model's first layer) norms ``x`` and returns it as ``t``. ``sum_out`` takes ``t``;
+    unrounded sum. The weight is taken in bf16. ``residual=None`` (a model's first layer) norms ``x`` and returns it as ``t``. ``sum_out`` takes ``t``;
     it may be ``x`` or ``residual``, otherwise it must not overlap them. A row with an infinity or a NaN in its norm gets
     the scale NaN (``KIND_BF16``: the NaNs that arise).
     """

@@ -48,8 +48,8 @@ def _output(out, shape, device):
         return torch.empty(shape, dtype=torch.bfloat16, device=device)
     if tuple(out.shape) != tuple(shape) or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
         raise ValueError(f"out must be a bf16 {list(shape)} tensor with a contiguous last dim")
-    if not _lib.in_place(out):
-        raise ValueError("out must be 16-byte aligned with strides that are multiples of 8 elements")
+    if not _lib.in_place(out) or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError("out must be 16-byte aligned with strides that are multiples of 8 elements and not 0")
     return out
 
 
@@ -61,7 +61,8 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
     checked and copied, another integer type on the GPU is converted); row ``i`` of a sequence attends to its rows 0 to
     ``i``. Sequences may be empty. Rows outside every sequence are not written: in a new output they hold anything, in
     ``out`` what it held. Bounds on the GPU are not checked, but cut to ``[0, T]``. ``out`` must not overlap the inputs.
-    Head dims 64 and 128 run natively, others up to 128 with zero channels added.
+    Head dims 64 and 128 run natively, others up to 128 with zero channels added. Rows of k and v are at most 2**24 elements
+    apart.
     """
     if query.ndim != 3 or key.ndim != 3 or key.shape != value.shape or query.shape[0] != key.shape[0] or \
             query.shape[2] != key.shape[2]:
@@ -99,7 +100,7 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     new tokens' own keys and values (its last N rows) among them: token ``i`` attends to rows 0 to ``lengths[b] - N + i``.
     A token in front of the first row (``lengths[b] < N``) attends to nothing and gives zeros. Rows behind a length are
     not used, whatever they hold. Lengths are cut to ``[0, room]``. Head dims 64 and 128; the caches are read in place, so
-    their layout has to suit the kernel (16-byte rows). ``out`` must not overlap the inputs.
+    their layout has to suit the kernel (16-byte rows, at most 2**24 elements apart). ``out`` must not overlap the inputs.
     """
     if query.ndim != 4 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape or \
             query.shape[0] != key_cache.shape[0] or query.shape[3] != key_cache.shape[3]:

@@ -24,7 +24,8 @@ class RotaryAxes:
     ``sections[a]`` pairs belong to axis ``a``, in order; ``rot_dim = 2 * sum(sections)`` channels turn, pair ``i`` being
     channels ``i`` and ``i + rot_dim / 2`` (split-half, as in the block). Pair ``i`` turns by ``theta ** (-i / n)`` per
     position: with ``ladder="shared"`` over all ``n = rot_dim / 2`` pairs (one ladder of frequencies, cut into axes), with
-    ``"per_axis"`` over the ``n = sections[a]`` pairs of its own axis, counted from the axis's first pair.
+    ``"per_axis"`` over the ``n = sections[a]`` pairs of its own axis, counted from the axis's first pair. The object holds the
+    frequencies on the device: it has to outlive graphs that were captured with it.
     """
 
     def __init__(self, sections, theta: float = 10000.0, ladder: str = "shared"):

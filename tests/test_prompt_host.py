@@ -118,6 +118,15 @@ def test_c_entry_points_refuse_before_any_launch(built_lib):
                 dict(dim=60), dict(dim=136), dict(w=p + 2)]:
         assert rotary(**bad) == _lib.VDNH3_ERR_INVALID, bad
 
+    def far_rotary():
+        return lib.vdnh3_qk_rotary_axes(p, 256, 64, None, float("nan"), p, 256, 64, 4, p, 128, 64, None, 1e-6, p, 128, 64, 2, p,
+                                        1, 3, 1, p, p, 64, 3, 64, None)
+
+    assert far_rotary() == _lib.VDNH3_ERR_INVALID and "eps" in _lib.last_error()
+    # more threads than a launch holds
+    assert norm(rows=1 << 24) == _lib.VDNH3_ERR_INVALID and "too many" in _lib.last_error()
+    assert rotary(rows=1 << 26) == _lib.VDNH3_ERR_INVALID and "too many" in _lib.last_error()
+
     def packed(q=p, q_row=256, k=p, out=p, cu=p, n=1, rows=4, h=4, kh=2, dim=64, scale=0.1):
         return lib.vdnh3_causal_attn_packed(q, q_row, 64, k, 128, 64, p, 128, 64, out, 256, 64, cu, n, rows, h, kh, dim, scale,
                                             None)
@@ -126,3 +135,61 @@ def test_c_entry_points_refuse_before_any_launch(built_lib):
                 dict(rows=0), dict(h=5), dict(kh=0), dict(h=0), dict(dim=80), dict(scale=0.0), dict(scale=-1.0),
                 dict(scale=float("nan")), dict(scale=float("inf"))]:
         assert packed(**bad) == _lib.VDNH3_ERR_INVALID, bad
+    assert packed(rows=1 << 30, h=64, kh=2) == _lib.VDNH3_ERR_INVALID and "too many" in _lib.last_error()
+    assert packed(rows=1 << 26, h=64, kh=64, n=1 << 23) == _lib.VDNH3_ERR_INVALID and "too many" in _lib.last_error()
+
+    def cached(q=p, k=p, k_row=128, lengths=p, batch=2, new=1, room=64, h=4, kh=2, dim=64, scale=0.1, ranges=0, part=None,
+               size=0):
+        return lib.vdnh3_causal_attn_cached(q, 256, 256, 64, k, 8192, k_row, 64, p, 8192, 128, 64, p, 256, 256, 64, lengths,
+                                            batch, new, room, h, kh, dim, scale, ranges, part, size, None)
+
+    for bad in [dict(q=None), dict(k=p + 2), dict(k_row=(1 << 24) + 8), dict(k_row=-8), dict(lengths=None), dict(batch=0),
+                dict(new=0), dict(room=0), dict(h=3), dict(dim=96), dict(scale=float("inf")), dict(ranges=-1),
+                dict(ranges=2), dict(ranges=2, part=p, size=8), dict(ranges=2, part=p + 8, size=1 << 20),
+                dict(ranges=1, batch=1 << 20, new=1 << 12), dict(ranges=1, batch=1 << 16, room=1 << 25)]:
+        assert cached(**bad) == _lib.VDNH3_ERR_INVALID, bad
+
+
+def test_ranges_of_a_call(built_lib):
+    """The host's rule: never more parts than the buffer's size counts, one range where one takes the caches, the prompt
+    kernel (0) for many tokens over short caches, and nothing for sizes that are none."""
+    from vdn_h3_amd import _lib
+
+    lib = _lib.lib()
+    assert lib.vdnh3_causal_cached_ranges(1, 1, 64, 40, 8) == 1
+    assert lib.vdnh3_causal_cached_ranges(64, 1, 8192, 40, 8) == 32
+    assert lib.vdnh3_causal_cached_ranges(16, 64, 2048, 40, 8) == 0
+    assert lib.vdnh3_causal_cached_ranges(1, 32, 40960, 40, 8) > 1
+    for bad in [(0, 1, 1, 1, 1), (1, 0, 1, 1, 1), (1, 1, 0, 1, 1), (1, 1, 1, 3, 2), (1, 1, 1, 0, 1), (1, 1, 1, 1, 0)]:
+        assert lib.vdnh3_causal_cached_ranges(*bad) == 0
+    assert lib.vdnh3_causal_partial_bytes(3, 10, 64, 1) == 0
+    assert lib.vdnh3_causal_partial_bytes(3, 10, 64, 4) == 4 * 2 * 30 * 66 * 4
+
+
+def test_launch_makes_the_tensors_device_current(monkeypatch):
+    from vdn_h3_amd import _lib
+
+    entered = []
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+
+        def __exit__(self, *_):
+            entered.append(None)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(_lib, "stream_handle", lambda device: 77)
+    seen = []
+
+    def call(*args):
+        seen.append((args, list(entered)))
+        return 0
+
+    _lib.launch("x", call, torch.device("cuda:0"), 1, 2)
+    _lib.launch("x", call, torch.device("cuda:1"), 3)
+    assert seen[0] == ((1, 2, 77), []) and seen[1] == ((3, 77), [torch.device("cuda:1")]) and entered[-1] is None
