@@ -860,6 +860,11 @@ __global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, 
   finish_row<D>(q, k, v, out, sequence_at(seqs, b), b, kvh, group, row, o, l, scale_log2, lane);
 }
 
+// A dimension of one element has no stride, whatever a caller passes for it.
+Operand operand(const uint16_t *p, int64_t batch, int64_t row, int64_t head, int batches, int rows, int heads) {
+  return Operand{p, batches > 1 ? batch : 0, rows > 1 ? row : 0, heads > 1 ? head : 0};
+}
+
 int check_operand(const Operand &o, const char *name) {
   VDNH3_HOST_CHECK(o.p != nullptr, VDNH3_ERR_INVALID, "causal attention: %s is null", name);
   VDNH3_HOST_CHECK(o.batch % 8 == 0 && o.row % 8 == 0 && o.head % 8 == 0 && reinterpret_cast<uintptr_t>(o.p) % 16 == 0,
@@ -952,7 +957,8 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
                                         int64_t o_row, int64_t o_head, const int32_t *cu_seqlens, int sequences, int rows,
                                         int heads, int kv_heads, int head_dim, float scale, void *stream) {
   using namespace vdnh3;
-  const Operand qo{q, 0, q_row, q_head}, ko{k, 0, k_row, k_head}, vo{v, 0, v_row, v_head}, oo{out, 0, o_row, o_head};
+  const Operand qo = operand(q, 0, q_row, q_head, 1, rows, heads), ko = operand(k, 0, k_row, k_head, 1, rows, kv_heads),
+                vo = operand(v, 0, v_row, v_head, 1, rows, kv_heads), oo = operand(out, 0, o_row, o_head, 1, rows, heads);
   int rc = check_causal(qo, ko, vo, oo, heads, kv_heads, head_dim, scale);
   if (rc) return rc;
   VDNH3_HOST_CHECK(cu_seqlens && sequences > 0 && rows > 0, VDNH3_ERR_INVALID,
@@ -996,8 +1002,10 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
                                         int new_tokens, int room, int heads, int kv_heads, int head_dim, float scale,
                                         int ranges, float *partial, size_t partial_bytes, void *stream) {
   using namespace vdnh3;
-  const Operand qo{q, q_batch, q_row, q_head}, ko{k, k_batch, k_row, k_head}, vo{v, v_batch, v_row, v_head},
-      oo{out, o_batch, o_row, o_head};
+  const Operand qo = operand(q, q_batch, q_row, q_head, batch, new_tokens, heads),
+                ko = operand(k, k_batch, k_row, k_head, batch, room, kv_heads),
+                vo = operand(v, v_batch, v_row, v_head, batch, room, kv_heads),
+                oo = operand(out, o_batch, o_row, o_head, batch, new_tokens, heads);
   int rc = check_causal(qo, ko, vo, oo, heads, kv_heads, head_dim, scale);
   if (rc) return rc;
   VDNH3_HOST_CHECK(lengths && batch > 0 && new_tokens > 0 && room > 0, VDNH3_ERR_INVALID,

@@ -302,6 +302,7 @@ extern "C" int vdnh3_residual_rmsnorm_quant_rows(int kind, const uint16_t *x, in
                    "residual_rmsnorm: rows must be positive and the width a positive multiple of 8, got %d x %d", rows,
                    hidden);
   VDNH3_HOST_CHECK(eps >= 0.f && eps < INFINITY, VDNH3_ERR_INVALID, "residual_rmsnorm: eps must be finite and not negative");
+  if (rows == 1) x_row = residual_row = out_row = sum_row = hidden;  // one row has no stride, whatever a caller passes for it
   int rc = check_bf16_rows(x, x_row, hidden, "x", true);
   if (!rc && residual) rc = check_bf16_rows(residual, residual_row, hidden, "the residual", true);
   if (!rc) rc = check_bf16_rows(weight, hidden, hidden, "the weight");

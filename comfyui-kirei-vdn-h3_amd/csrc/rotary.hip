@@ -172,8 +172,12 @@ extern "C" int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_
   VDNH3_HOST_CHECK(rows > 0 && q_heads > 0 && k_heads > 0, VDNH3_ERR_INVALID, "rotary: rows and heads must be positive");
   VDNH3_HOST_CHECK(positions && turns && axis_of_pair && position_type >= 0 && position_type <= 2, VDNH3_ERR_INVALID,
                    "rotary: null positions or frequencies, or a position type other than 0 (int32), 1 (int64), 2 (fp32)");
-  const Vectors qs{q, q_row, q_head, q_weight, q_eps, q_out, qo_row, qo_head, q_heads};
-  const Vectors ks{k, k_row, k_head, k_weight, k_eps, k_out, ko_row, ko_head, k_heads};
+  // a dimension of one element has no stride, whatever a caller passes for it
+  auto stride = [](int64_t s, int extent) { return extent > 1 ? s : 0; };
+  const Vectors qs{q, stride(q_row, rows), stride(q_head, q_heads), q_weight, q_eps, q_out, stride(qo_row, rows),
+                   stride(qo_head, q_heads), q_heads};
+  const Vectors ks{k, stride(k_row, rows), stride(k_head, k_heads), k_weight, k_eps, k_out, stride(ko_row, rows),
+                   stride(ko_head, k_heads), k_heads};
   int rc = check_vectors(qs, "q");
   if (!rc) rc = check_vectors(ks, "k");
   if (!rc) rc = check_grid(rows, 64, "rotary");  // four rows a workgroup of 256, or fewer rows

@@ -189,20 +189,14 @@ def stream_handle(device: torch.device) -> int:
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
-def strides(t) -> tuple[int, ...]:
-    """The strides of every dim but the last; one of size 1 has none (torch may report anything for it)."""
-    if 1 in t.shape:
-        return tuple(0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()))
-    return t.stride()[:-1]
-
-
 def in_place(t) -> bool:
     """Whether a kernel can take a bf16 tensor where it lies: 16-byte aligned rows of contiguous channels."""
     if t.data_ptr() % 16:
         return False
-    if t.is_contiguous() and t.shape[-1] % 8 == 0:
-        return True
-    return (t.stride(-1) == 1 or t.shape[-1] == 1) and not any(s % 8 for s in strides(t))
+    if t.is_contiguous():
+        return t.shape[-1] % 8 == 0 or t.numel() == t.shape[-1]
+    *outer, inner = zip(t.shape, t.stride())
+    return (inner[1] == 1 or inner[0] == 1) and not any(s % 8 for n, s in outer if n > 1)
 
 
 def operand(t):

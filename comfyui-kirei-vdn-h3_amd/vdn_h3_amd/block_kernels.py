@@ -275,12 +275,10 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
     if rows == 0:
         return out, scale, total
 
-    def operand(t):  # address and row stride; one row's stride may be anything
-        return (None, 0) if t is None else (t.data_ptr(), t.stride(0) if rows > 1 else width)
-
+    summed = (None, 0) if rr is None else (total.data_ptr(), total.stride(0))
     _lib.launch("vdnh3_residual_rmsnorm_quant_rows", _lib.lib().vdnh3_residual_rmsnorm_quant_rows, device, kind,
-                *operand(xr), *operand(rr), w.data_ptr(), eps, rows, width, out.data_ptr(), width, _lib.ptr(scale),
-                *operand(None if rr is None else total))
+                xr.data_ptr(), xr.stride(0), _lib.ptr(rr), 0 if rr is None else rr.stride(0), w.data_ptr(), eps, rows, width,
+                out.data_ptr(), width, _lib.ptr(scale), *summed)
     return out, scale, total
 
 

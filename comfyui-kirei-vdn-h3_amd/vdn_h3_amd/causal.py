@@ -10,6 +10,8 @@ can be replayed with other lengths. Forward-only; there is no CPU path.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _lib
@@ -86,9 +88,17 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
         return out
     q, k, v = _lib.operand(query), _lib.operand(key), _lib.operand(value)
     _lib.launch("causal_softmax_packed", _lib.lib().vdnh3_causal_attn_packed, device,
-                q.data_ptr(), *_lib.strides(q), k.data_ptr(), *_lib.strides(k), v.data_ptr(), *_lib.strides(v),
-                out.data_ptr(), *_lib.strides(out), cu.data_ptr(), cu.numel() - 1, rows, heads, key.shape[1], dim, scale)
+                q.data_ptr(), *q.stride()[:-1], k.data_ptr(), *k.stride()[:-1], v.data_ptr(), *v.stride()[:-1],
+                out.data_ptr(), *out.stride()[:-1], cu.data_ptr(), cu.numel() - 1, rows, heads, key.shape[1], dim, scale)
     return out
+
+
+@lru_cache(maxsize=1024)
+def _cut(batch: int, new: int, room: int, heads: int, kv_heads: int, dim: int) -> tuple[int, int]:
+    """The ranges of keys that a call of these sizes takes and the bytes of their partial results."""
+    lib = _lib.lib()
+    ranges = lib.vdnh3_causal_cached_ranges(batch, new, room, heads, kv_heads)
+    return ranges, lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
 
 
 def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, lengths: torch.Tensor,
@@ -126,13 +136,11 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
         return out.zero_()
     if lengths.dtype != torch.int32 or not lengths.is_contiguous():
         lengths = lengths.to(torch.int32).contiguous()
-    lib = _lib.lib()
-    ranges = lib.vdnh3_causal_cached_ranges(batch, new, room, heads, kv_heads)
-    size = lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
+    ranges, size = _cut(batch, new, room, heads, kv_heads, dim)
     partial = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _lib.launch("causal_softmax_cached", lib.vdnh3_causal_attn_cached, device,
-                q.data_ptr(), *_lib.strides(q), key_cache.data_ptr(), *_lib.strides(key_cache), value_cache.data_ptr(),
-                *_lib.strides(value_cache), out.data_ptr(), *_lib.strides(out), lengths.data_ptr(), batch, new, room, heads,
+    _lib.launch("causal_softmax_cached", _lib.lib().vdnh3_causal_attn_cached, device,
+                q.data_ptr(), *q.stride()[:-1], key_cache.data_ptr(), *key_cache.stride()[:-1], value_cache.data_ptr(),
+                *value_cache.stride()[:-1], out.data_ptr(), *out.stride()[:-1], lengths.data_ptr(), batch, new, room, heads,
                 kv_heads, dim, scale, ranges, _lib.ptr(partial), size)
     return out
 

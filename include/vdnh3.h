@@ -512,7 +512,8 @@ int vdnh3_fill_rows_bf16(uint16_t *p, int64_t ld, int rows, int cols, float valu
 
 /* ------------------------------------------------------------------------------
  * Operators of the language model that encodes the prompts (not in the reference). Strides in
- * elements; bf16 operands 16-byte aligned with strides that are multiples of 8 elements.
+ * elements; bf16 operands 16-byte aligned with strides that are multiples of 8 elements (a stride
+ * of a dimension of one element is not looked at).
  * ------------------------------------------------------------------------------ */
 
 /* t = x + residual; y = t / sqrt(mean(t^2) + eps) * weight, in fp32. kind 0: out = bf16(y) (uint16_t, 16-byte

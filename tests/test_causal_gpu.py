@@ -251,6 +251,31 @@ def test_offsets_past_32_bits(device, new):
     _check(got, po.cached(q, hk[None], hv[None], [room - 1], 0.125), 64)
 
 
+def test_strides_of_single_elements_do_not_count(device):
+    from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
+    from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
+    from vdn_h3_amd.rotary import RotaryAxes, normalise_qk_axes
+
+    def odd(t):  # a stride of 3 wherever a dimension has one element
+        return torch.as_strided(t, t.shape, tuple(3 if n == 1 else s for n, s in zip(t.shape, t.stride())))
+
+    for rows, heads, kv in ((1, 4, 1), (1, 1, 1), (40, 1, 1)):
+        q, k, v = (t.to(device) for t in _qkv(rows, heads, kv, 64, 60))
+        want = causal_softmax_packed(q, k, v, [0, rows], 0.125)
+        assert torch.equal(causal_softmax_packed(odd(q), odd(k), odd(v), [0, rows], 0.125), want)
+        n = torch.tensor([rows], dtype=torch.int32, device=device)
+        got = causal_softmax_cached(odd(q[None, -1:]), odd(k[None]), odd(v[None]), n, 0.125)
+        _check(got[0], [t[-1:] for t in po.packed(q.cpu(), k.cpu(), v.cpu(), [0, rows], 0.125)], 64)
+        pos = torch.arange(rows, device=device)
+        axes = RotaryAxes((32,))
+        assert all(torch.equal(a, b) for a, b in zip(normalise_qk_axes(odd(q), odd(k), pos, axes),
+                                                     normalise_qk_axes(q, k, pos, axes)))
+    x, w = torch.randn(1, 64, device=device).to(BF), torch.ones(64, dtype=BF, device=device)
+    out = torch.empty_like(x)
+    got = residual_rmsnorm_quantize(odd(x), odd(x), w, 1e-6, 1, sum_out=odd(out))
+    assert torch.equal(got[0], residual_rmsnorm_quantize(x, x, w, 1e-6, 1)[0]) and torch.equal(out, 2 * x)
+
+
 def test_cache_layout_and_lengths_are_checked(device):
     from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
 
@@ -269,6 +294,8 @@ def test_cache_layout_and_lengths_are_checked(device):
             causal_softmax_packed(q[:, 0], good[:, 0], good[:, 0], [0, 2], scale)
     with pytest.raises(RuntimeError, match="CPU"):
         causal_softmax_cached(q, good, good, n.cpu(), 0.1)
+    with pytest.raises(ValueError, match="out"):
+        causal_softmax_cached(q, good, good, n, 0.1, out=torch.zeros(1, 1, 4, 64, dtype=BF, device=device).expand(2, 1, 4, 64))
     empty = causal_softmax_cached(q, good[:, :0], good[:, :0], n, 0.1)
     assert (empty == 0).all()
     assert causal_softmax_packed(q[:0, 0], good[:0, 0], good[:0, 0], [0], 0.1).shape == (0, 4, 64)
