@@ -95,12 +95,18 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
 // wavefront's two 16-query blocks and 24 of a tile's 96 keys, and its probabilities are operands of O^T += V^T P^T as
 // they lie. V tiles are loaded as they are, key by key, and read transposed (ds_read_b64_tr_b16: 16 lanes get 4 keys of
 // 16 channels), so no pass writes a transposed copy first.
+//
+// What bounds it: the issue of the SIMD that two wavefronts share. A phase's 102 MFMAs of 16 cycles and the softmax beside
+// them, about 1,400 cycles of VALU (a third of it the exponentials), take 2,500 cycles together; LDS is busy for 28% of
+// the time, without bank conflicts, and fragment reads 2 to 6 ahead measure the same. 8,296 rows x 40 / 8 heads x 128 take
+// 585 us, 1,205 TFLOP/s, where the library's 8,192^3 product reaches 1,367. Short prompts are bound by a workgroup's start
+// and end, about 6 us (its block, the first loads, two more phases than tiles, the stores): 512 rows take 15.0 us.
 constexpr int kBN = 96;        // keys per tile
 constexpr int kThreads = 512;
 constexpr int kRing = 3;       // LDS slots per K and V ring (144 KB at D = 128): loads run kRing - 1 tiles ahead
 constexpr int kAhead = 4;      // fragments a wavefront's LDS reads run ahead of its MFMAs
 constexpr float kLazy = 8.0f;  // log2 of the largest probability a stale running max allows
-constexpr float kNoMax = -3.402823466e38f;  // the running max before any score: finite, so a masked score gives exp2(-inf) = 0
+constexpr float kNoMax = -3.402823466e38f;  // the running max before any score: finite, so exp2(-inf - max) is 0
 
 // LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). K: the 16 rows of a fragment read hit 16 different
 // 16-byte bank groups. V: the 8 rows that half a wavefront reads 32 bytes of hit 8 different 32-byte ones.
@@ -130,9 +136,9 @@ struct Block {
   Sequence s;
 };
 
-// Blocks of packed sequences are numbered without a count on the host: sequence b's begin at floor(cu[b] group / BM) + b, which
-// leaves room for those before. Every wavefront looks for its own, a lane per sequence: one load, a ballot. Numbers that
-// are no block's give no rows.
+// Blocks of packed sequences are numbered without a count on the host: sequence b's begin at floor(cu[b] group / BM) + b,
+// which leaves room for those before. Every wavefront looks for its own, a lane per sequence: one load, a ballot. Numbers
+// that are no block's give no rows.
 template <int BM>
 __device__ __forceinline__ Block packed_block(const Sequences &seqs, int block, int group) {
   const int lane = threadIdx.x & 63;
@@ -270,8 +276,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
     const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
 
     // K(t) and V(t) live in slot t % kRing. Phase 0 needs K(0), by group A, and the queries; K(1 .. kRing-2) by group A and
-    // V(0 .. kRing-3) by group B, which phase 2 needs, follow behind its barrier. V(-1), which the product of tile 0 reads with
-    // P(-1) = 0, is zeroed. Group B's first issue in its turn (phase 0) is V(kRing-2).
+    // V(0 .. kRing-3) by group B, which phase 2 needs, follow behind its barrier. V(-1), which the product of tile 0 reads
+    // with P(-1) = 0, is zeroed. Group B's first issue in its turn (phase 0) is V(kRing-2).
     if (turn == 0) tile_dma(0, 0);
     bf16x8_t qf[NQ][NS];
 #pragma unroll
@@ -288,8 +294,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
     for (int p = 0; p < phases; ++p) {
       const int t_mfma = p >> 1, t_valu = (p - 1) >> 1;
       if (turn == (p & 1)) {
-        // t = w_tiles has no scores to make and t = 0 no product with values: those halves run on what is there (leaving them out
-        // in code of their own carries both operands through the loop, which spills)
+        // t = w_tiles has no scores to make and t = 0 no product with values: those halves run on what is there (leaving
+        // them out in code of their own carries both operands through the loop, which spills)
         const int t = t_mfma;
         if (t <= w_tiles && w_tiles > 0) {
           const uint16_t *vtile = Vs[(t + kRing - 1) % kRing];
@@ -374,7 +380,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
               for (int m = 0; m < NO; ++m) oacc[m][n] *= corr;
             }
           }
-          // P in bf16 pairs (the values the PV product and the row sums use)
+          // P in bf16 pairs, the matrix cores' operand, for the PV product and the row sums alike: up to 2^-8 of a
+          // probability, 2.0e-3 of the result in 2-norm with its own rounding's 1.6e-3
 #pragma unroll
           for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -387,8 +394,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
               }
         }
       }
-      // before an even phase 2(t+1): K(t+1) and V(t) have landed. While there are tiles to load, each group's latest one, K(t+2)
-      // or V(t+1), may still be in flight; after that there is none later.
+      // before an even phase 2(t+1): K(t+1) and V(t) have landed. While there are tiles to load, each group's latest one,
+      // K(t+2) or V(t+1), may still be in flight; after that there is none later.
       if (p & 1) {
         if (t_valu + kRing - 1 < T) wait_vm_lds<(kRing - 2) * CG>();
         else wait_vm_lds<0>();
@@ -437,8 +444,8 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
       }
     }
   }
-  // A value that is not finite behind a row, in a tile that the row sees a part of, times the row's probability 0 is a NaN in
-  // its sum. Rows whose result is not finite are computed once more without the keys that they do not see: never for
+  // A value that is not finite behind a row, in a tile that the row sees a part of, times the row's probability 0 is a NaN
+  // in its sum. Rows whose result is not finite are computed once more without the keys that they do not see: never for
   // finite inputs whose result bf16 holds.
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -455,21 +462,25 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   }
 }
 
-// ---------------------------------------------------------------------------------
-// Few rows over long caches (new tokens): what counts is to stream the keys and values once. The 32-key tiles of all
-// sequences, one behind another, are cut into `ranges` equal ranges for each key / value head, one workgroup each and about
-// one workgroup per CU: whatever the lengths are, every CU streams the same number of tiles, in one round. A range crosses
-// from one sequence into the next; only the sequences at its two ends can be shared with other ranges. Such a part is
-// written unnormalised in fp32 with its max and sum and combined by a second launch; a sequence inside a range is
-// finished at once. The cut follows from the lengths on the device, in both kernels alike.
-// A workgroup takes up to 16 NQ of a head's (token, head) rows. Its wavefronts take the tiles in turn, each through two LDS
-// slots of its own (one tile in flight while it works on the other, no barrier), with a running softmax of its own; they
-// are merged in LDS at the end of a sequence.
+// --------------------------------------------------------------------------------- Few rows over long caches (new tokens):
+// what counts is to stream the keys and values once. The 32-key tiles of all sequences, one behind another, are cut into
+// `ranges` equal ranges for each key / value head, one workgroup each and about one workgroup per CU: whatever the lengths
+// are, every CU streams the same number of tiles, in one round. A range crosses from one sequence into the next; only the
+// sequences at its two ends can be shared with other ranges. Such a part is written unnormalised in fp32 with its max and
+// sum and combined by a second launch; a sequence inside a range is finished at once. The cut follows from the lengths on
+// the device, in both kernels alike. A workgroup takes up to 16 NQ of a head's (token, head) rows. Its wavefronts take the
+// tiles in turn, each through two LDS slots of its own (one tile in flight while it works on the other, no barrier), with a
+// running softmax of its own; they are merged in LDS at the end of a sequence. HBM bounds it: 64 requests of up to 8,192
+// keys x 8 heads x 128 (1.05 GB) take 196 us, 5.3 TB/s where a copy reaches 4.8; one request of 40,688 keys (167 MB) 34 us
+// and 5 for the combination. With fixed chunks of keys instead of equal ranges the first took 215 to 244 us, whole rounds
+// of workgroups each with a pipeline to fill.
 constexpr int kFewKeys = 32;      // keys per tile: one k-step of the PV product
 constexpr int kFewRing = 2;
-// Tiles of a range, at least: one per wavefront (one request of 1,000 keys x 40 / 8 heads: 16 ranges 11.1 us, 8 11.3, 4 12.2).
+// Tiles of a range, at least: one per wavefront (one request of 1,000 keys x 40 / 8 heads: 16 ranges 11.1 us, 8 11.3, 4
+// 12.2).
 constexpr int kFewLeast = 4;
-// Tiles of all caches up to which one range takes them and no second launch is needed (600 keys 11.1 us against 11.2 to 12.9).
+// Tiles of all caches up to which one range takes them and no second launch is needed (600 keys 11.1 us against 11.2 to
+// 12.9).
 constexpr int kFewOne = 18;
 constexpr int kFewThreads = 256;  // of both kernels
 
@@ -489,8 +500,8 @@ __device__ __forceinline__ int tiles_of(const Sequences &seqs, int b) {
   return max(1, (keys + kFewKeys - 1) / kFewKeys);
 }
 
-// How the tiles of all sequences are cut: `each` per range, the first `more` ranges one more. Each of the workgroup's threads
-// counts the tiles of `per` sequences; before[i] is what the threads in front of i counted.
+// How the tiles of all sequences are cut: `each` per range, the first `more` ranges one more. Each of the workgroup's
+// threads counts the tiles of `per` sequences; before[i] is what the threads in front of i counted.
 struct Cut {
   int total, per, ranges, each, more;
   const int *before;
@@ -689,8 +700,8 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
               if (at_key > last[n] || at_key >= k1) sacc[h][n][i] = -INFINITY;
           }
       }
-      // P as bf16 and what that leaves, again as bf16 (16 bits of each probability): the matrix cores are idle beside the loads,
-      // and the result is then as exact as its own rounding
+      // P as bf16 and what that leaves, again as bf16 (16 bits of each probability): the matrix cores are idle beside the
+      // loads, and the result is then as exact as its own rounding
       u32x4_t pb[NQ], pl[NQ];
       float mt[NQ];
 #pragma unroll
@@ -907,8 +918,10 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
   return check_launch("causal attention");
 }
 
-// Workgroups of 256 rows from which on they are taken; with fewer, workgroups of 128 leave fewer CUs without one and end closer
-// together.
+// Workgroups of 256 rows from which on they are taken; with fewer, workgroups of 128 (which read twice the LDS for the same
+// products) leave fewer CUs without one and end closer together. 512 rows x 40 / 8 x 128 15 us against 23, 4,148 x 16 / 2
+// (260 workgroups) 88 against 98, 2,000 x 40 / 8 (313) 67 against 60, 8,296 751 against 588; with 64 channels, where two
+// fit a CU, 4,000 x 20 / 20 (313) 65 against 74, 8,000 x 32 / 8 (1,000) 325 against 296.
 constexpr int kHighGroups128 = 288, kHighGroups64 = 512;
 
 int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int heads,
@@ -967,12 +980,12 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
                        static_cast<hipStream_t>(stream));
 }
 
-// The ranges of a call, or 0 for the kernel above: what its caches take at full length either way, in us. The prompt kernel goes
-// through all keys of a block of 128 rows in one workgroup (1.3 us per 96 keys), which is little at a time where there are
-// few blocks. Here 256 workgroups are at work always, but on 32 rows each (1.9 us per 4 tiles of 32 keys). 40 / 8 heads x
-// 128, measured: 40,688 keys and 32 new tokens 139 us against 560, 128 tokens 399 against 563, 256 tokens 759 against 566; 16
-// requests of 2,000 keys and 16 tokens 93 against 38. With up to 16 rows it is the loads that count, and this kernel
-// always.
+// The ranges of a call, or 0 for the kernel above: what its caches take at full length either way, in us. The prompt kernel
+// goes through all keys of a block of 128 rows in one workgroup (1.3 us per 96 keys), which is little at a time where there
+// are few blocks. Here 256 workgroups are at work always, but on 32 rows each (1.9 us per 4 tiles of 32 keys). 40 / 8 heads
+// x 128, measured: 40,688 keys and 32 new tokens 139 us against 560, 128 tokens 399 against 563, 256 tokens 759 against
+// 566; 16 requests of 2,000 keys and 16 tokens 93 against 38. With up to 16 rows it is the loads that count, and this
+// kernel always.
 extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads) {
   using namespace vdnh3;
   if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
