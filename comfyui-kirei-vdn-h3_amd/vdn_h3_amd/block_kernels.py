@@ -277,8 +277,8 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
 
     summed = (None, 0) if rr is None else (total.data_ptr(), total.stride(0))
     _lib.launch("vdnh3_residual_rmsnorm_quant_rows", _lib.lib().vdnh3_residual_rmsnorm_quant_rows, device, kind,
-                xr.data_ptr(), xr.stride(0), _lib.ptr(rr), 0 if rr is None else rr.stride(0), w.data_ptr(), eps, rows, width,
-                out.data_ptr(), width, _lib.ptr(scale), *summed)
+                xr.data_ptr(), xr.stride(0), _lib.ptr(rr), 0 if rr is None else rr.stride(0), w.data_ptr(), float(eps),
+                rows, width, out.data_ptr(), width, _lib.ptr(scale), *summed)
     return out, scale, total
 
 

@@ -17,6 +17,8 @@ import torch
 from . import _lib
 from .window import KERNEL_HEAD_DIMS, padded_head_dim, zero_pad_channels
 
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
 
 def _check_heads(query, key, value, name):
     if query.dtype != torch.bfloat16 or key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
@@ -29,8 +31,8 @@ def _check_heads(query, key, value, name):
 def _sequence_bounds(cu_seqlens, rows: int, device) -> torch.Tensor:
     """``cu_seqlens`` as a contiguous int32 device tensor; bounds that the host holds are checked."""
     if not isinstance(cu_seqlens, torch.Tensor):
-        cu_seqlens = torch.tensor(list(cu_seqlens), dtype=torch.int64)
-    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
+        cu_seqlens = torch.tensor(list(cu_seqlens))
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in _INTEGERS:
         raise ValueError("cu_seqlens must hold the sequences + 1 integer bounds")
     if cu_seqlens.device.type == "cpu":
         bounds = cu_seqlens.tolist()
@@ -63,7 +65,7 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
     checked and copied, another integer type on the GPU is converted); row ``i`` of a sequence attends to its rows 0 to
     ``i``. Sequences may be empty. Rows outside every sequence are not written: in a new output they hold anything, in
     ``out`` what it held. Bounds on the GPU are not checked, but cut to ``[0, T]``. ``out`` must not overlap the inputs.
-    Head dims 64 and 128 run natively, others up to 128 with zero channels added. Rows of k and v are at most 2**24 elements
+    Head dims 64 and 128 run natively, others up to 128 with zero channels added. Rows of k and v are at most 2**23 elements
     apart.
     """
     if query.ndim != 3 or key.ndim != 3 or key.shape != value.shape or query.shape[0] != key.shape[0] or \
@@ -89,7 +91,8 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
     q, k, v = _lib.operand(query), _lib.operand(key), _lib.operand(value)
     _lib.launch("causal_softmax_packed", _lib.lib().vdnh3_causal_attn_packed, device,
                 q.data_ptr(), *q.stride()[:-1], k.data_ptr(), *k.stride()[:-1], v.data_ptr(), *v.stride()[:-1],
-                out.data_ptr(), *out.stride()[:-1], cu.data_ptr(), cu.numel() - 1, rows, heads, key.shape[1], dim, scale)
+                out.data_ptr(), *out.stride()[:-1], cu.data_ptr(), cu.numel() - 1, rows, heads, key.shape[1], dim,
+                float(scale))
     return out
 
 
@@ -110,7 +113,7 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     new tokens' own keys and values (its last N rows) among them: token ``i`` attends to rows 0 to ``lengths[b] - N + i``.
     A token in front of the first row (``lengths[b] < N``) attends to nothing and gives zeros. Rows behind a length are
     not used, whatever they hold. Lengths are cut to ``[0, room]``. Head dims 64 and 128; the caches are read in place, so
-    their layout has to suit the kernel (16-byte rows, at most 2**24 elements apart). ``out`` must not overlap the inputs.
+    their layout has to suit the kernel (16-byte rows, at most 2**23 elements apart). ``out`` must not overlap the inputs.
     """
     if query.ndim != 4 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape or \
             query.shape[0] != key_cache.shape[0] or query.shape[3] != key_cache.shape[3]:
@@ -119,7 +122,7 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     _check_heads(query, key_cache, value_cache, "causal_softmax_cached")
     batch, new, heads, dim = query.shape
     room, kv_heads = key_cache.shape[1], key_cache.shape[2]
-    if lengths.ndim != 1 or lengths.numel() != batch or lengths.is_floating_point():
+    if lengths.ndim != 1 or lengths.numel() != batch or lengths.dtype not in _INTEGERS:
         raise ValueError(f"lengths must hold {batch} integers, got {tuple(lengths.shape)} {lengths.dtype}")
     if dim not in KERNEL_HEAD_DIMS:
         raise ValueError(f"causal_softmax_cached supports head dims {KERNEL_HEAD_DIMS}, got {dim}")
@@ -141,7 +144,7 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     _lib.launch("causal_softmax_cached", _lib.lib().vdnh3_causal_attn_cached, device,
                 q.data_ptr(), *q.stride()[:-1], key_cache.data_ptr(), *key_cache.stride()[:-1], value_cache.data_ptr(),
                 *value_cache.stride()[:-1], out.data_ptr(), *out.stride()[:-1], lengths.data_ptr(), batch, new, room, heads,
-                kv_heads, dim, scale, ranges, _lib.ptr(partial), size)
+                kv_heads, dim, float(scale), ranges, _lib.ptr(partial), size)
     return out
 
 

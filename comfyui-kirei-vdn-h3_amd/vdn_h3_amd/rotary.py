@@ -110,8 +110,8 @@ def normalise_qk_axes(q_raw: torch.Tensor, k_raw: torch.Tensor, positions: torch
         return qn, kn
     turns, axis = axes.table(device)
     _lib.launch("vdnh3_qk_rotary_axes", _lib.lib().vdnh3_qk_rotary_axes, device,
-                q.data_ptr(), q.stride(0), q.stride(1), _lib.ptr(wq), eps, qn.data_ptr(), heads * dim, dim, heads,
-                k.data_ptr(), k.stride(0), k.stride(1), _lib.ptr(wk), eps if k_eps is None else k_eps, kn.data_ptr(),
+                q.data_ptr(), q.stride(0), q.stride(1), _lib.ptr(wq), float(eps), qn.data_ptr(), heads * dim, dim, heads,
+                k.data_ptr(), k.stride(0), k.stride(1), _lib.ptr(wk), float(eps if k_eps is None else k_eps), kn.data_ptr(),
                 kv_heads * dim, dim, kv_heads, positions.data_ptr(), code, *positions.stride(), turns.data_ptr(),
                 axis.data_ptr(), axes.rot_dim, seq, dim)
     return qn, kn

@@ -218,6 +218,13 @@ def test_many_sequences(device):
         cu = torch.tensor(bounds, dtype=torch.int32, device=device)
         got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), cu, 0.125)
         _check(got, po.packed(q, k, v, bounds, 0.125), dim)
+    # thousands, nearly all of them empty or of one row
+    lengths = (torch.rand(9000, generator=g) < 0.1).long()
+    lengths[[0, 4095, 4097, 8999]] = torch.tensor([3, 70, 130, 2])
+    bounds = [0] + lengths.cumsum(0).tolist()
+    q, k, v = _qkv(bounds[-1], 4, 2, 64, 54)
+    got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), bounds, 0.125)
+    _check(got, po.packed(q, k, v, bounds, 0.125), 64)
 
 
 def test_cached_infinities_behind_a_new_token(device):
@@ -234,13 +241,13 @@ def test_cached_infinities_behind_a_new_token(device):
         assert got[:, -2:].isnan().all()
 
 
-@pytest.mark.parametrize("new", [1, 40])
-def test_offsets_past_32_bits(device, new):
+# row 1,199 starts at element 2.5e9; rows as far apart as they may be
+@pytest.mark.parametrize("new,room,row", [(1, 1200, 1 << 21), (40, 1200, 1 << 21), (1, 300, 1 << 23), (70, 300, 1 << 23)])
+def test_offsets_past_32_bits(device, new, room, row):
     """Caches whose rows lie more than 2^32 bytes, and 2^31 elements, behind their first."""
     from vdn_h3_amd.causal import causal_softmax_cached
 
-    print(f"case cached far {new}", flush=True)
-    room, row = 1200, 1 << 21  # row 1199 starts at element 2.5e9
+    print(f"case cached far {new} {room} x {row}", flush=True)
     store = torch.empty(room * row, dtype=BF, device=device)
     k, v = (torch.as_strided(store, (1, room, 2, 64), (8, row, 64, 1), off) for off in (0, 1 << 20))
     q, hk, hv = _qkv(room, 4, 2, 64, 15)

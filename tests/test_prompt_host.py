@@ -86,7 +86,8 @@ def test_bounds_that_the_host_holds_are_checked():
     from vdn_h3_amd.causal import _sequence_bounds
 
     device = torch.device("cuda:0")
-    for bad in ([0, 7], [-1, 3], [0, 4, 3], [], torch.tensor([0.0, 3.0]), torch.tensor([[0, 3]]), torch.tensor([0, 9])):
+    for bad in ([0, 7], [-1, 3], [0, 4, 3], [], torch.tensor([0.0, 3.0]), [0, 2.5], [False, True],
+                torch.tensor([[0, 3]]), torch.tensor([0, 9])):
         with pytest.raises(ValueError):
             _sequence_bounds(bad, 6, device)
 
@@ -143,7 +144,7 @@ def test_c_entry_points_refuse_before_any_launch(built_lib):
         return lib.vdnh3_causal_attn_cached(q, 256, 256, 64, k, 8192, k_row, 64, p, 8192, 128, 64, p, 256, 256, 64, lengths,
                                             batch, new, room, h, kh, dim, scale, ranges, part, size, None)
 
-    for bad in [dict(q=None), dict(k=p + 2), dict(k_row=(1 << 24) + 8), dict(k_row=-8), dict(lengths=None), dict(batch=0),
+    for bad in [dict(q=None), dict(k=p + 2), dict(k_row=(1 << 23) + 8), dict(k_row=-8), dict(lengths=None), dict(batch=0),
                 dict(new=0), dict(room=0), dict(h=3), dict(dim=96), dict(scale=float("inf")), dict(ranges=-1),
                 dict(ranges=2), dict(ranges=2, part=p, size=8), dict(ranges=2, part=p + 8, size=1 << 20),
                 dict(ranges=1, batch=1 << 20, new=1 << 12), dict(ranges=1, batch=1 << 16, room=1 << 25)]:
