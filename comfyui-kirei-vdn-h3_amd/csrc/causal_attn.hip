@@ -45,7 +45,8 @@ __device__ __forceinline__ Sequence sequence_at(const Sequences &s, int b) {
 }
 
 // The output row of one query by one wavefront: a lane takes a key of each 64, then two (one) channels of the sum.
-// Keys that the query does not see are not read.
+// Keys that the query does not see are not read. Probabilities carry a factor of 2^-24, which cancels, so that up to 2^24
+// values of bf16's largest sum up inside fp32.
 template <int D>
 __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k, int64_t k_row, const uint16_t *v,
                                            int64_t v_row, int keys, float scale_log2, uint16_t *out, int lane) {
@@ -67,7 +68,7 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
       s = dot * scale_log2;
     }
     const float m_new = fmaxf(m, wave_max(s)), base = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = exp2f(m - base), p = exp2f(s - base);  // 0 for a lane without a key
+    const float corr = exp2f(m - base), p = exp2f(s - base - 24.f);  // 0 for a lane without a key
     m = m_new;
     l *= corr;
 #pragma unroll
@@ -545,9 +546,9 @@ __device__ __forceinline__ Cut make_cut(const Sequences &seqs, int ranges, int (
   return Cut{total, per, n, each, total - n * each, before};
 }
 
-// O / l of one row, two (one) channels per lane. Where new tokens stand behind one another (`masked`), a value that is not
-// finite behind the row, in a tile that it sees a part of, times the probability 0 is a NaN in its sum: such a row is
-// computed once more without the keys that it does not see.
+// O / l of one row, two (one) channels per lane. A value that is not finite gives a NaN where it meets a probability of 0: that
+// of a key behind the row, of a last key that stands in for one, or what the rounding of its own probability left. Values
+// near fp32's largest can sum up past it. A row with such a result is computed once more, from the keys that it sees.
 template <int D>
 __device__ __forceinline__ void finish_row(const Operand &q, const Operand &k, const Operand &v, const Operand &out,
                                            const Sequence &s, int b, int kvh, int group, int row, const float (&o)[D / 64],
@@ -562,7 +563,7 @@ __device__ __forceinline__ void finish_row(const Operand &q, const Operand &k, c
     y[c] = keys > 0 ? o[c] / l : 0.f;
     fine = fine && fabsf(y[c]) < INFINITY;
   }
-  if (s.n > 1 && __any(!fine)) {
+  if (__any(!fine)) {
     attend_row<D>(q.at(b, s.q0 + token, head), k.at(b, s.k0, kvh), k.row, v.at(b, s.k0, kvh), v.row, keys, scale_log2, op,
                   lane);
     return;
@@ -875,6 +876,9 @@ __global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, 
   finish_row<D>(q, k, v, out, sequence_at(seqs, b), b, kvh, group, row, o, l, scale_log2, lane);
 }
 
+// Rows of a cache: keys are counted in 32 bits, up to the end of a tile behind the last.
+constexpr int kMostRoom = INT32_MAX - 4 * kBN;
+
 // A dimension of one element has no stride, whatever a caller passes for it.
 Operand operand(const uint16_t *p, int64_t batch, int64_t row, int64_t head, int batches, int rows, int heads) {
   return Operand{p, batches > 1 ? batch : 0, rows > 1 ? row : 0, heads > 1 ? head : 0};
@@ -912,11 +916,13 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
                  int kv_heads, float scale, hipStream_t s) {
   constexpr int BM = 128 * NQ;
   const int group = heads / kv_heads;
-  const int64_t blocks = seqs.cu ? (int64_t)seqs.rows * group / BM + seqs.count
-                                 : seqs.count * (((int64_t)seqs.rows * group + BM - 1) / BM);
   VDNH3_HOST_CHECK((int64_t)seqs.rows * group <= INT32_MAX - BM, VDNH3_ERR_INVALID,
                    "causal attention: %d rows of %d heads are too many", seqs.rows, heads);
-  if (int rc = check_grid(blocks * kv_heads, kThreads, "causal attention")) return rc;
+  const int64_t blocks = seqs.cu ? (int64_t)seqs.rows * group / BM + seqs.count
+                                 : seqs.count * (((int64_t)seqs.rows * group + BM - 1) / BM);
+  int rc = check_grid(blocks, kThreads, "causal attention");
+  if (!rc) rc = check_grid(blocks * kv_heads, kThreads, "causal attention");
+  if (rc) return rc;
   hipLaunchKernelGGL((causal_tile_kernel<D, NQ>), dim3((unsigned)(blocks * kv_heads)), dim3(kThreads), 0, s, q, k, v, out, seqs,
                      (int)blocks, kv_heads, group, scale * 1.4426950408889634f);
   return check_launch("causal attention");
@@ -930,7 +936,7 @@ constexpr int kHighGroups128 = 288, kHighGroups64 = 512;
 
 int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int heads,
                   int kv_heads, int head_dim, float scale, hipStream_t s) {
-  const bool high = (int64_t)seqs.rows * (seqs.cu ? 1 : seqs.count) * heads / 256 >=
+  const bool high = (double)seqs.rows * (seqs.cu ? 1 : seqs.count) * heads / 256 >=
                     (head_dim == 128 ? kHighGroups128 : kHighGroups64);
   if (head_dim == 128)
     return high ? launch_tiles<128, 2>(q, k, v, out, seqs, heads, kv_heads, scale, s)
@@ -993,8 +999,8 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
 extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads) {
   using namespace vdnh3;
   if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
-  const int64_t rows = (int64_t)new_tokens * (heads / kv_heads), tiles = (int64_t)batch * ((room + kFewKeys - 1) / kFewKeys);
-  if (tiles > INT32_MAX || rows * batch * kv_heads > INT32_MAX) return 0;
+  const int64_t rows = (int64_t)new_tokens * (heads / kv_heads), tiles = batch * (((int64_t)room + kFewKeys - 1) / kFewKeys);
+  if (room > kMostRoom || tiles > INT32_MAX || rows * batch > INT32_MAX || rows * batch * kv_heads > INT32_MAX) return 0;
   const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
   if (rows > 16) {
     const double groups = (double)((rows + 127) / 128) * batch * kv_heads;
@@ -1027,15 +1033,15 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
   if (rc) return rc;
   VDNH3_HOST_CHECK(lengths && batch > 0 && new_tokens > 0 && room > 0, VDNH3_ERR_INVALID,
                    "causal attention: null lengths, or no sequences, new tokens or room in the cache");
+  VDNH3_HOST_CHECK(room <= kMostRoom, VDNH3_ERR_INVALID, "causal attention: caches of %d rows are too long", room);
   const Sequences seqs{nullptr, lengths, batch, new_tokens, room};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (ranges == 0) return launch_causal(qo, ko, vo, oo, seqs, heads, kv_heads, head_dim, scale, s);
   const int group = heads / kv_heads;
   const int64_t rows = (int64_t)new_tokens * group;
-  VDNH3_HOST_CHECK(ranges > 0 && room <= INT32_MAX - kFewKeys, VDNH3_ERR_INVALID,
-                   "causal attention: the ranges must not be negative, got %d", ranges);
-  VDNH3_HOST_CHECK(rows * batch * kv_heads <= INT32_MAX && (int64_t)batch * (room / kFewKeys + 1) <= INT32_MAX,
-                   VDNH3_ERR_INVALID, "causal attention: %d x %d new tokens or caches of %d rows are too many for ranges",
+  VDNH3_HOST_CHECK(ranges > 0, VDNH3_ERR_INVALID, "causal attention: the ranges must not be negative, got %d", ranges);
+  VDNH3_HOST_CHECK(rows * batch <= INT32_MAX && rows * batch * kv_heads <= INT32_MAX &&
+                       (int64_t)batch * (room / kFewKeys + 1) <= INT32_MAX, VDNH3_ERR_INVALID, "causal attention: %d x %d new tokens or caches of %d rows are too many for ranges",
                    batch, new_tokens, room);
   const size_t need = vdnh3_causal_partial_bytes(new_tokens, heads, head_dim, ranges);
   VDNH3_HOST_CHECK(need == 0 || (partial && reinterpret_cast<uintptr_t>(partial) % 16 == 0 && partial_bytes >= need),

@@ -216,6 +216,13 @@ def launch(what: str, fn, device: torch.device, *args) -> None:
         check(rc, what)
 
 
+def int32_sizes(what: str, *sizes: int) -> None:
+    """Sizes that the library takes as 32-bit numbers (ctypes would cut longer ones without a word)."""
+    for n in sizes:
+        if n >= 2 ** 31:
+            raise ValueError(f"{what}: a size of {n} is too large")
+
+
 def forward_only(what: str, *tensors) -> None:
     """The HIP ops have no backward: in gradient mode an input that requires grad is an error, since the
     result would silently carry no gradient."""

@@ -245,9 +245,9 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
     ``kind`` (``linear.KIND_I8`` / ``KIND_F8``): the row-wise int8 / e4m3 codes and scales of ``rms_norm(t, weight, eps)``,
     as ``quantize_rows`` gives them for ``gemm_w8a8``; ``KIND_BF16``: the norm itself in bf16, and no scale. The sum, the
     norm and the codes are computed in fp32 from the bf16 inputs, each output rounded once: the norm is that of the
-    unrounded sum. The weight is taken in bf16. ``residual=None`` (a model's first layer) norms ``x`` and returns it as ``t``. ``sum_out`` takes ``t``;
-    it may be ``x`` or ``residual``, otherwise it must not overlap them. A row with an infinity or a NaN in its norm gets
-    the scale NaN (``KIND_BF16``: the NaNs that arise).
+    unrounded sum. The weight is taken in bf16. ``residual=None`` (a model's first layer) norms ``x`` and returns it as
+    ``t``. ``sum_out`` takes ``t``; it may be ``x`` or ``residual``, otherwise it must not overlap them. A row with an
+    infinity or a NaN in its norm gets the scale NaN (``KIND_BF16``: the NaNs that arise).
     """
     if x.ndim != 2 or x.dtype != torch.bfloat16:
         raise ValueError("residual_rmsnorm_quantize expects bf16 [rows, hidden]")
@@ -256,12 +256,13 @@ def residual_rmsnorm_quantize(x: torch.Tensor, residual: torch.Tensor | None, we
     if kind not in _NORM_DTYPES:
         raise ValueError(f"unknown kind {kind!r}; expected KIND_BF16, KIND_I8 or KIND_F8")
     rows, width = x.shape
+    _lib.int32_sizes("residual_rmsnorm_quantize", rows, width)
     if weight.numel() != width or width == 0 or width % 8:
         raise ValueError(f"the width must be a positive multiple of 8 and the weight's, got {width} and {weight.numel()}")
     if sum_out is not None and (residual is None or sum_out.shape != x.shape or sum_out.dtype != torch.bfloat16
                                 or not _lib.in_place(sum_out) or (rows > 1 and sum_out.stride(0) < width)):
         raise ValueError("sum_out needs a residual, x's shape, bf16 and 16-byte rows")
-    _lib.forward_only("residual_rmsnorm_quantize", x, residual, weight)
+    _lib.forward_only("residual_rmsnorm_quantize", x, residual, weight, sum_out)
     device = _lib.require_device(x, residual, weight, sum_out)
     if weight.ndim != 1 or weight.dtype != torch.bfloat16:
         weight = weight.reshape(-1).to(torch.bfloat16)

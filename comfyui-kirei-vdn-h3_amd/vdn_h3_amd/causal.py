@@ -42,9 +42,16 @@ def _sequence_bounds(cu_seqlens, rows: int, device) -> torch.Tensor:
         return cu_seqlens.to(torch.int32).to(device)
     if cu_seqlens.device != device:
         raise RuntimeError(f"tensors on different devices: {device} and {cu_seqlens.device}")
-    if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous():
-        return cu_seqlens
-    return cu_seqlens.to(torch.int32).contiguous()
+    return _int32(cu_seqlens, rows)
+
+
+def _int32(counts: torch.Tensor, most: int) -> torch.Tensor:
+    """Counts on the GPU as contiguous int32; wider ones are cut to ``[0, most]`` first, as the kernels cut."""
+    if counts.dtype == torch.int32 and counts.is_contiguous():
+        return counts
+    if counts.dtype == torch.int64:
+        counts = counts.clamp(0, most)
+    return counts.to(torch.int32).contiguous()
 
 
 def _output(out, shape, device):
@@ -73,9 +80,10 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
         raise ValueError("query must be [rows, heads, dim], key and value [rows, kv_heads, dim]; got "
                          f"{tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}")
     _check_heads(query, key, value, "causal_softmax_packed")
-    _lib.forward_only("causal_softmax_packed", query, key, value)
-    device = _lib.require_device(query, key, value, out)
+    _lib.forward_only("causal_softmax_packed", query, key, value, out)
     rows, heads, dim = query.shape
+    _lib.int32_sizes("causal_softmax_packed", rows, heads)
+    device = _lib.require_device(query, key, value, out)
     if dim not in KERNEL_HEAD_DIMS:
         width = padded_head_dim(dim)
         if out is not None and (out.shape != query.shape or out.dtype != torch.bfloat16):
@@ -122,11 +130,12 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     _check_heads(query, key_cache, value_cache, "causal_softmax_cached")
     batch, new, heads, dim = query.shape
     room, kv_heads = key_cache.shape[1], key_cache.shape[2]
+    _lib.int32_sizes("causal_softmax_cached", batch, new, room, heads)
     if lengths.ndim != 1 or lengths.numel() != batch or lengths.dtype not in _INTEGERS:
         raise ValueError(f"lengths must hold {batch} integers, got {tuple(lengths.shape)} {lengths.dtype}")
     if dim not in KERNEL_HEAD_DIMS:
         raise ValueError(f"causal_softmax_cached supports head dims {KERNEL_HEAD_DIMS}, got {dim}")
-    _lib.forward_only("causal_softmax_cached", query, key_cache, value_cache)
+    _lib.forward_only("causal_softmax_cached", query, key_cache, value_cache, out)
     device = _lib.require_device(query, key_cache, value_cache, lengths, out)
     if not (_lib.in_place(key_cache) and _lib.in_place(value_cache)):
         raise ValueError("the caches must be 16-byte aligned with contiguous channels and strides that are multiples of 8 "
@@ -137,8 +146,7 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
         return out
     if room == 0:
         return out.zero_()
-    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
-        lengths = lengths.to(torch.int32).contiguous()
+    lengths = _int32(lengths, room)
     ranges, size = _cut(batch, new, room, heads, kv_heads, dim)
     partial = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.launch("causal_softmax_cached", _lib.lib().vdnh3_causal_attn_cached, device,

@@ -90,9 +90,10 @@ def normalise_qk_axes(q_raw: torch.Tensor, k_raw: torch.Tensor, positions: torch
     if q_raw.dtype != torch.bfloat16 or k_raw.dtype != torch.bfloat16:
         raise TypeError(f"normalise_qk_axes computes in bf16; got {q_raw.dtype}/{k_raw.dtype}")
     _lib.forward_only("normalise_qk_axes", q_raw, k_raw, q_weight, k_weight, positions)
-    device = _lib.require_device(q_raw, k_raw, q_weight, k_weight, positions)
     seq, heads, dim = q_raw.shape
     kv_heads = k_raw.shape[1]
+    _lib.int32_sizes("normalise_qk_axes", seq, heads, kv_heads)
+    device = _lib.require_device(q_raw, k_raw, q_weight, k_weight, positions)
     code = _POSITION_CODES.get(positions.dtype)
     if code is None:
         raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")

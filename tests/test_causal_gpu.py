@@ -241,6 +241,42 @@ def test_cached_infinities_behind_a_new_token(device):
         assert got[:, -2:].isnan().all()
 
 
+@pytest.mark.parametrize("new", [1, 4, 40, 200])
+def test_infinities_and_largest_numbers_that_a_row_sees(device, new):
+    """An infinity among the values gives an infinity, values near the largest number sum to numbers; the other channels and
+    the tokens in front do not change. New tokens over caches of one part and of several, and whole prompts."""
+    from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
+
+    for room, dim in ((60, 128), (900, 64), (900, 128)):
+        new = min(new, room)
+        print(f"case infinities seen {new} of {room} x {dim}", flush=True)
+        q, k, v = _qkv(room, 4, 2, dim, 16)
+        big = (torch.rand(room, generator=torch.Generator().manual_seed(17)) * 0.1 + 0.9) * 3e38
+        v[room // 2, :, 3], v[-1, :, 5] = torch.inf, -torch.inf
+        v[:, :, 7], v[:, :, 8] = big[:, None].to(BF), -big[:, None].to(BF)
+        whole = po.packed(q, k, v, [0, room], dim ** -0.5)
+        n = torch.tensor([room], dtype=torch.int32, device=device)
+        some = causal_softmax_cached(q[None, -new:].to(device), k[None].to(device), v[None].to(device), n, dim ** -0.5)
+        full = causal_softmax_packed(q.to(device), k.to(device), v.to(device), [0, room], dim ** -0.5)
+        for got, want in ((some[0], [t[-new:] for t in whole]), (full, whole)):
+            odd = want[0].isinf()
+            assert odd.any() and torch.equal(got.cpu()[odd], want[0][odd].to(BF))
+            rest = [want[0].masked_fill(odd, 0), want[1].masked_fill(odd, 0), want[2]]
+            assert got.cpu()[~odd].isfinite().all()
+            _check(got.cpu().masked_fill(odd, 0), rest, dim)
+
+
+def test_counts_past_32_bits_are_cut(device):
+    from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
+
+    q, k, v = _qkv(90, 4, 2, 64, 18)
+    far = torch.tensor([2 ** 32 + 5, -2 ** 32 + 5], dtype=torch.int64, device=device)
+    got = causal_softmax_cached(q[:2, None].to(device), *(t.expand(2, -1, -1, -1).to(device) for t in (k, v)), far, 0.125)
+    _check(got, po.cached(q[:2, None], *(t.expand(2, -1, -1, -1) for t in (k, v)), [90, 0], 0.125), 64)
+    got = causal_softmax_packed(q.to(device), k.to(device), v.to(device), far.flip(0), 0.125)
+    _check(got, po.packed(q, k, v, [0, 90], 0.125), 64)
+
+
 # row 1,199 starts at element 2.5e9; rows as far apart as they may be
 @pytest.mark.parametrize("new,room,row", [(1, 1200, 1 << 21), (40, 1200, 1 << 21), (1, 300, 1 << 23), (70, 300, 1 << 23)])
 def test_offsets_past_32_bits(device, new, room, row):

@@ -29,6 +29,10 @@ def test_norm_refusals(built_lib):
         op(x, x, w, 1e-6, linear.KIND_I8)
     with pytest.raises(RuntimeError, match="residual_rmsnorm_quantize is forward-only"):
         op(x, x.clone().requires_grad_(), w, 1e-6, linear.KIND_I8)
+    with pytest.raises(RuntimeError, match="residual_rmsnorm_quantize is forward-only"):
+        op(x, x, w, 1e-6, linear.KIND_I8, sum_out=_z(4, 64).requires_grad_())
+    with pytest.raises(ValueError, match="too large"):
+        op(x[:1].expand(2 ** 31, 64), None, w, 1e-6, 1)
 
 
 def test_rotary_refusals(built_lib):
@@ -51,6 +55,8 @@ def test_rotary_refusals(built_lib):
             bad()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         op(q, k, pos, axes)
+    with pytest.raises(ValueError, match="too large"):
+        op(q[:1].expand(2 ** 32 + 5, 4, 64), k[:1].expand(2 ** 32 + 5, 2, 64), pos[:, :1].expand(3, 2 ** 32 + 5), axes)
     with pytest.raises(RuntimeError, match="normalise_qk_axes is forward-only"):
         op(q.requires_grad_(), k, pos, axes)
 
@@ -70,6 +76,11 @@ def test_attention_refusals(built_lib):
         packed(q, k, k, [0, 6], 0.1)
     with pytest.raises(RuntimeError, match="causal_softmax_packed is forward-only"):
         packed(q.clone().requires_grad_(), k, k, [0, 6], 0.1)
+    with pytest.raises(RuntimeError, match="causal_softmax_packed is forward-only"):
+        packed(q, k, k, [0, 6], 0.1, out=_z(6, 4, 64).requires_grad_())
+    far, near = q[:1].expand(2 ** 32 + 6, 4, 64), k[:1].expand(2 ** 32 + 6, 2, 64)
+    with pytest.raises(ValueError, match="too large"):
+        packed(far, near, near, [0, 6], 0.1)
     q, k, n = _z(2, 1, 4, 64), _z(2, 9, 2, 64), torch.zeros(2, dtype=torch.int32)
     for bad in [lambda: cached(q, k[:1], k[:1], n, 0.1), lambda: cached(q, k, _z(2, 8, 2, 64), n, 0.1),
                 lambda: cached(q, k, k, n[:1], 0.1), lambda: cached(q, k, k, n.float(), 0.1),
@@ -80,6 +91,9 @@ def test_attention_refusals(built_lib):
         cached(q, k, k, n, 0.1)
     with pytest.raises(RuntimeError, match="causal_softmax_cached is forward-only"):
         cached(q, k.clone().requires_grad_(), k, n, 0.1)
+    far = k[:, :1].expand(2, 2 ** 32 + 9, 2, 64)
+    with pytest.raises(ValueError, match="too large"):
+        cached(q, far, far, n, 0.1)
 
 
 def test_bounds_that_the_host_holds_are_checked():
@@ -147,7 +161,10 @@ def test_c_entry_points_refuse_before_any_launch(built_lib):
     for bad in [dict(q=None), dict(k=p + 2), dict(k_row=(1 << 23) + 8), dict(k_row=-8), dict(lengths=None), dict(batch=0),
                 dict(new=0), dict(room=0), dict(h=3), dict(dim=96), dict(scale=float("inf")), dict(ranges=-1),
                 dict(ranges=2), dict(ranges=2, part=p, size=8), dict(ranges=2, part=p + 8, size=1 << 20),
-                dict(ranges=1, batch=1 << 20, new=1 << 12), dict(ranges=1, batch=1 << 16, room=1 << 25)]:
+                dict(room=(1 << 31) - 1), dict(ranges=2, room=(1 << 31) - 100),
+                dict(batch=1 << 30, new=1 << 20, h=1 << 10, kh=1 << 10),
+                dict(ranges=1, batch=1 << 30, new=1 << 30, h=1 << 10, kh=1 << 10), dict(ranges=1, batch=1 << 20, new=1 << 12),
+                dict(ranges=1, batch=1 << 16, room=1 << 25)]:
         assert cached(**bad) == _lib.VDNH3_ERR_INVALID, bad
 
 
@@ -161,7 +178,8 @@ def test_ranges_of_a_call(built_lib):
     assert lib.vdnh3_causal_cached_ranges(64, 1, 8192, 40, 8) == 32
     assert lib.vdnh3_causal_cached_ranges(16, 64, 2048, 40, 8) == 0
     assert lib.vdnh3_causal_cached_ranges(1, 32, 40960, 40, 8) > 1
-    for bad in [(0, 1, 1, 1, 1), (1, 0, 1, 1, 1), (1, 1, 0, 1, 1), (1, 1, 1, 3, 2), (1, 1, 1, 0, 1), (1, 1, 1, 1, 0)]:
+    for bad in [(0, 1, 1, 1, 1), (1, 0, 1, 1, 1), (1, 1, 0, 1, 1), (1, 1, 1, 3, 2), (1, 1, 1, 0, 1), (1, 1, 1, 1, 0),
+                (1, 1, 2 ** 31 - 1, 4, 4), (2 ** 31 - 1, 2 ** 31 - 1, 64, 2 ** 31 - 1, 1)]:
         assert lib.vdnh3_causal_cached_ranges(*bad) == 0
     assert lib.vdnh3_causal_partial_bytes(3, 10, 64, 1) == 0
     assert lib.vdnh3_causal_partial_bytes(3, 10, 64, 4) == 4 * 2 * 30 * 66 * 4
