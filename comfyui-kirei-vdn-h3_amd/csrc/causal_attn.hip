@@ -990,27 +990,32 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
                        static_cast<hipStream_t>(stream));
 }
 
-// The ranges of a call, or 0 for the kernel above: what its caches take at full length either way, in us. The prompt kernel
-// goes through all keys of a block of 128 rows in one workgroup (1.3 us per 96 keys), which is little at a time where there
-// are few blocks. Here 256 workgroups are at work always, but on 32 rows each (1.9 us per 4 tiles of 32 keys). 40 / 8 heads
-// x 128, measured: 40,688 keys and 32 new tokens 139 us against 560, 128 tokens 399 against 563, 256 tokens 759 against
-// 566; 16 requests of 2,000 keys and 16 tokens 93 against 38. With up to 16 rows it is the loads that count, and this
-// kernel always.
+// The ranges of a call, or 0 for the kernel above, by what its caches take at full length, in us. Ranges: rounds of 256
+// workgroups; each takes 7.4 to start and again for every sequence that it crosses into, and 2.1 for each 4 tiles of 32 keys.
+// One round is the least where it fills the CUs, several where they leave fewer idle. The kernel above
+// goes through all keys of a block of 128 rows in one workgroup, 1.3 per 96 keys. With up to 16 rows it is the loads that
+// count, and this kernel always. Measured, 128 channels: one token of 40 / 40 heads over 8,192 keys in 6 ranges 40, in 25 55; 32
+// tokens of 40 / 8 heads over 8,192 keys 6: 35, 12: 43, 25: 57, 0: 118; over 40,688 keys 6: 117, 25: 134, 0: 559; 128 tokens 3:
+// 415, 8: 400, 0: 564; 200 tokens 2: 613, 0: 564; 16 requests of 2,048 keys and 16 tokens 8: 93, 0: 38.
 extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads) {
   using namespace vdnh3;
   if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
   const int64_t rows = (int64_t)new_tokens * (heads / kv_heads), tiles = batch * (((int64_t)room + kFewKeys - 1) / kFewKeys);
   if (room > kMostRoom || tiles > INT32_MAX || rows * batch > INT32_MAX || rows * batch * kv_heads > INT32_MAX) return 0;
+  if (rows <= 16 && tiles <= kFewOne) return 1;
   const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
+  int64_t ranges = 1;
+  double least = INFINITY;
+  for (int rounds = 1; rounds <= 8; ++rounds) {
+    const int64_t r = std::max<int64_t>(std::min<int64_t>(256 * rounds / blocks, tiles / kFewLeast), 1);
+    const double us = 5. + (double)((blocks * r + 255) / 256) * (7.4 * (1. + (double)batch / r) + 2.1 / 4 * ((tiles + r - 1) / r));
+    if (us < least) least = us, ranges = r;
+  }
   if (rows > 16) {
     const double groups = (double)((rows + 127) / 128) * batch * kv_heads;
-    const double whole = 8. + 1.3 * std::ceil(groups / 256) * ((room + kBN - 1) / kBN);
-    if (whole < 14. + 1.9 * (double)blocks * tiles / (256 * 4)) return 0;
+    if (8. + 1.3 * std::ceil(groups / 256) * (((int64_t)room + kBN - 1) / kBN) < least) return 0;
   }
-  if (tiles <= kFewOne) return 1;
-  // one round of workgroups, or several where one would leave CUs idle
-  const int64_t ranges = blocks <= 24 ? 256 / blocks : (1024 + blocks - 1) / blocks;
-  return (int)std::max<int64_t>(std::min<int64_t>(ranges, tiles / kFewLeast), 1);
+  return tiles <= kFewOne ? 1 : (int)ranges;
 }
 
 extern "C" size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges) {
