@@ -499,11 +499,10 @@ struct Parts {
   }
 };
 
+__device__ __forceinline__ int keys_of(const Sequences &seqs, int b) { return min(max(seqs.lengths[b], 0), seqs.room); }
 // The tiles of a sequence; one without keys has one, which writes its rows.
-__device__ __forceinline__ int tiles_of(const Sequences &seqs, int b) {
-  const int keys = min(max(seqs.lengths[b], 0), seqs.room);
-  return max(1, (keys + kFewKeys - 1) / kFewKeys);
-}
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kFewKeys - 1) / kFewKeys); }
+__device__ __forceinline__ int tiles_of(const Sequences &seqs, int b) { return tiles_of(keys_of(seqs, b)); }
 
 // How the tiles of all sequences are cut: `each` per range, the first `more` ranges one more. Each of the workgroup's
 // threads counts the tiles of `per` sequences; before[i] is what the threads in front of i counted.
@@ -546,39 +545,23 @@ __device__ __forceinline__ Cut make_cut(const Sequences &seqs, int ranges, int (
   return Cut{total, per, n, each, total - n * each, before};
 }
 
-// O / l of one row, two (one) channels per lane. A value that is not finite gives a NaN where it meets a probability of 0: that
-// of a key behind the row, of a last key that stands in for one, or what the rounding of its own probability left. Values
-// near fp32's largest can sum up past it. A row with such a result is computed once more, from the keys that it sees.
+// A row of the result by `attend_row`. A value that is not finite gives a NaN where it meets a probability of 0: that of a key
+// behind the row, of a last key that stands in for one, or what the rounding of its own probability left. Values near
+// fp32's largest can sum up past it. Rows with such a result are computed once more, from the keys that they see.
 template <int D>
-__device__ __forceinline__ void finish_row(const Operand &q, const Operand &k, const Operand &v, const Operand &out,
-                                           const Sequence &s, int b, int kvh, int group, int row, const float (&o)[D / 64],
-                                           float l, float scale_log2, int lane) {
-  constexpr int C = D / 64;
-  const int token = row / group, head = kvh * group + (row - token * group), keys = min(s.keys - s.n + token + 1, s.keys);
-  uint16_t *op = const_cast<uint16_t *>(out.at(b, s.q0 + token, head));
-  float y[C];
-  bool fine = true;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    y[c] = keys > 0 ? o[c] / l : 0.f;
-    fine = fine && fabsf(y[c]) < INFINITY;
-  }
-  if (__any(!fine)) {
-    attend_row<D>(q.at(b, s.q0 + token, head), k.at(b, s.k0, kvh), k.row, v.at(b, s.k0, kvh), v.row, keys, scale_log2, op,
-                  lane);
-    return;
-  }
-  if constexpr (C == 2) *reinterpret_cast<uint32_t *>(op + 2 * lane) = pack_bf2(y[0], y[1]);
-  else op[lane] = f2bf(y[0]);
+__device__ __forceinline__ void again_row(const Operand &q, const Operand &k, const Operand &v, const Operand &out,
+                                          const Sequence &s, int b, int kvh, int group, int row, float scale_log2, int lane) {
+  const int token = row / group, head = kvh * group + (row - token * group);
+  attend_row<D>(q.at(b, s.q0 + token, head), k.at(b, s.k0, kvh), k.row, v.at(b, s.k0, kvh), v.row,
+                min(s.keys - s.n + token + 1, s.keys), scale_log2, const_cast<uint16_t *>(out.at(b, s.q0 + token, head)), lane);
 }
 
 template <int D, int NQ>
 __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Operand k, Operand v, Operand out, Sequences seqs,
                                                                  int kv_heads, int group, int row_blocks, float scale_log2,
                                                                  Parts parts) {
-  constexpr int KC = D / 8, NS = D / 32, NO = D / 16, C = D / 64, ROWS = 16 * NQ, W = kFewThreads / 64;
+  constexpr int KC = D / 8, NS = D / 32, NO = D / 16, ROWS = 16 * NQ, W = kFewThreads / 64;
   constexpr int TILE = kFewKeys * D;  // elements
-  static_assert(NQ <= 2, "one exchange reduces the maxima of two queries");
   static_assert(ROWS * D * 2 <= kFewRing * 2 * TILE, "a wavefront's sums fit its tiles' place");
   __shared__ __attribute__((aligned(16))) uint16_t tiles[W][kFewRing][2][TILE];
   __shared__ float2 stats[W][ROWS];
@@ -607,13 +590,15 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
     b = lo * cut.per;
   }
   int front = before[b / cut.per];
-  int here = tiles_of(seqs, b);
+  int keys = keys_of(seqs, b), here = tiles_of(keys);
   while (front + here <= u) {
     front += here;
-    here = tiles_of(seqs, ++b);
+    keys = keys_of(seqs, ++b);
+    here = tiles_of(keys);
   }
   for (bool first_part = true; u < u1; first_part = false) {
-    const Sequence s = sequence_at(seqs, b);
+    const Sequence s{0, seqs.rows, 0, keys};
+    const int next_keys = keys_of(seqs, min(b + 1, seqs.count - 1));  // on its way while this one is worked on
     const int behind = s.keys - s.n;
     const int k0 = (u - front) * kFewKeys;
     const int n_units = min(u1, front + here) - u;
@@ -670,15 +655,21 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
     const u32x4_t ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // eight bf16 1.0
 
     if (wave < n_tiles) load_tile(wave, 0);
+    if (wave + W < n_tiles) load_tile(wave + W, 1);
+    // The queries arrive here: the compiler counts its own loads only, so that its wait for them, in the loop, would be one
+    // for every tile on its way.
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        u32x4_t x = __builtin_bit_cast(u32x4_t, qf[n][st]);
+        asm volatile("" : "+v"(x));
+        qf[n][st] = as_bf16x8(x);
+      }
     int ring = 0;
     for (int t = wave; t < n_tiles; t += W, ring ^= 1) {
-      // the reads of the slot that is loaded now ended with the products of the last tile
-      if (t + W < n_tiles) {
-        load_tile(t + W, ring ^ 1);
-        wait_vm_lds<2 * LOADS>();
-      } else {
-        wait_vm_lds<0>();
-      }
+      if (t + W < n_tiles) wait_vm_lds<2 * LOADS>();
+      else wait_vm_lds<0>();
       asm volatile("" ::: "memory");
       const uint16_t *ktile = tiles[wave][ring][0], *vtile = tiles[wave][ring][1];
       f32x4_t sacc[2][NQ];
@@ -714,7 +705,8 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
         const f32x4_t x = sacc[0][n], y = sacc[1][n];
         mt[n] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
       }
-      group_max(mt[0], mt[NQ - 1]);
+#pragma unroll
+      for (int n = 0; n < NQ; n += 2) group_max(mt[n], mt[min(n + 1, NQ - 1)]);
       bool grow = false;
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
@@ -757,7 +749,8 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
           oacc[m][n] = mfma_bf16_16x16x32(a, as_bf16x8(pl[n]), oacc[m][n]);
         }
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this tile is read: the next trip loads over it
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this tile is read: the one after the next comes over it
+      if (t + 2 * W < n_tiles) load_tile(t + 2 * W, ring);
     }
 
     // Each wavefront's sums into its tiles' place: row 16 n + l16, 16-byte chunk 4 m + g at chunk ^ (row % 16).
@@ -771,53 +764,70 @@ __global__ __launch_bounds__(kFewThreads) void causal_few_kernel(Operand q, Oper
       if (g == 0) stats[wave][r] = make_float2(m_run[n], l_run[n][0]);
     }
     __syncthreads();
-    for (int r = wave; r < r1 - r0; r += W) {
-      float top = kNoMax;
-#pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w][r].x);
-      float o[C] = {}, l = 0.f;
+    constexpr int LANES = D / 4, AT_ONCE = kFewThreads / LANES;  // of a row, four channels each; rows at once
+    for (int first_row = 0; first_row < r1 - r0; first_row += AT_ONCE) {
+      const int r = min(first_row + tid / LANES, r1 - r0 - 1), c = tid % LANES;
+      const bool live = first_row + tid / LANES < r1 - r0;
+      float top = kNoMax, l = 0.f;
+      float2 ml[W];
+      f32x4_t o = {};
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float2 ml = stats[w][r];
-        const float by = __builtin_amdgcn_exp2f(ml.x - top);
-        const float *from = reinterpret_cast<const float *>(&tiles[w][0][0][0]) + r * D;
-        l = fmaf(by, ml.y, l);
+        ml[w] = stats[w][r];
+        top = fmaxf(top, ml[w].x);
+      }
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const int d = C * lane + c;
-          o[c] = fmaf(by, from[4 * ((d >> 2) ^ (r & 15)) + (d & 3)], o[c]);
-        }
+      for (int w = 0; w < W; ++w) {
+        const float by = __builtin_amdgcn_exp2f(ml[w].x - top);
+        l = fmaf(by, ml[w].y, l);
+        o += by * *reinterpret_cast<const f32x4_t *>(reinterpret_cast<const float *>(&tiles[w][0][0][0]) + r * D + 4 * (c ^ (r & 15)));
       }
       if (n_units == here) {
-        finish_row<D>(q, k, v, out, s, b, kvh, group, r0 + r, o, l, scale_log2, lane);
-      } else {
+        const int token = (r0 + r) / group, head = kvh * group + (r0 + r - token * group);
+        const float inv = behind + token >= 0 && s.keys > 0 ? 1.f / l : 0.f;
+        o *= inv;
+        const bool odd = live && !(fmaf(o[0], 0.f, fmaf(o[1], 0.f, fmaf(o[2], 0.f, o[3] * 0.f))) == 0.f);
+        if (live)
+          *reinterpret_cast<uint2 *>(const_cast<uint16_t *>(out.at(b, s.q0 + token, head)) + 4 * c) =
+              make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+        const uint64_t odds = __ballot(odd);
+        if (odds) {
+          wait_vm_lds<0>();  // the stores above come first
+          for (int i = 0; i < 64 / LANES; ++i)
+            if ((odds >> (i * LANES)) & ((1ull << LANES) - 1))
+              again_row<D>(q, k, v, out, s, b, kvh, group, r0 + first_row + wave * (64 / LANES) + i, scale_log2, lane);
+        }
+      } else if (live) {
         const int64_t to = parts.at(kvh, range, first_part ? 0 : 1, rows) + r0 + r;
-#pragma unroll
-        for (int c = 0; c < C; ++c) parts.o[to * D + C * lane + c] = o[c];
-        if (lane == 0) parts.ml[to] = make_float2(top, l);
+        *reinterpret_cast<f32x4_t *>(parts.o + to * D + 4 * c) = o;
+        if (c == 0) parts.ml[to] = make_float2(top, l);
       }
     }
     u += n_units;
     if (u < u1) {
       front += here;
-      here = tiles_of(seqs, ++b);
+      ++b;
+      keys = next_keys;
+      here = tiles_of(keys);
       __syncthreads();  // the sums are read: the next sequence's tiles load over them
     }
   }
 }
 
-// One workgroup per row of a sequence that several ranges share: its wavefronts take the parts in turn, eight at once (their
-// loads do not wait for one another's maxima), and are merged in LDS.
+// The rows of sequences that several ranges share, `per` rows of one sequence and key / value head per workgroup: of few
+// parts a row per wavefront, of many all wavefronts on one row, merged in LDS. A wavefront has eight parts on their way at
+// once (its loads do not wait for one another's maxima).
 template <int D>
 __global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, Operand k, Operand v, Operand out,
-                                                                     Sequences seqs, int kv_heads, int group,
+                                                                     Sequences seqs, int kv_heads, int group, int per,
                                                                      float scale_log2, Parts parts) {
   constexpr int C = D / 64, W = kFewThreads / 64, AT_ONCE = 8;
   __shared__ float sums[W][D];
   __shared__ float2 stats[W];
   __shared__ int before[kFewThreads];
-  const int rows = seqs.rows * group;
-  const int row = (int)blockIdx.x % rows, bh = (int)blockIdx.x / rows, b = bh / kv_heads, kvh = bh - b * kv_heads;
+  const int rows = seqs.rows * group, row_blocks = (rows + per - 1) / per;
+  const int bh = (int)blockIdx.x / row_blocks, row0 = ((int)blockIdx.x - bh * row_blocks) * per, b = bh / kv_heads;
+  const int kvh = bh - b * kv_heads, row1 = min(row0 + per, rows);
   const Cut cut = make_cut(seqs, parts.ranges, before);
   const int u = cut.in_front(seqs, b);
   const int first = cut.range_of(u), past = cut.range_of(u + tiles_of(seqs, b) - 1) + 1;
@@ -825,55 +835,91 @@ __global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // a range's part of the sequence is its first one, but in a range that began in an earlier sequence
   const int early = cut.start(first) < u ? first : -1;
-  float o[C] = {}, l = 0.f, m = kNoMax;
-  for (int i0 = first + wave; i0 < past; i0 += W * AT_ONCE) {
-    float2 ml[AT_ONCE];
-    float x[AT_ONCE][C];
+  const Sequence s = sequence_at(seqs, b);
+  // parts begin, begin + step, ... of a row: their sum, weight and max
+  auto gather = [&](int row, int begin, int step, float (&o)[C], float &l, float &m) __device__ {
+    m = kNoMax;
+    l = 0.f;
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      const int i = min(i0 + W * j, past - 1);
-      const int64_t from = parts.at(kvh, i, i == early, rows) + row;
-      ml[j] = parts.ml[from];
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
+    for (int i0 = begin; i0 < past; i0 += step * AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float x[AT_ONCE][C];
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[j][c] = parts.o[from * D + C * lane + c];
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int i = min(i0 + step * j, past - 1);
+        const int64_t from = parts.at(kvh, i, i == early, rows) + row;
+        ml[j] = parts.ml[from];
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[j][c] = parts.o[from * D + C * lane + c];
+      }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j)
+        if (i0 + step * j < past) top = fmaxf(top, ml[j].x);
+      const float by = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= by;
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] *= by;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        if (i0 + step * j >= past) break;
+        const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+        l = fmaf(f, ml[j].y, l);
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = fmaf(f, x[j][c], o[c]);
+      }
     }
-    float top = m;
+  };
+  auto finish = [&](int row, float (&o)[C], float l) __device__ {
+    const int token = row / group, head = kvh * group + (row - token * group);
+    const float inv = s.keys - s.n + token >= 0 ? 1.f / l : 0.f;
+    float odd = 0.f;
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j)
-      if (i0 + W * j < past) top = fmaxf(top, ml[j].x);
-    const float by = __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    l *= by;
-#pragma unroll
-    for (int c = 0; c < C; ++c) o[c] *= by;
-#pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      if (i0 + W * j >= past) break;
-      const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
-      l = fmaf(f, ml[j].y, l);
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(f, x[j][c], o[c]);
+    for (int c = 0; c < C; ++c) {
+      o[c] *= inv;
+      odd = fmaf(o[c], 0.f, odd);
     }
+    if (__any(!(odd == 0.f))) {
+      again_row<D>(q, k, v, out, s, b, kvh, group, row, scale_log2, lane);
+      return;
+    }
+    uint16_t *op = const_cast<uint16_t *>(out.at(b, s.q0 + token, head));
+    if constexpr (C == 2) *reinterpret_cast<uint32_t *>(op + 2 * lane) = pack_bf2(o[0], o[1]);
+    else op[lane] = f2bf(o[0]);
+  };
+  float o[C], l, m;
+  if (past - first <= AT_ONCE && per >= W) {
+    for (int row = row0 + wave; row < row1; row += W) {
+      gather(row, first, 1, o, l, m);
+      finish(row, o, l);
+    }
+    return;
   }
+  for (int row = row0; row < row1; ++row) {
+    gather(row, first + wave, W, o, l, m);
+    if (row > row0) __syncthreads();  // the last row's sums are read
 #pragma unroll
-  for (int c = 0; c < C; ++c) sums[wave][C * lane + c] = o[c];
-  if (lane == 0) stats[wave] = make_float2(m, l);
-  __syncthreads();
-  if (wave) return;
-  float top = kNoMax;
+    for (int c = 0; c < C; ++c) sums[wave][C * lane + c] = o[c];
+    if (lane == 0) stats[wave] = make_float2(m, l);
+    __syncthreads();
+    if (wave) continue;
+    float top = kNoMax;
 #pragma unroll
-  for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w].x);
-  l = 0.f;
+    for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w].x);
+    l = 0.f;
 #pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = 0.f;
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const float by = __builtin_amdgcn_exp2f(stats[w].x - top);
-    l = fmaf(by, stats[w].y, l);
+    for (int w = 0; w < W; ++w) {
+      const float by = __builtin_amdgcn_exp2f(stats[w].x - top);
+      l = fmaf(by, stats[w].y, l);
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = fmaf(by, sums[w][C * lane + c], o[c]);
+      for (int c = 0; c < C; ++c) o[c] = fmaf(by, sums[w][C * lane + c], o[c]);
+    }
+    finish(row, o, l);
   }
-  finish_row<D>(q, k, v, out, sequence_at(seqs, b), b, kvh, group, row, o, l, scale_log2, lane);
 }
 
 // Rows of a cache: keys are counted in 32 bits, up to the end of a tile behind the last.
@@ -945,7 +991,11 @@ int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Op
               : launch_tiles<64, 1>(q, k, v, out, seqs, heads, kv_heads, scale, s);
 }
 
-int few_block(int64_t rows) { return rows <= 16 ? 16 : 32; }
+// Rows of a workgroup: equal blocks of up to 48, in 16s.
+int few_block(int64_t rows) {
+  const int64_t blocks = (rows + 47) / 48;
+  return (int)((rows + 16 * blocks - 1) / (16 * blocks)) * 16;
+}
 
 template <int D, int NQ>
 int launch_few(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int kv_heads,
@@ -953,23 +1003,29 @@ int launch_few(const Operand &q, const Operand &k, const Operand &v, const Opera
   const int rows = seqs.rows * group, row_blocks = (rows + 16 * NQ - 1) / (16 * NQ);
   const int64_t blocks = (int64_t)kv_heads * row_blocks * parts.ranges;
   int rc = check_grid(blocks, kFewThreads, "causal attention over caches");
-  if (!rc) rc = check_grid((int64_t)seqs.count * kv_heads * rows, kFewThreads, "causal attention over caches");
+  // a row per workgroup up to four workgroups a CU, then fours of rows: every workgroup has the cut to make first
+  const int64_t all = (int64_t)seqs.count * kv_heads * rows;
+  const int per = all <= 1024 ? 1 : (int)std::min<int64_t>((all + 4095) / 4096 * 4, rows);
+  const int64_t combines = (int64_t)seqs.count * kv_heads * ((rows + per - 1) / per);
+  if (!rc) rc = check_grid(combines, kFewThreads, "causal attention over caches");
   if (rc) return rc;
   hipLaunchKernelGGL((causal_few_kernel<D, NQ>), dim3((unsigned)blocks), dim3(kFewThreads), 0, s, q, k, v, out, seqs, kv_heads,
                      group, row_blocks, scale_log2, parts);
   rc = check_launch("causal attention over caches");
   if (rc || parts.ranges == 1) return rc;
-  hipLaunchKernelGGL(causal_combine_kernel<D>, dim3((unsigned)(seqs.count * kv_heads * rows)), dim3(kFewThreads), 0, s, q, k,
-                     v, out, seqs, kv_heads, group, scale_log2, parts);
+  hipLaunchKernelGGL(causal_combine_kernel<D>, dim3((unsigned)combines), dim3(kFewThreads), 0, s, q, k, v, out, seqs,
+                     kv_heads, group, per, scale_log2, parts);
   return check_launch("causal attention's ranges");
 }
 
 template <int D>
 int launch_few_rows(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs,
                     int kv_heads, int group, float scale_log2, const Parts &parts, hipStream_t s) {
-  if (few_block((int64_t)seqs.rows * group) == 16)
-    return launch_few<D, 1>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
-  return launch_few<D, 2>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
+  switch (few_block((int64_t)seqs.rows * group)) {
+    case 16: return launch_few<D, 1>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
+    case 32: return launch_few<D, 2>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
+    default: return launch_few<D, 3>(q, k, v, out, seqs, kv_heads, group, scale_log2, parts, s);
+  }
 }
 
 }  // namespace
@@ -1006,9 +1062,11 @@ extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, i
   const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
   int64_t ranges = 1;
   double least = INFINITY;
-  for (int rounds = 1; rounds <= 8; ++rounds) {
-    const int64_t r = std::max<int64_t>(std::min<int64_t>(256 * rounds / blocks, tiles / kFewLeast), 1);
-    const double us = 5. + (double)((blocks * r + 255) / 256) * (7.4 * (1. + (double)batch / r) + 2.1 / 4 * ((tiles + r - 1) / r));
+  const double step = few_block(rows) == 16 ? 1.1 : few_block(rows) == 32 ? 2.0 : 2.3;
+  for (int quarters = 1; quarters <= 32; ++quarters) {
+    const int64_t r = std::max<int64_t>(std::min<int64_t>(64 * quarters / blocks, tiles / kFewLeast), 1);
+    const int64_t rounds = (blocks * r + 255) / 256, steps = (tiles + 4 * r - 1) / (4 * r);
+    const double us = 5. + 0.07 * r / batch + (double)rounds * (7.4 * (1. + (double)batch / r) + step * steps);
     if (us < least) least = us, ranges = r;
   }
   if (rows > 16) {
