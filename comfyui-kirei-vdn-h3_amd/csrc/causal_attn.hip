@@ -484,9 +484,6 @@ constexpr int kFewRing = 2;
 // Tiles of a range, at least: one per wavefront (one request of 1,000 keys x 40 / 8 heads: 16 ranges 11.1 us, 8 11.3, 4
 // 12.2).
 constexpr int kFewLeast = 4;
-// Tiles of all caches up to which one range takes them and no second launch is needed (600 keys 11.1 us against 11.2 to
-// 12.9).
-constexpr int kFewOne = 18;
 constexpr int kFewThreads = 256;  // of both kernels
 
 // Unnormalised results of the ranges' ends: [kv head][range][end][row] of D floats, then the same of (max, sum).
@@ -1046,34 +1043,42 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
                        static_cast<hipStream_t>(stream));
 }
 
-// The ranges of a call, or 0 for the kernel above, by what its caches take at full length, in us. Ranges: rounds of 256
-// workgroups; each takes 7.4 to start and again for every sequence that it crosses into, and 2.1 for each 4 tiles of 32 keys.
-// One round is the least where it fills the CUs, several where they leave fewer idle. The kernel above
-// goes through all keys of a block of 128 rows in one workgroup, 1.3 per 96 keys. With up to 16 rows it is the loads that
-// count, and this kernel always. Measured, 128 channels: one token of 40 / 40 heads over 8,192 keys in 6 ranges 40, in 25 55; 32
-// tokens of 40 / 8 heads over 8,192 keys 6: 35, 12: 43, 25: 57, 0: 118; over 40,688 keys 6: 117, 25: 134, 0: 559; 128 tokens 3:
-// 415, 8: 400, 0: 564; 200 tokens 2: 613, 0: 564; 16 requests of 2,048 keys and 16 tokens 8: 93, 0: 38.
-extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads) {
+// The ranges of a call, or 0 for the kernel above: whichever an estimate says takes the least time, in us. The lengths are not
+// known here: caches are taken to be 64% full, the longest whole.
+//   0      : 4 + the longer of the bytes at 7.5 TB/s (partly out of the last-level cache) and 0.9 (64 channels: 0.75) per 96
+//            keys of the longest cache and round of workgroups (128 rows of one sequence and key / value head each)
+//   ranges : 10 (of more than 16 rows a workgroup: 13), 5.3 less for a single range, which needs no combination, + 0.08 per
+//            range of a sequence + 4.2 per further round of workgroups + the longer of the bytes at 8 TB/s and, for every round,
+//            1.45 (48 rows: 1.85) per 4 tiles of 32 keys and 4.3 (9.6) for every sequence that a range crosses into; those
+//            0.84 times with 64 channels
+// The constants are a fit to 4,477 calls: 1 to 64 requests, 64 to 40,960 rows of cache, 1 to 64 new tokens, 7 layouts of heads, up
+// to 7 ways each. The choice then takes 0.9% longer than the best of them in the mean, 4.5% at the 95th percentile; ranges
+// for all calls up to 16 rows, one round of them, and a coarser estimate for more took 19% and 2.3 times. E.g. one token of
+// 40 / 8 heads x 128 over 40,688 keys: 32 ranges 41, 0: 452; over 300 keys of 2 requests 5: 12, 0: 9; 64 requests of 512 keys and 3
+// tokens 32: 42, 0: 33; of 8,192 keys at most 32: 190, 0: 215.
+extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads, int head_dim) {
   using namespace vdnh3;
-  if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads) return 0;
+  if (batch <= 0 || new_tokens <= 0 || room <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
   const int64_t rows = (int64_t)new_tokens * (heads / kv_heads), tiles = batch * (((int64_t)room + kFewKeys - 1) / kFewKeys);
   if (room > kMostRoom || tiles > INT32_MAX || rows * batch > INT32_MAX || rows * batch * kv_heads > INT32_MAX) return 0;
-  if (rows <= 16 && tiles <= kFewOne) return 1;
-  const int64_t blocks = (rows + few_block(rows) - 1) / few_block(rows) * kv_heads;
-  int64_t ranges = 1;
-  double least = INFINITY;
-  const double step = few_block(rows) == 16 ? 1.1 : few_block(rows) == 32 ? 2.0 : 2.3;
-  for (int quarters = 1; quarters <= 32; ++quarters) {
+  constexpr double kFull = 0.64;
+  const bool narrow = head_dim <= 64;
+  const double megabytes = kFull * batch * room * kv_heads * head_dim * 4e-6;
+  const double groups = (double)((rows + 127) / 128) * batch * kv_heads;
+  double least = 4. + std::max(megabytes / 7.5, (narrow ? 0.75 : 0.9) * std::ceil(groups / 256) * ((room + kBN - 1) / kBN));
+  int64_t ranges = 0;
+  const int height = few_block(rows);
+  const int64_t blocks = (rows + height - 1) / height * kv_heads;
+  const double slow = narrow ? 0.84 : 1., step = slow * (height > 32 ? 1.85 : 1.45), cross = slow * (height > 16 ? 9.6 : 4.3);
+  for (const int quarters : {0, 1, 2, 4, 8, 12}) {  // of a round; 0: one range
     const int64_t r = std::max<int64_t>(std::min<int64_t>(64 * quarters / blocks, tiles / kFewLeast), 1);
-    const int64_t rounds = (blocks * r + 255) / 256, steps = (tiles + 4 * r - 1) / (4 * r);
-    const double us = 5. + 0.07 * r / batch + (double)rounds * (7.4 * (1. + (double)batch / r) + step * steps);
+    const double rounds = std::ceil((double)blocks * r / 256), steps = std::ceil(kFull * tiles / (4. * r));
+    const double crossings = batch > 1 ? std::max(1., (double)batch / r) : 0.;
+    const double us = (height > 16 ? 13. : 10.) - (r == 1 ? 5.3 : 0.) + 0.08 * r / batch + 4.2 * (rounds - 1) +
+                      std::max(rounds * (step * steps + cross * crossings), megabytes / 8.);
     if (us < least) least = us, ranges = r;
   }
-  if (rows > 16) {
-    const double groups = (double)((rows + 127) / 128) * batch * kv_heads;
-    if (8. + 1.3 * std::ceil(groups / 256) * (((int64_t)room + kBN - 1) / kBN) < least) return 0;
-  }
-  return tiles <= kFewOne ? 1 : (int)ranges;
+  return (int)ranges;
 }
 
 extern "C" size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges) {

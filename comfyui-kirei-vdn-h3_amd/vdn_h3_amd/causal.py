@@ -108,7 +108,7 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
 def _cut(batch: int, new: int, room: int, heads: int, kv_heads: int, dim: int) -> tuple[int, int]:
     """The ranges of keys that a call of these sizes takes and the bytes of their partial results."""
     lib = _lib.lib()
-    ranges = lib.vdnh3_causal_cached_ranges(batch, new, room, heads, kv_heads)
+    ranges = lib.vdnh3_causal_cached_ranges(batch, new, room, heads, kv_heads, dim)
     return ranges, lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
 
 

@@ -174,12 +174,13 @@ def test_ranges_of_a_call(built_lib):
     from vdn_h3_amd import _lib
 
     lib = _lib.lib()
-    assert lib.vdnh3_causal_cached_ranges(1, 1, 64, 40, 8) == 1
-    assert lib.vdnh3_causal_cached_ranges(64, 1, 8192, 40, 8) == 32
-    assert lib.vdnh3_causal_cached_ranges(16, 64, 2048, 40, 8) == 0
-    assert lib.vdnh3_causal_cached_ranges(1, 32, 40960, 40, 8) > 1
-    for bad in [(0, 1, 1, 1, 1), (1, 0, 1, 1, 1), (1, 1, 0, 1, 1), (1, 1, 1, 3, 2), (1, 1, 1, 0, 1), (1, 1, 1, 1, 0),
-                (1, 1, 2 ** 31 - 1, 4, 4), (2 ** 31 - 1, 2 ** 31 - 1, 64, 2 ** 31 - 1, 1)]:
+    assert lib.vdnh3_causal_cached_ranges(1, 1, 64, 40, 8, 128) <= 1
+    assert lib.vdnh3_causal_cached_ranges(64, 1, 8192, 40, 8, 128) == 32
+    assert lib.vdnh3_causal_cached_ranges(16, 64, 2048, 40, 8, 128) == 0
+    assert lib.vdnh3_causal_cached_ranges(1, 32, 40960, 40, 8, 128) > 1
+    for bad in [(0, 1, 1, 1, 1, 64), (1, 0, 1, 1, 1, 64), (1, 1, 0, 1, 1, 64), (1, 1, 1, 3, 2, 64), (1, 1, 1, 0, 1, 64),
+                (1, 1, 1, 1, 0, 64), (1, 1, 1, 1, 1, 0), (1, 1, 2 ** 31 - 1, 4, 4, 64),
+                (2 ** 31 - 1, 2 ** 31 - 1, 64, 2 ** 31 - 1, 1, 128)]:
         assert lib.vdnh3_causal_cached_ranges(*bad) == 0
     assert lib.vdnh3_causal_partial_bytes(3, 10, 64, 1) == 0
     assert lib.vdnh3_causal_partial_bytes(3, 10, 64, 4) == 4 * 2 * 30 * 66 * 4
