@@ -37,6 +37,22 @@ def _check(got, want, dim):
     assert (d <= bar[live]).all(), (d / bar[live].clamp_min(1e-30)).max()
 
 
+def _cached_in(ranges, q, k, v, lengths, scale):
+    """``vdnh3_causal_attn_cached`` in that many ranges, into an output of sevens and a buffer of NaNs."""
+    from vdn_h3_amd import _lib
+
+    lib = _lib.lib()
+    (batch, new, heads, dim), (room, kv) = q.shape, k.shape[1:3]
+    size = lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
+    partial = torch.full((max(size, 16),), 0xFF, dtype=torch.uint8, device=q.device)
+    out = torch.full(q.shape, 7.0, dtype=BF, device=q.device)
+    _lib.check(lib.vdnh3_causal_attn_cached(
+        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], out.data_ptr(),
+        *out.stride()[:3], lengths.data_ptr(), batch, new, room, heads, kv, dim, scale, ranges, partial.data_ptr(), size,
+        _lib.stream_handle(q.device)), "cached")
+    return out
+
+
 PACKED = [  # lengths, heads, kv heads, dim
     ([1], 1, 1, 64), ([2], 5, 1, 128), ([5, 1, 33], 4, 4, 64), ([0, 3, 0, 1, 64, 0], 8, 2, 128), ([95, 96, 97], 5, 1, 128),
     ([255, 256, 257], 2, 2, 128), ([51, 52, 103], 10, 2, 128), ([640], 40, 8, 128), ([1, 500, 63], 14, 2, 64),
@@ -162,7 +178,8 @@ def test_cached_against_float64(device, new, room, lengths, heads, kv, dim):
     assert torch.equal(got2, got) and (wide[:, :, heads:] == 9).all()
 
 
-@pytest.mark.parametrize("new,heads,kv,dim", [(1, 5, 1, 128), (1, 4, 4, 64), (3, 12, 2, 64), (7, 10, 2, 128)])
+@pytest.mark.parametrize("new,heads,kv,dim", [(1, 5, 1, 128), (1, 4, 4, 64), (3, 12, 2, 64), (7, 10, 2, 128), (9, 10, 2, 128),
+                                                (7, 20, 4, 64), (20, 10, 2, 128), (33, 3, 1, 64)])
 def test_cached_however_it_is_cut(device, new, heads, kv, dim):
     """Whole rows and every number of ranges, more than there are tiles for among them; lengths of every kind at once."""
     from vdn_h3_amd import _lib
@@ -174,18 +191,11 @@ def test_cached_however_it_is_cut(device, new, heads, kv, dim):
     want = po.cached(q, k, v, lengths, 0.1)
     n = torch.tensor(lengths, dtype=torch.int32, device=device)
     dq, dk, dv = q.to(device), k.to(device), v.to(device)
-    lib = _lib.lib()
     for ranges in (0, 1, 2, 3, 5, 8, 13, 17, 40, 256):
         print(f"case {ranges} ranges, {new} new tokens {heads}/{kv}x{dim}", flush=True)
-        size = lib.vdnh3_causal_partial_bytes(new, heads, dim, ranges)
-        partial = torch.full((max(size, 16),), 0xFF, dtype=torch.uint8, device=device)  # NaNs where nothing is written
-        out = torch.full_like(dq, 7.0)
-        rc = lib.vdnh3_causal_attn_cached(
-            dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(), *dv.stride()[:3], out.data_ptr(),
-            *out.stride()[:3], n.data_ptr(), batch, new, room, heads, kv, dim, 0.1, ranges, partial.data_ptr(), size,
-            _lib.stream_handle(device))
-        _lib.check(rc, "cached")
+        out = _cached_in(ranges, dq, dk, dv, n, 0.1)
         _check(out, want, dim)
+    lib, partial = _lib.lib(), torch.empty(64, dtype=torch.uint8, device=device)
     assert lib.vdnh3_causal_attn_cached(
         dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3], dv.data_ptr(), *dv.stride()[:3], out.data_ptr(),
         *out.stride()[:3], n.data_ptr(), batch, new, room, heads, kv, dim, 0.1, 4, partial.data_ptr(), 64,
@@ -201,8 +211,12 @@ def test_many_requests(device):
     lengths = torch.randint(0, room + 1, (batch,), generator=g)
     q, k, v = _qkv(batch * room, 4, 2, 64, 51)
     q, k, v = q[:batch * 2].view(batch, 2, 4, 64), k.view(batch, room, 2, 64), v.view(batch, room, 2, 64)
-    got = causal_softmax_cached(q.to(device), k.to(device), v.to(device), lengths.to(device), 0.125)
-    _check(got, po.cached(q, k, v, lengths.tolist(), 0.125), 64)
+    want = po.cached(q, k, v, lengths.tolist(), 0.125)
+    dq, dk, dv = q.to(device), k.to(device), v.to(device)
+    _check(causal_softmax_cached(dq, dk, dv, lengths.to(device), 0.125), want, 64)
+    for ranges in (1, 7, 64, 300):
+        print(f"case {ranges} ranges of {batch} requests", flush=True)
+        _check(_cached_in(ranges, dq, dk, dv, lengths.to(device, torch.int32), 0.125), want, 64)
 
 
 def test_many_sequences(device):
@@ -235,10 +249,12 @@ def test_cached_infinities_behind_a_new_token(device):
         q, k, v = q[None, :new], k[None], v[None]
         v[0, 199], k[0, 198] = torch.nan, torch.nan  # what only the last two tokens see
         n = torch.tensor([200], dtype=torch.int32, device=device)
-        got = causal_softmax_cached(q.to(device), k.to(device), v.to(device), n, 0.125).cpu()
         want = po.cached(q, k, v, [200], 0.125)
-        _check(got[:, :-2], [t[:, :-2] for t in want], 64)
-        assert got[:, -2:].isnan().all()
+        dq, dk, dv = q.to(device), k.to(device), v.to(device)
+        for got in [causal_softmax_cached(dq, dk, dv, n, 0.125)] + [_cached_in(r, dq, dk, dv, n, 0.125) for r in (0, 1, 3)]:
+            got = got.cpu()
+            _check(got[:, :-2], [t[:, :-2] for t in want], 64)
+            assert got[:, -2:].isnan().all()
 
 
 @pytest.mark.parametrize("new", [1, 4, 40, 200])
@@ -256,9 +272,10 @@ def test_infinities_and_largest_numbers_that_a_row_sees(device, new):
         v[:, :, 7], v[:, :, 8] = big[:, None].to(BF), -big[:, None].to(BF)
         whole = po.packed(q, k, v, [0, room], dim ** -0.5)
         n = torch.tensor([room], dtype=torch.int32, device=device)
-        some = causal_softmax_cached(q[None, -new:].to(device), k[None].to(device), v[None].to(device), n, dim ** -0.5)
+        caches = (q[None, -new:].to(device), k[None].to(device), v[None].to(device), n, dim ** -0.5)
+        some = [causal_softmax_cached(*caches)] + [_cached_in(r, *caches) for r in (0, 1, 3)]
         full = causal_softmax_packed(q.to(device), k.to(device), v.to(device), [0, room], dim ** -0.5)
-        for got, want in ((some[0], [t[-new:] for t in whole]), (full, whole)):
+        for got, want in [(t[0], [w[-new:] for w in whole]) for t in some] + [(full, whole)]:
             odd = want[0].isinf()
             assert odd.any() and torch.equal(got.cpu()[odd], want[0][odd].to(BF))
             rest = [want[0].masked_fill(odd, 0), want[1].masked_fill(odd, 0), want[2]]
@@ -290,8 +307,10 @@ def test_offsets_past_32_bits(device, new, room, row):
     k.copy_(hk[None]), v.copy_(hv[None])
     q = q[None, :new]
     n = torch.tensor([room - 1], dtype=torch.int32, device=device)
-    got = causal_softmax_cached(q.to(device), k, v, n, 0.125)
-    _check(got, po.cached(q, hk[None], hv[None], [room - 1], 0.125), 64)
+    want = po.cached(q, hk[None], hv[None], [room - 1], 0.125)
+    _check(causal_softmax_cached(q.to(device), k, v, n, 0.125), want, 64)
+    for ranges in (0, 1, 5):
+        _check(_cached_in(ranges, q.to(device), k, v, n, 0.125), want, 64)
 
 
 def test_strides_of_single_elements_do_not_count(device):
