@@ -467,18 +467,21 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
   }
 }
 
-// --------------------------------------------------------------------------------- Few rows over long caches (new tokens):
-// what counts is to stream the keys and values once. The 32-key tiles of all sequences, one behind another, are cut into
-// `ranges` equal ranges for each key / value head, one workgroup each and about one workgroup per CU: whatever the lengths
-// are, every CU streams the same number of tiles, in one round. A range crosses from one sequence into the next; only the
-// sequences at its two ends can be shared with other ranges. Such a part is written unnormalised in fp32 with its max and
-// sum and combined by a second launch; a sequence inside a range is finished at once. The cut follows from the lengths on
-// the device, in both kernels alike. A workgroup takes up to 16 NQ of a head's (token, head) rows. Its wavefronts take the
-// tiles in turn, each through two LDS slots of its own (one tile in flight while it works on the other, no barrier), with a
-// running softmax of its own; they are merged in LDS at the end of a sequence. HBM bounds it: 64 requests of up to 8,192
-// keys x 8 heads x 128 (1.05 GB) take 196 us, 5.3 TB/s where a copy reaches 4.8; one request of 40,688 keys (167 MB) 34 us
-// and 5 for the combination. With fixed chunks of keys instead of equal ranges the first took 215 to 244 us, whole rounds
-// of workgroups each with a pipeline to fill.
+// ---------------------------------------------------------------------------------
+// Few rows over long caches (new tokens): what counts is to stream the keys and values once. The 32-key tiles of all
+// sequences, one behind another, are cut into `ranges` equal ranges for each key / value head, one workgroup each and mostly
+// one workgroup per CU: whatever the lengths are, every CU streams the same number of tiles, in one round. A range crosses
+// from one sequence into the next; only the sequences at its two ends can be shared with other ranges. Such a part is
+// written unnormalised in fp32 with its max and sum and combined by a second launch; a sequence inside a range is finished at
+// once. The cut follows from the lengths on the device, in both kernels alike.
+//
+// A workgroup takes 16 NQ of a head's (token, head) rows, up to 48 (64 spill). Its wavefronts take the tiles in turn, each
+// through two LDS slots of its own (one tile in flight while it works on the other, no barrier), with a running softmax of its
+// own; they are merged in LDS at the end of a sequence. HBM bounds it: 64 requests of up to 8,192 keys x 8 heads x 128
+// (1.1 GB) take 190 us, 5.7 TB/s where a copy reaches 4.8; one request of 40,688 keys (167 MB) 30 us and 6 for the
+// combination, which is a launch and a chain of three loads. 32 new tokens over them (four blocks of rows, 78 MFMAs a tile) take
+// 93 us: a chain too, of a tile's products, maxima and exponentials in the only wavefront of a SIMD. With fixed chunks of keys
+// instead of equal ranges the 64 requests took 215 to 244 us, whole rounds of workgroups each with a pipeline to fill.
 constexpr int kFewKeys = 32;      // keys per tile: one k-step of the PV product
 constexpr int kFewRing = 2;
 // Tiles of a range, at least: one per wavefront (one request of 1,000 keys x 40 / 8 heads: 16 ranges 11.1 us, 8 11.3, 4
