@@ -3,8 +3,9 @@
 * ``causal_softmax_packed``: whole prompts of different lengths, packed one behind another;
 * ``causal_softmax_cached``: one or several new tokens of each request over the requests' key / value caches.
 
-Both compute in bf16 with fp32 scores, sums and softmax statistics and round once. Query head ``h`` reads key / value head
-``h // (heads // kv_heads)``. Sequence bounds are read on the device: a call needs no copy to the host, and a captured one
+Both take bf16 and hold scores, sums and softmax statistics in fp32. The products with the values take the probabilities as
+bf16 (2.0e-3 of the result, with the result's own rounding of 1.6e-3), in ranges of long caches as two bf16 numbers (1.7e-3).
+Query head ``h`` reads key / value head ``h // (heads // kv_heads)``. Sequence bounds are read on the device: a call needs no copy to the host, and a captured one
 can be replayed with other lengths. Forward-only; there is no CPU path.
 """
 
