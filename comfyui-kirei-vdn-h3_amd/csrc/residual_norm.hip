@@ -265,16 +265,18 @@ __global__ __launch_bounds__(256) void residual_norm_sweep_kernel(Rows p) {
   });
 }
 
-// A workgroup per row, but for many narrow rows in 8 bits, which leave its threads one chunk each or less: a wavefront per row.
-// 40,688 rows x 5,120 in int8: 253 us against 282 with a wavefront and ten chunks a lane; x 2,048: 113 against 106. HBM is
-// the bound: 246 us are 5.9 TB/s for the 7 bytes of an element, where a copy reaches 4.8.
-constexpr int kWaveWidth = 2048, kWaveRows = 4096;
+// A workgroup per row, but for many narrow rows, which leave its threads one chunk each or less: a wavefront per row. 40,688
+// rows x 5,120 in int8: 253 us against 282 with a wavefront and ten chunks a lane; x 2,048: 118 against 104, x 1,024: 93
+// against 55. In bf16 the workgroup has less to do per row: x 2,048 113 against 117, x 1,024 68 against 53. 2,048 rows x 1,024
+// in int8 6.9 against 5.6, 512 rows 3.5 against 3.8. HBM is the bound: 246 us for the 5,120 are 5.9 TB/s for the 7 bytes of
+// an element, where a copy reaches 4.8.
+constexpr int kWaveWidth = 2048, kWaveWidthBf16 = 1024, kWaveRows = 2048;
 
 template <int KIND>
 void launch_residual_norm(const Rows &p, hipStream_t s) {
   if (p.hidden > 8 * 256 * 4)
     hipLaunchKernelGGL(residual_norm_sweep_kernel<KIND>, dim3(p.rows), dim3(256), 0, s, p);
-  else if (KIND != 0 && p.hidden <= kWaveWidth && p.rows >= kWaveRows)
+  else if (p.hidden <= (KIND ? kWaveWidth : kWaveWidthBf16) && p.rows >= kWaveRows)
     hipLaunchKernelGGL((residual_norm_kernel<KIND, 64, 4>), dim3((p.rows + 3) / 4), dim3(256), 0, s, p);
   else
     hipLaunchKernelGGL((residual_norm_kernel<KIND, 256, 4>), dim3(p.rows), dim3(256), 0, s, p);

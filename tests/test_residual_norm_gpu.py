@@ -68,13 +68,13 @@ def test_against_float64(device, kind, rows, hidden):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("hidden", [1024, 5120, 8200])
-def test_strided_repeated_and_in_place(device, kind, hidden):
+@pytest.mark.parametrize("rows,hidden", [(9, 1024), (9, 5120), (9, 8200), (2100, 1024)])
+def test_strided_repeated_and_in_place(device, kind, rows, hidden):
     from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
 
-    print(f"case residual norm strides {kind} {hidden}", flush=True)
-    x, res, w = _case(9, hidden, 5)
-    wide = torch.full((9, hidden + 64), 7.0, dtype=BF, device=device)
+    print(f"case residual norm strides {kind} {rows} {hidden}", flush=True)
+    x, res, w = _case(rows, hidden, 5)
+    wide = torch.full((rows, hidden + 64), 7.0, dtype=BF, device=device)
     wide[:, 8:8 + hidden] = x.to(device)
     want = residual_rmsnorm_quantize(x.to(device), res.to(device), w.to(device), 1e-5, KINDS[kind])
 
@@ -83,18 +83,18 @@ def test_strided_repeated_and_in_place(device, kind, hidden):
         assert torch.equal(got[2], want[2])
 
     same(residual_rmsnorm_quantize(wide[:, 8:8 + hidden], res.to(device), w.to(device), 1e-5, KINDS[kind]))
-    odd = torch.empty(9 * hidden + 1, dtype=BF, device=device)[1:].view(9, hidden).copy_(x)  # rows off 16 bytes: copied
+    odd = torch.empty(rows * hidden + 1, dtype=BF, device=device)[1:].view(rows, hidden).copy_(x)  # rows off 16 bytes: copied
     same(residual_rmsnorm_quantize(odd, res.to(device), w.to(device), 1e-5, KINDS[kind]))
     for which in range(2):  # the sum over x or over the residual
         a, b = x.to(device), res.to(device)
         got = residual_rmsnorm_quantize(a, b, w.to(device), 1e-5, KINDS[kind], sum_out=(a, b)[which])
         assert got[2] is (a, b)[which]
         same(got)
-    out = torch.full((9, hidden + 16), 5.0, dtype=BF, device=device)
+    out = torch.full((rows, hidden + 16), 5.0, dtype=BF, device=device)
     same(residual_rmsnorm_quantize(x.to(device), res.to(device), w.to(device), 1e-5, KINDS[kind], sum_out=out[:, :hidden]))
     assert (out[:, hidden:] == 5).all() and (wide[:, :8] == 7).all()
-    one = residual_rmsnorm_quantize(x.to(device), res[:1].to(device).expand(9, hidden), w.to(device), 1e-5, KINDS[kind])
-    _check(one, kind, x, res[:1].expand(9, hidden), w, 1e-5)
+    one = residual_rmsnorm_quantize(x.to(device), res[:1].to(device).expand(rows, hidden), w.to(device), 1e-5, KINDS[kind])
+    _check(one, kind, x, res[:1].expand(rows, hidden), w, 1e-5)
 
 
 def test_squares_under_the_smallest_numbers(device):
@@ -110,12 +110,12 @@ def test_squares_under_the_smallest_numbers(device):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("hidden", [512, 5120, 9216])
-def test_borders(device, kind, hidden):
+@pytest.mark.parametrize("hidden,times", [(512, 1), (5120, 1), (9216, 1), (512, 300), (2048, 300)])
+def test_borders(device, kind, hidden, times):
     """Zero rows, rows far up and far down in bf16's range, and rows that are not finite."""
     from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
 
-    print(f"case residual norm borders {kind} {hidden}", flush=True)
+    print(f"case residual norm borders {kind} {hidden} x {times}", flush=True)
     x, res, w = _case(8, hidden, 6)
     x[0], res[0] = 0, 0
     x[1], res[1] = x[1] * 2.0 ** 100, res[1] * 2.0 ** 100  # the squares pass fp32
@@ -124,7 +124,12 @@ def test_borders(device, kind, hidden):
     x[4, hidden // 2] = torch.inf
     res[5, hidden - 1] = torch.nan
     x[6, 0], res[6, 0] = -3e38, -3e38  # the sum passes fp32
-    got = residual_rmsnorm_quantize(x.to(device), res.to(device), w.to(device), 1e-6, KINDS[kind])
+    got = residual_rmsnorm_quantize(x.to(device).repeat(times, 1), res.to(device).repeat(times, 1), w.to(device), 1e-6, KINDS[kind])
+    for t in got:  # the same rows give the same results
+        if t is not None:
+            bits = t.view(torch.uint8).view(times, 8, -1)
+            assert torch.equal(bits, bits[:1].expand_as(bits))
+    got = [None if t is None else t[:8] for t in got]
     fine = [0, 1, 2, 3, 7]
     _check([None if t is None else t[fine] for t in got], kind, x[fine], res[fine], w, 1e-6)
     for row in (4, 5, 6):
