@@ -137,20 +137,20 @@ int check_vectors(const Vectors &s, const char *name) {
   return VDNH3_OK;
 }
 
-// Rows up to which each has a workgroup of its own: with 40 + 8 heads of 128, 512 rows take 7.9 us against 12.4 with four rows a
-// workgroup, 2,048 15.1 against 15.5, 4,096 30.9 against 23.7. HBM is the bound of many rows: 40,688 x 80 heads x 128 take
-// 327 us with the norms, 5.1 TB/s; 2 or 8 vectors in flight instead of 4 and non-temporal loads are no faster.
-constexpr int kSingleRows = 2048;
+// Rows of a workgroup: as few as keep the launch within one round, 4 workgroups a CU; more rows share a workgroup's other
+// threads for the angles. 40 + 8 heads of 128: 512 rows 7.8 us (1 row), 9.0 (2), 12.3 (4); 2,048 rows 15.3, 13.8, 15.5; 4,096
+// rows 30, 27, 23; 32 + 8 heads of 64: 2,048 rows 10.5, 8.1, 11.0 (8). HBM is the bound of many rows: 40,688 x 80 heads x 128
+// take 327 us with the norms, 5.1 TB/s; 2 or 8 vectors in flight instead of 4 and non-temporal loads are no faster.
+constexpr int kRound = 1024;
 
-template <int LANES>
+template <int LANES, int R>
 void launch_rotary(const Vectors &q, const Vectors &k, const Positions &pos, const double *turns, const int32_t *axis, int rot,
                    int dim, int rows, hipStream_t s) {
-  constexpr int R = 64 / LANES;  // a pair per thread
-  if (rows <= kSingleRows)
-    hipLaunchKernelGGL((rotary_kernel<LANES, 1>), dim3(rows), dim3(256), 0, s, q, k, pos, turns, axis, rot, dim, rows);
-  else
-    hipLaunchKernelGGL((rotary_kernel<LANES, R>), dim3((rows + R - 1) / R), dim3(256), 0, s, q, k, pos, turns, axis, rot, dim,
-                       rows);
+  if constexpr (R < 64 / LANES) {  // at most a pair per thread
+    if (rows > R * kRound) return launch_rotary<LANES, 2 * R>(q, k, pos, turns, axis, rot, dim, rows, s);
+  }
+  hipLaunchKernelGGL((rotary_kernel<LANES, R>), dim3((rows + R - 1) / R), dim3(256), 0, s, q, k, pos, turns, axis, rot, dim,
+                     rows);
 }
 
 }  // namespace
@@ -180,13 +180,13 @@ extern "C" int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_
                    stride(ko_head, k_heads), k_heads};
   int rc = check_vectors(qs, "q");
   if (!rc) rc = check_vectors(ks, "k");
-  if (!rc) rc = check_grid(rows, 64, "rotary");  // four rows a workgroup of 256, or fewer rows
+  if (!rc) rc = check_grid(rows, 64, "rotary");  // four rows a workgroup of 256 threads or more, or few rows
   if (rc) return rc;
   const Positions pos{positions, p_axis, p_row, position_type};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim <= 64)
-    launch_rotary<8>(qs, ks, pos, turns, axis_of_pair, rot_dim, head_dim, rows, s);
+    launch_rotary<8, 1>(qs, ks, pos, turns, axis_of_pair, rot_dim, head_dim, rows, s);
   else
-    launch_rotary<16>(qs, ks, pos, turns, axis_of_pair, rot_dim, head_dim, rows, s);
+    launch_rotary<16, 1>(qs, ks, pos, turns, axis_of_pair, rot_dim, head_dim, rows, s);
   return check_launch("rotary");
 }

@@ -41,7 +41,9 @@ CASES = [  # rows, heads, kv heads, dim, sections, ladder, with norm
     (1001, 40, 8, 128, (8, 28, 28), "per_axis", True), (130, 5, 5, 128, (16, 16), "shared", True),
     (257, 28, 4, 128, (64,), "shared", True), (333, 14, 2, 64, (4, 14, 14), "per_axis", True),
     (65, 16, 2, 64, (0, 8, 0, 8), "shared", False), (77, 6, 3, 80, (10, 14, 16), "shared", True),
-    (50, 3, 1, 96, (24,), "shared", True), (31, 7, 1, 40, (3, 5), "per_axis", True), (4500, 8, 1, 128, (64,), "shared", True)]
+    (50, 3, 1, 96, (24,), "shared", True), (31, 7, 1, 40, (3, 5), "per_axis", True), (4500, 8, 1, 128, (64,), "shared", True),
+    (1025, 2, 1, 128, (8, 28, 28), "per_axis", True), (2047, 3, 1, 64, (12, 12), "shared", True),
+    (2049, 2, 2, 64, (32,), "shared", False), (4099, 1, 1, 64, (16, 16), "per_axis", True), (2050, 1, 1, 24, (8,), "shared", True)]
 
 
 @pytest.mark.parametrize("rows,heads,kv,dim,sections,ladder,norm", CASES)
