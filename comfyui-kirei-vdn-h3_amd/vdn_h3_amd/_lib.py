@@ -195,8 +195,13 @@ def in_place(t) -> bool:
         return False
     if t.is_contiguous():
         return t.shape[-1] % 8 == 0 or t.numel() == t.shape[-1]
-    *outer, inner = zip(t.shape, t.stride())
-    return (inner[1] == 1 or inner[0] == 1) and not any(s % 8 for n, s in outer if n > 1)
+    shape, strides = t.shape, t.stride()
+    if strides[-1] != 1 and shape[-1] != 1:
+        return False
+    for n, s in zip(shape[:-1], strides):
+        if s % 8 and n > 1:
+            return False
+    return True
 
 
 def operand(t):
