@@ -86,13 +86,13 @@ __device__ __forceinline__ u32x2_t codes8(const float *y, float by) {
   }
 }
 
-// What turns a row's t * w into y and into codes. With z = t w and r = 1 / sqrt(mean(t^2) + eps), y = z r, and
+// What turns a row into its norm and its codes. With z = t w and r = 1 / sqrt(mean(t^2) + eps), y = z r, and
 // scale = max|z| r / q with q = 127 or 448: both reductions of a row are of its inputs alone and take one pass, and
 // y / scale = z (q / max|z|). Each is the row's by one more rounding than (t r) w would take.
 constexpr float kLeastMean = 0x1p-90f;  // below it the squares lose bits under fp32's smallest normal number
 template <int KIND>
 struct RowFactors {
-  float mean, y, code, scale;
+  float mean, y, code, scale;  // y: the factor r
   bool plain;  // else the squares or the products pass fp32 either way, or are not numbers
   __device__ __forceinline__ RowFactors(const Reduced &red, int hidden, float eps) {
     constexpr float kMost = KIND == 1 ? kI8Max : kF8Max;
@@ -135,14 +135,11 @@ struct Rows {
     }
   }
   __device__ __forceinline__ void weights(int c, float *wf) const { unpack8r(ld16(w + 8 * c), wf); }
-  // the outputs of chunk c: y * by is the norm (KIND 0) or the value that is coded
+  // the outputs of chunk c: y is the norm (KIND 0), y * by the value that is coded
   template <int KIND>
   __device__ __forceinline__ void store(int64_t row, int c, const float *t, const float *y, float by) const {
     if constexpr (KIND == 0) {
-      float n[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) n[j] = y[j] * by;
-      st16(static_cast<uint16_t *>(out) + row * out_row + 8 * c, pack8r(n));
+      st16(static_cast<uint16_t *>(out) + row * out_row + 8 * c, pack8r(y));
     } else {
       *reinterpret_cast<u32x2_t *>(static_cast<uint8_t *>(out) + row * out_row + 8 * c) = codes8<KIND>(y, by);
     }
@@ -173,9 +170,10 @@ __device__ __forceinline__ void norm_row(const Rows &p, int64_t row, bool leader
     each([&](int c, const float *t) __device__ {
       float z[8];
       p.weights(c, z);
+      // bf16: (t r) w, whose |t r| is at most sqrt(hidden); t w alone can pass fp32, and no reduction has looked at it
 #pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] *= t[j];
-      p.template store<KIND>(row, c, t, z, KIND == 0 ? f.y : f.code);
+      for (int j = 0; j < 8; ++j) z[j] *= KIND == 0 ? t[j] * f.y : t[j];
+      p.template store<KIND>(row, c, t, z, KIND == 0 ? 1.f : f.code);
     });
     return;
   }

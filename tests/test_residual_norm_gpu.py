@@ -187,3 +187,20 @@ def test_no_rows(device):
     x = torch.empty(0, 64, dtype=BF, device=device)
     q, s, t = residual_rmsnorm_quantize(x, x, torch.ones(64, dtype=BF, device=device), 1e-6, 2)
     assert q.shape == (0, 64) and s.shape == (0, 1) and t.shape == (0, 64)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("hidden,times", [(512, 1), (5120, 1), (9216, 1), (512, 300), (2048, 300)])
+def test_weights_whose_products_pass_fp32(device, kind, hidden, times):
+    """t w is past fp32's largest number, or under its smallest, while the norm, t r w, is one that bf16 holds."""
+    from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
+
+    print(f"case residual norm products {kind} {hidden} x {times}", flush=True)
+    for t_up, w_up, eps in ((45, 90, 1e-6), (-42, -105, 0.0)):
+        x, res, w = _case(8, hidden, 31)
+        x, res, w = ((t.float() * 2.0 ** up).to(BF) for t, up in ((x, t_up), (res, t_up), (w, w_up)))
+        z = (x.float() + res.float()).abs() * w.float().abs()
+        assert (z.amax(1).isinf() if t_up > 0 else z.median(1).values < 2.0 ** -140).all()
+        got = residual_rmsnorm_quantize(x.to(device).repeat(times, 1), res.to(device).repeat(times, 1), w.to(device), eps,
+                                        KINDS[kind])
+        _check([None if t is None else t[-8:] for t in got], kind, x, res, w, eps)
