@@ -57,6 +57,21 @@ __device__ __forceinline__ Reduced reduce_row(float v, uint32_t top, uint2 *red)
   return Reduced{v, top};
 }
 
+// The same of sums in 64 bits.
+template <int THREADS>
+__device__ __forceinline__ double sum_row(double v, uint2 *red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __builtin_bit_cast(uint2, v);
+    __syncthreads();
+    v = 0.;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) v += __builtin_bit_cast(double, red[w]);
+  }
+  return v;
+}
+
 // Eight int8 (KIND 1) or e4m3fn (KIND 2) codes of y * by, |y * by| at most the kind's largest number but for rounding.
 template <int KIND>
 __device__ __forceinline__ u32x2_t codes8(const float *y, float by) {
@@ -92,11 +107,11 @@ __device__ __forceinline__ u32x2_t codes8(const float *y, float by) {
 constexpr float kLeastMean = 0x1p-90f;  // below it the squares lose bits under fp32's smallest normal number
 template <int KIND>
 struct RowFactors {
-  float mean, y, code, scale;  // y: the factor r
-  bool plain;  // else the squares or the products pass fp32 either way, or are not numbers
+  float y, code, scale;  // y: the factor r
+  bool plain;          // else the squares or the products pass fp32 either way, or are not numbers
   __device__ __forceinline__ RowFactors(const Reduced &red, int hidden, float eps) {
     constexpr float kMost = KIND == 1 ? kI8Max : kF8Max;
-    mean = red.sum / (float)hidden + eps;
+    const float mean = red.sum / (float)hidden + eps;
     plain = mean > kLeastMean && red.sum < INFINITY && red.top < kInfBits;
     y = 1.f / sqrtf(mean);
     if constexpr (KIND != 0) {
@@ -107,13 +122,6 @@ struct RowFactors {
     }
   }
 };
-
-// The rest of a row's outputs, where fp32 does not hold them that way: t scaled by a power of two for the squares, y =
-// (t r) w, and a row whose y is not finite gets the scale NaN and zero codes.
-template <int KIND>
-__device__ __forceinline__ float row_scale(uint32_t top) {
-  return top < kInfBits ? fmaxf(__uint_as_float(top) / (KIND == 1 ? kI8Max : kF8Max), 1e-12f) : __builtin_nanf("");
-}
 
 struct Rows {
   const uint16_t *x, *res, *w;
@@ -148,11 +156,57 @@ struct Rows {
   }
 };
 
-// One row on THREADS threads: `each` calls a function with every chunk of the row that the thread has and its t. The outputs
-// are written after every read of the row, each thread's over what it alone read, so the sum may lie over x or the
-// residual.
+// A row that fp32 does not hold that way, read and made once more: its squares, their sum, r and (t r) w in 64 bits, which
+// hold them for any t and w (a power of two for the row would not do: t reaches from 2^-133 to 2^128, and what passed fp32 may
+// be t w alone). A row whose y is not finite gets the scale NaN and zero codes. Loops over memory: the registers stay few.
+template <int KIND, int THREADS>
+__device__ __forceinline__ void norm_row_again(const Rows &p, int64_t row, int tid, uint2 (*red)[THREADS / 64]) {
+  const int chunks = p.hidden / 8;
+  asm volatile("" : "+v"(tid));  // no address of the ordinary pass is kept for this one
+  double squares = 0.;
+  float t[8], y[8];
+#pragma unroll 1
+  for (int c = tid; c < chunks; c += THREADS) {
+    p.load(row, c, t);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) squares = fma((double)t[j], (double)t[j], squares);
+  }
+  const double r = 1. / sqrt(sum_row<THREADS>(squares, red[0]) / p.hidden + p.eps);
+  auto normed = [&](int c) __device__ {
+    p.load(row, c, t);
+    p.weights(c, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = (float)((double)t[j] * r * y[j]);
+  };
+  float by = 1.f;
+  if constexpr (KIND != 0) {
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int c = tid; c < chunks; c += THREADS) {
+      normed(c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(y[j]));
+    }
+    top = reduce_row<THREADS>(0.f, top, red[1]).top;
+    const float s = top < kInfBits ? fmaxf(__uint_as_float(top) / (KIND == 1 ? kI8Max : kF8Max), 1e-12f) : __builtin_nanf("");
+    if (tid == 0) p.scale[row] = s;
+    by = top < kInfBits ? 1.f / s : 0.f;
+  }
+#pragma unroll 1
+  for (int c = tid; c < chunks; c += THREADS) {
+    normed(c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (KIND != 0 && by == 0.f) y[j] = 0.f;
+    p.template store<KIND>(row, c, t, y, by);
+  }
+}
+
+// One row on THREADS threads: `each` calls a function with every chunk of the row that the thread has (`tid`, tid + THREADS,
+// ...) and its t. The outputs are written after every read of the row by another thread, each thread's over what it alone
+// read, so the sum may lie over x or the residual.
 template <int KIND, int THREADS, class Each>
-__device__ __forceinline__ void norm_row(const Rows &p, int64_t row, bool leader, uint2 (*red)[THREADS / 64], Each each) {
+__device__ __forceinline__ void norm_row(const Rows &p, int64_t row, int tid, uint2 (*red)[THREADS / 64], Each each) {
   float ss = 0.f;
   uint32_t top = 0;
   each([&](int c, const float *t) __device__ {
@@ -165,59 +219,24 @@ __device__ __forceinline__ void norm_row(const Rows &p, int64_t row, bool leader
     }
   });
   const RowFactors<KIND> f(reduce_row<THREADS>(ss, top, red[0]), p.hidden, p.eps);
-  if (f.plain) {
-    if (KIND != 0 && leader) p.scale[row] = f.scale;
-    each([&](int c, const float *t) __device__ {
-      float z[8];
-      p.weights(c, z);
-      // bf16: (t r) w, whose |t r| is at most sqrt(hidden); t w alone can pass fp32, and no reduction has looked at it
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] *= KIND == 0 ? t[j] * f.y : t[j];
-      p.template store<KIND>(row, c, t, z, KIND == 0 ? 1.f : f.code);
-    });
-    return;
-  }
-  const float shift = f.mean > 1.f || !(f.mean == f.mean) ? 0x1p-64f : 0x1p64f;
-  ss = 0.f;
-  each([&](int, const float *t) __device__ {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(t[j] * shift, t[j] * shift, ss);
-  });
-  const float r = shift / sqrtf(reduce_row<THREADS>(ss, 0, red[1]).sum / (float)p.hidden + p.eps * shift * shift);
-  auto normed = [&](int c, const float *t, float *y) __device__ {
-    p.weights(c, y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] *= t[j] * r;
-  };
-  float by = 1.f;
-  if constexpr (KIND != 0) {
-    top = 0;
-    each([&](int c, const float *t) __device__ {
-      float y[8];
-      normed(c, t, y);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, abs_bits(y[j]));
-    });
-    const float s = row_scale<KIND>(reduce_row<THREADS>(0.f, top, red[2]).top);
-    if (leader) p.scale[row] = s;
-    by = 1.f / s;
-  }
+  if (!f.plain) return norm_row_again<KIND, THREADS>(p, row, tid, red + 1);
+  if (KIND != 0 && tid == 0) p.scale[row] = f.scale;
   each([&](int c, const float *t) __device__ {
-    float y[8];
-    normed(c, t, y);
+    float z[8];
+    p.weights(c, z);
+    // bf16: (t r) w, whose |t r| is at most sqrt(hidden); t w alone can pass fp32, and no reduction has looked at it
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (KIND != 0 && !(by > 0.f)) y[j] = 0.f;
-    p.template store<KIND>(row, c, t, y, KIND != 0 && !(by > 0.f) ? 0.f : by);
+    for (int j = 0; j < 8; ++j) z[j] *= KIND == 0 ? t[j] * f.y : t[j];
+    p.template store<KIND>(row, c, t, z, KIND == 0 ? 1.f : f.code);
   });
 }
 
 // Rows of up to 8 THREADS NCH channels: the row's sum stays in registers (fp32) from the loads, all in flight at once, to the
-// outputs. THREADS 64: a wavefront per row, four rows per workgroup, no barrier; 256: a workgroup per row. Six wavefronts a SIMD
-// instead of the five that 86 registers leave: 20,000 rows x 2,560 in int8 73 -> 69 us, x 5,120 127 -> 125 (the rows that are
-// taken again spill 24 bytes).
+// outputs. THREADS 64: a wavefront per row, four rows per workgroup, no barrier; 256: a workgroup per row. Eight wavefronts a
+// SIMD in bf16 (with six 20,000 rows x 2,048 take 49.5 us instead of 47.2; rows that are taken again spill 28 bytes then), six
+// or more of the 8-bit kinds (with five x 2,560 in int8 took 73 instead of 69, x 5,120 127 instead of 125).
 template <int KIND, int THREADS, int NCH>
-__global__ __launch_bounds__(256, 6) void residual_norm_kernel(Rows p) {
+__global__ __launch_bounds__(256, KIND ? 6 : 8) void residual_norm_kernel(Rows p) {
   __shared__ uint2 red[3][4];
   const int64_t row = THREADS == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= p.rows) return;  // a whole wavefront (THREADS 64) or none
@@ -244,7 +263,7 @@ __global__ __launch_bounds__(256, 6) void residual_norm_kernel(Rows p) {
       }
     }
   }
-  norm_row<KIND, THREADS>(p, row, tid == 0, reinterpret_cast<uint2 (*)[THREADS / 64]>(red), [&](auto f) __device__ {
+  norm_row<KIND, THREADS>(p, row, tid, reinterpret_cast<uint2 (*)[THREADS / 64]>(red), [&](auto f) __device__ {
 #pragma unroll
     for (int u = 0; u < NCH; ++u)
       if (tid + THREADS * u < chunks) f(tid + THREADS * u, t[u]);
@@ -256,7 +275,7 @@ template <int KIND>
 __global__ __launch_bounds__(256) void residual_norm_sweep_kernel(Rows p) {
   __shared__ uint2 red[3][4];
   const int64_t row = blockIdx.x;
-  norm_row<KIND, 256>(p, row, threadIdx.x == 0, red, [&](auto f) __device__ {
+  norm_row<KIND, 256>(p, row, threadIdx.x, red, [&](auto f) __device__ {
     for (int c = threadIdx.x; c < p.hidden / 8; c += 256) {
       float t[8];
       p.load(row, c, t);

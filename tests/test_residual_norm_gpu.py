@@ -204,3 +204,53 @@ def test_weights_whose_products_pass_fp32(device, kind, hidden, times):
         got = residual_rmsnorm_quantize(x.to(device).repeat(times, 1), res.to(device).repeat(times, 1), w.to(device), eps,
                                         KINDS[kind])
         _check([None if t is None else t[-8:] for t in got], kind, x, res, w, eps)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("hidden,times", [(512, 1), (5120, 1), (9216, 1), (512, 300), (2048, 300)])
+def test_rows_near_the_largest_and_the_smallest_numbers(device, kind, hidden, times):
+    """Whole rows up to bf16's largest numbers and down to its smallest: their norm is an ordinary one."""
+    from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
+
+    print(f"case residual norm ends of the range {kind} {hidden} x {times}", flush=True)
+    x, res, w = _case(8, hidden, 32)
+    sign = x.float().sign()
+    x[0], res[0] = sign[0] * 1e37, 0
+    x[1], res[1] = sign[1] * 3e38, 0
+    x[2], res[2] = sign[2] * 1.6e38, sign[2] * 1.6e38
+    x[3], res[3] = x[3] * 1e36, res[3] * 1e34
+    x[4, 1:], res[4], x[4, 0] = 0, 0, 3e38  # one channel alone
+    x[5], res[5] = x[5] * 2.0 ** -120, res[5] * 2.0 ** -120
+    x[6], res[6] = sign[6] * 2.0 ** -133, 0  # the smallest number
+    got = residual_rmsnorm_quantize(x.to(device).repeat(times, 1), res.to(device).repeat(times, 1), w.to(device), 0.0, KINDS[kind])
+    over = x.to(device).repeat(times, 1)  # the sum over x
+    got2 = residual_rmsnorm_quantize(over, res.to(device).repeat(times, 1), w.to(device), 0.0, KINDS[kind], sum_out=over)
+    assert all(a is b or torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, got2))
+    for t in got:  # the same rows give the same results
+        if t is not None:
+            bits = t.view(torch.uint8).view(times, 8, -1)
+            assert torch.equal(bits, bits[:1].expand_as(bits))
+    _check([None if t is None else t[:8] for t in got], kind, x, res, w, 0.0)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("hidden,times", [(512, 1), (5120, 1), (9216, 1), (512, 300), (2048, 300)])
+def test_norms_past_fp32(device, kind, hidden, times):
+    """A row whose norm, not only a product on its way, is past fp32: the 8-bit kinds have the scale NaN, bf16 the infinity."""
+    from vdn_h3_amd.block_kernels import residual_rmsnorm_quantize
+
+    print(f"case residual norm past fp32 {kind} {hidden} x {times}", flush=True)
+    x, res, w = _case(8, hidden, 33)
+    x[:] = res[:] = 0
+    x[:6, 3], x[:6, 5], w[3], w[5] = 1.5, -0.75, 3e38, 1.0  # t w overflows, and t r w the more
+    x[6:, 5] = 1.0  # y = sqrt(hidden) in a channel, none in the others
+    x[5, 3], res[5, 3] = 0.01, 0.01  # t w does not overflow, t r w does
+    x[5, 5] = 0
+    got = residual_rmsnorm_quantize(x.to(device).repeat(times, 1), res.to(device).repeat(times, 1), w.to(device), 0.0, KINDS[kind])
+    assert (po.residual_rmsnorm(x, res, w, 0.0)[1][:6, 3].abs() > 2.0 ** 128).all()
+    codes, scale, _ = (None if t is None else t[-8:] for t in got)
+    if kind == "bf16":
+        assert (codes[:6, 3] == torch.inf).all() and codes[:, [i for i in range(hidden) if i != 3]].isfinite().all()
+    else:
+        assert scale[:6].isnan().all() and (codes[:6].float() == 0).all()
+    _check([None if t is None else t[-2:] for t in got], kind, x[6:], res[6:], w, 0.0)
