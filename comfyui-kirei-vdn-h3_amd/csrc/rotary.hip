@@ -1,6 +1,6 @@
 // q / k RMSNorm (optional) and the rotary embedding of positions on several axes (HBM-bound):
 //
-//   y_d = x_d * r * w_d (with weights; y = x without), the arithmetic of qk_norm.h
+//   y_d = x_d * r * w_d (with weights; y = x without), the arithmetic of qk_norm.h; in 64 bits for vectors whose squares leave fp32
 //   pair i of rot / 2 turns by angle_i = 2 pi * position[axis_i][row] * turns_i:
 //   out_i = y_i cos - y_{i+h} sin,  out_{i+h} = y_i sin + y_{i+h} cos,  h = rot / 2; channels >= rot pass
 //
@@ -49,6 +49,8 @@ struct Vectors {
 template <int LANES, int RB>
 __device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j, int step, int c, int dim, bool rotated,
                                            bool row_turn, int partner, const float2 (&cs)[8]) {
+  // of a mean below 2^-90 the squares fall under what fp32 holds with all bits
+  constexpr float kMostFactor = 0x1p45f;
   const bool live = 8 * c < dim;
   const uint16_t *x = s.x + row * s.row + 8 * c;
   uint16_t *out = s.out + row * s.out_row + 8 * c;
@@ -58,6 +60,30 @@ __device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j,
 #pragma unroll
     for (int i = 0; i < 8; ++i) wf[i] = __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
   }
+  // the turn of a normalised vector, and its store
+  auto finish = [&](float (&y)[8], int h, bool keep) __device__ {
+    float o[8];
+    if (row_turn) {  // the partner is 8 lanes away in a 16-lane DPP row (row_ror:8)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        o[i] = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y[i]), 0x128, 0xf, 0xf, false));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = __shfl(y[i], partner);
+    }
+    if (rotated) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = fmaf(cs[i].x, y[i], cs[i].y * o[i]);
+    }
+    if (live && keep)
+      st16(out + h * s.out_head,
+           u32x4_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7])});
+  };
+  auto unpack = [&](const u32x4_t &raw, float (&y)[8]) __device__ {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __uint_as_float((i & 1) ? (raw[i >> 1] & 0xffff0000u) : (raw[i >> 1] << 16));
+  };
+  bool again = false;
   for (int h0 = j; h0 < s.heads; h0 += RB * step) {
     u32x4_t raw[RB];
 #pragma unroll
@@ -68,31 +94,37 @@ __device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j,
 #pragma unroll
     for (int u = 0; u < RB; ++u) {
       if (h0 + u * step >= s.heads) break;  // a whole lane group
-      float y[8], o[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        y[i] = __uint_as_float((i & 1) ? (raw[u][i >> 1] & 0xffff0000u) : (raw[u][i >> 1] << 16));
+      float y[8];
+      unpack(raw[u], y);
+      bool fits = true;
       if (s.w) {
-        const float r = rms_factor(group_tree_sum<LANES>(chunk_sumsq(y)), dim, s.eps);
+        const float ss = group_tree_sum<LANES>(chunk_sumsq(y)), r = rms_factor(ss, dim, s.eps);
+        fits = r < kMostFactor && ss < INFINITY;
+        again = again || !fits;
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = y[i] * r * wf[i];
       }
-      if (row_turn) {  // the partner is 8 lanes away in a 16-lane DPP row (row_ror:8)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          o[i] = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y[i]), 0x128, 0xf, 0xf, false));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = __shfl(y[i], partner);
-      }
-      if (rotated) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = fmaf(cs[i].x, y[i], cs[i].y * o[i]);
-      }
-      if (live)
-        st16(out + (h0 + u * step) * s.out_head,
-             u32x4_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7])});
+      finish(y, h0 + u * step, fits);
     }
+  }
+  if (!again) return;
+  // Vectors whose squares fp32 does not hold, the norm in 64 bits: in a loop of their own, since in the one above its registers
+  // took a wavefront a SIMD (this way 40,688 rows x 80 heads take 306.6 us, 305.6 without; 512 x 48 6.6, 6.4).
+#pragma unroll 1
+  for (int h = j; h < s.heads; h += step) {
+    float y[8];
+    unpack(live ? ld16(x + h * s.head) : u32x4_t{0, 0, 0, 0}, y);
+    const float fp32 = group_tree_sum<LANES>(chunk_sumsq(y));
+    if (rms_factor(fp32, dim, s.eps) < kMostFactor && fp32 < INFINITY) continue;  // a whole lane group
+    double ss = 0.;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fma((double)y[i], (double)y[i], ss);
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) ss += __shfl_xor(ss, o);
+    const double r = 1. / sqrt(ss / dim + s.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (float)(y[i] * r * wf[i]);
+    finish(y, h, true);
   }
 }
 
@@ -100,7 +132,7 @@ __device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j,
 // widths that R is made for), and share them through LDS. LANES lanes hold a head vector, 8 channels each (dim <= 8 LANES,
 // lanes past it idle), 256 / LANES / R lane groups a row; a group keeps its row's pairs in registers and walks the heads.
 template <int LANES, int R>
-__global__ __launch_bounds__(256) void rotary_kernel(Vectors q, Vectors k, Positions pos, const double *__restrict__ turns,
+__global__ __launch_bounds__(256, LANES == 16 ? 5 : 4) void rotary_kernel(Vectors q, Vectors k, Positions pos, const double *__restrict__ turns,
                                                      const int32_t *__restrict__ axis, int rot, int dim, int rows) {
   constexpr int PAIRS = 4 * LANES, STEP = 256 / LANES / R;
   __shared__ __attribute__((aligned(16))) float2 table[R][PAIRS];

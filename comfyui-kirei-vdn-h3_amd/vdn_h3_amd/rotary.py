@@ -82,7 +82,8 @@ def normalise_qk_axes(q_raw: torch.Tensor, k_raw: torch.Tensor, positions: torch
 
     ``positions``: ``[axes, S]`` int32, int64 or float32 on the GPU, any strides, or ``[S]`` for the same position on every
     axis; positions past 2**53 turns lose their fraction. ``eps`` is q's epsilon, ``k_eps`` k's (``eps`` when ``None``).
-    D is a multiple of 8 up to 128. Returns new contiguous bf16 tensors (fp32 inside, one rounding).
+    D is a multiple of 8 up to 128. Returns new contiguous bf16 tensors (fp32 inside, 64 bits for the norm of vectors whose squares
+    leave it, one rounding).
     """
     if q_raw.ndim != 3 or k_raw.ndim != 3 or q_raw.shape[0] != k_raw.shape[0] or q_raw.shape[2] != k_raw.shape[2]:
         raise ValueError("q must be [sequence, heads, dim] and k [sequence, kv_heads, dim]; "

@@ -139,3 +139,29 @@ def test_refusals_streams_and_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, normalise_qk_axes(q, k, pos, axes)))
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim,sections", [(9, 5, 1, 128, (64,)), (2100, 2, 1, 64, (8, 8)), (5000, 3, 3, 80, (10, 14, 16))])
+def test_vectors_near_the_largest_and_the_smallest_numbers(device, rows, heads, kv, dim, sections):
+    """The norm of a vector does not depend on its size, where its squares pass fp32 and where they fall under it; an infinity
+    or a NaN stays in its vector."""
+    from vdn_h3_amd.rotary import RotaryAxes, normalise_qk_axes
+
+    print(f"case rotary ends of the range {rows}x{heads}/{kv}x{dim}", flush=True)
+    axes = RotaryAxes(sections)
+    qkv, wq, wk, g = _case(rows, heads, kv, dim, 70)
+    for row, by in ((0, 2.0 ** 70), (1, 2.0 ** 120), (2, 2.0 ** -80), (3, 2.0 ** -120), (rows - 1, 2.0 ** 100)):
+        qkv[row] = (qkv[row].float() * by).to(BF)
+    qkv[4, 0], qkv[4, 1] = qkv[4, 0].sign() * 3e38, qkv[4, 1].sign() * 2.0 ** -133
+    pos = torch.randint(0, 4000, (len(sections), rows), generator=g)
+    dev = qkv.to(device)
+    call = lambda x: normalise_qk_axes(x[:, :heads], x[:, heads:heads + kv], pos.to(device), axes, wq.to(device), wk.to(device), 0.0)
+    want = call(dev)
+    _check(want[0], qkv[:, :heads], wq, 0.0, pos, axes)
+    _check(want[1], qkv[:, heads:heads + kv], wk, 0.0, pos, axes)
+    dev[6, 1, 3], dev[7, 0, 5] = torch.nan, torch.inf
+    got = call(dev)
+    for (row, head) in ((6, 1), (7, 0)):
+        assert got[0][row, head].isnan().any()
+        got[0][row, head] = want[0][row, head] = 0
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
