@@ -46,7 +46,8 @@ __device__ __forceinline__ Sequence sequence_at(const Sequences &s, int b) {
 
 // The output row of one query by one wavefront: a lane takes a key of each 64, then two (one) channels of the sum.
 // Keys that the query does not see are not read. Probabilities carry a factor of 2^-24, which cancels, so that up to 2^24
-// values of bf16's largest sum up inside fp32. L2 bounds it, since no two rows share their reads: 2,048 tokens of 40 / 8 heads x
+// values of bf16's largest sum up inside fp32. An infinite value counts as such also where its key's probability, or what a
+// larger score leaves of it, is under fp32's smallest number: the softmax has no zeros but for scores of -inf. L2 bounds it, since no two rows share their reads: 2,048 tokens of 40 / 8 heads x
 // 128 that all see an infinite value take 10 ms (0.09 without), but 0.8 where a token is no number, which ends its rows at once.
 template <int D>
 __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k, int64_t k_row, const uint16_t *v,
@@ -73,14 +74,28 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
     m = m_new;
     l *= corr;
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] *= corr;
+    for (int c = 0; c < C; ++c) o[c] = fabsf(o[c]) == INFINITY ? o[c] : o[c] * corr;
     const int n = min(64, keys - j0);
-    for (int j = 0; j < n; ++j) {
-      const float pj = __shfl(p, j);
-      const uint16_t *vp = v + (int64_t)(j0 + j) * v_row + C * lane;
-      l += pj;
+    const uint64_t faint = __ballot(p == 0.f && s > -INFINITY);
+    if (faint == 0) {
+      for (int j = 0; j < n; ++j) {
+        const float pj = __shfl(p, j);
+        const uint16_t *vp = v + (int64_t)(j0 + j) * v_row + C * lane;
+        l += pj;
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(pj, bf2f(vp[c]), o[c]);
+        for (int c = 0; c < C; ++c) o[c] = fmaf(pj, bf2f(vp[c]), o[c]);
+      }
+    } else {
+      for (int j = 0; j < n; ++j) {
+        const float pj = __shfl(p, j);
+        const uint16_t *vp = v + (int64_t)(j0 + j) * v_row + C * lane;
+        l += pj;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float x = bf2f(vp[c]);
+          o[c] += ((faint >> j) & 1) && fabsf(x) == INFINITY ? x : pj * x;
+        }
+      }
     }
     bool number = false;
 #pragma unroll

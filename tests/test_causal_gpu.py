@@ -396,3 +396,39 @@ def test_repeatable_on_streams_and_in_graphs(device):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, calls())), (first, lengths)
     assert math.isfinite(got[0].float().abs().max().item())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinities_far_below_a_rows_maximum(device, dim):
+    """An infinite value counts however small its key's probability is (an exponential under fp32's smallest number), in
+    front of larger scores and behind them; opposite infinities give a NaN; a score of minus infinity leaves none of it."""
+    from vdn_h3_amd.causal import causal_softmax_cached, causal_softmax_packed
+
+    room, heads, kv = 700, 4, 2
+    g = torch.Generator().manual_seed(61)
+    q = torch.zeros(room, heads, dim)
+    q[..., 0] = 8.0
+    k = 0.1 * torch.randn(room, kv, dim, generator=g)
+    v = torch.randn(room, kv, dim, generator=g).to(BF)
+    k[..., 0] = 0.0
+    for j, score in ((5, -110.0), (40, -400.0), (300, -600.0), (301, -130.0), (302, -88.0), (640, -650.0)):
+        k[j, :, 0] = score / 8
+    k[400:, :, 0] += 12.0  # scores 96 above those in front
+    k[640, :, 0] = -600.0 / 8
+    q, k = q.to(BF), k.to(BF)
+    v[5, :, 1], v[40, :, 2], v[300, :, 3], v[640, :, 4] = torch.inf, -torch.inf, torch.inf, -torch.inf
+    v[301, :, 5], v[302, :, 5] = torch.inf, -torch.inf
+    for new in (1, 60, 350):
+        print(f"case infinities far below {new} of {room} x {dim}", flush=True)
+        out, size, score = po.packed(q, k, v, [0, room], 1.0)
+        assert (out[-1, :, [1, 3]] == torch.inf).all() and (out[-1, :, [2, 4]] == -torch.inf).all() and out[-1, :, 5].isnan().all()
+        n = torch.tensor([room], dtype=torch.int32, device=device)
+        caches = (q[None, -new:].to(device), k[None].to(device), v[None].to(device), n, 1.0)
+        some = [causal_softmax_cached(*caches)] + [_cached_in(r, *caches) for r in (0, 1, 3, 9)]
+        full = causal_softmax_packed(q.to(device), k.to(device), v.to(device), [0, room], 1.0)
+        for got, want in [(t[0], [w[-new:] for w in (out, size, score)]) for t in some] + [(full, (out, size, score))]:
+            got = got.cpu()
+            odd = ~want[0].isfinite()
+            assert torch.equal(got[odd].nan_to_num(7.0), want[0][odd].to(BF).nan_to_num(7.0))
+            assert got[~odd].isfinite().all()
+            _check(got.masked_fill(odd, 0), [want[0].masked_fill(odd, 0), want[1].masked_fill(odd, 0), want[2]], dim)
