@@ -942,6 +942,8 @@ __global__ __launch_bounds__(kFewThreads) void causal_combine_kernel(Operand q, 
   }
 }
 
+constexpr float kLog2E = 1.4426950408889634f;
+
 // Rows of a cache: keys are counted in 32 bits, up to the end of a tile behind the last.
 constexpr int kMostRoom = INT32_MAX - 4 * kBN;
 
@@ -964,8 +966,8 @@ int check_causal(const Operand &q, const Operand &k, const Operand &v, const Ope
                    "causal attention supports head_dim 64 or 128, got %d", head_dim);
   VDNH3_HOST_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, VDNH3_ERR_INVALID,
                    "causal attention: heads (%d) must be a multiple of the key / value heads (%d)", heads, kv_heads);
-  VDNH3_HOST_CHECK(scale > 0.f && scale < INFINITY, VDNH3_ERR_INVALID,
-                   "causal attention: scale must be positive and finite");
+  VDNH3_HOST_CHECK(scale > 0.f && scale * kLog2E < INFINITY, VDNH3_ERR_INVALID,
+                   "causal attention: scale must be positive, and finite times log2(e)");
   int rc = check_operand(q, "q");
   if (!rc) rc = check_operand(k, "k");
   if (!rc) rc = check_operand(v, "v");
@@ -990,7 +992,7 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
   if (!rc) rc = check_grid(blocks * kv_heads, kThreads, "causal attention");
   if (rc) return rc;
   hipLaunchKernelGGL((causal_tile_kernel<D, NQ>), dim3((unsigned)(blocks * kv_heads)), dim3(kThreads), 0, s, q, k, v, out, seqs,
-                     (int)blocks, kv_heads, group, scale * 1.4426950408889634f);
+                     (int)blocks, kv_heads, group, scale * kLog2E);
   return check_launch("causal attention");
 }
 
@@ -1139,7 +1141,7 @@ extern "C" int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int6
                    VDNH3_ERR_INVALID, "causal attention: the ranges' buffer must be 16-byte aligned and hold %zu bytes, got %zu",
                    need, partial_bytes);
   const Parts parts{partial, reinterpret_cast<float2 *>(partial + (size_t)ranges * 2 * new_tokens * heads * head_dim), ranges};
-  const float scale_log2 = scale * 1.4426950408889634f;
+  const float scale_log2 = scale * kLog2E;
   return head_dim == 128 ? launch_few_rows<128>(qo, ko, vo, oo, seqs, kv_heads, group, scale_log2, parts, s)
                          : launch_few_rows<64>(qo, ko, vo, oo, seqs, kv_heads, group, scale_log2, parts, s);
 }

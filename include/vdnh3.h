@@ -539,7 +539,8 @@ int vdnh3_qk_rotary_axes(const uint16_t *q, int64_t q_row, int64_t q_head, const
 
 /* Causal softmax attention of packed sequences, query head h on key / value head h / (heads / kv_heads): sequence b
  * is the rows [cu_seqlens[b], cu_seqlens[b + 1]) (device, sequences + 1 values, cut to [0, rows]) of q, k, v and
- * out; its row i sees its rows 0 .. i. Rows of no sequence are not written. head_dim 64 or 128, scale > 0. */
+ * out; its row i sees its rows 0 .. i. Rows of no sequence are not written. head_dim 64 or 128, scale > 0
+ * and finite times log2(e). */
 int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_t q_head, const uint16_t *k, int64_t k_row,
                              int64_t k_head, const uint16_t *v, int64_t v_row, int64_t v_head, uint16_t *out,
                              int64_t o_row, int64_t o_head, const int32_t *cu_seqlens, int sequences, int rows, int heads,

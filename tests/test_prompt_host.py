@@ -213,3 +213,18 @@ def test_launch_makes_the_tensors_device_current(monkeypatch):
     _lib.launch("x", call, torch.device("cuda:0"), 1, 2)
     _lib.launch("x", call, torch.device("cuda:1"), 3)
     assert seen[0] == ((1, 2, 77), []) and seen[1] == ((3, 77), [torch.device("cuda:1")]) and entered[-1] is None
+
+
+def test_scales_past_fp32_are_refused(built_lib):
+    """The kernels take scale * log2(e): a finite scale whose product is none gave NaNs. Nothing is launched either way: the null
+    bounds and lengths are refused behind the scale."""
+    from vdn_h3_amd import _lib
+
+    lib, p = _lib.lib(), 1 << 20
+    for scale, word in ((3e38, "scale"), (2.4e38, "scale"), (2.3e38, "null")):
+        assert lib.vdnh3_causal_attn_packed(p, 256, 64, p, 128, 64, p, 128, 64, p, 256, 64, None, 1, 4, 4, 2, 64, scale,
+                                            None) == _lib.VDNH3_ERR_INVALID
+        assert word in _lib.last_error(), (scale, _lib.last_error())
+        assert lib.vdnh3_causal_attn_cached(p, 256, 256, 64, p, 8192, 128, 64, p, 8192, 128, 64, p, 256, 256, 64, None, 2, 1, 64, 4,
+                                            2, 64, scale, 0, None, 0, None) == _lib.VDNH3_ERR_INVALID
+        assert word in _lib.last_error(), (scale, _lib.last_error())
