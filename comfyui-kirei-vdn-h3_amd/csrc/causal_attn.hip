@@ -1002,10 +1002,13 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
 // fit a CU, 4,000 x 20 / 20 (313) 65 against 74, 8,000 x 32 / 8 (1,000) 325 against 296.
 constexpr int kHighGroups128 = 288, kHighGroups64 = 512;
 
+bool high_blocks(int sequences, int rows, int heads, int head_dim) {
+  return (double)rows * sequences * heads / 256 >= (head_dim == 128 ? kHighGroups128 : kHighGroups64);
+}
+
 int launch_causal(const Operand &q, const Operand &k, const Operand &v, const Operand &out, const Sequences &seqs, int heads,
                   int kv_heads, int head_dim, float scale, hipStream_t s) {
-  const bool high = (double)seqs.rows * (seqs.cu ? 1 : seqs.count) * heads / 256 >=
-                    (head_dim == 128 ? kHighGroups128 : kHighGroups64);
+  const bool high = high_blocks(seqs.cu ? 1 : seqs.count, seqs.rows, heads, head_dim);
   if (head_dim == 128)
     return high ? launch_tiles<128, 2>(q, k, v, out, seqs, heads, kv_heads, scale, s)
                 : launch_tiles<128, 1>(q, k, v, out, seqs, heads, kv_heads, scale, s);
@@ -1104,6 +1107,13 @@ extern "C" int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, i
     if (us < least) least = us, ranges = r;
   }
   return (int)ranges;
+}
+
+extern "C" int vdnh3_causal_block_rows(int batch, int new_tokens, int heads, int kv_heads, int head_dim, int ranges) {
+  using namespace vdnh3;
+  if (batch <= 0 || new_tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || ranges < 0) return 0;
+  if (ranges > 0) return few_block((int64_t)new_tokens * (heads / kv_heads));
+  return high_blocks(batch, new_tokens, heads, head_dim) ? 256 : 128;
 }
 
 extern "C" size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges) {

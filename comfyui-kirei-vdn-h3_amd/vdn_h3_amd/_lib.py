@@ -120,6 +120,7 @@ SIGNATURES = {
                                           _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int, _c_int, _c_int, _c_int,
                                           _c_int, _c_int, _c_float, _c_int, _vp, _c_size, _vp]),
     "vdnh3_causal_cached_ranges": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "vdnh3_causal_block_rows": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "vdnh3_causal_partial_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
     "vdnh3_head_gate": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int, _vp]),
     "vdnh3_mfma_peak": (_c_int, [_c_int, _vp, _vp, _c_int, _c_int, _vp, _vp]),

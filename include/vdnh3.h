@@ -553,6 +553,9 @@ int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_t q_head, c
  * (vdnh3_causal_partial_bytes, 16-byte aligned; 0 bytes for one range) and combined. vdnh3_causal_cached_ranges gives
  * the number that suits a call (0 where the kernel of whole prompts is faster). */
 int vdnh3_causal_cached_ranges(int batch, int new_tokens, int room, int heads, int kv_heads, int head_dim);
+/* Rows, (token, query head) pairs, of a workgroup of such a call: 16, 32 or 48 with ranges, 128 or 256 without (whole
+ * prompts: batch 1 and all rows as its new tokens). */
+int vdnh3_causal_block_rows(int batch, int new_tokens, int heads, int kv_heads, int head_dim, int ranges);
 size_t vdnh3_causal_partial_bytes(int new_tokens, int heads, int head_dim, int ranges);
 int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
                              int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch,
