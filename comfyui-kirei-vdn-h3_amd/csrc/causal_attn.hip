@@ -47,8 +47,9 @@ __device__ __forceinline__ Sequence sequence_at(const Sequences &s, int b) {
 // The output row of one query by one wavefront: a lane takes a key of each 64, then two (one) channels of the sum.
 // Keys that the query does not see are not read. Probabilities carry a factor of 2^-24, which cancels, so that up to 2^24
 // values of bf16's largest sum up inside fp32. An infinite value counts as such also where its key's probability, or what a
-// larger score leaves of it, is under fp32's smallest number: the softmax has no zeros but for scores of -inf. L2 bounds it, since no two rows share their reads: 2,048 tokens of 40 / 8 heads x
-// 128 that all see an infinite value take 10 ms (0.09 without), but 0.8 where a token is no number, which ends its rows at once.
+// larger score leaves of it, is under fp32's smallest number: the softmax has no zeros but for scores of -inf. L2 bounds it,
+// since no two rows share their reads: 2,048 tokens of 40 / 8 heads x 128 that all see an infinite value take 10.7 ms (0.09
+// without), 4,096 take 30, but 2,048 take 0.8 where a token is no number, which ends its rows at once.
 template <int D>
 __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k, int64_t k_row, const uint16_t *v,
                                            int64_t v_row, int keys, float scale_log2, uint16_t *out, int lane) {
@@ -120,8 +121,9 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
 // What bounds it: the issue of the SIMD that two wavefronts share. A phase's 102 MFMAs of 16 cycles and the softmax beside
 // them, about 1,400 cycles of VALU (a third of it the exponentials), take 2,500 cycles together; LDS is busy for 28% of
 // the time, without bank conflicts, and fragment reads 2 to 6 ahead measure the same. 8,296 rows x 40 / 8 heads x 128 take
-// 585 us, 1,205 TFLOP/s, where the library's 8,192^3 product reaches 1,367. Short prompts are bound by a workgroup's start
-// and end, about 6 us (its block, the first loads, two more phases than tiles, the stores): 512 rows take 15.0 us.
+// 605 us, 1,165 TFLOP/s, where the library's 8,192^3 product reaches 1,367 (585 us on another card). With 64 channels a tile has
+// half the products and the same softmax: 8,000 rows x 32 / 8 take 300 us, VALU 55% and matrix cores 39% of them. Short prompts are bound by a workgroup's start
+// and end, about 6 us (its block, the first loads, two more phases than tiles, the stores): 512 rows take 15.1 us.
 constexpr int kBN = 96;        // keys per tile
 constexpr int kThreads = 512;
 constexpr int kRing = 3;       // LDS slots per K and V ring (144 KB at D = 128): loads run kRing - 1 tiles ahead
@@ -498,9 +500,9 @@ __global__ __launch_bounds__(kThreads, 1) void causal_tile_kernel(Operand q, Ope
 // A workgroup takes 16 NQ of a head's (token, head) rows, up to 48 (64 spill). Its wavefronts take the tiles in turn, each
 // through two LDS slots of its own (one tile in flight while it works on the other, no barrier), with a running softmax of its
 // own; they are merged in LDS at the end of a sequence. HBM bounds it: 64 requests of up to 8,192 keys x 8 heads x 128
-// (1.1 GB) take 190 us, 5.7 TB/s where a copy reaches 4.8; one request of 40,688 keys (167 MB) 30 us and 6 for the
+// (1.1 GB) take 196 us, 5.6 TB/s where a copy reaches 4.8; one request of 40,688 keys (167 MB) 30 us and 6 for the
 // combination, which is a launch and a chain of three loads. 32 new tokens over them (four blocks of rows, 78 MFMAs a tile) take
-// 93 us: a chain too, of a tile's products, maxima and exponentials in the only wavefront of a SIMD. With fixed chunks of keys
+// 91 us: a chain too, of a tile's products, maxima and exponentials in the only wavefront of a SIMD. With fixed chunks of keys
 // instead of equal ranges the 64 requests took 215 to 244 us, whole rounds of workgroups each with a pipeline to fill.
 constexpr int kFewKeys = 32;      // keys per tile: one k-step of the PV product
 constexpr int kFewRing = 2;
@@ -999,7 +1001,7 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
 // Workgroups of 256 rows from which on they are taken; with fewer, workgroups of 128 (which read twice the LDS for the same
 // products) leave fewer CUs without one and end closer together. 512 rows x 40 / 8 x 128 15 us against 23, 4,148 x 16 / 2
 // (260 workgroups) 88 against 98, 2,000 x 40 / 8 (313) 67 against 60, 8,296 751 against 588; with 64 channels, where two
-// fit a CU, 4,000 x 20 / 20 (313) 65 against 74, 8,000 x 32 / 8 (1,000) 325 against 296.
+// of 128 rows fit a CU (125 registers; 256 rows take 186), 4,000 x 20 / 20 (313) 65 against 74, 8,000 x 32 / 8 (1,000) 325 against 296.
 constexpr int kHighGroups128 = 288, kHighGroups64 = 512;
 
 bool high_blocks(int sequences, int rows, int heads, int head_dim) {
@@ -1080,7 +1082,7 @@ extern "C" int vdnh3_causal_attn_packed(const uint16_t *q, int64_t q_row, int64_
 //            1.45 (48 rows: 1.85) per 4 tiles of 32 keys and 4.3 (9.6) for every sequence that a range crosses into; those
 //            0.84 times with 64 channels
 // The constants are a fit to 4,477 calls: 1 to 64 requests, 64 to 40,960 rows of cache, 1 to 64 new tokens, 7 layouts of heads, up
-// to 7 ways each. The choice then takes 0.9% longer than the best of them in the mean, 4.5% at the 95th percentile; ranges
+// to 7 ways each. The choice then takes 0.9% longer than the best of them in the mean, 4.8% at the 95th percentile; ranges
 // for all calls up to 16 rows, one round of them, and a coarser estimate for more took 19% and 2.3 times. E.g. one token of
 // 40 / 8 heads x 128 over 40,688 keys: 32 ranges 41, 0: 452; over 300 keys of 2 requests 5: 12, 0: 9; 64 requests of 512 keys and 3
 // tokens 32: 42, 0: 33; of 8,192 keys at most 32: 190, 0: 215.

@@ -3,10 +3,11 @@
 * ``causal_softmax_packed``: whole prompts of different lengths, packed one behind another;
 * ``causal_softmax_cached``: one or several new tokens of each request over the requests' key / value caches.
 
-Both take bf16 and hold scores, sums and softmax statistics in fp32. The products with the values take the probabilities as
-bf16 (2.0e-3 of the result, with the result's own rounding of 1.6e-3), in ranges of long caches as two bf16 numbers (1.7e-3).
-Query head ``h`` reads key / value head ``h // (heads // kv_heads)``. Sequence bounds are read on the device: a call needs no copy to the host, and a captured one
-can be replayed with other lengths. Forward-only; there is no CPU path.
+Both take bf16 and hold scores, sums and softmax statistics in fp32 (q . k, before the scale too, has to stay inside its range).
+The products with the values take the probabilities as bf16 (2.0e-3 of the result, with the result's own rounding of 1.6e-3), in
+ranges of long caches as two bf16 numbers (1.7e-3). Query head ``h`` reads key / value head ``h // (heads // kv_heads)``. Sequence
+bounds are read on the device: a call needs no copy to the host, and a captured one can be replayed with other lengths. Rows that
+see an infinity are computed one by one, in a time that grows with the square of the tokens. Forward-only; there is no CPU path.
 """
 
 from __future__ import annotations
@@ -121,7 +122,8 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     ``lengths`` (``[B]`` int32 on the GPU, another integer type is converted) counts a request's valid cache rows, the
     new tokens' own keys and values (its last N rows) among them: token ``i`` attends to rows 0 to ``lengths[b] - N + i``.
     A token in front of the first row (``lengths[b] < N``) attends to nothing and gives zeros. Rows behind a length are
-    not used, whatever they hold. Lengths are cut to ``[0, room]``. Head dims 64 and 128; the caches are read in place, so
+    not used, whatever they hold. Lengths are cut to ``[0, room]``. Kernel and ranges go by the whole batch, so that a request's last
+    bits can differ with the requests beside it. Head dims 64 and 128; the caches are read in place, so
     their layout has to suit the kernel (16-byte rows, at most 2**23 elements apart). ``out`` must not overlap the inputs.
     """
     if query.ndim != 4 or key_cache.ndim != 4 or key_cache.shape != value_cache.shape or \

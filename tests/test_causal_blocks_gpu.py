@@ -164,3 +164,17 @@ def test_high_blocks_against_float64(device, built_lib, lengths, heads, kv, dim,
         odd = ~out.isfinite()
         _check(got[a:e][at].masked_fill(odd, 0), (out.masked_fill(odd, 0), size.masked_fill(odd, 0), score), dim)
         assert got[e - 30:e].isnan().all()
+
+
+@pytest.mark.parametrize("new,heads,kv,dim", [(1, 10, 2, 128), (5, 8, 1, 64), (40, 6, 2, 128)])
+def test_a_request_beside_others_of_other_lengths(device, new, heads, kv, dim):
+    """By the prompt kernel and in one range a request's result does not depend on the lengths beside it."""
+    print(f"case beside others {new} {heads}/{kv}x{dim}", flush=True)
+    q, k, v = (t.view(4, -1, t.shape[1], dim).to(device) for t in _qkv(4 * 600, heads, kv, dim, 72, loud=2.0))
+    q = q[:, :new]
+    for ranges in (0, 1):
+        seen = []
+        for lengths in ([600, 431, 0, 77], [3, 431, 600, 599], [431, 431, 431, 1]):
+            n = torch.tensor(lengths, dtype=torch.int32, device=device)
+            seen.append(_cached_in(ranges, q, k, v, n, 0.1)[1])
+        assert torch.equal(seen[0], seen[1]) and torch.equal(seen[0], seen[2]), ranges
