@@ -82,6 +82,8 @@ def causal_softmax_packed(query: torch.Tensor, key: torch.Tensor, value: torch.T
         raise ValueError("query must be [rows, heads, dim], key and value [rows, kv_heads, dim]; got "
                          f"{tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}")
     _check_heads(query, key, value, "causal_softmax_packed")
+    if not 0 < query.shape[2] <= KERNEL_HEAD_DIMS[-1]:
+        raise ValueError(f"causal_softmax_packed supports head dims 1 to {KERNEL_HEAD_DIMS[-1]}, got {query.shape[2]}")
     _lib.forward_only("causal_softmax_packed", query, key, value, out)
     rows, heads, dim = query.shape
     _lib.int32_sizes("causal_softmax_packed", rows, heads)
@@ -134,6 +136,8 @@ def causal_softmax_cached(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     batch, new, heads, dim = query.shape
     room, kv_heads = key_cache.shape[1], key_cache.shape[2]
     _lib.int32_sizes("causal_softmax_cached", batch, new, room, heads)
+    if not isinstance(lengths, torch.Tensor):
+        raise TypeError(f"lengths must be a tensor of {batch} integers, got {type(lengths).__name__}")
     if lengths.ndim != 1 or lengths.numel() != batch or lengths.dtype not in _INTEGERS:
         raise ValueError(f"lengths must hold {batch} integers, got {tuple(lengths.shape)} {lengths.dtype}")
     if dim not in KERNEL_HEAD_DIMS:

@@ -228,3 +228,17 @@ def test_scales_past_fp32_are_refused(built_lib):
         assert lib.vdnh3_causal_attn_cached(p, 256, 256, 64, p, 8192, 128, 64, p, 8192, 128, 64, p, 256, 256, 64, None, 2, 1, 64, 4,
                                             2, 64, scale, 0, None, 0, None) == _lib.VDNH3_ERR_INVALID
         assert word in _lib.last_error(), (scale, _lib.last_error())
+
+
+def test_attention_names_itself_where_it_refuses(built_lib):
+    """Head dims that no kernel takes, and lengths that are no tensor."""
+    from vdn_h3_amd.causal import causal_softmax_cached as cached, causal_softmax_packed as packed
+
+    for dim in (0, 136):
+        q, k = _z(6, 4, dim), _z(6, 2, dim)
+        with pytest.raises(ValueError, match="causal_softmax_packed supports head dims"):
+            packed(q, k, k, [0, 6], 0.1)
+    q, k = _z(2, 1, 4, 64), _z(2, 9, 2, 64)
+    for lengths in ([3, 4], 3, None):
+        with pytest.raises(TypeError, match="lengths must be a tensor"):
+            cached(q, k, k, lengths, 0.1)
