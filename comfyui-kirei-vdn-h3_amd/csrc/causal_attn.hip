@@ -122,8 +122,9 @@ __device__ __forceinline__ void attend_row(const uint16_t *q, const uint16_t *k,
 // them, about 1,400 cycles of VALU (a third of it the exponentials), take 2,500 cycles together; LDS is busy for 28% of
 // the time, without bank conflicts, and fragment reads 2 to 6 ahead measure the same. 8,296 rows x 40 / 8 heads x 128 take
 // 605 us, 1,165 TFLOP/s, where the library's 8,192^3 product reaches 1,367 (585 us on another card). With 64 channels a tile has
-// half the products and the same softmax: 8,000 rows x 32 / 8 take 300 us, VALU 55% and matrix cores 39% of them. Short prompts are bound by a workgroup's start
-// and end, about 6 us (its block, the first loads, two more phases than tiles, the stores): 512 rows take 15.1 us.
+// half the products and the same softmax: 8,000 rows x 32 / 8 take 300 us, VALU 55% and matrix cores 39% of them. Short prompts
+// are bound by a workgroup's start and end, about 6 us (its block, the first loads, two more phases than tiles, the stores): 512
+// rows take 15.1 us.
 constexpr int kBN = 96;        // keys per tile
 constexpr int kThreads = 512;
 constexpr int kRing = 3;       // LDS slots per K and V ring (144 KB at D = 128): loads run kRing - 1 tiles ahead
@@ -1000,8 +1001,9 @@ int launch_tiles(const Operand &q, const Operand &k, const Operand &v, const Ope
 
 // Workgroups of 256 rows from which on they are taken; with fewer, workgroups of 128 (which read twice the LDS for the same
 // products) leave fewer CUs without one and end closer together. 512 rows x 40 / 8 x 128 15 us against 23, 4,148 x 16 / 2
-// (260 workgroups) 88 against 98, 2,000 x 40 / 8 (313) 67 against 60, 8,296 751 against 588; with 64 channels, where two
-// of 128 rows fit a CU (125 registers; 256 rows take 186), 4,000 x 20 / 20 (313) 65 against 74, 8,000 x 32 / 8 (1,000) 325 against 296.
+// (260 workgroups) 88 against 98, 2,000 x 40 / 8 (313) 67 against 60, 8,296 751 against 588; with 64 channels, where two of 128
+// rows fit a CU (125 registers; 256 rows take 186, one workgroup), 4,000 x 20 / 20 (313) 65 against 74, 8,000 x 32 / 8 (1,000)
+// 325 against 296.
 constexpr int kHighGroups128 = 288, kHighGroups64 = 512;
 
 bool high_blocks(int sequences, int rows, int heads, int head_dim) {

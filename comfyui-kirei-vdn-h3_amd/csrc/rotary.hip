@@ -109,7 +109,8 @@ __device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j,
   }
   if (!again) return;
   // Vectors whose squares fp32 does not hold, the norm in 64 bits: in a loop of their own, since in the one above its registers
-  // took a wavefront a SIMD (this way 40,688 rows x 80 heads take 306.6 us, 305.6 without; 512 x 48 6.6, 6.4).
+  // took a wavefront a SIMD (of contiguous operands 40,688 rows x 80 heads take 306.6 us this way, 305.6 without; 512 x 48 6.6
+  // and 6.4).
 #pragma unroll 1
   for (int h = j; h < s.heads; h += step) {
     float y[8];
@@ -132,8 +133,10 @@ __device__ __forceinline__ void turn_heads(const Vectors &s, int64_t row, int j,
 // widths that R is made for), and share them through LDS. LANES lanes hold a head vector, 8 channels each (dim <= 8 LANES,
 // lanes past it idle), 256 / LANES / R lane groups a row; a group keeps its row's pairs in registers and walks the heads.
 template <int LANES, int R>
-__global__ __launch_bounds__(256, LANES == 16 ? 5 : 4) void rotary_kernel(Vectors q, Vectors k, Positions pos, const double *__restrict__ turns,
-                                                     const int32_t *__restrict__ axis, int rot, int dim, int rows) {
+__global__ __launch_bounds__(256, LANES == 16 ? 5 : 4) void rotary_kernel(Vectors q, Vectors k, Positions pos,
+                                                                          const double *__restrict__ turns,
+                                                                          const int32_t *__restrict__ axis, int rot, int dim,
+                                                                          int rows) {
   constexpr int PAIRS = 4 * LANES, STEP = 256 / LANES / R;
   __shared__ __attribute__((aligned(16))) float2 table[R][PAIRS];
   const int half = rot >> 1, tid = threadIdx.x;

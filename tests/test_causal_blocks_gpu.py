@@ -91,8 +91,8 @@ def test_every_key_of_a_cache_counts_once(device, built_lib, new, lengths, room,
 
 
 HIGH_CACHED = [  # new tokens, lengths, room, heads, kv heads, dim: the prompt kernel over caches, 256 rows a workgroup
-    (1000, [1500, 600, 0], 1500, 40, 8, 128), (700, [700, 1100, 33, 2], 1100, 28, 4, 128), (1100, [1100, 0, 40, 2000], 2000, 32, 8, 64),
-    (2300, [2300, 2301, 5], 2304, 20, 20, 64)]
+    (1000, [1500, 600, 0], 1500, 40, 8, 128), (700, [700, 1100, 33, 2], 1100, 28, 4, 128),
+    (1100, [1100, 0, 40, 2000], 2000, 32, 8, 64), (2300, [2300, 2301, 5], 2304, 20, 20, 64)]
 
 
 @pytest.mark.parametrize("new,lengths,room,heads,kv,dim", HIGH_CACHED)
