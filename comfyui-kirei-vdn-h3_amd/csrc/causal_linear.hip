@@ -1,0 +1,526 @@
+// Causal linear attention with a decay for each head on gfx950, bf16, states fp32: whole prompts of several sequences
+// packed one behind another. (New tokens over a pool of states: state_step.hip.)
+//
+//   S_t = a_h S_{t-1} + v_t k_t^T,   o_t = scale S_t q_t,   a_h = exp(log_decay_h)       S: [dv, dk] per value head h
+//
+// Value head h reads query / key head h / (heads / qk_heads). Sequence b is the rows [cu[b], cu[b + 1]); its state
+// starts from initial[b] or zeros. With chunks of C = 64 tokens that begin with their sequence, row r of a chunk of n:
+//   o_r = scale (a^{r+1} S q_r + sum_{j <= r} a^{r-j} (q_r . k_j) v_j),   S' = a^n S + sum_j a^{n-1-j} v_j k_j^T
+#include <cmath>
+
+#include "common.h"
+
+namespace vdnh3 {
+namespace {
+
+constexpr int kLinC = 64;  // tokens of a chunk
+
+struct LinOperand {
+  const uint16_t *p;
+  int64_t row, head;
+};
+
+struct LinCall {
+  LinOperand q, k, v;
+  uint16_t *out;
+  int64_t o_row, o_head;
+  const float *log_decay;
+  const int32_t *cu;
+  const float *initial;
+  float *final_state;
+  float *carry;    // [ranges, heads, D, D]: the state at the end of a range, where its last sequence goes on
+  int32_t *meta;   // [ranges]: tokens of a range that lies in one sequence begun before it, -1 for others
+  int sequences, rows, heads, group, ranges;
+  float scale;
+};
+
+// a^n of a head from log2 a. 0 * -inf (a head that keeps nothing) is 1 here.
+__device__ __forceinline__ float decay_pow(float log2a, int n) {
+  return n == 0 ? 1.f : __builtin_amdgcn_exp2f(log2a * (float)n);
+}
+
+__device__ __forceinline__ int lin_bound(const LinCall &p, int b) { return min(max(p.cu[b], 0), p.rows); }
+
+// Where a workgroup is: sequence b (rows [s0, s1)), the chunk that begins at row `row` of q, k and v.
+struct LinPlace {
+  int b, s0, s1, row;
+};
+
+// The workgroup's range of the chunks of all sequences, one sequence behind another: equal ranges, whatever the lengths, and
+// none empty in front of one that is not. Every thread adds up the chunks of sequences next to each other; the one that has the
+// range's first chunk finds its sequence. `count` chunks begin at `at`.
+struct LinRange {
+  int64_t count;
+  LinPlace at;
+};
+template <int THREADS>
+__device__ __forceinline__ LinRange lin_range(const LinCall &p, int range, int64_t *sums, int *found) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (p.sequences + THREADS - 1) / THREADS;
+  const int b0 = (int)min((int64_t)tid * per, (int64_t)p.sequences), b1 = min(b0 + per, p.sequences);
+  auto chunks_of = [&](int b, int &s, int &e) __device__ {
+    s = lin_bound(p, b);
+    e = max(lin_bound(p, b + 1), s);
+    return (e - s + kLinC - 1) / kLinC;
+  };
+  int64_t mine = 0;
+  int s, e;
+  for (int b = b0; b < b1; ++b) mine += chunks_of(b, s, e);
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t x = __shfl_up(upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) upto += sums[w];
+    total += sums[w];
+  }
+  const int64_t ranges = min((int64_t)p.ranges, total);
+  if (range >= ranges) return LinRange{0, LinPlace{0, 0, 0, 0}};
+  const int64_t c0 = total * range / ranges, c1 = total * (range + 1) / ranges;
+  int64_t c = c0 - (upto - mine);
+  if (c >= 0 && c0 < upto) {
+    int b = b0, n = chunks_of(b, s, e);
+    while (c >= n) {  // the thread's sequences hold more than c chunks
+      c -= n;
+      n = chunks_of(++b, s, e);
+    }
+    found[0] = b;
+    found[1] = s;
+    found[2] = e;
+    found[3] = s + (int)c * kLinC;
+  }
+  __syncthreads();
+  return LinRange{c1 - c0, LinPlace{__builtin_amdgcn_readfirstlane(found[0]), __builtin_amdgcn_readfirstlane(found[1]),
+                                    __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3])}};
+}
+
+// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Q and K: the 16 rows of a fragment read hit 16
+// different 16-byte bank groups, and the transposed reads of K, 8 bytes of four chunks of eight rows, cover all banks as
+// evenly as halves of chunks can. V: the 8 rows that half a wavefront reads 32 bytes of hit 8 different 32-byte groups.
+template <int D>
+__device__ __forceinline__ int qk_swizzle(int r) {
+  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int r) {
+  if constexpr (D == 128) return 2 * (r & 7);
+  else return 2 * ((r >> 1) & 3);
+}
+
+typedef short lin_s16x4_t __attribute__((ext_vector_type(4)));
+// Four rows of one channel per lane: 16 lanes read 4 rows of 16 channels (lane i: 4 channels of row i / 4) and get their
+// transpose (lane i: channel i of the 4 rows).
+__device__ __forceinline__ u32x2_t lin_read_transposed(const uint16_t *p) {
+  typedef __attribute__((address_space(3))) lin_s16x4_t *lds_ptr;
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)));
+}
+
+// x as bf16 numbers that add up to it: hi + lo hold 16 bits of it, hi + mid + lo all 24.
+struct Split2 {
+  u32x4_t hi, lo;
+};
+__device__ __forceinline__ float lo_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ Split2 split2(const float *x) {
+  Split2 s;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    s.hi[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
+    s.lo[j] = pack_bf2(x[2 * j] - lo_half(s.hi[j]), x[2 * j + 1] - hi_half(s.hi[j]));
+  }
+  return s;
+}
+
+// A workgroup of D / 16 wavefronts walks a range of a head's chunks; a wavefront carries 16 rows (dv) of the state in
+// accumulators, as C[dk][dv] tiles whose dk are ordered so that a lane's registers are the operand of S q as they lie:
+// row m of tile t is dk = 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. Outputs are computed transposed, O^T[dv][row].
+// CARRY: only the state at the range's end, where the last sequence goes on behind it.
+template <int D, bool CARRY>
+__global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
+  constexpr int C = kLinC, KC = D / 8, NW = D / 16, THREADS = 64 * NW, TILE = C * D;
+  constexpr int NS = D / 32;            // k-steps over dk
+  constexpr int PT = NW == 8 ? 2 : 4;   // 16 x 16 tiles of P that a wavefront makes at most
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][TILE], Vs[2][TILE];
+  __shared__ __attribute__((aligned(16))) uint16_t Qs[CARRY ? 1 : 2][CARRY ? 8 : TILE];
+  __shared__ __attribute__((aligned(16))) u32x4_t Ps[CARRY ? 1 : 2][CARRY ? 1 : 8][64];  // hi / lo, (row tile, k-step), lane
+  __shared__ int64_t sums[NW];
+  __shared__ int found[4];
+
+  const int h = (int)blockIdx.x % p.heads, range = (int)blockIdx.x / p.heads, hk = h / p.group;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const float log2a = p.log_decay[h] * 1.44269504088896341f;
+  LinRange rg = lin_range<THREADS>(p, range, sums, found);
+  const int dv = 16 * wave + l16;  // the lane's row of the state
+
+  // ---- states between memory and the accumulators -----------------------------------------------------------------
+  f32x4_t s[D / 16];
+  auto load_state = [&](const float *from) __device__ {
+    if (from == nullptr) {
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) s[t] = f32x4_t{};
+      return;
+    }
+    const float *r = from + (int64_t)dv * D + 8 * g;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) s[t] = *reinterpret_cast<const f32x4_t *>(r + 32 * (t / 2) + 4 * (t % 2));
+  };
+  auto store_state = [&](float *to) __device__ {
+    float *r = to + (int64_t)dv * D + 8 * g;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t *>(r + 32 * (t / 2) + 4 * (t % 2)) = s[t];
+  };
+  const int64_t state_at = (int64_t)h * D * D, state_step = (int64_t)p.heads * D * D;
+  auto initial_of = [&](int b) __device__ { return p.initial ? p.initial + b * state_step + state_at : nullptr; };
+  // empty sequences from b on end as they began; the first that is not empty
+  auto pass_empty = [&](int b) __device__ {
+    for (; b < p.sequences && lin_bound(p, b + 1) <= lin_bound(p, b); ++b) {
+      if (CARRY || !p.final_state) continue;
+      const float *from = initial_of(b);
+      float *to = p.final_state + b * state_step + state_at;
+      for (int i = 4 * tid; i < D * D; i += 4 * THREADS)
+        *reinterpret_cast<f32x4_t *>(to + i) = from ? *reinterpret_cast<const f32x4_t *>(from + i) : f32x4_t{};
+    }
+    return b;
+  };
+
+  if (CARRY) {
+    if (tid == 0 && h == 0) p.meta[range] = -1;
+    if (rg.count <= 0) return;
+    // the range's last chunk and the sequence that it is of; nothing to do where that ends here
+    LinPlace at = rg.at;
+    int64_t left = rg.count;
+    bool open = at.row > at.s0;
+    while (true) {
+      const int chunks = (at.s1 - at.row + C - 1) / C;
+      if (chunks == left) return;
+      if (chunks > left) break;
+      left -= chunks;
+      int b = at.b + 1;
+      while (lin_bound(p, b + 1) <= lin_bound(p, b)) ++b;  // there is a chunk left, so one of them is not empty
+      at = LinPlace{b, lin_bound(p, b), lin_bound(p, b + 1), lin_bound(p, b)};
+      open = false;
+    }
+    rg = LinRange{left, at};
+    if (tid == 0 && h == 0 && open) p.meta[range] = (int)left * C;
+    load_state(open ? nullptr : initial_of(at.b));
+  } else {
+    if (range == 0) pass_empty(0);
+    if (rg.count <= 0) return;
+    load_state(rg.at.row > rg.at.s0 ? p.carry + (range - 1) * state_step + state_at : initial_of(rg.at.b));
+  }
+
+  // ---- tile loads, straight to LDS: thread chunk i fills position THREADS i + tid: row P / KC, slot P % KC ----------
+  constexpr int CG = C * KC / THREADS;
+  static_assert(CG == 2 && THREADS / KC % 16 == 0, "the swizzle is the same for a thread's rows");
+  const int kr0 = tid / KC, slot = tid % KC;
+  const uint32_t qk_chunk = (slot ^ qk_swizzle<D>(kr0)) * 8, v_chunk = (slot ^ v_swizzle<D>(kr0)) * 8;
+  const uint16_t *kp = p.k.p + hk * p.k.head, *vp = p.v.p + h * p.v.head, *qp = p.q.p + hk * p.q.head;
+  const uint32_t wave_lds = __builtin_amdgcn_readfirstlane(wave * 1024);
+  // rows behind the chunk's last repeat it: their weights are zero and their outputs are not stored
+  auto load_tiles = [&](int row, int n, int buf) __device__ {
+#pragma unroll
+    for (int i = 0; i < CG; ++i) {
+      const uint32_t r = min(kr0 + i * (THREADS / KC), n - 1), to = wave_lds + i * THREADS * 16;
+      global_to_lds16_sbase(kp + (int64_t)row * p.k.row, 2u * (r * (uint32_t)p.k.row + qk_chunk), lds_address(Ks[buf]) + to);
+      global_to_lds16_sbase(vp + (int64_t)row * p.v.row, 2u * (r * (uint32_t)p.v.row + v_chunk), lds_address(Vs[buf]) + to);
+      if constexpr (!CARRY)
+        global_to_lds16_sbase(qp + (int64_t)row * p.q.row, 2u * (r * (uint32_t)p.q.row + qk_chunk), lds_address(Qs[buf]) + to);
+    }
+  };
+
+  // ---- what stays the same over a head's chunks ----------------------------------------------------------------------
+  // fragment of row l16 of a 16-row tile of Q or K, k-step s: 16 bytes; transposed reads of K by pairs of dk tiles and of V
+  int qk_at[NS], kt_at[NS];
+  const int tr = 4 * g + (l16 >> 2);
+#pragma unroll
+  for (int t = 0; t < NS; ++t) {
+    qk_at[t] = l16 * D + ((4 * t + g) ^ qk_swizzle<D>(l16)) * 8;
+    kt_at[t] = tr * D + ((4 * t + (l16 & 3)) ^ qk_swizzle<D>(tr)) * 8;
+  }
+  const int vt_at = tr * D + ((2 * wave + ((l16 >> 1) & 1)) ^ v_swizzle<D>(tr)) * 8 + 4 * (l16 & 1);
+  // the wavefront's tiles of P^T: row tile prt, token tiles pu, pu + PS, ... up to the diagonal
+  constexpr int PS = NW / 4;
+  const int prt = wave / PS, pu = wave % PS;
+  float pw[PT][4], row_weight[4];
+  if constexpr (!CARRY) {
+#pragma unroll
+    for (int x = 0; x < PT; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pw[x][i] = decay_pow(log2a, max(16 * (prt - pu - PS * x) + l16 - 4 * g - i, 0));
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) row_weight[rt] = decay_pow(log2a, 16 * rt + l16 + 1);
+    // tiles of P behind the diagonal that share a k-step with one on it
+    for (int i = tid; i < 2 * 8 * 64; i += THREADS) (&Ps[0][0][0])[i] = u32x4_t{};
+  }
+  float vw[16];  // a^{n-1-j} of the lane's tokens j of a chunk of n
+  int vw_n = -1;
+
+  LinPlace at = rg.at;
+  int n = min(C, at.s1 - at.row), buf = 0;
+  load_tiles(at.row, n, 0);
+  for (int64_t left = rg.count; left > 0; --left, buf ^= 1) {
+    wait_vm_lds<0>();
+    bare_barrier();
+    // the next chunk
+    LinPlace next = at;
+    next.row = at.row + C;
+    const bool ends = next.row >= at.s1;
+    if (ends && (left > 1 || !CARRY)) {
+      const int b = pass_empty(at.b + 1);
+      if (left > 1) next = LinPlace{b, lin_bound(p, b), lin_bound(p, b + 1), lin_bound(p, b)};
+    }
+    const int next_n = min(C, next.s1 - next.row);
+    if (left > 1) load_tiles(next.row, next_n, buf ^ 1);
+
+    if (n != vw_n) {
+      vw_n = n;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int back = n - 1 - (16 * (x / 4) + 4 * g + x % 4);
+        vw[x] = back < 0 ? 0.f : decay_pow(log2a, back);
+      }
+    }
+    const uint16_t *kt = Ks[buf], *vt = Vs[buf];
+    u32x4_t vf[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const u32x2_t a = lin_read_transposed(vt + 32 * ks * D + vt_at), b = lin_read_transposed(vt + (32 * ks + 16) * D + vt_at);
+      vf[ks] = u32x4_t{a[0], a[1], b[0], b[1]};
+    }
+
+    if constexpr (!CARRY) {
+      const uint16_t *qt = Qs[buf];
+      // P^T = K Q^T with the decays, as two bf16 numbers
+#pragma unroll
+      for (int x = 0; x < PT; ++x) {
+        const int u = pu + PS * x;
+        if (u > prt) break;
+        f32x4_t c = {};
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+          c = mfma_bf16_16x16x32(as_bf16x8(ld16(kt + 16 * u * D + qk_at[t])), as_bf16x8(ld16(qt + 16 * prt * D + qk_at[t])), c);
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // behind the diagonal nothing is taken, whatever the key holds
+          w[i] = u < prt || l16 >= 4 * g + i ? c[i] * pw[x][i] : 0.f;
+        }
+        const uint32_t h0 = pack_bf2(w[0], w[1]), h1 = pack_bf2(w[2], w[3]);
+        const uint32_t e0 = pack_bf2(w[0] - lo_half(h0), w[1] - hi_half(h0)), e1 = pack_bf2(w[2] - lo_half(h1), w[3] - hi_half(h1));
+        const int f = 2 * prt + (u >> 1);
+        reinterpret_cast<u32x2_t *>(&Ps[0][f][lane])[u & 1] = u32x2_t{h0, h1};
+        reinterpret_cast<u32x2_t *>(&Ps[1][f][lane])[u & 1] = u32x2_t{e0, e1};
+      }
+      // O^T = S Q^T, rows by a^{r+1}
+      f32x4_t o[4] = {};
+#pragma unroll
+      for (int t = 0; t < NS; ++t) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s[2 * t + j / 4][j % 4];
+        const Split2 sp = split2(x);
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) {
+          const bf16x8_t qf = as_bf16x8(ld16(qt + 16 * rt * D + qk_at[t]));
+          o[rt] = mfma_bf16_16x16x32(as_bf16x8(sp.hi), qf, o[rt]);
+          o[rt] = mfma_bf16_16x16x32(as_bf16x8(sp.lo), qf, o[rt]);
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[rt][i] *= row_weight[rt];
+      // a value that is no finite number would reach rows in front of it as 0 * inf: it is left out of the product, and its
+      // channel ends there
+      uint32_t worst = 0;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) worst = max(worst, max(vf[ks][j] & 0x7fffu, (vf[ks][j] >> 16) & 0x7fffu));
+      const bool careful = __any(worst >= 0x7f80u);
+      u32x4_t vc[2] = {vf[0], vf[1]};
+      int bad = C;
+      if (careful) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t mask = j & 1 ? 0xffff0000u : 0xffffu, most = j & 1 ? 0x7f800000u : 0x7f80u;
+            if ((vf[ks][j / 2] & most) == most) {
+              bad = min(bad, 32 * ks + 16 * (j / 4) + 4 * g + j % 4);
+              vc[ks][j / 2] &= ~mask;
+            }
+          }
+        bad = min(bad, __shfl_xor(bad, 16));
+        bad = min(bad, __shfl_xor(bad, 32));
+      }
+      wait_vm_lds<63>();
+      bare_barrier();
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+        for (int ks = 0; ks <= rt / 2; ++ks) {
+          o[rt] = mfma_bf16_16x16x32(as_bf16x8(vc[ks]), as_bf16x8(Ps[0][2 * rt + ks][lane]), o[rt]);
+          o[rt] = mfma_bf16_16x16x32(as_bf16x8(vc[ks]), as_bf16x8(Ps[1][2 * rt + ks][lane]), o[rt]);
+        }
+      if (careful) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int from = __shfl(bad, 4 * g + i);
+#pragma unroll
+          for (int rt = 0; rt < 4; ++rt)
+            if (16 * rt + l16 >= from) o[rt][i] = __builtin_nanf("");
+        }
+      }
+      uint16_t *op = p.out + (int64_t)at.row * p.o_row + h * p.o_head + 16 * wave + 4 * g;
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+        const int r = 16 * rt + l16;
+        if (r < n)
+          *reinterpret_cast<u32x2_t *>(op + r * p.o_row) =
+              u32x2_t{pack_bf2(o[rt][0] * p.scale, o[rt][1] * p.scale), pack_bf2(o[rt][2] * p.scale, o[rt][3] * p.scale)};
+      }
+    }
+
+    // S' = a^n S + K^T V, the weighted values as three bf16 numbers, which hold them whole
+    const float all = decay_pow(log2a, n);
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] *= all;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u32x4_t w0, w1, w2;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x0 = lo_half(vf[ks][j]) * vw[8 * ks + 2 * j], x1 = hi_half(vf[ks][j]) * vw[8 * ks + 2 * j + 1];
+        w0[j] = pack_bf2(x0, x1);
+        const float y0 = x0 - lo_half(w0[j]), y1 = x1 - hi_half(w0[j]);
+        w1[j] = pack_bf2(y0, y1);
+        w2[j] = pack_bf2(y0 - lo_half(w1[j]), y1 - hi_half(w1[j]));
+      }
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        const uint16_t *kr = kt + 32 * ks * D + kt_at[t / 2] + 4 * (t & 1);
+        const u32x2_t a = lin_read_transposed(kr), b = lin_read_transposed(kr + 16 * D);
+        const bf16x8_t kf = as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
+        s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w2), s[t]);
+        s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w1), s[t]);
+        s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w0), s[t]);
+      }
+    }
+    if (!CARRY && ends) {
+      if (p.final_state) store_state(p.final_state + at.b * state_step + state_at);
+      if (left > 1) load_state(initial_of(next.b));
+    }
+    at = next;
+    n = next_n;
+  }
+  if (CARRY) store_state(p.carry + range * state_step + state_at);
+}
+
+// The states at the ranges' ends from those that each range adds: carry[w] += a^{tokens of w} carry[w - 1] where range w lies
+// in a sequence that began before it. Four numbers a thread, range after range.
+__global__ __launch_bounds__(256) void carry_scan_kernel(LinCall p, int numbers) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)p.heads * numbers;
+  if (i >= all) return;
+  const float log2a = p.log_decay[i / numbers] * 1.44269504088896341f;
+  f32x4_t acc = *reinterpret_cast<const f32x4_t *>(p.carry + i);
+  for (int w = 1; w + 1 < p.ranges; ++w) {
+    float *at = p.carry + w * all + i;
+    f32x4_t x = *reinterpret_cast<const f32x4_t *>(at);
+    const int tokens = p.meta[w];
+    if (tokens >= 0) {
+      const float a = decay_pow(log2a, tokens);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = fmaf(a, acc[j], x[j]);
+      *reinterpret_cast<f32x4_t *>(at) = x;
+    }
+    acc = x;
+  }
+}
+
+template <int D>
+int launch_causal_linear(const LinCall &p, hipStream_t s) {
+  if (p.ranges > 1) {
+    hipLaunchKernelGGL((causal_linear_kernel<D, true>), dim3(p.ranges * p.heads), dim3(D * 4), 0, s, p);
+    int rc = check_launch("causal_linear");
+    if (rc) return rc;
+    if (p.ranges > 2) {
+      hipLaunchKernelGGL(carry_scan_kernel, dim3((unsigned)(((int64_t)p.heads * D * D / 4 + 255) / 256)), dim3(256), 0, s, p, D * D);
+      rc = check_launch("causal_linear");
+      if (rc) return rc;
+    }
+  }
+  hipLaunchKernelGGL((causal_linear_kernel<D, false>), dim3(p.ranges * p.heads), dim3(D * 4), 0, s, p);
+  return check_launch("causal_linear");
+}
+
+int check_lin_operand(const void *p, int64_t row, int64_t head, const char *name) {
+  VDNH3_HOST_CHECK(p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && head % 8 == 0 && row >= 0 &&
+                       head >= 0 && row <= (1 << 23),
+                   VDNH3_ERR_INVALID, "causal_linear: %s must be 16-byte aligned with strides that are multiples of 8, rows at "
+                   "most 2^23 elements apart", name);
+  return VDNH3_OK;
+}
+
+}  // namespace
+}  // namespace vdnh3
+
+extern "C" int vdnh3_causal_linear_ranges(int rows, int sequences, int heads, int head_dim) {
+  if (rows <= 0 || sequences <= 0 || heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  const int64_t chunks = (int64_t)rows / vdnh3::kLinC + 1, slots = head_dim == 128 ? 256 : 512;
+  const int64_t ranges = slots / heads;
+  return (int)(ranges < 1 ? 1 : ranges > chunks / 4 ? (chunks / 4 > 1 ? chunks / 4 : 1) : ranges);
+}
+
+extern "C" size_t vdnh3_causal_linear_workspace_bytes(int ranges, int heads, int head_dim) {
+  if (ranges <= 1 || heads <= 0 || head_dim <= 0) return 0;
+  return (size_t)ranges * heads * head_dim * head_dim * 4 + (size_t)ranges * 4;
+}
+
+extern "C" int vdnh3_causal_linear_packed(const uint16_t *q, int64_t q_row, int64_t q_head, const uint16_t *k, int64_t k_row,
+                                          int64_t k_head, const uint16_t *v, int64_t v_row, int64_t v_head, uint16_t *out,
+                                          int64_t o_row, int64_t o_head, const float *log_decay, const int32_t *cu_seqlens,
+                                          const float *initial_state, float *final_state, int sequences, int rows,
+                                          int heads, int qk_heads, int head_dim, float scale, int ranges, void *workspace,
+                                          size_t workspace_bytes, void *stream) {
+  using namespace vdnh3;
+  VDNH3_HOST_CHECK(head_dim == 64 || head_dim == 128, VDNH3_ERR_INVALID, "causal_linear: head_dim must be 64 or 128, got %d",
+                   head_dim);
+  VDNH3_HOST_CHECK(rows > 0 && sequences > 0 && heads > 0 && qk_heads > 0 && heads % qk_heads == 0, VDNH3_ERR_INVALID,
+                   "causal_linear: rows, sequences and heads must be positive and heads a multiple of qk_heads, got %d rows, "
+                   "%d sequences, %d / %d heads", rows, sequences, heads, qk_heads);
+  int rc = check_lin_operand(q, q_row, q_head, "q");
+  if (!rc) rc = check_lin_operand(k, k_row, k_head, "k");
+  if (!rc) rc = check_lin_operand(v, v_row, v_head, "v");
+  if (!rc) rc = check_lin_operand(out, o_row, o_head, "out");
+  if (rc) return rc;
+  VDNH3_HOST_CHECK(log_decay && cu_seqlens, VDNH3_ERR_INVALID, "causal_linear: decays and sequence bounds are needed");
+  VDNH3_HOST_CHECK(reinterpret_cast<uintptr_t>(initial_state) % 16 == 0 && reinterpret_cast<uintptr_t>(final_state) % 16 == 0,
+                   VDNH3_ERR_INVALID, "causal_linear: states must be 16-byte aligned");
+  VDNH3_HOST_CHECK(std::isfinite(scale), VDNH3_ERR_INVALID, "causal_linear: scale must be finite");
+  VDNH3_HOST_CHECK(ranges >= 1 && ranges <= (1 << 20), VDNH3_ERR_INVALID, "causal_linear: ranges must be positive, got %d", ranges);
+  VDNH3_HOST_CHECK(ranges == 1 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                                   workspace_bytes >= vdnh3_causal_linear_workspace_bytes(ranges, heads, head_dim)),
+                   VDNH3_ERR_INVALID, "causal_linear: %d ranges need a 16-byte aligned workspace of %zu bytes", ranges,
+                   vdnh3_causal_linear_workspace_bytes(ranges, heads, head_dim));
+  VDNH3_HOST_CHECK((int64_t)rows + sequences < (1ll << 31) - 64, VDNH3_ERR_INVALID, "causal_linear: %d rows are too many", rows);
+  rc = check_grid((int64_t)ranges * heads, head_dim * 4, "causal_linear");
+  if (!rc) rc = check_grid((int64_t)heads * head_dim * head_dim / 1024, 256, "causal_linear");
+  if (rc) return rc;
+  float *carry = static_cast<float *>(workspace);
+  const LinCall p{{q, q_row, q_head}, {k, k_row, k_head}, {v, v_row, v_head}, out, o_row, o_head, log_decay, cu_seqlens,
+                  initial_state, final_state, carry,
+                  reinterpret_cast<int32_t *>(carry + (ranges > 1 ? (int64_t)ranges * heads * head_dim * head_dim : 0)),
+                  sequences, rows, heads, heads / qk_heads, ranges, scale};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return head_dim == 128 ? launch_causal_linear<128>(p, s) : launch_causal_linear<64>(p, s);
+}

@@ -122,6 +122,18 @@ SIGNATURES = {
     "vdnh3_causal_cached_ranges": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "vdnh3_causal_block_rows": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "vdnh3_causal_partial_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
+    "vdnh3_causal_linear_ranges": (_c_int, [_c_int, _c_int, _c_int, _c_int]),
+    "vdnh3_causal_linear_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "vdnh3_causal_linear_packed": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64,
+                                            _c_i64, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
+                                            _c_int, _vp, _c_size, _vp]),
+    "vdnh3_causal_linear_step": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                                          _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_int, _vp, _c_int,
+                                          _c_int, _c_int, _c_int, _c_int, _c_float, _vp]),
+    "vdnh3_gated_delta_step": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                                        _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                                        _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                        _vp]),
     "vdnh3_head_gate": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int, _vp]),
     "vdnh3_mfma_peak": (_c_int, [_c_int, _vp, _vp, _c_int, _c_int, _vp, _vp]),
     "vdnh3_mfma_peak_ops": (ctypes.c_double, [_c_int, _c_int, _c_int]),

@@ -7,7 +7,8 @@ is the published Gated DeltaNet recurrence in chunk (WY) form, the workload a to
 
     S_t = a_t S_{t-1} (I - b_t k_t k_t^T) + b_t v_t k_t^T,   o_t = S_t q_t,   a_t = exp(g_t)
 
-``chunk_gated_delta_rule`` keeps the argument names of the common Gated DeltaNet operator.
+``chunk_gated_delta_rule`` keeps the argument names of the common Gated DeltaNet operator; ``gated_delta_step`` takes the new
+tokens of many requests over a pool of their states.
 """
 
 from __future__ import annotations
@@ -18,6 +19,7 @@ import threading
 import torch
 
 from . import _lib
+from .causal_linear import _pool, _rows, _slots, _step_operands, _step_output
 
 
 class _Pipe:
@@ -174,6 +176,38 @@ def chunk_gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, be
     return out, final
 
 
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, g: torch.Tensor,
+                     state: torch.Tensor, *, slots: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The recurrent form for new tokens: q and k ``[B, N, H_qk, D]``, v ``[B, N, H, D]`` bf16, ``beta`` and ``g`` ``[B, N, H]``
+    (computed in fp32); returns ``[B, N, H, D]``. D up to 128; value head ``h`` reads query / key head ``h // (H // H_qk)``.
+
+    ``state`` is a pool ``[slots, H, D, D]`` fp32 of states as ``chunk_gated_delta_rule`` gives and takes them, updated in place;
+    ``slots`` and ``out`` as in ``causal_linear.causal_linear_step``: request ``b`` has ``state[slots[b]]`` (``state[b]`` without
+    slots), one outside the pool gives zeros, a slot that an earlier request has gives NaN rows.
+    """
+    name = "gated_delta_step"
+    _step_operands(q, k, v, name)
+    batch, new, heads, dim = v.shape
+    if tuple(beta.shape) != (batch, new, heads) or tuple(g.shape) != (batch, new, heads):
+        raise ValueError(f"beta and g must have shape [{batch}, {new}, {heads}]")
+    _lib.forward_only(name, q, k, v, beta, g, state, out)
+    strides = _pool(state, heads, dim, name)
+    slots = _slots(slots, batch, state.shape[0], name)
+    device = _lib.require_device(q, k, v, beta, g, state, slots, out)
+    out = _step_output(out, v.shape, device)
+    if v.numel() == 0:
+        return out
+    if state.shape[0] == 0:
+        return out.zero_()
+    q, k, v, beta, g = _rows(q), _rows(k), _rows(v), beta.float(), g.float()
+    _lib.launch(name, _lib.lib().vdnh3_gated_delta_step, device,
+                q.data_ptr(), *q.stride()[:-1], k.data_ptr(), *k.stride()[:-1], v.data_ptr(), *v.stride()[:-1],
+                out.data_ptr(), *out.stride()[:-1], beta.data_ptr(), *beta.stride(), g.data_ptr(), *g.stride(),
+                state.data_ptr(), *strides, state.shape[0], _lib.ptr(slots), batch, new, heads, q.shape[2], dim)
+    return out
+
+
 def gdn_flops(tokens: int, heads: int, dim: int = 128, chunk: int = 64) -> float:
     """Algorithmic work of the chunk form per call: per chunk and head K K^T and Q K^T (2 C^2 D each),
     the two triangular solves (C^2 D each), U = U~ - W S^T and Q S^T (2 C D^2 each), P U (2 C^2 D) and
@@ -184,4 +218,4 @@ def gdn_flops(tokens: int, heads: int, dim: int = 128, chunk: int = 64) -> float
     return chunks * heads * per
 
 
-__all__ = ["chunk_gated_delta_rule", "gdn_flops", "gdn_forward_into", "side_stream"]
+__all__ = ["chunk_gated_delta_rule", "gated_delta_step", "gdn_flops", "gdn_forward_into", "side_stream"]

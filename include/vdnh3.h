@@ -563,6 +563,41 @@ int vdnh3_causal_attn_cached(const uint16_t *q, int64_t q_batch, int64_t q_row, 
                              const int32_t *lengths, int batch, int new_tokens, int room, int heads, int kv_heads,
                              int head_dim, float scale, int ranges, float *partial, size_t partial_bytes, void *stream);
 
+/* Causal linear attention with a decay for each head, packed sequences as above: per value head h, which reads query / key
+ * head h / (heads / qk_heads), S_t = exp(log_decay[h]) S_{t-1} + v_t k_t^T, o_t = scale S_t q_t, S [dv, dk] fp32, from
+ * initial_state[b] (null: zeros) to final_state[b] (null: not kept), both [sequences, heads, head_dim, head_dim]. Rows of no
+ * sequence are not written; final_state is, for empty sequences too. head_dim 64 or 128; rows at most 2^23 elements apart,
+ * strides of q, k and v may be 0. The chunks of all sequences are cut into `ranges` equal ranges that run beside each other;
+ * with more than one the states between them lie in `workspace` (16-byte aligned). vdnh3_causal_linear_ranges gives the number
+ * that suits a call. */
+int vdnh3_causal_linear_ranges(int rows, int sequences, int heads, int head_dim);
+size_t vdnh3_causal_linear_workspace_bytes(int ranges, int heads, int head_dim);
+int vdnh3_causal_linear_packed(const uint16_t *q, int64_t q_row, int64_t q_head, const uint16_t *k, int64_t k_row,
+                               int64_t k_head, const uint16_t *v, int64_t v_row, int64_t v_head, uint16_t *out, int64_t o_row,
+                               int64_t o_head, const float *log_decay, const int32_t *cu_seqlens, const float *initial_state,
+                               float *final_state, int sequences, int rows, int heads, int qk_heads, int head_dim,
+                               float scale, int ranges, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Its recurrent form for new_tokens tokens of each of `batch` requests: the states of request b are those at
+ * pool + slots[b] slot_stride + h head_stride (contiguous [head_dim, head_dim] each; slots null: b), updated in place. A request
+ * whose slot lies outside [0, slot_count) is idle: its rows are zeros. Of requests with the same slot the first has it; the
+ * others' rows are NaN. head_dim 1 to 128, no alignment needed (16-byte states and 8-byte q / k rows are faster). */
+int vdnh3_causal_linear_step(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
+                             int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch, int64_t v_row,
+                             int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row, int64_t o_head,
+                             const float *log_decay, float *pool, int64_t slot_stride, int64_t head_stride, int slot_count,
+                             const int32_t *slots, int batch, int new_tokens, int heads, int qk_heads, int head_dim,
+                             float scale, void *stream);
+
+/* The same for the Gated DeltaNet (vdnh3_gdn_*): S_t = a S_{t-1} (I - beta k k^T) + beta v k^T, o = S_t q, a = exp(log_decay),
+ * beta and log_decay one number per request, token and value head. */
+int vdnh3_gated_delta_step(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
+                           int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch, int64_t v_row,
+                           int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row, int64_t o_head, const float *beta,
+                           int64_t b_batch, int64_t b_row, int64_t b_head, const float *log_decay, int64_t g_batch,
+                           int64_t g_row, int64_t g_head, float *pool, int64_t slot_stride, int64_t head_stride, int slot_count,
+                           const int32_t *slots, int batch, int new_tokens, int heads, int qk_heads, int head_dim, void *stream);
+
 /* ------------------------------------------------------------------------------
  * Calibration (no counterpart in the reference): the sustained MFMA rate of the part on
  * caller-supplied operand bits, the ceiling the kernels' rates are read against besides the
