@@ -1,0 +1,113 @@
+"""Low-rank adapters of many requests beside a shared projection on MI355X.
+
+A projection runs once for the rows of all requests; each row's own adapter is added to its output::
+
+    out_t = y_t + s_i B_i (A_i x_t),   i = index[t]
+
+``LowRankAdapters`` holds the adapters of one projection, ``add`` applies them; ``linear.HipLinear`` takes both
+(``adapters=``, ``adapter_index=``). The index is read on the device: a captured call can be replayed with another.
+Forward-only; there is no CPU path.
+"""
+
+from __future__ import annotations
+
+from functools import lru_cache
+
+import torch
+
+from . import _lib
+
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, width: int, adapters: int, rank: int) -> int:
+    return _lib.lib().vdnh3_adapter_workspace_bytes(rows, width, adapters, rank)
+
+
+class LowRankAdapters:
+    """The adapters of one projection ``[out, width]``: ``down`` ``[n, rank, width]`` (A) and ``up`` ``[n, out, rank]`` (B), bf16 on
+    the GPU, and ``scales``, ``n`` numbers (a tensor or a sequence; ``None``: ones), kept in fp32.
+
+    Widths are multiples of 8; a rank that is none is filled up with zeros. Contiguous tensors of such a rank are used where they
+    lie (a later change of theirs counts), others are copied. ``from_pairs`` takes adapters of different ranks. The object holds
+    the tensors on the device: it has to outlive graphs that were captured with it.
+    """
+
+    def __init__(self, down: torch.Tensor, up: torch.Tensor, scales=None):
+        if not isinstance(down, torch.Tensor) or not isinstance(up, torch.Tensor) or down.ndim != 3 or up.ndim != 3 or \
+                down.shape[0] != up.shape[0] or down.shape[1] != up.shape[2] or 0 in down.shape or 0 in up.shape:
+            raise ValueError("down must be [adapters, rank, width] and up [adapters, out, rank]")
+        if down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16:
+            raise TypeError(f"LowRankAdapters computes in bf16; got {down.dtype}/{up.dtype}")
+        self.count, self.rank, self.width = (int(n) for n in down.shape)
+        self.out_width = int(up.shape[1])
+        if self.width % 8 or self.out_width % 8:
+            raise ValueError(f"the projection's widths must be multiples of 8, got {self.width} -> {self.out_width}")
+        fill = -self.rank % 8
+        if self.rank + fill > 1024:
+            raise ValueError(f"ranks up to 1024 are supported, got {self.rank}")
+        _lib.forward_only("LowRankAdapters", down, up, scales)
+        if scales is not None:
+            scales = torch.as_tensor(scales, dtype=torch.float32, device=down.device).reshape(-1).contiguous()
+            if scales.numel() != self.count:
+                raise ValueError(f"scales must be {self.count} numbers, got {scales.numel()}")
+        self.device = _lib.require_device(down, up, scales)
+        if fill:
+            down = torch.nn.functional.pad(down, (0, 0, 0, fill))
+            up = torch.nn.functional.pad(up, (0, fill))
+        self.down, self.up = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else
+                              t.clone(memory_format=torch.contiguous_format) for t in (down.detach(), up.detach()))
+        self.scales = None if scales is None else scales.detach()
+
+    @classmethod
+    def from_pairs(cls, pairs, scales=None) -> "LowRankAdapters":
+        """From ``(down [rank_i, width], up [out, rank_i])`` of each adapter; smaller ranks are filled up with zeros."""
+        pairs = list(pairs)
+        if not pairs or any(a.ndim != 2 or b.ndim != 2 or a.shape[0] != b.shape[1] or a.shape[1] != pairs[0][0].shape[1] or
+                            b.shape[0] != pairs[0][1].shape[0] for a, b in pairs):
+            raise ValueError("pairs must be (down [rank, width], up [out, rank]) of one projection")
+        rank = max(a.shape[0] for a, _ in pairs)
+        pad = torch.nn.functional.pad
+        return cls(torch.stack([pad(a, (0, 0, 0, rank - a.shape[0])) for a, _ in pairs]),
+                   torch.stack([pad(b, (0, rank - b.shape[1])) for _, b in pairs]), scales)
+
+    def add(self, y: torch.Tensor, x: torch.Tensor, index: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+        """``y`` ``[T, out]`` with each row's adapter applied to ``x`` ``[T, width]`` added, both bf16: a new tensor, or ``out``, which
+        may be ``y`` itself (but not overlap it, or x, otherwise).
+
+        ``index`` (``[T]`` integers on the GPU) names a row's adapter; a number outside ``[0, n)`` (-1 by custom) names none, and
+        the row keeps ``y``. The sum is rounded once; ``A x`` is fp32. Rows of one adapter are fastest next to each other.
+        """
+        name = "LowRankAdapters.add"
+        rows = x.shape[0] if x.ndim == 2 else -1
+        if x.ndim != 2 or tuple(x.shape) != (rows, self.width) or tuple(y.shape) != (rows, self.out_width):
+            raise ValueError(f"y must be [rows, {self.out_width}] and x [rows, {self.width}]; got {tuple(y.shape)} and {tuple(x.shape)}")
+        if x.dtype != torch.bfloat16 or y.dtype != torch.bfloat16:
+            raise TypeError(f"{name} computes in bf16; got {y.dtype}/{x.dtype}")
+        if not isinstance(index, torch.Tensor) or index.ndim != 1 or index.numel() != rows or index.dtype not in _INTEGERS:
+            raise ValueError(f"index must be a tensor of {rows} integers, one per row")
+        _lib.forward_only(name, y, x, out)
+        _lib.int32_sizes(name, rows)
+        device = _lib.require_device(self.down, y, x, index, out)
+        if out is None:
+            out = torch.empty(rows, self.out_width, dtype=torch.bfloat16, device=device)
+        elif tuple(out.shape) != (rows, self.out_width) or out.dtype != torch.bfloat16 or not _lib.in_place(out) or \
+                (rows > 1 and out.stride(0) < self.out_width):
+            raise ValueError(f"out must be a bf16 [{rows}, {self.out_width}] tensor with 16-byte aligned rows that do not overlap")
+        if rows == 0:
+            return out
+        if index.dtype == torch.int64:
+            index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
+        index = index.to(torch.int32).contiguous()
+        x, y = _lib.operand(x), _lib.operand(y)
+        size = _workspace_bytes(rows, self.width, self.count, self.down.shape[1])
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        _lib.launch(name, _lib.lib().vdnh3_adapter_add, device,
+                    y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), self.down.data_ptr(), self.up.data_ptr(),
+                    _lib.ptr(self.scales), index.data_ptr(), out.data_ptr(), out.stride(0), rows, self.width, self.out_width,
+                    self.count, self.down.shape[1], workspace.data_ptr(), size)
+        return out
+
+
+__all__ = ["LowRankAdapters"]

@@ -197,7 +197,19 @@ class HipLinear(torch.nn.Module):
             self.register_buffer("weight", q)
             self.register_buffer("weight_scale", s.reshape(1, -1))
 
-    def forward(self, x: torch.Tensor, *, out: torch.Tensor | None = None, accumulate: bool = False):
+    def forward(self, x: torch.Tensor, *, out: torch.Tensor | None = None, accumulate: bool = False, adapters=None,
+                adapter_index: torch.Tensor | None = None):
+        """The projection of ``x``; with ``adapters`` (``adapters.LowRankAdapters``) each row's low-rank adapter
+        (``adapter_index``) is applied to the bf16 ``x`` and added to the projection's bf16 output, in place."""
+        if adapters is not None:
+            if accumulate:
+                raise ValueError("adapters are added to the projection's own output: not with accumulate")
+            if x.dtype != torch.bfloat16:
+                x = x.to(torch.bfloat16)
+            y = self.forward(x, out=out)
+            return adapters.add(y, x, adapter_index, out=y)
+        if adapter_index is not None:
+            raise ValueError("adapter_index without adapters")
         if x.ndim != 2 or x.shape[1] != self.in_features:
             raise ValueError(f"expected [rows, {self.in_features}] input, got {tuple(x.shape)}")
         if x.dtype != torch.bfloat16:

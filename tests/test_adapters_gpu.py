@@ -1,0 +1,160 @@
+"""Low-rank adapters of many requests against float64 (GPU).
+
+Bar, from the arithmetic, relative to the absolute values of the terms (`size`, y among them): the products with A are fp32 sums
+of `width` terms, width 2^-24; s A x is one product more and meets B as two bf16 numbers, 2^-16; the products with B are sums of
+`rank` terms, 2 rank 2^-24, and the sum with y one more. The result is rounded once, 2^-8 of itself.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import recurrent_oracle as ro
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+def _case(rows, width, out, n, rank, device, seed=0):
+    g = torch.Generator().manual_seed(rows + width + seed)
+    x, y = torch.randn(rows, width, generator=g).to(BF), torch.randn(rows, out, generator=g).to(BF)
+    down = (torch.randn(n, rank, width, generator=g) * width ** -0.5).to(BF)
+    up = torch.randn(n, out, rank, generator=g).to(BF)
+    return [t.to(device) for t in (x, y, down, up, torch.rand(n, generator=g) - 0.3)], g
+
+
+def _check(got, x, y, down, up, scales, index):
+    want, size = ro.adapters(y, x, down, up, scales if scales is not None else [1.0] * down.shape[0], index)
+    bar = ((x.shape[1] + 2 * down.shape[1] + 8) * 2.0 ** -24 + 2.0 ** -16) * size + 2.0 ** -8 * want.abs()
+    d = (got.double() - want).abs()
+    assert (d <= bar).all(), (d / bar.clamp_min(1e-30)).max()
+    none = (index < 0) | (index >= down.shape[0])
+    assert torch.equal(got[none], y[none])
+
+
+def _runs(rows, lengths, choices):
+    index = torch.full((rows,), -1, dtype=torch.int32)
+    at = 0
+    for n, c in zip(lengths, choices):
+        index[at:at + n] = c
+        at += n
+    return index
+
+
+CASES = [  # rows, width, out, adapters, rank
+    (1, 64, 64, 1, 8), (1, 5120, 640, 8, 16), (3, 8, 8, 2, 8), (17, 136, 264, 3, 16), (64, 512, 512, 16, 16), (65, 1000, 72, 70, 8),
+    (130, 256, 1032, 4, 24), (200, 2048, 256, 3, 64), (333, 640, 320, 5, 40), (64, 384, 128, 2, 128), (100, 256, 64, 3, 136),
+    (70, 128, 64, 2, 264), (20000, 64, 64, 3, 32), (48, 5120, 64, 2, 48)]
+
+
+@pytest.mark.parametrize("rows,width,out,n,rank", CASES)
+def test_against_float64(device, rows, width, out, n, rank):
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    print(f"case adapters {rows} x {width} -> {out}, {n} of rank {rank}", flush=True)
+    (x, y, down, up, scales), g = _case(rows, width, out, n, rank, device)
+    handle = LowRankAdapters(down, up, scales)
+    any_order = torch.randint(-1, n + 1, (rows,), generator=g, dtype=torch.int32)
+    runs = torch.randint(-1, n, (rows,), generator=g, dtype=torch.int32).sort()[0]
+    same = torch.full((rows,), n - 1, dtype=torch.int32)
+    none = torch.full((rows,), -1, dtype=torch.int32)
+    for index in (any_order, runs, same, none):
+        index = index.to(device)
+        got = handle.add(y, x, index)
+        _check(got, x, y, down, up, scales, index)
+        again = y.clone()
+        assert handle.add(again, x, index.long(), out=again) is again and torch.equal(again, got)
+    # views: columns of wider matrices, off 16 bytes, one row for all
+    wide_x = torch.cat([x, x], 1)[:, width:]
+    wide_y = torch.cat([y, y], 1)[:, :out]
+    off = torch.empty(x.numel() + 1, dtype=BF, device=device)[1:].view_as(x).copy_(x)
+    index = any_order.to(device)
+    got = handle.add(y, x, index)
+    for args in ((wide_y, wide_x), (y, off)):
+        assert torch.equal(handle.add(*args, index), got)
+    to = torch.full((rows, out + 8), 7.0, dtype=BF, device=device)
+    assert torch.equal(handle.add(y, x, index, out=to[:, :out]), got) and (to[:, out:] == 7).all()
+    one = handle.add(y[:1].expand(rows, out), x[:1].expand(rows, width), index)
+    assert torch.equal(one, handle.add(y[:1].expand(rows, out).contiguous(), x[:1].expand(rows, width).contiguous(), index))
+
+
+def test_ranks_scales_and_pairs(device):
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    (x, y, down, up, scales), g = _case(50, 128, 96, 3, 12, device)
+    index = torch.randint(0, 3, (50,), generator=g).to(device)
+    _check(LowRankAdapters(down, up).add(y, x, index), x, y, down, up, None, index)
+    _check(LowRankAdapters(down, up, scales.tolist()).add(y, x, index), x, y, down, up, scales, index)
+    _check(LowRankAdapters(down, up, scales.double().cpu()).add(y, x, index), x, y, down, up, scales, index)
+    lone = LowRankAdapters.from_pairs([(down[0], up[0]), (down[1, :5], up[1, :, :5]), (down[2, :1], up[2, :, :1])], scales)
+    down, up = down.clone(), up.clone()
+    down[1, 5:], down[2, 1:], up[1, :, 5:], up[2, :, 1:] = 0, 0, 0, 0
+    _check(lone.add(y, x, index), x, y, down, up, scales, index)
+    turned = LowRankAdapters(down.transpose(1, 2).contiguous().transpose(1, 2), up, scales)
+    assert torch.equal(turned.add(y, x, index), lone.add(y, x, index))
+
+
+def test_a_row_keeps_to_itself(device):
+    """Infinities and NaN of a row, or of an adapter that others use, stay there."""
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    (x, y, down, up, scales), g = _case(90, 256, 128, 4, 16, device)
+    index = torch.randint(0, 3, (90,), generator=g, dtype=torch.int32).to(device)
+    index[7] = 3
+    want = LowRankAdapters(down, up, scales).add(y, x, index)
+    for value in (torch.inf, torch.nan):
+        bad = x.clone()
+        bad[11, 5] = value
+        got = LowRankAdapters(down, up, scales).add(y, bad, index)
+        assert not got[11].isfinite().any() and torch.equal(got[:11], want[:11]) and torch.equal(got[12:], want[12:])
+        poisoned = down.clone()
+        poisoned[3] = value
+        got = LowRankAdapters(poisoned, up, scales).add(y, x, index)
+        assert not got[7].isfinite().any()
+        got[7] = want[7]
+        assert torch.equal(got, want)
+
+
+def test_beside_a_projection(device):
+    from vdn_h3_amd.adapters import LowRankAdapters
+    from vdn_h3_amd.linear import HipLinear
+
+    (x, _, down, up, scales), g = _case(77, 256, 384, 3, 16, device)
+    weight = (torch.randn(384, 256, generator=g) / 16).to(BF).to(device)
+    index = torch.randint(-1, 3, (77,), generator=g, dtype=torch.int32).to(device)
+    handle = LowRankAdapters(down, up, scales)
+    for precision in ("bf16", "int8", "fp8"):
+        layer = HipLinear(weight, precision)
+        base = layer(x)
+        got = layer(x, adapters=handle, adapter_index=index)
+        assert torch.equal(got, handle.add(base, x, index))
+        out = torch.zeros(77, 384, dtype=BF, device=device)
+        assert layer(x.float(), out=out, adapters=handle, adapter_index=index) is out and torch.equal(out, got)
+        with pytest.raises(ValueError):
+            layer(x, out=out, accumulate=True, adapters=handle, adapter_index=index)
+        with pytest.raises(ValueError):
+            layer(x, adapter_index=index)
+
+
+def test_replays_take_another_index(device):
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    (x, y, down, up, scales), g = _case(40, 512, 256, 5, 16, device)
+    index = torch.zeros(40, dtype=torch.int32, device=device)
+    handle, out = LowRankAdapters(down, up, scales), torch.zeros_like(y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        handle.add(y, x, index, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        handle.add(y, x, index, out=out)
+    for seed in range(4):
+        index.copy_(torch.randint(-1, 6, (40,), generator=g, dtype=torch.int32))
+        x.add_(0.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, handle.add(y, x, index))
