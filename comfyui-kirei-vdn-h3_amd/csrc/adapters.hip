@@ -13,8 +13,8 @@
 namespace vdnh3 {
 namespace {
 
-constexpr int kBlockRows = 64;
-constexpr int kRankGroup = 128;  // ranks that a shrinking workgroup takes at most
+constexpr int kBlockRows = 64;  // of an expanding workgroup; the most that a list holds
+constexpr int kShrinkWaves = 8;
 
 struct AdapterCall {
   const uint16_t *x, *y, *down, *up;
@@ -22,32 +22,30 @@ struct AdapterCall {
   int64_t x_row, y_row, out_row;
   const float *scales;
   const int32_t *index;
-  float *h;  // [parts, rows, rank rounded up to 16]
-  int rows, width, out_width, adapters, rank, rank16, parts, part_width, shares, copy;
+  uint16_t *h;  // [rows, rank rounded up to 32 in eights, 2, 8]: s A x as two bf16 numbers
+  int rows, width, out_width, adapters, rank, rank32, shares, copy;
 };
 
 // The adapter of each of a block's rows, a lane a row: -1 for none and behind the last row.
-__device__ __forceinline__ int adapter_of(const AdapterCall &p, int row0) {
-  const int r = row0 + ((int)threadIdx.x & 63);
-  const int i = r < p.rows ? p.index[r] : -1;
+__device__ __forceinline__ int adapter_of(const AdapterCall &p, int row0, int block_rows) {
+  const int lane = threadIdx.x & 63;
+  const int i = lane < block_rows && row0 + lane < p.rows ? p.index[row0 + lane] : -1;
   return i >= 0 && i < p.adapters ? i : -1;
 }
 
 // The rows of `mask`, one behind another, as a wavefront's list; the last one repeats behind its end.
 __device__ __forceinline__ void list_rows(uint64_t mask, int *list) {
   const int lane = threadIdx.x & 63, at = __popcll(mask & ((1ull << lane) - 1)), count = __popcll(mask);
-  if ((mask >> lane) & 1) {
-    list[at] = lane;
-    if (at == count - 1)
-      for (int i = count; i < kBlockRows; ++i) list[i] = lane;
-  }
+  if ((mask >> lane) & 1) list[at] = lane;
+  if (lane >= count) list[lane] = 63 - __builtin_clzll(mask);
 }
 
-// h = A x of one block, adapter and part of the width: four wavefronts, each with a quarter of the part, whose sums meet in LDS.
-// C[rank][row] tiles: a lane keeps four ranks of a row.
+// s A x of the rows of one adapter in a block: the wavefronts take steps of 64 channels in turn and add their sums up in LDS.
+// C[rank][row] tiles: a lane has four ranks of a row.
 template <int MT, int NT>
-__device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int part,
-                                            int rank0, f32x4_t (*sums)[4 * NT][64]) {
+__device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int rank0,
+                                            f32x4_t (*sums)[64]) {
+  constexpr int T = MT * NT, W = kShrinkWaves;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
   const uint16_t *xp[MT], *ap[NT];
   bool has[NT];
@@ -59,63 +57,74 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
     has[t] = r < p.rank;
     ap[t] = p.down + ((int64_t)adapter * p.rank + (has[t] ? r : 0)) * p.width;
   }
-  f32x4_t acc[NT][MT] = {};
-  const int begin = part * p.part_width, end = min(begin + p.part_width, p.width);
-  for (int c0 = begin + 32 * wave; c0 < end; c0 += 128) {
-    const int c = c0 + 8 * g;
-    const bool in = c < end;
+  f32x4_t acc[T] = {};
+  auto products = [&](const u32x4_t *a, const u32x4_t *x) __device__ {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[t * MT + m] = mfma_bf16_16x16x32(as_bf16x8(a[t]), as_bf16x8(x[m]), acc[t * MT + m]);
+  };
+  int c0 = 64 * wave;
+  for (; c0 + 64 <= p.width; c0 += 64 * W) {
+    u32x4_t a[2][NT], x[2][MT];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = c0 + 32 * k + 8 * g;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[k][m] = ld16(xp[m] + c);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) a[k][t] = has[t] ? ld16(ap[t] + c) : u32x4_t{};
+    }
+    products(a[0], x[0]);
+    products(a[1], x[1]);
+  }
+  for (int c1 = c0; c1 < p.width && c1 < c0 + 64; c1 += 32) {
+    const int c = c1 + 8 * g;
+    const bool in = c < p.width;
     u32x4_t a[NT], x[MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) a[t] = in && has[t] ? ld16(ap[t] + c) : u32x4_t{};
 #pragma unroll
     for (int m = 0; m < MT; ++m) x[m] = in ? ld16(xp[m] + c) : u32x4_t{};
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(a[t]), as_bf16x8(x[m]), acc[t][m]);
+    products(a, x);
   }
-  // wavefronts 2 and 3 give their sums to 0 and 1, then 1 to 0
+  // tile i is added up and written by wavefront i % W
+  constexpr int KEPT = (T + W - 1) / W;
+  const float scale = p.scales ? p.scales[adapter] : 1.f;
 #pragma unroll
-  for (int half = 2; half > 0; half >>= 1) {
-    if (wave >= half && wave < 2 * half) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) sums[wave - half][t * MT + m][lane] = acc[t][m];
-    }
+  for (int k = 0; k < KEPT; ++k) {
+    const int tiles = T - k * W < W ? T - k * W : W;  // the tiles of this turn
     __syncthreads();
-    if (wave < half) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[t][m] += sums[wave][t * MT + m][lane];
-    }
+    for (int i = 0; i < tiles; ++i) sums[wave * W + i][lane] = acc[k * W + i];
     __syncthreads();
-  }
-  if (wave != 0) return;
+    if (wave >= tiles) continue;
+    f32x4_t all = sums[wave][lane];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (16 * m + l16 >= count) continue;
-    float *to = p.h + ((int64_t)part * p.rows + row0 + list[16 * m + l16]) * p.rank16 + rank0 + 4 * g;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      if (rank0 + 16 * t < p.rank16) *reinterpret_cast<f32x4_t *>(to + 16 * t) = acc[t][m];
+    for (int w = 1; w < W; ++w) all += sums[w * W + wave][lane];
+    const int i = k * W + wave, m = i % MT, r = rank0 + 16 * (i / MT) + 4 * g;
+    if (16 * m + l16 >= count || r >= p.rank32) continue;
+    all *= scale;
+    const u32x2_t hi = {pack_bf2(all[0], all[1]), pack_bf2(all[2], all[3])};
+    const u32x2_t lo = {pack_bf2(all[0] - __uint_as_float(hi[0] << 16), all[1] - __uint_as_float(hi[0] & 0xffff0000u)),
+                        pack_bf2(all[2] - __uint_as_float(hi[1] << 16), all[3] - __uint_as_float(hi[1] & 0xffff0000u))};
+    uint16_t *to = p.h + ((int64_t)(row0 + list[16 * m + l16]) * p.rank32 + (r & ~7)) * 2 + (r & 4);
+    *reinterpret_cast<u32x2_t *>(to) = hi;
+    *reinterpret_cast<u32x2_t *>(to + 8) = lo;
   }
 }
 
-// grid: parts x shares x rank groups x blocks; a workgroup takes every `shares`-th adapter of its block
-template <int NT>
-__global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterCall p, int groups) {
-  __shared__ f32x4_t sums[2][4 * NT][64];
-  __shared__ int lists[4][kBlockRows];
+// grid: shares x rank groups x blocks of 16 MT rows; a workgroup takes every `shares`-th adapter of its block
+template <int MT, int NT>
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdapterCall p, int groups) {
+  __shared__ f32x4_t sums[kShrinkWaves * kShrinkWaves][64];
+  __shared__ int lists[kShrinkWaves][kBlockRows];
   int at = blockIdx.x;
-  const int part = at % p.parts;
-  at /= p.parts;
   const int share = at % p.shares;
   at /= p.shares;
-  const int rank0 = at % groups * (16 * NT), row0 = at / groups * kBlockRows;
+  const int rank0 = at % groups * (16 * NT), row0 = at / groups * (16 * MT);
   int *list = lists[threadIdx.x >> 6];
-  const int mine = adapter_of(p, row0);
+  const int mine = adapter_of(p, row0, 16 * MT);
   uint64_t left = __ballot(mine >= 0);
   for (int n = 0; left; ++n) {
     const int adapter = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
@@ -124,117 +133,162 @@ __global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterCall p, int 
     if (n % p.shares != share) continue;
     list_rows(rows, list);
     const int count = __popcll(rows);
-    if (count <= 16) shrink_rows<1, NT>(p, row0, list, count, adapter, part, rank0, sums);
-    else if (count <= 32) shrink_rows<2, NT>(p, row0, list, count, adapter, part, rank0, sums);
-    else shrink_rows<4, NT>(p, row0, list, count, adapter, part, rank0, sums);
+    if (MT > 1 && count > 16) {
+      if (MT > 2 && count > 32) shrink_rows<MT, NT>(p, row0, list, count, adapter, rank0, sums);
+      else shrink_rows<(MT > 1 ? 2 : 1), NT>(p, row0, list, count, adapter, rank0, sums);
+    } else {
+      shrink_rows<1, NT>(p, row0, list, count, adapter, rank0, sums);
+    }
   }
 }
 
-// out = y + s B h of a wavefront's 64 columns and the rows of one adapter in a block. C[column][row] tiles whose columns are
-// ordered so that a pair of tiles gives a lane eight neighbours: row m of tile t is column 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4.
-template <int MT>
-__device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int col0) {
+// s A x of a row, eight ranks, as the operand's two bf16 numbers
+struct HalfPair {
+  u32x4_t hi, lo;
+};
+__device__ __forceinline__ HalfPair load_h(const uint16_t *row, int r) { return HalfPair{ld16(row + 2 * r), ld16(row + 2 * r + 8)}; }
+
+// out = y + s B h of the rows of one adapter in a block, a wavefront's 64 of each 256 columns of the workgroup's span.
+// C[column][row] tiles whose columns are ordered so that a pair of tiles gives a lane eight neighbours: row m of tile t is
+// column 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. KS: the ranks in 32s, kept as operands over the columns; 0: any number of
+// them, read again for each 64 columns.
+template <int MT, int KS>
+__device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int col0,
+                                            int col_end) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  f32x4_t acc[4][MT] = {};
-  const float scale = p.scales ? p.scales[adapter] : 1.f;
-  for (int r0 = 0; r0 < p.rank; r0 += 32) {
-    const int r = r0 + 8 * g;
-    u32x4_t hi[MT], lo[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      f32x4_t a = {}, b = {};
-      if (r < p.rank) {
-        const float *from = p.h + (int64_t)(row0 + list[16 * m + l16]) * p.rank16 + r;
-        for (int part = 0; part < p.parts; ++part) {
-          const f32x4_t *f = reinterpret_cast<const f32x4_t *>(from + (int64_t)part * p.rows * p.rank16);
-          a += f[0];
-          b += f[1];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x0 = (j < 2 ? a[2 * j] : b[2 * j - 4]) * scale, x1 = (j < 2 ? a[2 * j + 1] : b[2 * j - 3]) * scale;
-        hi[m][j] = pack_bf2(x0, x1);
-        lo[m][j] = pack_bf2(x0 - __uint_as_float(hi[m][j] << 16), x1 - __uint_as_float(hi[m][j] & 0xffff0000u));
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int c = col0 + 32 * (t / 2) + 8 * (l16 / 4) + 4 * (t % 2) + l16 % 4;
-      const u32x4_t b = r < p.rank && c < p.out_width ? ld16(p.up + ((int64_t)adapter * p.out_width + c) * p.rank + r) : u32x4_t{};
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(b), as_bf16x8(hi[m]), acc[t][m]);
-        acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(b), as_bf16x8(lo[m]), acc[t][m]);
-      }
-    }
-  }
+  const uint16_t *hp[MT];
+  int64_t row[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    if (16 * m + l16 >= count) continue;
-    const int row = row0 + list[16 * m + l16];
+    row[m] = row0 + list[16 * m + l16];
+    hp[m] = p.h + row[m] * p.rank32 * 2;
+  }
+  HalfPair h[KS ? KS : 1][MT];
 #pragma unroll
-    for (int t = 0; t < 4; t += 2) {
-      const int c = col0 + 16 * t + 8 * g;
-      if (c >= p.out_width) continue;
-      const u32x4_t y = ld16(p.y + (int64_t)row * p.y_row + c);
-      u32x4_t o;
+  for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4_t &d = acc[t + j / 2][m];
-        o[j] = pack_bf2(__uint_as_float(y[j] << 16) + d[2 * (j % 2)], __uint_as_float(y[j] & 0xffff0000u) + d[2 * (j % 2) + 1]);
+    for (int m = 0; m < MT; ++m) h[k][m] = load_h(hp[m], 32 * k + 8 * g);
+  const uint16_t *up = p.up + (int64_t)adapter * p.out_width * p.rank;
+  for (; col0 < col_end; col0 += 256) {
+    u32x4_t y[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int c = col0 + 32 * t + 8 * g;
+        y[m][t] = c < p.out_width && 16 * m + l16 < count ? ld16(p.y + row[m] * p.y_row + c) : u32x4_t{};
       }
-      st16(p.out + (int64_t)row * p.out_row + c, o);
+    f32x4_t acc[4][MT] = {};
+    auto products = [&](int r0, const HalfPair *hk) __device__ {
+      const int r = r0 + 8 * g;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int c = col0 + 32 * (t / 2) + 8 * (l16 / 4) + 4 * (t % 2) + l16 % 4;
+        const u32x4_t b = r < p.rank && c < p.out_width ? ld16(up + (int64_t)c * p.rank + r) : u32x4_t{};
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(b), as_bf16x8(hk[m].hi), acc[t][m]);
+          acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(b), as_bf16x8(hk[m].lo), acc[t][m]);
+        }
+      }
+    };
+    if constexpr (KS > 0) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) products(32 * k, h[k]);
+    } else {
+      for (int r0 = 0; r0 < p.rank; r0 += 32) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) h[0][m] = load_h(hp[m], r0 + 8 * g);
+        products(r0, h[0]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (16 * m + l16 >= count) continue;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int c = col0 + 32 * t + 8 * g;
+        if (c >= p.out_width) continue;
+        u32x4_t o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4_t &d = acc[2 * t + j / 2][m];
+          o[j] = pack_bf2(__uint_as_float(y[m][t][j] << 16) + d[2 * (j % 2)],
+                          __uint_as_float(y[m][t][j] & 0xffff0000u) + d[2 * (j % 2) + 1]);
+        }
+        st16(p.out + row[m] * p.out_row + c, o);
+      }
     }
   }
 }
 
-// grid: column tiles of 256 x blocks
-__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterCall p, int column_tiles) {
+// grid: spans of columns x shares x blocks; a workgroup takes every `shares`-th adapter of its block
+template <int KS>
+__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterCall p, int spans, int span, int shares) {
   __shared__ int lists[4][kBlockRows];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col0 = (int)blockIdx.x % column_tiles * 256 + 64 * wave, row0 = (int)blockIdx.x / column_tiles * kBlockRows;
-  if (col0 >= p.out_width) return;
+  int at = blockIdx.x;
+  const int first = at % spans * span, col0 = first + 64 * wave, col_end = min(first + span, p.out_width);
+  at /= spans;
+  const int share = at % shares, row0 = at / shares * kBlockRows;
+  if (col0 >= col_end) return;
   int *list = lists[wave];
-  const int mine = adapter_of(p, row0);
+  const int mine = adapter_of(p, row0, kBlockRows);
   uint64_t left = __ballot(mine >= 0);
   if (p.copy) {  // rows without an adapter: y as it is
     const uint64_t none = __ballot(mine < 0 && row0 + lane < p.rows);
-    list_rows(none, list);
-    const int count = __popcll(none), c = col0 + 8 * (lane & 7);
-    for (int i = lane >> 3; i < count; i += 8) {
-      const int64_t row = row0 + list[i];
-      if (c < p.out_width) st16(p.out + row * p.out_row + c, ld16(p.y + row * p.y_row + c));
+    if (none) {
+      list_rows(none, list);
+      const int count = __popcll(none);
+      for (int i = share * 8 + (lane >> 3); i < count; i += 8 * shares) {
+        const int64_t row = row0 + list[i];
+        for (int c = col0 + 8 * (lane & 7); c < col_end; c += 256) st16(p.out + row * p.out_row + c, ld16(p.y + row * p.y_row + c));
+      }
     }
   }
-  while (left) {
+  for (int n = 0; left; ++n) {
     const int adapter = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
     const uint64_t rows = __ballot(mine == adapter);
     left &= ~rows;
+    if (n % shares != share) continue;
     list_rows(rows, list);
     const int count = __popcll(rows);
-    if (count <= 16) expand_rows<1>(p, row0, list, count, adapter, col0);
-    else if (count <= 32) expand_rows<2>(p, row0, list, count, adapter, col0);
-    else expand_rows<4>(p, row0, list, count, adapter, col0);
+    if (count <= 16) expand_rows<1, KS>(p, row0, list, count, adapter, col0, col_end);
+    else if (count <= 32) expand_rows<2, KS>(p, row0, list, count, adapter, col0, col_end);
+    else expand_rows<4, KS>(p, row0, list, count, adapter, col0, col_end);
   }
 }
 
+#ifndef ROWS64
+#define ROWS64 16384
+#endif
+#ifndef ROWS32
+#define ROWS32 8192
+#endif
+#ifndef EX_WG
+#define EX_WG 2048
+#endif
 struct AdapterCut {
-  int blocks, rank16, tiles, groups, parts, part_width, shares;
+  int rank32, row_tiles, rank_tiles, groups, shares, span, expand_shares;
+  int64_t shrink, expand;  // workgroups
 };
-AdapterCut adapter_cut(int rows, int width, int adapters, int rank) {
+AdapterCut adapter_cut(int rows, int out_width, int adapters, int rank) {
   AdapterCut c;
-  c.blocks = (rows + kBlockRows - 1) / kBlockRows;
-  c.rank16 = (rank + 15) / 16 * 16;
-  const int tiles = std::min(c.rank16, kRankGroup) / 16;
-  c.tiles = tiles <= 1 ? 1 : tiles <= 2 ? 2 : tiles <= 4 ? 4 : 8;
-  c.groups = (c.rank16 + 16 * c.tiles - 1) / (16 * c.tiles);
-  c.shares = c.blocks >= 256 ? 1 : std::min(std::min(rows, adapters), 16);
-  // parts of the width until the workgroups are two a CU, of 128 channels or more
-  const int64_t wanted = 512 / ((int64_t)c.blocks * c.groups * std::min(c.shares, 4)), most = (width + 127) / 128;
-  c.parts = (int)std::max<int64_t>(1, std::min(std::min(wanted, most), (int64_t)16));
-  c.part_width = ((width + c.parts - 1) / c.parts + 127) / 128 * 128;
-  c.parts = (width + c.part_width - 1) / c.part_width;
+  c.rank32 = (rank + 31) / 32 * 32;
+  c.row_tiles = rows >= ROWS64 ? 4 : rows >= ROWS32 ? 2 : 1;
+  const int most = c.row_tiles == 4 ? 4 : 8;
+  c.rank_tiles = 2;
+  while (c.rank_tiles < most && 16 * c.rank_tiles < c.rank32) c.rank_tiles *= 2;
+  c.groups = (c.rank32 + 16 * c.rank_tiles - 1) / (16 * c.rank_tiles);
+  const int64_t blocks = (rows + 16 * c.row_tiles - 1) / (16 * c.row_tiles), of = std::min(rows, adapters);
+  c.shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16 * c.row_tiles, 512 / (blocks * c.groups)}));
+  c.shrink = blocks * c.groups * c.shares;
+  // columns of an expanding workgroup: fewer than all where that leaves too few workgroups
+  const int64_t tall = (rows + kBlockRows - 1) / kBlockRows, column_tiles = (out_width + 255) / 256;
+  c.expand_shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16, EX_WG / (tall * column_tiles)}));
+  const int64_t spans = std::min(column_tiles, std::max<int64_t>(1, EX_WG / (tall * c.expand_shares)));
+  c.span = (int)((column_tiles + spans - 1) / spans) * 256;
+  c.expand = tall * c.expand_shares * ((out_width + c.span - 1) / c.span);
   return c;
 }
 
@@ -248,10 +302,9 @@ int check_adapter_rows(const void *p, int64_t row, int width, const char *name, 
 }  // namespace
 }  // namespace vdnh3
 
-extern "C" size_t vdnh3_adapter_workspace_bytes(int rows, int width, int adapters, int rank) {
-  if (rows <= 0 || width <= 0 || adapters <= 0 || rank <= 0) return 0;
-  const vdnh3::AdapterCut c = vdnh3::adapter_cut(rows, width, adapters, rank);
-  return (size_t)c.parts * rows * c.rank16 * 4;
+extern "C" size_t vdnh3_adapter_workspace_bytes(int rows, int rank) {
+  if (rows <= 0 || rank <= 0 || rank > 1024) return 0;
+  return (size_t)rows * ((rank + 31) / 32 * 32) * 4;
 }
 
 extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_t *x, int64_t x_row, const uint16_t *down,
@@ -274,26 +327,27 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   if (!rc) rc = check_adapter_rows(up, rank, rank, "up", true);
   if (rc) return rc;
   VDNH3_HOST_CHECK(out != y || out_row == y_row, VDNH3_ERR_INVALID, "adapter_add: out over y needs y's row stride");
-  const AdapterCut c = adapter_cut(rows, width, adapters, rank);
-  VDNH3_HOST_CHECK(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
-                       workspace_bytes >= vdnh3_adapter_workspace_bytes(rows, width, adapters, rank),
-                   VDNH3_ERR_INVALID, "adapter_add: needs a 16-byte aligned workspace of %zu bytes",
-                   vdnh3_adapter_workspace_bytes(rows, width, adapters, rank));
-  const int column_tiles = (out_width + 255) / 256;
-  const int64_t shrink = (int64_t)c.blocks * c.groups * c.shares * c.parts, expand = (int64_t)c.blocks * column_tiles;
-  rc = check_grid(shrink, 256, "adapter_add");
-  if (!rc) rc = check_grid(expand, 256, "adapter_add");
+  const size_t needed = vdnh3_adapter_workspace_bytes(rows, rank);
+  VDNH3_HOST_CHECK(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= needed,
+                   VDNH3_ERR_INVALID, "adapter_add: needs a 16-byte aligned workspace of %zu bytes", needed);
+  const AdapterCut c = adapter_cut(rows, out_width, adapters, rank);
+  rc = check_grid(c.shrink, 64 * kShrinkWaves, "adapter_add");
+  if (!rc) rc = check_grid(c.expand, 256, "adapter_add");
   if (rc) return rc;
-  const AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<float *>(workspace), rows, width,
-                      out_width, adapters, rank, c.rank16, c.parts, c.part_width, c.shares, out != y};
+  const AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<uint16_t *>(workspace), rows, width,
+                      out_width, adapters, rank, c.rank32, c.shares, out != y};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)shrink), threads(256);
-  if (c.tiles == 1) hipLaunchKernelGGL(adapter_shrink_kernel<1>, grid, threads, 0, s, p, c.groups);
-  else if (c.tiles == 2) hipLaunchKernelGGL(adapter_shrink_kernel<2>, grid, threads, 0, s, p, c.groups);
-  else if (c.tiles == 4) hipLaunchKernelGGL(adapter_shrink_kernel<4>, grid, threads, 0, s, p, c.groups);
-  else hipLaunchKernelGGL(adapter_shrink_kernel<8>, grid, threads, 0, s, p, c.groups);
+  auto shrink = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.shrink), dim3(64 * kShrinkWaves), 0, s, p, c.groups); };
+  if (c.row_tiles == 4)
+    c.rank_tiles == 2 ? shrink(adapter_shrink_kernel<4, 2>) : shrink(adapter_shrink_kernel<4, 4>);
+  else if (c.row_tiles == 2)
+    c.rank_tiles == 2 ? shrink(adapter_shrink_kernel<2, 2>) : c.rank_tiles == 4 ? shrink(adapter_shrink_kernel<2, 4>) : shrink(adapter_shrink_kernel<2, 8>);
+  else
+    c.rank_tiles == 2 ? shrink(adapter_shrink_kernel<1, 2>) : c.rank_tiles == 4 ? shrink(adapter_shrink_kernel<1, 4>) : shrink(adapter_shrink_kernel<1, 8>);
   rc = check_launch("adapter_add");
   if (rc) return rc;
-  hipLaunchKernelGGL(adapter_expand_kernel, dim3((unsigned)expand), threads, 0, s, p, column_tiles);
+  const int spans = (out_width + c.span - 1) / c.span;
+  auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.expand), dim3(256), 0, s, p, spans, c.span, c.expand_shares); };
+  rank <= 32 ? expand(adapter_expand_kernel<1>) : rank <= 64 ? expand(adapter_expand_kernel<2>) : expand(adapter_expand_kernel<0>);
   return check_launch("adapter_add");
 }

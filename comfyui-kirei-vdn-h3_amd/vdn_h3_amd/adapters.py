@@ -21,8 +21,8 @@ _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
 @lru_cache(maxsize=1024)
-def _workspace_bytes(rows: int, width: int, adapters: int, rank: int) -> int:
-    return _lib.lib().vdnh3_adapter_workspace_bytes(rows, width, adapters, rank)
+def _workspace_bytes(rows: int, rank: int) -> int:
+    return _lib.lib().vdnh3_adapter_workspace_bytes(rows, rank)
 
 
 class LowRankAdapters:
@@ -101,7 +101,7 @@ class LowRankAdapters:
             index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
         index = index.to(torch.int32).contiguous()
         x, y = _lib.operand(x), _lib.operand(y)
-        size = _workspace_bytes(rows, self.width, self.count, self.down.shape[1])
+        size = _workspace_bytes(rows, self.down.shape[1])
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         _lib.launch(name, _lib.lib().vdnh3_adapter_add, device,
                     y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), self.down.data_ptr(), self.up.data_ptr(),

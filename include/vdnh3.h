@@ -602,8 +602,8 @@ int vdnh3_gated_delta_step(const uint16_t *q, int64_t q_batch, int64_t q_row, in
  * [adapters, rank, width] and up [adapters, out_width, rank] contiguous, beside a projection's output y [rows, out_width].
  * scales null: ones. An index outside [0, adapters) names no adapter: out[t] = y[t]. out may be y. Widths and rank are
  * multiples of 8, the rank at most 1024; row strides of x and y may be 0. workspace (vdnh3_adapter_workspace_bytes, 16-byte
- * aligned) holds the products with down in fp32. */
-size_t vdnh3_adapter_workspace_bytes(int rows, int width, int adapters, int rank);
+ * aligned) holds the products with down as two bf16 numbers each. */
+size_t vdnh3_adapter_workspace_bytes(int rows, int rank);
 int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_t *x, int64_t x_row, const uint16_t *down,
                       const uint16_t *up, const float *scales, const int32_t *index, uint16_t *out, int64_t out_row, int rows,
                       int width, int out_width, int adapters, int rank, void *workspace, size_t workspace_bytes, void *stream);
