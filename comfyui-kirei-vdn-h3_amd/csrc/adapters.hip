@@ -6,14 +6,22 @@
 // the parts of the width that different workgroups take; s h meets B as two bf16 numbers (16 bits of it), and the sum with y is
 // rounded once. Rows are taken in blocks of 64 neighbours; a block finds the adapters in it by ballots and takes their rows
 // together, so the rows of one request share each fragment of its adapter, in whatever order requests lie.
+//
+// A and B are kept in the order in which the wavefronts read them, a kilobyte of neighbours per load: fragments of 16 ranks x 32
+// channels of A (strided rows of A took 18 us of 31 at 3,939 rows x 5,120 of rank 32) and of 32 columns x 32 (16) ranks of B.
+// x, y and out move in runs of 128 bytes of a row. HBM bounds both passes where there are many rows: 40,688 rows x 5,120 -> 5,120
+// of rank 64 take 84 us (x, 5.0 TB/s) and 183 us (y and out, 4.6 TB/s), a copy's rate; one row x 5,120 -> 15,360 of rank 16
+// 4.9 and 3.2 us, launches and chains of loads.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
 namespace vdnh3 {
 namespace {
 
-constexpr int kBlockRows = 64;  // of an expanding workgroup; the most that a list holds
+constexpr int kListRows = 64;    // the most rows of a block
+constexpr int kExpandRows = 32;  // 64 leave one wavefront a SIMD: 286 us for 40,688 rows x 5,120 of rank 64 instead of 183
 constexpr int kShrinkWaves = 8;
 
 struct AdapterCall {
@@ -22,9 +30,16 @@ struct AdapterCall {
   int64_t x_row, y_row, out_row;
   const float *scales;
   const int32_t *index;
-  uint16_t *h;  // [rows, rank rounded up to 32 in eights, 2, 8]: s A x as two bf16 numbers
-  int rows, width, out_width, adapters, rank, rank32, shares, copy;
+  uint16_t *h;  // [rows, ranks, in eights: 8 first numbers, 8 second ones]: s A x as two bf16 numbers
+  int rows, width, out_width, adapters, ranks, shares, copy;  // ranks: 16, or the rank rounded up to 32
 };
+
+// Between what lanes of a wavefront write to LDS and what others of them read: its LDS operations run in order, but the compiler
+// may leave out or move accesses of which no lane's own reads tell.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 // The adapter of each of a block's rows, a lane a row: -1 for none and behind the last row.
 __device__ __forceinline__ int adapter_of(const AdapterCall &p, int row0, int block_rows) {
@@ -36,57 +51,54 @@ __device__ __forceinline__ int adapter_of(const AdapterCall &p, int row0, int bl
 // The rows of `mask`, one behind another, as a wavefront's list; the last one repeats behind its end.
 __device__ __forceinline__ void list_rows(uint64_t mask, int *list) {
   const int lane = threadIdx.x & 63, at = __popcll(mask & ((1ull << lane) - 1)), count = __popcll(mask);
+  wave_sync();
   if ((mask >> lane) & 1) list[at] = lane;
   if (lane >= count) list[lane] = 63 - __builtin_clzll(mask);
+  wave_sync();
 }
 
-// s A x of the rows of one adapter in a block: the wavefronts take steps of 64 channels in turn and add their sums up in LDS.
+// s A x of the rows of one adapter in a block, in two bf16 numbers, 2^-17 of it: one would add 1.1e-3 of the product to the
+// result's own 1.7e-3 of rounding. The wavefronts take steps of 64 channels in turn and add their sums up in LDS.
 // C[rank][row] tiles: a lane has four ranks of a row.
 template <int MT, int NT>
 __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int rank0,
-                                            f32x4_t (*sums)[64]) {
-  constexpr int T = MT * NT, W = kShrinkWaves;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-  const uint16_t *xp[MT], *ap[NT];
-  bool has[NT];
+                                            u32x4_t (*sums)[64]) {
+  constexpr int T = MT * NT, W = kShrinkWaves, TURN = T < W ? T : W;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+  const int steps = (p.width + 63) / 64, tiles16 = p.ranks / 16, r8 = lane >> 3, c8 = lane & 7;
+  // x is read in runs of 128 bytes of a row, eight rows at a time, and turns into fragments in the wavefront's part of LDS:
+  // chunk c (16 bytes) of row r lies at slot c ^ (r % 8)
+  u32x4_t *stage = &sums[0][0] + wave * (16 * MT * 8);
+  const uint16_t *xp[2 * MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xp[m] = p.x + (int64_t)(row0 + list[16 * m + l16]) * p.x_row;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = rank0 + 16 * t + l16;
-    has[t] = r < p.rank;
-    ap[t] = p.down + ((int64_t)adapter * p.rank + (has[t] ? r : 0)) * p.width;
-  }
+  for (int i = 0; i < 2 * MT; ++i) xp[i] = p.x + (int64_t)(row0 + list[8 * i + r8]) * p.x_row;
+  // ranks behind the last tile read it again; their sums are not used
+  const uint16_t *ap = p.down + ((int64_t)adapter * steps * tiles16 + rank0 / 16) * 1024 + lane * 8;
+  const int most = tiles16 - rank0 / 16 - 1;
   f32x4_t acc[T] = {};
-  auto products = [&](const u32x4_t *a, const u32x4_t *x) __device__ {
+  __syncthreads();  // the sums of another adapter have been read
+  for (int step = wave; step < steps; step += W) {
+    u32x4_t a[2][NT], x[2 * MT];
+    // channels behind the width: A holds zeros for them, x is read again
+    const int c = min(64 * step + 8 * c8, p.width - 8);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < 2 * MT; ++i) x[i] = ld16(xp[i] + c);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[t * MT + m] = mfma_bf16_16x16x32(as_bf16x8(a[t]), as_bf16x8(x[m]), acc[t * MT + m]);
-  };
-  int c0 = 64 * wave;
-  for (; c0 + 64 <= p.width; c0 += 64 * W) {
-    u32x4_t a[2][NT], x[2][MT];
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = c0 + 32 * k + 8 * g;
+      for (int t = 0; t < NT; ++t) a[k][t] = ld16(ap + ((int64_t)step * tiles16 + min(t, most)) * 1024 + 512 * k);
+    wave_sync();
 #pragma unroll
-      for (int m = 0; m < MT; ++m) x[k][m] = ld16(xp[m] + c);
+    for (int i = 0; i < 2 * MT; ++i) stage[(8 * i + r8) * 8 + (c8 ^ r8)] = x[i];
+    wave_sync();
 #pragma unroll
-      for (int t = 0; t < NT; ++t) a[k][t] = has[t] ? ld16(ap[t] + c) : u32x4_t{};
-    }
-    products(a[0], x[0]);
-    products(a[1], x[1]);
-  }
-  for (int c1 = c0; c1 < p.width && c1 < c0 + 64; c1 += 32) {
-    const int c = c1 + 8 * g;
-    const bool in = c < p.width;
-    u32x4_t a[NT], x[MT];
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) a[t] = in && has[t] ? ld16(ap[t] + c) : u32x4_t{};
+      for (int m = 0; m < MT; ++m) {
+        const bf16x8_t f = as_bf16x8(stage[(16 * m + l16) * 8 + ((4 * k + g) ^ (l16 & 7))]);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) x[m] = in ? ld16(xp[m] + c) : u32x4_t{};
-    products(a, x);
+        for (int t = 0; t < NT; ++t) acc[t * MT + m] = mfma_bf16_16x16x32(as_bf16x8(a[k][t]), f, acc[t * MT + m]);
+      }
   }
   // tile i is added up and written by wavefront i % W
   constexpr int KEPT = (T + W - 1) / W;
@@ -96,19 +108,19 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
     const int tiles = T - k * W < W ? T - k * W : W;  // the tiles of this turn
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < tiles; ++i) sums[wave * W + i][lane] = acc[k * W + i];
+    for (int i = 0; i < tiles; ++i) sums[wave * TURN + i][lane] = __builtin_bit_cast(u32x4_t, acc[k * W + i]);
     __syncthreads();
     if (wave >= tiles) continue;
-    f32x4_t all = sums[wave][lane];
+    f32x4_t all = __builtin_bit_cast(f32x4_t, sums[wave][lane]);
 #pragma unroll
-    for (int w = 1; w < W; ++w) all += sums[w * W + wave][lane];
+    for (int w = 1; w < W; ++w) all += __builtin_bit_cast(f32x4_t, sums[w * TURN + wave][lane]);
     const int i = k * W + wave, m = i % MT, r = rank0 + 16 * (i / MT) + 4 * g;
-    if (16 * m + l16 >= count || r >= p.rank32) continue;
+    if (16 * m + l16 >= count || r >= p.ranks) continue;
     all *= scale;
     const u32x2_t hi = {pack_bf2(all[0], all[1]), pack_bf2(all[2], all[3])};
     const u32x2_t lo = {pack_bf2(all[0] - __uint_as_float(hi[0] << 16), all[1] - __uint_as_float(hi[0] & 0xffff0000u)),
                         pack_bf2(all[2] - __uint_as_float(hi[1] << 16), all[3] - __uint_as_float(hi[1] & 0xffff0000u))};
-    uint16_t *to = p.h + ((int64_t)(row0 + list[16 * m + l16]) * p.rank32 + (r & ~7)) * 2 + (r & 4);
+    uint16_t *to = p.h + ((int64_t)(row0 + list[16 * m + l16]) * p.ranks + (r & ~7)) * 2 + (r & 4);
     *reinterpret_cast<u32x2_t *>(to) = hi;
     *reinterpret_cast<u32x2_t *>(to + 8) = lo;
   }
@@ -117,8 +129,10 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
 // grid: shares x rank groups x blocks of 16 MT rows; a workgroup takes every `shares`-th adapter of its block
 template <int MT, int NT>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(AdapterCall p, int groups) {
-  __shared__ f32x4_t sums[kShrinkWaves * kShrinkWaves][64];
-  __shared__ int lists[kShrinkWaves][kBlockRows];
+  // sums of the wavefronts, a kilobyte a tile; before that 2 MT of them as each wavefront's part for x
+  constexpr int TURN = MT * NT < kShrinkWaves ? MT * NT : kShrinkWaves;
+  __shared__ u32x4_t sums[kShrinkWaves * (TURN > 2 * MT ? TURN : 2 * MT)][64];
+  __shared__ int lists[kShrinkWaves][kListRows];
   int at = blockIdx.x;
   const int share = at % p.shares;
   at /= p.shares;
@@ -142,81 +156,117 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
   }
 }
 
-// s A x of a row, eight ranks, as the operand's two bf16 numbers
-struct HalfPair {
-  u32x4_t hi, lo;
-};
-__device__ __forceinline__ HalfPair load_h(const uint16_t *row, int r) { return HalfPair{ld16(row + 2 * r), ld16(row + 2 * r + 8)}; }
+// Four k-values a lane: A[m = l % 16][k = 4 (l / 16) + j], B[k][n] alike
+__device__ __forceinline__ f32x4_t mfma_bf16_16x16x16(u32x2_t a, u32x2_t b, f32x4_t c) {
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, a), __builtin_bit_cast(s16x4_t, b), c, 0, 0, 0);
+}
 
-// out = y + s B h of the rows of one adapter in a block, a wavefront's 64 of each 256 columns of the workgroup's span.
+// A wavefront's 16 x 64 tile in LDS on its way from columns to rows
+constexpr int kTurnRow = 68, kTurn = 16 * kTurnRow;
+
+// out = y + B h of the rows of one adapter in a block, a wavefront's 64 of each 256 columns of the workgroup's span.
 // C[column][row] tiles whose columns are ordered so that a pair of tiles gives a lane eight neighbours: row m of tile t is
-// column 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. KS: the ranks in 32s, kept as operands over the columns; 0: any number of
-// them, read again for each 64 columns.
+// column 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. They turn in LDS so that y and out are read and written in runs of 128
+// bytes of a row, eight rows at a time: 833 MB take 150 us that way, and 197 as 64 bytes of 16 rows, as the tiles lie. KS: the ranks in 32s, kept as operands over the columns; 0: 16 ranks;
+// -1: any number of 32s, read again for each 64 columns.
 template <int MT, int KS>
 __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int col0,
-                                            int col_end) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+                                            int col_end, float *turn) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, r8 = lane >> 3, c8 = lane & 7;
   const uint16_t *hp[MT];
-  int64_t row[MT];
+  int64_t row[2 * MT];  // the lane's rows of y and out: 8 i + r8 of the list
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) row[i] = row0 + list[8 * i + r8];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    row[m] = row0 + list[16 * m + l16];
-    hp[m] = p.h + row[m] * p.rank32 * 2;
+    hp[m] = p.h + (int64_t)(row0 + list[16 * m + l16]) * p.ranks * 2 + (KS ? 16 * g : 16 * (g / 2) + 4 * (g % 2));
   }
-  HalfPair h[KS ? KS : 1][MT];
+  constexpr int KEPT = KS > 0 ? KS : 1;
+  u32x4_t hi[KEPT][MT], lo[KEPT][MT];  // 16 ranks: the first halves
+  auto load_h = [&](int i, int k) __device__ {
 #pragma unroll
-  for (int k = 0; k < KS; ++k)
+    for (int m = 0; m < MT; ++m) {
+      if constexpr (KS == 0) {
+        const u32x2_t a = *reinterpret_cast<const u32x2_t *>(hp[m]), b = *reinterpret_cast<const u32x2_t *>(hp[m] + 8);
+        hi[i][m] = u32x4_t{a[0], a[1], 0, 0};
+        lo[i][m] = u32x4_t{b[0], b[1], 0, 0};
+      } else {
+        hi[i][m] = ld16(hp[m] + 64 * k);
+        lo[i][m] = ld16(hp[m] + 64 * k + 8);
+      }
+    }
+  };
+  if constexpr (KS >= 0) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) h[k][m] = load_h(hp[m], 32 * k + 8 * g);
-  const uint16_t *up = p.up + (int64_t)adapter * p.out_width * p.rank;
+    for (int k = 0; k < KEPT; ++k) load_h(k, k);
+  }
+  const int ks = KS < 0 ? p.ranks / 32 : KEPT, pairs = (p.out_width + 31) / 32, piece = KS ? 1024 : 512;
+  const uint16_t *up = p.up + (int64_t)adapter * pairs * ks * piece + lane * 8;
   for (; col0 < col_end; col0 += 256) {
-    u32x4_t y[MT][2];
+    const int c = col0 + 8 * c8;
+    u32x4_t y[2 * MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int i = 0; i < 2 * MT; ++i) y[i] = c < p.out_width && 8 * i + r8 < count ? ld16(p.y + row[i] * p.y_row + c) : u32x4_t{};
+    f32x4_t acc[4][MT] = {};
+    auto products = [&](int i, int k) __device__ {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int c = col0 + 32 * t + 8 * g;
-        y[m][t] = c < p.out_width && 16 * m + l16 < count ? ld16(p.y + row[m] * p.y_row + c) : u32x4_t{};
-      }
-    f32x4_t acc[4][MT] = {};
-    auto products = [&](int r0, const HalfPair *hk) __device__ {
-      const int r = r0 + 8 * g;
+        // columns behind the last read the last pair again and are not stored
+        const uint16_t *b = up + ((int64_t)min(col0 / 32 + t, pairs - 1) * ks + k) * piece;
+        if constexpr (KS == 0) {
+          const u32x4_t both = ld16(b);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int c = col0 + 32 * (t / 2) + 8 * (l16 / 4) + 4 * (t % 2) + l16 % 4;
-        const u32x4_t b = r < p.rank && c < p.out_width ? ld16(up + (int64_t)c * p.rank + r) : u32x4_t{};
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(b), as_bf16x8(hk[m].hi), acc[t][m]);
-          acc[t][m] = mfma_bf16_16x16x32(as_bf16x8(b), as_bf16x8(hk[m].lo), acc[t][m]);
+            for (int m = 0; m < MT; ++m) {
+              const u32x2_t f = {both[2 * half], both[2 * half + 1]};
+              f32x4_t &c = acc[2 * t + half][m];
+              c = mfma_bf16_16x16x16(f, u32x2_t{hi[i][m][0], hi[i][m][1]}, c);
+              c = mfma_bf16_16x16x16(f, u32x2_t{lo[i][m][0], lo[i][m][1]}, c);
+            }
+        } else {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const bf16x8_t f = as_bf16x8(ld16(b + 512 * half));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              f32x4_t &c = acc[2 * t + half][m];
+              c = mfma_bf16_16x16x32(f, as_bf16x8(hi[i][m]), c);
+              c = mfma_bf16_16x16x32(f, as_bf16x8(lo[i][m]), c);
+            }
+          }
         }
       }
     };
-    if constexpr (KS > 0) {
+    if constexpr (KS >= 0) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) products(32 * k, h[k]);
+      for (int k = 0; k < KEPT; ++k) products(k, k);
     } else {
-      for (int r0 = 0; r0 < p.rank; r0 += 32) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) h[0][m] = load_h(hp[m], r0 + 8 * g);
-        products(r0, h[0]);
+      for (int k = 0; k < ks; ++k) {
+        load_h(0, k);
+        products(0, k);
       }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (16 * m + l16 >= count) continue;
+      float *tile = turn + (m & 1) * kTurn;
+      wave_sync();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int c = col0 + 32 * t + 8 * g;
-        if (c >= p.out_width) continue;
+      for (int t = 0; t < 4; ++t)
+        *reinterpret_cast<f32x4_t *>(tile + l16 * kTurnRow + 32 * (t / 2) + 8 * g + 4 * (t % 2)) = acc[t][m];
+      wave_sync();
+#pragma unroll
+      for (int i = 2 * m; i < 2 * m + 2; ++i) {
+        const f32x4_t *d = reinterpret_cast<const f32x4_t *>(tile + (8 * (i & 1) + r8) * kTurnRow + 8 * c8);
+        const f32x4_t d0 = d[0], d1 = d[1];
         u32x4_t o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const f32x4_t &d = acc[2 * t + j / 2][m];
-          o[j] = pack_bf2(__uint_as_float(y[m][t][j] << 16) + d[2 * (j % 2)],
-                          __uint_as_float(y[m][t][j] & 0xffff0000u) + d[2 * (j % 2) + 1]);
+          const float x0 = j < 2 ? d0[2 * j] : d1[2 * j - 4], x1 = j < 2 ? d0[2 * j + 1] : d1[2 * j - 3];
+          o[j] = pack_bf2(__uint_as_float(y[i][j] << 16) + x0, __uint_as_float(y[i][j] & 0xffff0000u) + x1);
         }
-        st16(p.out + row[m] * p.out_row + c, o);
+        if (c < p.out_width && 8 * i + r8 < count) st16(p.out + row[i] * p.out_row + c, o);
       }
     }
   }
@@ -224,19 +274,20 @@ __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, cons
 
 // grid: spans of columns x shares x blocks; a workgroup takes every `shares`-th adapter of its block
 template <int KS>
-__global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterCall p, int spans, int span, int shares) {
-  __shared__ int lists[4][kBlockRows];
+__global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, int spans, int span, int shares) {
+  __shared__ int lists[4][kListRows];
+  __shared__ __attribute__((aligned(16))) float turns[4][2 * kTurn];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int at = blockIdx.x;
   const int first = at % spans * span, col0 = first + 64 * wave, col_end = min(first + span, p.out_width);
   at /= spans;
-  const int share = at % shares, row0 = at / shares * kBlockRows;
+  const int share = at % shares, row0 = at / shares * kExpandRows;
   if (col0 >= col_end) return;
   int *list = lists[wave];
-  const int mine = adapter_of(p, row0, kBlockRows);
+  const int mine = adapter_of(p, row0, kExpandRows);
   uint64_t left = __ballot(mine >= 0);
   if (p.copy) {  // rows without an adapter: y as it is
-    const uint64_t none = __ballot(mine < 0 && row0 + lane < p.rows);
+    const uint64_t none = __ballot(mine < 0 && lane < kExpandRows && row0 + lane < p.rows);
     if (none) {
       list_rows(none, list);
       const int count = __popcll(none);
@@ -253,40 +304,41 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(AdapterCall p, int 
     if (n % shares != share) continue;
     list_rows(rows, list);
     const int count = __popcll(rows);
-    if (count <= 16) expand_rows<1, KS>(p, row0, list, count, adapter, col0, col_end);
-    else if (count <= 32) expand_rows<2, KS>(p, row0, list, count, adapter, col0, col_end);
-    else expand_rows<4, KS>(p, row0, list, count, adapter, col0, col_end);
+    if (count <= 16) expand_rows<1, KS>(p, row0, list, count, adapter, col0, col_end, turns[wave]);
+    else expand_rows<kExpandRows / 16, KS>(p, row0, list, count, adapter, col0, col_end, turns[wave]);
   }
 }
 
-#ifndef ROWS64
-#define ROWS64 16384
-#endif
-#ifndef ROWS32
-#define ROWS32 8192
-#endif
-#ifndef EX_WG
-#define EX_WG 2048
-#endif
+// The ranks that are kept: 16, or a multiple of 32; zeros behind the adapter's own.
+int kept_ranks(int rank) { return rank <= 16 ? 16 : (rank + 31) / 32 * 32; }
+
+// Rows of a shrinking workgroup: 16 until there are workgroups enough without, since A is read for each (3,939 rows of rank 32:
+// 15.2 us with 16, 21 with 32, 35 with 64; 9,000 of rank 128: 59 with 16, 48 with 32; 40,688 of rank 64: 117, 85, 84).
+constexpr int kRows32 = 8192, kRows64 = 16384;
+// Adapters of a block go to workgroups of their own, and its columns, until there are about this many: 64 rows of 16 adapters x
+// 15,360 columns 6.3 us (all adapters in one workgroup 98, in 16 8.1), 256 of them 13.7 (18, 15); 40,688 rows x 5,120 columns
+// 183 us in six spans, 191 in three; 9,000 x 15,360 111 and 125.
+constexpr int kShrinkGroups = 512, kExpandShares = 1024, kExpandGroups = 8192;
+
 struct AdapterCut {
-  int rank32, row_tiles, rank_tiles, groups, shares, span, expand_shares;
+  int ranks, row_tiles, rank_tiles, groups, shares, span, expand_shares;
   int64_t shrink, expand;  // workgroups
 };
 AdapterCut adapter_cut(int rows, int out_width, int adapters, int rank) {
   AdapterCut c;
-  c.rank32 = (rank + 31) / 32 * 32;
-  c.row_tiles = rows >= ROWS64 ? 4 : rows >= ROWS32 ? 2 : 1;
+  c.ranks = kept_ranks(rank);
+  c.row_tiles = rows >= kRows64 ? 4 : rows >= kRows32 ? 2 : 1;
   const int most = c.row_tiles == 4 ? 4 : 8;
-  c.rank_tiles = 2;
-  while (c.rank_tiles < most && 16 * c.rank_tiles < c.rank32) c.rank_tiles *= 2;
-  c.groups = (c.rank32 + 16 * c.rank_tiles - 1) / (16 * c.rank_tiles);
+  c.rank_tiles = 1;
+  while (c.rank_tiles < most && 16 * c.rank_tiles < c.ranks) c.rank_tiles *= 2;
+  c.groups = (c.ranks + 16 * c.rank_tiles - 1) / (16 * c.rank_tiles);
   const int64_t blocks = (rows + 16 * c.row_tiles - 1) / (16 * c.row_tiles), of = std::min(rows, adapters);
-  c.shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16 * c.row_tiles, 512 / (blocks * c.groups)}));
+  c.shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16 * c.row_tiles, kShrinkGroups / (blocks * c.groups)}));
   c.shrink = blocks * c.groups * c.shares;
   // columns of an expanding workgroup: fewer than all where that leaves too few workgroups
-  const int64_t tall = (rows + kBlockRows - 1) / kBlockRows, column_tiles = (out_width + 255) / 256;
-  c.expand_shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16, EX_WG / (tall * column_tiles)}));
-  const int64_t spans = std::min(column_tiles, std::max<int64_t>(1, EX_WG / (tall * c.expand_shares)));
+  const int64_t tall = (rows + kExpandRows - 1) / kExpandRows, column_tiles = (out_width + 255) / 256;
+  c.expand_shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16, kExpandShares / (tall * column_tiles)}));
+  const int64_t spans = std::min(column_tiles, std::max<int64_t>(1, kExpandGroups / (tall * c.expand_shares)));
   c.span = (int)((column_tiles + spans - 1) / spans) * 256;
   c.expand = tall * c.expand_shares * ((out_width + c.span - 1) / c.span);
   return c;
@@ -304,7 +356,7 @@ int check_adapter_rows(const void *p, int64_t row, int width, const char *name, 
 
 extern "C" size_t vdnh3_adapter_workspace_bytes(int rows, int rank) {
   if (rows <= 0 || rank <= 0 || rank > 1024) return 0;
-  return (size_t)rows * ((rank + 31) / 32 * 32) * 4;
+  return (size_t)rows * vdnh3::kept_ranks(rank) * 4;
 }
 
 extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_t *x, int64_t x_row, const uint16_t *down,
@@ -315,17 +367,17 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   VDNH3_HOST_CHECK(rows > 0 && width > 0 && out_width > 0 && adapters > 0 && rank > 0, VDNH3_ERR_INVALID,
                    "adapter_add: rows, widths, adapters and rank must be positive, got %d rows, %d -> %d, %d of rank %d", rows, width,
                    out_width, adapters, rank);
-  VDNH3_HOST_CHECK(width % 8 == 0 && out_width % 8 == 0 && rank % 8 == 0 && rank <= 1024, VDNH3_ERR_INVALID,
-                   "adapter_add: widths and rank must be multiples of 8, the rank at most 1024, got %d -> %d, rank %d", width,
-                   out_width, rank);
+  VDNH3_HOST_CHECK(width % 8 == 0 && out_width % 8 == 0 && rank <= 1024, VDNH3_ERR_INVALID,
+                   "adapter_add: widths must be multiples of 8 and the rank at most 1024, got %d -> %d, rank %d", width, out_width,
+                   rank);
   VDNH3_HOST_CHECK(index != nullptr, VDNH3_ERR_INVALID, "adapter_add: an index is needed");
   if (rows == 1) y_row = out_row = out_width, x_row = width;  // one row has no stride, whatever a caller passes for it
   int rc = check_adapter_rows(x, x_row, width, "x", true);
   if (!rc) rc = check_adapter_rows(y, y_row, out_width, "y", true);
   if (!rc) rc = check_adapter_rows(out, out_row, out_width, "out", false);
-  if (!rc) rc = check_adapter_rows(down, width, width, "down", true);
-  if (!rc) rc = check_adapter_rows(up, rank, rank, "up", true);
   if (rc) return rc;
+  VDNH3_HOST_CHECK(down && up && reinterpret_cast<uintptr_t>(down) % 16 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0,
+                   VDNH3_ERR_INVALID, "adapter_add: down and up must be 16-byte aligned");
   VDNH3_HOST_CHECK(out != y || out_row == y_row, VDNH3_ERR_INVALID, "adapter_add: out over y needs y's row stride");
   const size_t needed = vdnh3_adapter_workspace_bytes(rows, rank);
   VDNH3_HOST_CHECK(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= needed,
@@ -335,19 +387,26 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   if (!rc) rc = check_grid(c.expand, 256, "adapter_add");
   if (rc) return rc;
   const AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<uint16_t *>(workspace), rows, width,
-                      out_width, adapters, rank, c.rank32, c.shares, out != y};
+                      out_width, adapters, c.ranks, c.shares, out != y};
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto shrink = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.shrink), dim3(64 * kShrinkWaves), 0, s, p, c.groups); };
-  if (c.row_tiles == 4)
-    c.rank_tiles == 2 ? shrink(adapter_shrink_kernel<4, 2>) : shrink(adapter_shrink_kernel<4, 4>);
-  else if (c.row_tiles == 2)
-    c.rank_tiles == 2 ? shrink(adapter_shrink_kernel<2, 2>) : c.rank_tiles == 4 ? shrink(adapter_shrink_kernel<2, 4>) : shrink(adapter_shrink_kernel<2, 8>);
-  else
-    c.rank_tiles == 2 ? shrink(adapter_shrink_kernel<1, 2>) : c.rank_tiles == 4 ? shrink(adapter_shrink_kernel<1, 4>) : shrink(adapter_shrink_kernel<1, 8>);
+  auto by_ranks = [&](auto rows16) {
+    constexpr int MT = decltype(rows16)::value;
+    if (c.rank_tiles == 1) shrink(adapter_shrink_kernel<MT, 1>);
+    else if (c.rank_tiles == 2) shrink(adapter_shrink_kernel<MT, 2>);
+    else if (c.rank_tiles == 4) shrink(adapter_shrink_kernel<MT, 4>);
+    else if constexpr (MT < 4) shrink(adapter_shrink_kernel<MT, 8>);
+  };
+  if (c.row_tiles == 4) by_ranks(std::integral_constant<int, 4>());
+  else if (c.row_tiles == 2) by_ranks(std::integral_constant<int, 2>());
+  else by_ranks(std::integral_constant<int, 1>());
   rc = check_launch("adapter_add");
   if (rc) return rc;
   const int spans = (out_width + c.span - 1) / c.span;
   auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.expand), dim3(256), 0, s, p, spans, c.span, c.expand_shares); };
-  rank <= 32 ? expand(adapter_expand_kernel<1>) : rank <= 64 ? expand(adapter_expand_kernel<2>) : expand(adapter_expand_kernel<0>);
+  if (c.ranks == 16) expand(adapter_expand_kernel<0>);
+  else if (c.ranks == 32) expand(adapter_expand_kernel<1>);
+  else if (c.ranks == 64) expand(adapter_expand_kernel<2>);
+  else expand(adapter_expand_kernel<-1>);
   return check_launch("adapter_add");
 }

@@ -25,13 +25,29 @@ def _workspace_bytes(rows: int, rank: int) -> int:
     return _lib.lib().vdnh3_adapter_workspace_bytes(rows, rank)
 
 
+def _layouts(down: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """A and B in the kernels' order (``include/vdnh3.h``), the rank filled up with zeros to 16 or a multiple of 32, the widths
+    to multiples of 64 and 32."""
+    n, rank, width = down.shape
+    out = up.shape[1]
+    ranks = 16 if rank <= 16 else -(-rank // 32) * 32
+    pad = torch.nn.functional.pad
+    a = pad(down, (0, -width % 64, 0, ranks - rank)).view(n, ranks // 16, 16, -1, 2, 4, 8)
+    b = pad(up, (0, ranks - rank, 0, -out % 32))
+    if ranks == 16:
+        b = b.view(n, -1, 4, 2, 4, 4, 4).permute(0, 1, 5, 2, 4, 3, 6)
+    else:
+        b = b.view(n, -1, 4, 2, 4, ranks // 32, 4, 8).permute(0, 1, 5, 3, 6, 2, 4, 7)
+    return a.permute(0, 3, 1, 4, 5, 2, 6).contiguous(), b.contiguous()
+
+
 class LowRankAdapters:
     """The adapters of one projection ``[out, width]``: ``down`` ``[n, rank, width]`` (A) and ``up`` ``[n, out, rank]`` (B), bf16 on
     the GPU, and ``scales``, ``n`` numbers (a tensor or a sequence; ``None``: ones), kept in fp32.
 
-    Widths are multiples of 8; a rank that is none is filled up with zeros. Contiguous tensors of such a rank are used where they
-    lie (a later change of theirs counts), others are copied. ``from_pairs`` takes adapters of different ranks. The object holds
-    the tensors on the device: it has to outlive graphs that were captured with it.
+    Widths are multiples of 8, ranks at most 1024. The object keeps both in the kernels' order, copied once (a later change of the
+    tensors is not seen), and has to outlive graphs that were captured with it. ``from_pairs`` takes adapters of different
+    ranks.
     """
 
     def __init__(self, down: torch.Tensor, up: torch.Tensor, scales=None):
@@ -44,8 +60,7 @@ class LowRankAdapters:
         self.out_width = int(up.shape[1])
         if self.width % 8 or self.out_width % 8:
             raise ValueError(f"the projection's widths must be multiples of 8, got {self.width} -> {self.out_width}")
-        fill = -self.rank % 8
-        if self.rank + fill > 1024:
+        if self.rank > 1024:
             raise ValueError(f"ranks up to 1024 are supported, got {self.rank}")
         _lib.forward_only("LowRankAdapters", down, up, scales)
         if scales is not None:
@@ -53,11 +68,7 @@ class LowRankAdapters:
             if scales.numel() != self.count:
                 raise ValueError(f"scales must be {self.count} numbers, got {scales.numel()}")
         self.device = _lib.require_device(down, up, scales)
-        if fill:
-            down = torch.nn.functional.pad(down, (0, 0, 0, fill))
-            up = torch.nn.functional.pad(up, (0, fill))
-        self.down, self.up = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else
-                              t.clone(memory_format=torch.contiguous_format) for t in (down.detach(), up.detach()))
+        self.down, self.up = _layouts(down.detach(), up.detach())
         self.scales = None if scales is None else scales.detach()
 
     @classmethod
@@ -101,12 +112,12 @@ class LowRankAdapters:
             index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
         index = index.to(torch.int32).contiguous()
         x, y = _lib.operand(x), _lib.operand(y)
-        size = _workspace_bytes(rows, self.down.shape[1])
+        size = _workspace_bytes(rows, self.rank)
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         _lib.launch(name, _lib.lib().vdnh3_adapter_add, device,
                     y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), self.down.data_ptr(), self.up.data_ptr(),
                     _lib.ptr(self.scales), index.data_ptr(), out.data_ptr(), out.stride(0), rows, self.width, self.out_width,
-                    self.count, self.down.shape[1], workspace.data_ptr(), size)
+                    self.count, self.rank, workspace.data_ptr(), size)
         return out
 
 

@@ -598,11 +598,17 @@ int vdnh3_gated_delta_step(const uint16_t *q, int64_t q_batch, int64_t q_row, in
                            int64_t g_row, int64_t g_head, float *pool, int64_t slot_stride, int64_t head_stride, int slot_count,
                            const int32_t *slots, int batch, int new_tokens, int heads, int qk_heads, int head_dim, void *stream);
 
-/* out[t] = bf16(y[t] + scales[i] up[i] (down[i] x[t])), i = index[t]: the low-rank adapters of many requests, down
- * [adapters, rank, width] and up [adapters, out_width, rank] contiguous, beside a projection's output y [rows, out_width].
- * scales null: ones. An index outside [0, adapters) names no adapter: out[t] = y[t]. out may be y. Widths and rank are
- * multiples of 8, the rank at most 1024; row strides of x and y may be 0. workspace (vdnh3_adapter_workspace_bytes, 16-byte
- * aligned) holds the products with down as two bf16 numbers each. */
+/* out[t] = bf16(y[t] + scales[i] B_i (A_i x[t])), i = index[t]: the low-rank adapters of many requests, A_i [rank, width] and
+ * B_i [out_width, rank], beside a projection's output y [rows, out_width]. scales null: ones. An index outside [0, adapters) names
+ * no adapter: out[t] = y[t]. out may be y. Widths are multiples of 8, the rank is at most 1024; row strides of x and y may be 0.
+ * A and B lie in the order of the wavefronts' operands, zeros behind their own numbers, with R = 16 ranks for ranks up to 16,
+ * else the rank rounded up to 32:
+ *   down [adapters][width / 64, rounded up][R / 16][2][4][16][8] bf16: the element [i][s][t][k][g][m][j] is
+ *        A_i[16 t + m][64 s + 32 k + 8 g + j];
+ *   up   [adapters][out_width / 32, rounded up][R / 32][2][4][16][8]: [i][p][k][t][g][m][j] is
+ *        B_i[32 p + 8 (m / 4) + 4 t + m % 4][32 k + 8 g + j]; for R = 16 [adapters][out_width / 32][4][16][2][4]: [i][p][g][m][t][j]
+ *        is B_i[32 p + 8 (m / 4) + 4 t + m % 4][4 g + j].
+ * workspace (vdnh3_adapter_workspace_bytes, 16-byte aligned) holds scales[i] A_i x[t] as two bf16 numbers each. */
 size_t vdnh3_adapter_workspace_bytes(int rows, int rank);
 int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_t *x, int64_t x_row, const uint16_t *down,
                       const uint16_t *up, const float *scales, const int32_t *index, uint16_t *out, int64_t out_row, int rows,
