@@ -100,13 +100,13 @@ __device__ __forceinline__ LinRange lin_range(const LinCall &p, int range, int64
                                     __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3])}};
 }
 
-// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Q and K: the 16 rows of a fragment read hit 16
-// different 16-byte bank groups, and the transposed reads of K, 8 bytes of four chunks of eight rows, cover all banks as
-// evenly as halves of chunks can. V: the 8 rows that half a wavefront reads 32 bytes of hit 8 different 32-byte groups.
+// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Q and K: the same chunk of the 16 rows of a fragment read
+// lies in 16 different 16-byte bank groups, and 32 bytes of the 8 rows that half a wavefront reads transposed in 8 different
+// 32-byte ones. V: only the latter.
 template <int D>
 __device__ __forceinline__ int qk_swizzle(int r) {
-  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
-  else return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  if constexpr (D == 128) return ((r & 7) << 1) | ((r >> 3) & 1);
+  else return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
 }
 template <int D>
 __device__ __forceinline__ int v_swizzle(int r) {
@@ -139,8 +139,9 @@ __device__ __forceinline__ Split2 split2(const float *x) {
 }
 
 // A workgroup of D / 16 wavefronts walks a range of a head's chunks; a wavefront carries 16 rows (dv) of the state in
-// accumulators, as C[dk][dv] tiles whose dk are ordered so that a lane's registers are the operand of S q as they lie:
-// row m of tile t is dk = 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. Outputs are computed transposed, O^T[dv][row].
+// accumulators, as C[dk][dv] tiles: a lane has dk = 16 t + 4 g + i of its dv, and two tiles are the operand of S q as they lie,
+// with k = 8 g + j standing for dk = 32 s + 16 (j / 4) + 4 g + j % 4; Q and K are read in that order too. Outputs are computed
+// transposed, O^T[dv][row].
 // CARRY: only the state at the range's end, where the last sequence goes on behind it.
 template <int D, bool CARRY>
 __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
@@ -167,14 +168,14 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       for (int t = 0; t < D / 16; ++t) s[t] = f32x4_t{};
       return;
     }
-    const float *r = from + (int64_t)dv * D + 8 * g;
+    const float *r = from + (int64_t)dv * D + 4 * g;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) s[t] = *reinterpret_cast<const f32x4_t *>(r + 32 * (t / 2) + 4 * (t % 2));
+    for (int t = 0; t < D / 16; ++t) s[t] = *reinterpret_cast<const f32x4_t *>(r + 16 * t);
   };
   auto store_state = [&](float *to) __device__ {
-    float *r = to + (int64_t)dv * D + 8 * g;
+    float *r = to + (int64_t)dv * D + 4 * g;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t *>(r + 32 * (t / 2) + 4 * (t % 2)) = s[t];
+    for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t *>(r + 16 * t) = s[t];
   };
   const int64_t state_at = (int64_t)h * D * D, state_step = (int64_t)p.heads * D * D;
   auto initial_of = [&](int b) __device__ { return p.initial ? p.initial + b * state_step + state_at : nullptr; };
@@ -236,14 +237,18 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
   };
 
   // ---- what stays the same over a head's chunks ----------------------------------------------------------------------
-  // fragment of row l16 of a 16-row tile of Q or K, k-step s: 16 bytes; transposed reads of K by pairs of dk tiles and of V
-  int qk_at[NS], kt_at[NS];
+  // fragment of row l16 of a 16-row tile of Q or K by 16 dk: 8 bytes; transposed reads of K by dk tiles, and of V
+  int qk_at[D / 16], kt_at[D / 16];
   const int tr = 4 * g + (l16 >> 2);
 #pragma unroll
-  for (int t = 0; t < NS; ++t) {
-    qk_at[t] = l16 * D + ((4 * t + g) ^ qk_swizzle<D>(l16)) * 8;
-    kt_at[t] = tr * D + ((4 * t + (l16 & 3)) ^ qk_swizzle<D>(tr)) * 8;
+  for (int t = 0; t < D / 16; ++t) {
+    qk_at[t] = l16 * D + ((2 * t + (g >> 1)) ^ qk_swizzle<D>(l16)) * 8 + 4 * (g & 1);
+    kt_at[t] = tr * D + ((2 * t + ((l16 >> 1) & 1)) ^ qk_swizzle<D>(tr)) * 8 + 4 * (l16 & 1);
   }
+  auto qk_frag = [&](const uint16_t *tile, int t) __device__ {
+    const u32x2_t a = *reinterpret_cast<const u32x2_t *>(tile + qk_at[2 * t]), b = *reinterpret_cast<const u32x2_t *>(tile + qk_at[2 * t + 1]);
+    return as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
+  };
   const int vt_at = tr * D + ((2 * wave + ((l16 >> 1) & 1)) ^ v_swizzle<D>(tr)) * 8 + 4 * (l16 & 1);
   // the wavefront's tiles of P^T: row tile prt, token tiles pu, pu + PS, ... up to the diagonal
   constexpr int PS = NW / 4;
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
         f32x4_t c = {};
 #pragma unroll
         for (int t = 0; t < NS; ++t)
-          c = mfma_bf16_16x16x32(as_bf16x8(ld16(kt + 16 * u * D + qk_at[t])), as_bf16x8(ld16(qt + 16 * prt * D + qk_at[t])), c);
+          c = mfma_bf16_16x16x32(qk_frag(kt + 16 * u * D, t), qk_frag(qt + 16 * prt * D, t), c);
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -328,7 +333,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
         const Split2 sp = split2(x);
 #pragma unroll
         for (int rt = 0; rt < 4; ++rt) {
-          const bf16x8_t qf = as_bf16x8(ld16(qt + 16 * rt * D + qk_at[t]));
+          const bf16x8_t qf = qk_frag(qt + 16 * rt * D, t);
           o[rt] = mfma_bf16_16x16x32(as_bf16x8(sp.hi), qf, o[rt]);
           o[rt] = mfma_bf16_16x16x32(as_bf16x8(sp.lo), qf, o[rt]);
         }
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       }
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        const uint16_t *kr = kt + 32 * ks * D + kt_at[t / 2] + 4 * (t & 1);
+        const uint16_t *kr = kt + 32 * ks * D + kt_at[t];
         const u32x2_t a = lin_read_transposed(kr), b = lin_read_transposed(kr + 16 * D);
         const bf16x8_t kf = as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
         s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w2), s[t]);
