@@ -186,63 +186,56 @@ bool fits4(const void *p, int64_t a, int64_t b, int64_t c, int bytes) {
 }
 
 template <bool DELTA>
-int state_step(const StepCall &p, int batch, int qk_heads, void *stream, const char *what) {
-  VDNH3_HOST_CHECK(batch > 0 && p.tokens > 0 && p.heads > 0 && qk_heads > 0 && p.heads % qk_heads == 0, VDNH3_ERR_INVALID,
-                   "%s: batch, tokens and heads must be positive and heads a multiple of qk_heads, got %d x %d, %d / %d heads",
-                   what, batch, p.tokens, p.heads, qk_heads);
-  VDNH3_HOST_CHECK(p.dim > 0 && p.dim <= 128, VDNH3_ERR_INVALID, "%s: head_dim must be 1 to 128, got %d", what, p.dim);
-  VDNH3_HOST_CHECK(p.q.p && p.k.p && p.v.p && p.out && p.pool && (DELTA ? p.beta.p && p.g.p : p.log_decay != nullptr),
-                   VDNH3_ERR_INVALID, "%s: an operand is missing", what);
-  VDNH3_HOST_CHECK(p.slot_count > 0 && (p.slots || batch <= p.slot_count), VDNH3_ERR_INVALID,
-                   "%s: %d requests need a state each, the pool has %d", what, batch, p.slot_count);
-  const int64_t own = (int64_t)p.dim * p.dim;
+int state_step(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out, const float *decay, const float *beta,
+               float *pool, const int32_t *slots, const vdnh3_step_layout *layout, float scale, void *stream, const char *what) {
+  VDNH3_HOST_CHECK(layout != nullptr, VDNH3_ERR_INVALID, "%s: a layout is needed", what);
+  const vdnh3_step_layout &l = *layout;
+  for (const int64_t n : {l.slots, l.batch, l.new_tokens, l.heads, l.qk_heads, l.head_dim})
+    VDNH3_HOST_CHECK(n > 0 && n <= INT32_MAX, VDNH3_ERR_INVALID, "%s: sizes must be positive and fit 32 bits, got %lld", what,
+                     (long long)n);
+  VDNH3_HOST_CHECK(l.heads % l.qk_heads == 0, VDNH3_ERR_INVALID, "%s: %lld heads are no multiple of %lld q / k heads", what,
+                   (long long)l.heads, (long long)l.qk_heads);
+  VDNH3_HOST_CHECK(l.head_dim <= 128, VDNH3_ERR_INVALID, "%s: head_dim must be 1 to 128, got %lld", what, (long long)l.head_dim);
+  VDNH3_HOST_CHECK(q && k && v && out && pool && decay && (beta || !DELTA), VDNH3_ERR_INVALID, "%s: an operand is missing", what);
+  VDNH3_HOST_CHECK(slots || l.batch <= l.slots, VDNH3_ERR_INVALID, "%s: %lld requests need a state each, the pool has %lld", what,
+                   (long long)l.batch, (long long)l.slots);
+  const int64_t own = l.head_dim * l.head_dim;
   // one state behind another, heads inside slots or slots inside heads; a stride of a single one is not looked at
   auto apart = [own](int64_t inner, int64_t count, int64_t outer) {
     return inner >= own && inner <= (INT64_MAX >> 32) && outer >= (count - 1) * inner + own;
   };
-  VDNH3_HOST_CHECK(p.heads == 1 || p.slot_count == 1
-                       ? (p.slot_count == 1 || p.slot_stride >= own) && (p.heads == 1 || p.head_stride >= own)
-                       : apart(p.head_stride, p.heads, p.slot_stride) || apart(p.slot_stride, p.slot_count, p.head_stride),
+  VDNH3_HOST_CHECK(l.heads == 1 || l.slots == 1
+                       ? (l.slots == 1 || l.slot >= own) && (l.heads == 1 || l.state_head >= own)
+                       : apart(l.state_head, l.heads, l.slot) || apart(l.slot, l.slots, l.state_head),
                    VDNH3_ERR_INVALID, "%s: states must not overlap", what);
-  VDNH3_HOST_CHECK(std::isfinite(p.scale), VDNH3_ERR_INVALID, "%s: scale must be finite", what);
-  const int64_t per_request = (int64_t)((p.dim + 31) / 32) * p.heads;
-  const int rc = check_grid(per_request > (1 << 24) ? per_request : per_request * batch, 256, what);
+  VDNH3_HOST_CHECK(std::isfinite(scale), VDNH3_ERR_INVALID, "%s: scale must be finite", what);
+  const int64_t per_request = (l.head_dim + 31) / 32 * l.heads;
+  const int rc = check_grid(per_request > (1 << 24) ? per_request : per_request * l.batch, 256, what);
   if (rc) return rc;
+  const StepCall p{{q, l.q_batch, l.q_row, l.q_head}, {k, l.k_batch, l.k_row, l.k_head}, {v, l.v_batch, l.v_row, l.v_head},
+                   out, l.o_batch, l.o_row, l.o_head, decay, {beta, l.beta_batch, l.beta_row, l.beta_head},
+                   {decay, l.g_batch, l.g_row, l.g_head}, pool, l.slot, l.state_head, slots, (int)l.slots, (int)l.new_tokens,
+                   (int)l.heads, (int)(l.heads / l.qk_heads), (int)l.head_dim, 1, scale};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool vec = p.dim % 4 == 0 && fits4(p.pool, p.slot_stride, p.head_stride, 0, 16) &&
-                   fits4(p.q.p, p.q.batch, p.q.row, p.q.head, 8) && fits4(p.k.p, p.k.batch, p.k.row, p.k.head, 8);
-  if (vec && p.dim % 64 == 0) launch_state_step<DELTA, 2>(p, batch, s);
-  else if (vec) launch_state_step<DELTA, 1>(p, batch, s);
-  else launch_state_step<DELTA, 0>(p, batch, s);
+  const bool vec = p.dim % 4 == 0 && fits4(pool, l.slot, l.state_head, 0, 16) && fits4(q, l.q_batch, l.q_row, l.q_head, 8) &&
+                   fits4(k, l.k_batch, l.k_row, l.k_head, 8);
+  if (vec && p.dim % 64 == 0) launch_state_step<DELTA, 2>(p, (int)l.batch, s);
+  else if (vec) launch_state_step<DELTA, 1>(p, (int)l.batch, s);
+  else launch_state_step<DELTA, 0>(p, (int)l.batch, s);
   return check_launch(what);
 }
 
 }  // namespace
 }  // namespace vdnh3
 
-extern "C" int vdnh3_causal_linear_step(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
-                                        int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch,
-                                        int64_t v_row, int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row,
-                                        int64_t o_head, const float *log_decay, float *pool, int64_t slot_stride,
-                                        int64_t head_stride, int slot_count, const int32_t *slots, int batch, int new_tokens,
-                                        int heads, int qk_heads, int head_dim, float scale, void *stream) {
-  using namespace vdnh3;
-  const StepCall p{{q, q_batch, q_row, q_head}, {k, k_batch, k_row, k_head}, {v, v_batch, v_row, v_head}, out, o_batch, o_row,
-                   o_head, log_decay, {}, {}, pool, slot_stride, head_stride, slots, slot_count, new_tokens, heads,
-                   qk_heads > 0 ? heads / qk_heads : 1, head_dim, 1, scale};
-  return state_step<false>(p, batch, qk_heads, stream, "causal_linear_step");
+extern "C" int vdnh3_causal_linear_step(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out,
+                                        const float *log_decay, float *pool, const int32_t *slots,
+                                        const vdnh3_step_layout *layout, float scale, void *stream) {
+  return vdnh3::state_step<false>(q, k, v, out, log_decay, nullptr, pool, slots, layout, scale, stream, "causal_linear_step");
 }
 
-extern "C" int vdnh3_gated_delta_step(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
-                                      int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch,
-                                      int64_t v_row, int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row,
-                                      int64_t o_head, const float *beta, int64_t b_batch, int64_t b_row, int64_t b_head,
-                                      const float *log_decay, int64_t g_batch, int64_t g_row, int64_t g_head, float *pool,
-                                      int64_t slot_stride, int64_t head_stride, int slot_count, const int32_t *slots, int batch,
-                                      int new_tokens, int heads, int qk_heads, int head_dim, void *stream) {
-  using namespace vdnh3;
-  const StepCall p{{q, q_batch, q_row, q_head}, {k, k_batch, k_row, k_head}, {v, v_batch, v_row, v_head}, out, o_batch, o_row,
-                   o_head, nullptr, {beta, b_batch, b_row, b_head}, {log_decay, g_batch, g_row, g_head}, pool, slot_stride,
-                   head_stride, slots, slot_count, new_tokens, heads, qk_heads > 0 ? heads / qk_heads : 1, head_dim, 1, 1.f};
-  return state_step<true>(p, batch, qk_heads, stream, "gated_delta_step");
+extern "C" int vdnh3_gated_delta_step(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out, const float *beta,
+                                      const float *log_decay, float *pool, const int32_t *slots, const vdnh3_step_layout *layout,
+                                      void *stream) {
+  return vdnh3::state_step<true>(q, k, v, out, log_decay, beta, pool, slots, layout, 1.f, stream, "gated_delta_step");
 }

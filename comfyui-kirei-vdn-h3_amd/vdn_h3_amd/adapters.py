@@ -20,9 +20,24 @@ from . import _lib
 _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
-@lru_cache(maxsize=1024)
-def _workspace_bytes(rows: int, rank: int) -> int:
-    return _lib.lib().vdnh3_adapter_workspace_bytes(rows, rank)
+@lru_cache(maxsize=4096)
+def _add_plan(xs, xt, xd, ys, yt, yd, ins, it, ind, width: int, out_width: int, rank: int) -> tuple[int, int, bool]:
+    """What the layouts of a call say, checked once for each set of them: ``(rows, workspace bytes, whether no operand has to be
+    copied but for an address off 16 bytes)``."""
+    rows = xs[0] if len(xs) == 2 else -1
+    if len(xs) != 2 or tuple(xs) != (rows, width) or tuple(ys) != (rows, out_width):
+        raise ValueError(f"y must be [rows, {out_width}] and x [rows, {width}]; got {tuple(ys)} and {tuple(xs)}")
+    if xd != torch.bfloat16 or yd != torch.bfloat16:
+        raise TypeError(f"LowRankAdapters.add computes in bf16; got {yd}/{xd}")
+    if tuple(ins) != (rows,) or ind not in _INTEGERS:
+        raise ValueError(f"index must be a tensor of {rows} integers, one per row")
+    _lib.int32_sizes("LowRankAdapters.add", rows)
+
+    def whole(t):
+        return t[1] == 1 and (rows < 2 or t[0] % 8 == 0)
+
+    as_they_lie = whole(xt) and whole(yt) and ind == torch.int32 and (rows < 2 or it[0] == 1)
+    return rows, _lib.lib().vdnh3_adapter_workspace_bytes(rows, rank) if rows else 0, as_they_lie
 
 
 def _layouts(down: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -91,28 +106,24 @@ class LowRankAdapters:
         the row keeps ``y``. The sum is rounded once; ``A x`` is fp32. Rows of one adapter are fastest next to each other.
         """
         name = "LowRankAdapters.add"
-        rows = x.shape[0] if x.ndim == 2 else -1
-        if x.ndim != 2 or tuple(x.shape) != (rows, self.width) or tuple(y.shape) != (rows, self.out_width):
-            raise ValueError(f"y must be [rows, {self.out_width}] and x [rows, {self.width}]; got {tuple(y.shape)} and {tuple(x.shape)}")
-        if x.dtype != torch.bfloat16 or y.dtype != torch.bfloat16:
-            raise TypeError(f"{name} computes in bf16; got {y.dtype}/{x.dtype}")
-        if not isinstance(index, torch.Tensor) or index.ndim != 1 or index.numel() != rows or index.dtype not in _INTEGERS:
-            raise ValueError(f"index must be a tensor of {rows} integers, one per row")
+        if not isinstance(index, torch.Tensor):
+            raise ValueError(f"index must be a tensor of integers, one per row, got {type(index).__name__}")
+        rows, size, as_they_lie = _add_plan(x.shape, x.stride(), x.dtype, y.shape, y.stride(), y.dtype, index.shape, index.stride(),
+                                            index.dtype, self.width, self.out_width, self.rank)
         _lib.forward_only(name, y, x, out)
-        _lib.int32_sizes(name, rows)
         device = _lib.require_device(self.down, y, x, index, out)
         if out is None:
             out = torch.empty(rows, self.out_width, dtype=torch.bfloat16, device=device)
-        elif tuple(out.shape) != (rows, self.out_width) or out.dtype != torch.bfloat16 or not _lib.in_place(out) or \
-                (rows > 1 and out.stride(0) < self.out_width):
+        elif out is not y and (tuple(out.shape) != (rows, self.out_width) or out.dtype != torch.bfloat16) or \
+                not _lib.in_place(out) or (rows > 1 and out.stride(0) < self.out_width):
             raise ValueError(f"out must be a bf16 [{rows}, {self.out_width}] tensor with 16-byte aligned rows that do not overlap")
         if rows == 0:
             return out
-        if index.dtype == torch.int64:
-            index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
-        index = index.to(torch.int32).contiguous()
-        x, y = _lib.operand(x), _lib.operand(y)
-        size = _workspace_bytes(rows, self.rank)
+        if not as_they_lie or x.data_ptr() % 16 or y.data_ptr() % 16:
+            x, y = _lib.operand(x), _lib.operand(y)
+            if index.dtype == torch.int64:
+                index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
+            index = index.to(torch.int32).contiguous()
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         _lib.launch(name, _lib.lib().vdnh3_adapter_add, device,
                     y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), self.down.data_ptr(), self.up.data_ptr(),

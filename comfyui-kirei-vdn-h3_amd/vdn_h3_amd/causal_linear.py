@@ -13,23 +13,23 @@ needs no copy to the host, and a captured one can be replayed with others. Forwa
 
 from __future__ import annotations
 
+import ctypes
 from functools import lru_cache
 
 import torch
 
 from . import _lib
-from .causal import _INTEGERS, _int32, _output, _sequence_bounds
+from .causal import _INTEGERS, _output, _sequence_bounds
 from .window import KERNEL_HEAD_DIMS, padded_head_dim, zero_pad_channels
 
 
-def _check_heads(query, key, value, name):
-    if query.dtype != torch.bfloat16 or key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
-        raise TypeError(f"{name} computes in bf16; got {query.dtype}/{key.dtype}/{value.dtype}")
-    heads, qk_heads = value.shape[-2], query.shape[-2]
+def _head_checks(name: str, dtypes, heads: int, qk_heads: int, dim: int) -> None:
+    if any(d != torch.bfloat16 for d in dtypes):
+        raise TypeError(f"{name} computes in bf16; got {dtypes[0]}/{dtypes[1]}/{dtypes[2]}")
     if (heads > 0 and qk_heads == 0) or (qk_heads and heads % qk_heads):
         raise ValueError(f"{heads} value heads are no multiple of {qk_heads} query / key heads")
-    if not 0 < query.shape[-1] <= KERNEL_HEAD_DIMS[-1]:
-        raise ValueError(f"{name} supports head dims 1 to {KERNEL_HEAD_DIMS[-1]}, got {query.shape[-1]}")
+    if not 0 < dim <= KERNEL_HEAD_DIMS[-1]:
+        raise ValueError(f"{name} supports head dims 1 to {KERNEL_HEAD_DIMS[-1]}, got {dim}")
 
 
 def _decays(log_decay, heads: int, name: str) -> torch.Tensor:
@@ -44,29 +44,6 @@ def _states(state, shape, name: str) -> torch.Tensor:
     if state.dtype != torch.float32:
         raise TypeError(f"{name} must be fp32, got {state.dtype}")
     return state
-
-
-def _pool(pool, heads: int, dim: int, name: str) -> tuple:
-    """The strides of slots and heads of a pool ``[slots, heads, dim, dim]`` that is updated in place."""
-    if not isinstance(pool, torch.Tensor) or pool.ndim != 4 or tuple(pool.shape[1:]) != (heads, dim, dim):
-        raise ValueError(f"{name}: state must be [slots, {heads}, {dim}, {dim}]")
-    if pool.dtype != torch.float32:
-        raise TypeError(f"{name}: state must be fp32, got {pool.dtype}")
-    if dim > 1 and (pool.stride(3) != 1 or pool.stride(2) != dim):
-        raise ValueError(f"{name}: each head's state must be contiguous (it is updated in place)")
-    return pool.stride(0), pool.stride(1)
-
-
-def _slots(slots, batch: int, count: int, name: str):
-    if slots is None:
-        if batch > count:
-            raise ValueError(f"{name}: {batch} requests need a state each, the pool has {count}")
-        return None
-    if not isinstance(slots, torch.Tensor) or slots.ndim != 1 or slots.numel() != batch or slots.dtype not in _INTEGERS:
-        raise ValueError(f"{name}: slots must be a tensor of {batch} integers")
-    if slots.dtype == torch.int64:
-        slots = slots.clamp(-1, count)  # outside the pool stays outside in 32 bits
-    return slots.to(torch.int32).contiguous()
 
 
 @lru_cache(maxsize=1024)
@@ -95,7 +72,7 @@ def causal_linear_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Te
             query.shape[2] != value.shape[2]:
         raise ValueError("query and key must be [rows, qk_heads, dim], value [rows, heads, dim]; got "
                          f"{tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}")
-    _check_heads(query, key, value, name)
+    _head_checks(name, (query.dtype, key.dtype, value.dtype), value.shape[1], query.shape[1], query.shape[2])
     _lib.forward_only(name, query, key, value, log_decay, initial_state, out)
     rows, heads, dim = value.shape
     _lib.int32_sizes(name, rows, heads)
@@ -139,26 +116,83 @@ def causal_linear_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     return out, final
 
 
-def _step_operands(query, key, value, name):
-    if query.ndim != 4 or query.shape != key.shape or value.ndim != 4 or query.shape[:2] != value.shape[:2] or \
-            query.shape[3] != value.shape[3]:
+@lru_cache(maxsize=4096)
+def _step_plan(name: str, *layouts) -> tuple:
+    """What the layouts of a step call say, checked and put down for the library once for each set of them, not per call (that
+    took more than half of a call's 15 us): shape, strides and dtype of q, k, v, the pool, slots, out (``None`` three times
+    without them) and the gates. Returns ``(vdnh3_step_layout, out's shape, whether operands have to be copied first)``."""
+    (qs, qt, qd), (ks, kt, kd), (vs, vt, vd), (ps, pt, pd), (ss, st, sd), (os, ot, od), *gates = zip(*[iter(layouts)] * 3)
+    if len(qs) != 4 or qs != ks or len(vs) != 4 or qs[:2] != vs[:2] or qs[3] != vs[3]:
         raise ValueError("query and key must be [batch, new, qk_heads, dim], value [batch, new, heads, dim]; got "
-                         f"{tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}")
-    _check_heads(query, key, value, name)
-    _lib.int32_sizes(name, *value.shape)
+                         f"{tuple(qs)}, {tuple(ks)} and {tuple(vs)}")
+    _head_checks(name, (qd, kd, vd), vs[2], qs[2], qs[3])
+    batch, new, heads, dim = vs
+    _lib.int32_sizes(name, *vs)
+    if len(ps) != 4 or tuple(ps[1:]) != (heads, dim, dim):
+        raise ValueError(f"{name}: state must be [slots, {heads}, {dim}, {dim}], got {tuple(ps)}")
+    if pd != torch.float32:
+        raise TypeError(f"{name}: state must be fp32, got {pd}")
+    if dim > 1 and (pt[3] != 1 or pt[2] != dim):
+        raise ValueError(f"{name}: each head's state must be contiguous (it is updated in place)")
+    _lib.int32_sizes(name, ps[0])
+    if ss is None:
+        if batch > ps[0]:
+            raise ValueError(f"{name}: {batch} requests need a state each, the pool has {ps[0]}")
+    elif tuple(ss) != (batch,) or sd not in _INTEGERS:
+        raise ValueError(f"{name}: slots must be a tensor of {batch} integers")
+    if os is None:
+        ot = (new * heads * dim, heads * dim, dim, 1)
+    elif os != vs or od != torch.bfloat16 or (dim > 1 and ot[3] != 1) or any(n > 1 and s == 0 for n, s in zip(os, ot)):
+        raise ValueError(f"out must be a bf16 {list(vs)} tensor with a contiguous last dim and no stride of 0")
+    shape = (heads,) if len(gates) == 1 else (batch, new, heads)
+    for gs, _, gd in gates:
+        if tuple(gs) != shape or not gd.is_floating_point:
+            what = "log_decay must be a tensor" if len(gates) == 1 else "beta and g must be tensors"
+            raise ValueError(f"{name}: {what} of shape {list(shape)}, floating-point")
+    # the channels next to each other; slots in 32 bits; gates in fp32, one per head next to each other
+    copies = any(t[3] != 1 and dim != 1 for t in (qt, kt, vt)) or (
+        ss is not None and (sd != torch.int32 or (batch > 1 and st[0] != 1))) or any(
+        gd != torch.float32 or (len(gates) == 1 and heads > 1 and gt[0] != 1) for _, gt, gd in gates)
+    gate_strides = (0,) * 6 if len(gates) == 1 else (*gates[0][1], *gates[1][1])
+    layout = (ctypes.c_int64 * 26)(*qt[:3], *kt[:3], *vt[:3], *ot[:3], pt[0], pt[1], *gate_strides, ps[0], batch, new, heads,
+                                   qs[2], dim)
+    return layout, tuple(vs), copies
 
 
-def _rows(t):
-    """A bf16 operand of the step kernels: any strides, the channels next to each other."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _step_copies(query, key, value, slots, gates, count: int):
+    """The operands as the kernels take them, where a call's layouts need copies."""
+    if slots is not None:
+        if slots.dtype == torch.int64:
+            slots = slots.clamp(-1, count)  # outside the pool stays outside in 32 bits
+        slots = slots.to(torch.int32).contiguous()
+    gates = tuple(g.float().contiguous() for g in gates)
+    return *(t if t.stride(-1) == 1 else t.contiguous() for t in (query, key, value)), slots, gates
 
 
-def _step_output(out, shape, device):
+def _step(name: str, fn, query, key, value, state, slots, gates, out, *scale):
+    """A step call of either rule: ``gates`` are its decays (one number a head), or beta and g (one a token and head)."""
+    try:
+        layouts = (query.shape, query.stride(), query.dtype, key.shape, key.stride(), key.dtype, value.shape, value.stride(),
+                   value.dtype, state.shape, state.stride(), state.dtype,
+                   *((None, None, None) if slots is None else (slots.shape, slots.stride(), slots.dtype)),
+                   *((None, None, None) if out is None else (out.shape, out.stride(), out.dtype)),
+                   *(x for g in gates for x in (g.shape, g.stride(), g.dtype)))
+    except AttributeError:
+        raise TypeError(f"{name} takes tensors (query, key, value, the gates, state, slots, out)") from None
+    layout, shape, copies = _step_plan(name, *layouts)
+    _lib.forward_only(name, query, key, value, state, out, *gates)
+    device = _lib.require_device(query, key, value, state, slots, out, *gates)
     if out is None:
-        return torch.empty(*shape, dtype=torch.bfloat16, device=device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != torch.bfloat16 or (shape[-1] > 1 and out.stride(-1) != 1) or \
-            any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise ValueError(f"out must be a bf16 {list(shape)} tensor with a contiguous last dim and no stride of 0")
+        out = torch.empty(*shape, dtype=torch.bfloat16, device=device)
+    if 0 in shape:
+        return out
+    if state.shape[0] == 0:
+        return out.zero_()
+    if copies:
+        query, key, value, slots, gates = _step_copies(query, key, value, slots, gates, state.shape[0])
+        return _step(name, fn, query, key, value, state, slots, gates, out, *scale)
+    _lib.launch(name, fn, device, query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(),
+                *[g.data_ptr() for g in gates], state.data_ptr(), None if slots is None else slots.data_ptr(), layout, *scale)
     return out
 
 
@@ -173,25 +207,8 @@ def causal_linear_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     earlier request of the batch names belongs to that one: the later request's rows are NaN. Head dims up to 128.
     ``out`` must not overlap the inputs.
     """
-    name = "causal_linear_step"
-    _step_operands(query, key, value, name)
-    batch, new, heads, dim = value.shape
-    _lib.forward_only(name, query, key, value, log_decay, state, out)
-    decays = _decays(log_decay, heads, name)
-    strides = _pool(state, heads, dim, name)
-    slots = _slots(slots, batch, state.shape[0], name)
-    device = _lib.require_device(query, key, value, decays, state, slots, out)
-    out = _step_output(out, value.shape, device)
-    if value.numel() == 0:
-        return out
-    if state.shape[0] == 0:
-        return out.zero_()
-    q, k, v = _rows(query), _rows(key), _rows(value)
-    _lib.launch(name, _lib.lib().vdnh3_causal_linear_step, device,
-                q.data_ptr(), *q.stride()[:-1], k.data_ptr(), *k.stride()[:-1], v.data_ptr(), *v.stride()[:-1],
-                out.data_ptr(), *out.stride()[:-1], decays.data_ptr(), state.data_ptr(), *strides, state.shape[0],
-                _lib.ptr(slots), batch, new, heads, query.shape[2], dim, float(scale))
-    return out
+    return _step("causal_linear_step", _lib.lib().vdnh3_causal_linear_step, query, key, value, state, slots, (log_decay,), out,
+                 float(scale))
 
 
 __all__ = ["causal_linear_packed", "causal_linear_step"]

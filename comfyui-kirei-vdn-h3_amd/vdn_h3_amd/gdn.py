@@ -19,7 +19,7 @@ import threading
 import torch
 
 from . import _lib
-from .causal_linear import _pool, _rows, _slots, _step_operands, _step_output
+from .causal_linear import _step
 
 
 class _Pipe:
@@ -186,26 +186,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
     ``slots`` and ``out`` as in ``causal_linear.causal_linear_step``: request ``b`` has ``state[slots[b]]`` (``state[b]`` without
     slots), one outside the pool gives zeros, a slot that an earlier request has gives NaN rows.
     """
-    name = "gated_delta_step"
-    _step_operands(q, k, v, name)
-    batch, new, heads, dim = v.shape
-    if tuple(beta.shape) != (batch, new, heads) or tuple(g.shape) != (batch, new, heads):
-        raise ValueError(f"beta and g must have shape [{batch}, {new}, {heads}]")
-    _lib.forward_only(name, q, k, v, beta, g, state, out)
-    strides = _pool(state, heads, dim, name)
-    slots = _slots(slots, batch, state.shape[0], name)
-    device = _lib.require_device(q, k, v, beta, g, state, slots, out)
-    out = _step_output(out, v.shape, device)
-    if v.numel() == 0:
-        return out
-    if state.shape[0] == 0:
-        return out.zero_()
-    q, k, v, beta, g = _rows(q), _rows(k), _rows(v), beta.float(), g.float()
-    _lib.launch(name, _lib.lib().vdnh3_gated_delta_step, device,
-                q.data_ptr(), *q.stride()[:-1], k.data_ptr(), *k.stride()[:-1], v.data_ptr(), *v.stride()[:-1],
-                out.data_ptr(), *out.stride()[:-1], beta.data_ptr(), *beta.stride(), g.data_ptr(), *g.stride(),
-                state.data_ptr(), *strides, state.shape[0], _lib.ptr(slots), batch, new, heads, q.shape[2], dim)
-    return out
+    return _step("gated_delta_step", _lib.lib().vdnh3_gated_delta_step, q, k, v, state, slots, (beta, g), out)
 
 
 def gdn_flops(tokens: int, heads: int, dim: int = 128, chunk: int = 64) -> float:

@@ -579,24 +579,25 @@ int vdnh3_causal_linear_packed(const uint16_t *q, int64_t q_row, int64_t q_head,
                                float scale, int ranges, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Its recurrent form for new_tokens tokens of each of `batch` requests: the states of request b are those at
- * pool + slots[b] slot_stride + h head_stride (contiguous [head_dim, head_dim] each; slots null: b), updated in place. A request
- * whose slot lies outside [0, slot_count) is idle: its rows are zeros. Of requests with the same slot the first has it; the
- * others' rows are NaN. head_dim 1 to 128, no alignment needed (16-byte states and 8-byte q / k rows are faster). */
-int vdnh3_causal_linear_step(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
-                             int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch, int64_t v_row,
-                             int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row, int64_t o_head,
-                             const float *log_decay, float *pool, int64_t slot_stride, int64_t head_stride, int slot_count,
-                             const int32_t *slots, int batch, int new_tokens, int heads, int qk_heads, int head_dim,
-                             float scale, void *stream);
+ * pool + slots[b] slot + h state_head (contiguous [head_dim, head_dim] each; slots null: b), updated in place. A request
+ * whose slot lies outside [0, layout->slots) is idle: its rows are zeros. Of requests with the same slot the first has it; the
+ * others' rows are NaN. head_dim 1 to 128, no alignment needed (16-byte states and 8-byte q / k rows are faster). `layout` is host
+ * memory, read before the call returns: strides in elements of requests, tokens and heads, of the pool's slots and heads, of beta
+ * and log_decay (the delta rule's, fp32, one number per request, token and value head; log_decay of the other is one per head,
+ * contiguous), and sizes. */
+typedef struct vdnh3_step_layout {
+  int64_t q_batch, q_row, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head, o_batch, o_row, o_head;
+  int64_t slot, state_head;
+  int64_t beta_batch, beta_row, beta_head, g_batch, g_row, g_head;
+  int64_t slots, batch, new_tokens, heads, qk_heads, head_dim;
+} vdnh3_step_layout;
+int vdnh3_causal_linear_step(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out, const float *log_decay,
+                             float *pool, const int32_t *slots, const vdnh3_step_layout *layout, float scale, void *stream);
 
-/* The same for the Gated DeltaNet (vdnh3_gdn_*): S_t = a S_{t-1} (I - beta k k^T) + beta v k^T, o = S_t q, a = exp(log_decay),
- * beta and log_decay one number per request, token and value head. */
-int vdnh3_gated_delta_step(const uint16_t *q, int64_t q_batch, int64_t q_row, int64_t q_head, const uint16_t *k,
-                           int64_t k_batch, int64_t k_row, int64_t k_head, const uint16_t *v, int64_t v_batch, int64_t v_row,
-                           int64_t v_head, uint16_t *out, int64_t o_batch, int64_t o_row, int64_t o_head, const float *beta,
-                           int64_t b_batch, int64_t b_row, int64_t b_head, const float *log_decay, int64_t g_batch,
-                           int64_t g_row, int64_t g_head, float *pool, int64_t slot_stride, int64_t head_stride, int slot_count,
-                           const int32_t *slots, int batch, int new_tokens, int heads, int qk_heads, int head_dim, void *stream);
+/* The same for the Gated DeltaNet (vdnh3_gdn_*): S_t = a S_{t-1} (I - beta k k^T) + beta v k^T, o = S_t q, a = exp(log_decay). */
+int vdnh3_gated_delta_step(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out, const float *beta,
+                           const float *log_decay, float *pool, const int32_t *slots, const vdnh3_step_layout *layout,
+                           void *stream);
 
 /* out[t] = bf16(y[t] + scales[i] B_i (A_i x[t])), i = index[t]: the low-rank adapters of many requests, A_i [rank, width] and
  * B_i [out_width, rank], beside a projection's output y [rows, out_width]. scales null: ones. An index outside [0, adapters) names
