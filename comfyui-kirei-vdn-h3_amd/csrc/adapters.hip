@@ -11,7 +11,7 @@
 // channels of A (strided rows of A took 18 us of 31 at 3,939 rows x 5,120 of rank 32) and of 32 columns x 32 (16) ranks of B.
 // x, y and out move in runs of 128 bytes of a row. HBM bounds both passes where there are many rows: 40,688 rows x 5,120 -> 5,120
 // of rank 64 take 84 us (x, 5.0 TB/s) and 183 us (y and out, 4.6 TB/s), a copy's rate; one row x 5,120 -> 15,360 of rank 16
-// 4.9 and 3.2 us, launches and chains of loads.
+// 5.9 us in one launch, a chain of loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,6 +23,7 @@ namespace {
 constexpr int kListRows = 64;    // the most rows of a block
 constexpr int kExpandRows = 32;  // 64 leave one wavefront a SIMD: 286 us for 40,688 rows x 5,120 of rank 64 instead of 183
 constexpr int kShrinkWaves = 8;
+constexpr int kFewRows = 64, kFewRanks = 64;  // up to which one launch makes both products
 
 struct AdapterCall {
   const uint16_t *x, *y, *down, *up;
@@ -60,9 +61,10 @@ __device__ __forceinline__ void list_rows(uint64_t mask, int *list) {
 // s A x of the rows of one adapter in a block, in two bf16 numbers, 2^-17 of it: one would add 1.1e-3 of the product to the
 // result's own 1.7e-3 of rounding. The wavefronts take steps of 64 channels in turn and add their sums up in LDS.
 // C[rank][row] tiles: a lane has four ranks of a row.
-template <int MT, int NT>
+// `h` holds the rows of the list one behind another (LISTED), or all rows.
+template <int MT, int NT, bool LISTED>
 __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int rank0,
-                                            u32x4_t (*sums)[64]) {
+                                            u32x4_t (*sums)[64], uint16_t *h) {
   constexpr int T = MT * NT, W = kShrinkWaves, TURN = T < W ? T : W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
   const int steps = (p.width + 63) / 64, tiles16 = p.ranks / 16, r8 = lane >> 3, c8 = lane & 7;
@@ -120,7 +122,8 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
     const u32x2_t hi = {pack_bf2(all[0], all[1]), pack_bf2(all[2], all[3])};
     const u32x2_t lo = {pack_bf2(all[0] - __uint_as_float(hi[0] << 16), all[1] - __uint_as_float(hi[0] & 0xffff0000u)),
                         pack_bf2(all[2] - __uint_as_float(hi[1] << 16), all[3] - __uint_as_float(hi[1] & 0xffff0000u))};
-    uint16_t *to = p.h + ((int64_t)(row0 + list[16 * m + l16]) * p.ranks + (r & ~7)) * 2 + (r & 4);
+    const int64_t row = LISTED ? 16 * m + l16 : row0 + list[16 * m + l16];
+    uint16_t *to = h + (row * p.ranks + (r & ~7)) * 2 + (r & 4);
     *reinterpret_cast<u32x2_t *>(to) = hi;
     *reinterpret_cast<u32x2_t *>(to + 8) = lo;
   }
@@ -148,10 +151,10 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
     list_rows(rows, list);
     const int count = __popcll(rows);
     if (MT > 1 && count > 16) {
-      if (MT > 2 && count > 32) shrink_rows<MT, NT>(p, row0, list, count, adapter, rank0, sums);
-      else shrink_rows<(MT > 1 ? 2 : 1), NT>(p, row0, list, count, adapter, rank0, sums);
+      if (MT > 2 && count > 32) shrink_rows<MT, NT, false>(p, row0, list, count, adapter, rank0, sums, p.h);
+      else shrink_rows<(MT > 1 ? 2 : 1), NT, false>(p, row0, list, count, adapter, rank0, sums, p.h);
     } else {
-      shrink_rows<1, NT>(p, row0, list, count, adapter, rank0, sums);
+      shrink_rows<1, NT, false>(p, row0, list, count, adapter, rank0, sums, p.h);
     }
   }
 }
@@ -165,14 +168,15 @@ __device__ __forceinline__ f32x4_t mfma_bf16_16x16x16(u32x2_t a, u32x2_t b, f32x
 // A wavefront's 16 x 64 tile in LDS on its way from columns to rows
 constexpr int kTurnRow = 68, kTurn = 16 * kTurnRow;
 
-// out = y + B h of the rows of one adapter in a block, a wavefront's 64 of each 256 columns of the workgroup's span.
+// out = y + B h of the rows of one adapter in a block, a wavefront's 64 of each STEP columns of the workgroup's span.
 // C[column][row] tiles whose columns are ordered so that a pair of tiles gives a lane eight neighbours: row m of tile t is
 // column 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. They turn in LDS so that y and out are read and written in runs of 128
 // bytes of a row, eight rows at a time: 833 MB take 150 us that way, and 197 as 64 bytes of 16 rows, as the tiles lie. KS: the ranks in 32s, kept as operands over the columns; 0: 16 ranks;
 // -1: any number of 32s, read again for each 64 columns.
-template <int MT, int KS>
+// STEP: the columns of the workgroup's wavefronts.
+template <int MT, int KS, int STEP, bool LISTED>
 __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int col0,
-                                            int col_end, float *turn) {
+                                            int col_end, float *turn, const uint16_t *h) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4, r8 = lane >> 3, c8 = lane & 7;
   const uint16_t *hp[MT];
   int64_t row[2 * MT];  // the lane's rows of y and out: 8 i + r8 of the list
@@ -180,7 +184,7 @@ __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, cons
   for (int i = 0; i < 2 * MT; ++i) row[i] = row0 + list[8 * i + r8];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    hp[m] = p.h + (int64_t)(row0 + list[16 * m + l16]) * p.ranks * 2 + (KS ? 16 * g : 16 * (g / 2) + 4 * (g % 2));
+    hp[m] = h + (LISTED ? 16 * m + l16 : (int64_t)row0 + list[16 * m + l16]) * p.ranks * 2 + (KS ? 16 * g : 16 * (g / 2) + 4 * (g % 2));
   }
   constexpr int KEPT = KS > 0 ? KS : 1;
   u32x4_t hi[KEPT][MT], lo[KEPT][MT];  // 16 ranks: the first halves
@@ -203,7 +207,7 @@ __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, cons
   }
   const int ks = KS < 0 ? p.ranks / 32 : KEPT, pairs = (p.out_width + 31) / 32, piece = KS ? 1024 : 512;
   const uint16_t *up = p.up + (int64_t)adapter * pairs * ks * piece + lane * 8;
-  for (; col0 < col_end; col0 += 256) {
+  for (; col0 < col_end; col0 += STEP) {
     const int c = col0 + 8 * c8;
     u32x4_t y[2 * MT];
 #pragma unroll
@@ -272,6 +276,19 @@ __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, cons
   }
 }
 
+// Rows without an adapter: y as it is, a wavefront's 64 of each STEP columns, eight of each 8 `shares` rows.
+template <int STEP>
+__device__ __forceinline__ void copy_rows(const AdapterCall &p, int row0, uint64_t rows, int *list, int share, int shares, int col0,
+                                          int col_end) {
+  if (rows == 0) return;
+  list_rows(rows, list);
+  const int lane = threadIdx.x & 63, count = __popcll(rows);
+  for (int i = share * 8 + (lane >> 3); i < count; i += 8 * shares) {
+    const int64_t row = row0 + list[i];
+    for (int c = col0 + 8 * (lane & 7); c < col_end; c += STEP) st16(p.out + row * p.out_row + c, ld16(p.y + row * p.y_row + c));
+  }
+}
+
 // grid: spans of columns x shares x blocks; a workgroup takes every `shares`-th adapter of its block
 template <int KS>
 __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, int spans, int span, int shares) {
@@ -286,17 +303,7 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, i
   int *list = lists[wave];
   const int mine = adapter_of(p, row0, kExpandRows);
   uint64_t left = __ballot(mine >= 0);
-  if (p.copy) {  // rows without an adapter: y as it is
-    const uint64_t none = __ballot(mine < 0 && lane < kExpandRows && row0 + lane < p.rows);
-    if (none) {
-      list_rows(none, list);
-      const int count = __popcll(none);
-      for (int i = share * 8 + (lane >> 3); i < count; i += 8 * shares) {
-        const int64_t row = row0 + list[i];
-        for (int c = col0 + 8 * (lane & 7); c < col_end; c += 256) st16(p.out + row * p.out_row + c, ld16(p.y + row * p.y_row + c));
-      }
-    }
-  }
+  if (p.copy) copy_rows<256>(p, row0, __ballot(mine < 0 && lane < kExpandRows && row0 + lane < p.rows), list, share, shares, col0, col_end);
   for (int n = 0; left; ++n) {
     const int adapter = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
     const uint64_t rows = __ballot(mine == adapter);
@@ -304,8 +311,47 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, i
     if (n % shares != share) continue;
     list_rows(rows, list);
     const int count = __popcll(rows);
-    if (count <= 16) expand_rows<1, KS>(p, row0, list, count, adapter, col0, col_end, turns[wave]);
-    else expand_rows<kExpandRows / 16, KS>(p, row0, list, count, adapter, col0, col_end, turns[wave]);
+    if (count <= 16) expand_rows<1, KS, 256, false>(p, row0, list, count, adapter, col0, col_end, turns[wave], p.h);
+    else expand_rows<kExpandRows / 16, KS, 256, false>(p, row0, list, count, adapter, col0, col_end, turns[wave], p.h);
+  }
+}
+
+// Both products in one launch for few rows: every workgroup of a span of columns makes s A x of its adapters' rows anew, in LDS.
+// Spans of 512 columns or more, as many workgroups as one round of the CUs: one row x 5,120 -> 15,360 of rank 16 takes 5.9 us
+// (two launches 7.7, and 4 us more of the host's), 64 rows of 16 adapters 11.0 in spans of 1,024 (512 16.7, 2,048 12.6, two
+// launches 13.9), but 64 rows of one adapter of rank 32 x 5,120 -> 5,120 14.5 (9.9).
+template <int NT, int KS>
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_few_rows_kernel(AdapterCall p, int spans, int span) {
+  constexpr int STEP = 64 * kShrinkWaves;
+  __shared__ u32x4_t sums[(kShrinkWaves * 2 * kTurn + 255) / 256][64];
+  __shared__ __attribute__((aligned(16))) uint16_t h[kFewRows * 16 * NT * 2];
+  __shared__ int lists[kShrinkWaves][kListRows];
+  static_assert(sizeof(sums) >= kShrinkWaves * 8 * 1024, "the tiles turn where x and the sums were");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int first = (int)blockIdx.x % spans * span, share = (int)blockIdx.x / spans;
+  const int col0 = first + 64 * wave, col_end = min(first + span, p.out_width);
+  int *list = lists[wave];
+  float *turn = reinterpret_cast<float *>(sums) + wave * 2 * kTurn;
+  const int mine = adapter_of(p, 0, kFewRows);
+  uint64_t left = __ballot(mine >= 0);
+  if (p.copy) copy_rows<STEP>(p, 0, __ballot(mine < 0 && lane < p.rows), list, share, p.shares, col0, col_end);
+  for (int n = 0; left; ++n) {
+    const int adapter = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    const uint64_t rows = __ballot(mine == adapter);
+    left &= ~rows;
+    if (n % p.shares != share) continue;
+    list_rows(rows, list);
+    const int count = __popcll(rows);
+    if (count <= 16) shrink_rows<1, NT, true>(p, 0, list, count, adapter, 0, sums, h);
+    else if (count <= 32) shrink_rows<2, NT, true>(p, 0, list, count, adapter, 0, sums, h);
+    else shrink_rows<4, NT, true>(p, 0, list, count, adapter, 0, sums, h);
+    __syncthreads();
+    if (count <= 16) {
+      expand_rows<1, KS, STEP, true>(p, 0, list, count, adapter, col0, col_end, turn, h);
+    } else {
+      for (int i = 0; i < count; i += 32)
+        expand_rows<2, KS, STEP, true>(p, 0, list + i, count - i, adapter, col0, col_end, turn, h + (int64_t)i * p.ranks * 2);
+    }
   }
 }
 
@@ -356,6 +402,7 @@ int check_adapter_rows(const void *p, int64_t row, int width, const char *name, 
 
 extern "C" size_t vdnh3_adapter_workspace_bytes(int rows, int rank) {
   if (rows <= 0 || rank <= 0 || rank > 1024) return 0;
+  if (rows <= vdnh3::kFewRows && rank <= vdnh3::kFewRanks) return 0;
   return (size_t)rows * vdnh3::kept_ranks(rank) * 4;
 }
 
@@ -380,15 +427,25 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
                    VDNH3_ERR_INVALID, "adapter_add: down and up must be 16-byte aligned");
   VDNH3_HOST_CHECK(out != y || out_row == y_row, VDNH3_ERR_INVALID, "adapter_add: out over y needs y's row stride");
   const size_t needed = vdnh3_adapter_workspace_bytes(rows, rank);
-  VDNH3_HOST_CHECK(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= needed,
+  VDNH3_HOST_CHECK(needed == 0 ||
+                       (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= needed),
                    VDNH3_ERR_INVALID, "adapter_add: needs a 16-byte aligned workspace of %zu bytes", needed);
   const AdapterCut c = adapter_cut(rows, out_width, adapters, rank);
   rc = check_grid(c.shrink, 64 * kShrinkWaves, "adapter_add");
   if (!rc) rc = check_grid(c.expand, 256, "adapter_add");
   if (rc) return rc;
-  const AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<uint16_t *>(workspace), rows, width,
-                      out_width, adapters, c.ranks, c.shares, out != y};
+  AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<uint16_t *>(workspace), rows, width,
+                out_width, adapters, c.ranks, c.shares, out != y};
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (needed == 0) {
+    p.shares = std::min({rows, adapters, 16});
+    const int wide = (out_width + 511) / 512, span = 512 * ((wide * p.shares + 255) / 256), few_spans = (out_width + span - 1) / span;
+    auto few = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(few_spans * p.shares), dim3(64 * kShrinkWaves), 0, s, p, few_spans, span); };
+    if (c.ranks == 16) few(adapter_few_rows_kernel<1, 0>);
+    else if (c.ranks == 32) few(adapter_few_rows_kernel<2, 1>);
+    else few(adapter_few_rows_kernel<4, 2>);
+    return check_launch("adapter_add");
+  }
   auto shrink = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.shrink), dim3(64 * kShrinkWaves), 0, s, p, c.groups); };
   auto by_ranks = [&](auto rows16) {
     constexpr int MT = decltype(rows16)::value;

@@ -124,11 +124,11 @@ class LowRankAdapters:
             if index.dtype == torch.int64:
                 index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
             index = index.to(torch.int32).contiguous()
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _lib.launch(name, _lib.lib().vdnh3_adapter_add, device,
                     y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), self.down.data_ptr(), self.up.data_ptr(),
                     _lib.ptr(self.scales), index.data_ptr(), out.data_ptr(), out.stride(0), rows, self.width, self.out_width,
-                    self.count, self.rank, workspace.data_ptr(), size)
+                    self.count, self.rank, _lib.ptr(workspace), size)
         return out
 
 
