@@ -51,10 +51,11 @@ __device__ __forceinline__ float sum16(float x) {
 
 // Columns of a row of the state: lane l16 has 4 l16 .. + 3 of each 64. The last of a head dim that is no multiple of 64 are
 // left out.
-template <bool VEC>
+template <bool VEC, bool STREAM>
 __device__ __forceinline__ f32x4_t load4(const float *p, int c, int dim) {
   if constexpr (VEC) {
-    return c < dim ? *reinterpret_cast<const f32x4_t *>(p + c) : f32x4_t{};
+    const f32x4_t *at = reinterpret_cast<const f32x4_t *>(p + c);
+    return c >= dim ? f32x4_t{} : STREAM ? __builtin_nontemporal_load(at) : *at;
   } else {
     f32x4_t x = {};
 #pragma unroll
@@ -92,6 +93,10 @@ __device__ __forceinline__ f32x4_t load4(const uint16_t *p, int c, int dim) {
 
 // MODE 0: any layout and head dim, number by number; 1: 16-byte columns; 2: the same, and the head dim is the lanes' 16 E.
 // A workgroup takes 16 G rows of one request's state of one head: a wavefront 4 G of them, 16 lanes a row, E columns a lane.
+// HBM is the bound: 64 requests x 40 heads x 128 (335 MB) take 58.6 us, 5.7 TB/s, where a large copy reaches 4.8; one request
+// 4.5 us, a launch and two chains of loads. 32 rows a workgroup (16: 74 us, 64: 69, 128: 79, one request 4.2, 5.3, 7.2). States of
+// more than 64 channels are read past the caches (65.1 us without; of 64 channels 23.1 without and 25.1 with); written so too
+// they take 60.8.
 template <bool DELTA, int E, int G, int MODE>
 __global__ __launch_bounds__(256) void state_step_kernel(StepCall p) {
   constexpr int Q = E / 4;
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(256) void state_step_kernel(StepCall p) {
   for (int g = 0; g < G; ++g) {
     const int r = row0 + 4 * g + r4;
 #pragma unroll
-    for (int c = 0; c < Q; ++c) s[g][c] = live && r < dim ? load4<VEC>(state + (int64_t)r * dim, 64 * c + 4 * l16, dim) : f32x4_t{};
+    for (int c = 0; c < Q; ++c) s[g][c] = live && r < dim ? load4<VEC, (E > 4)>(state + (int64_t)r * dim, 64 * c + 4 * l16, dim) : f32x4_t{};
   }
   // one request a slot: the first that names it has it, whatever order the workgroups run in
   bool taken = false;
