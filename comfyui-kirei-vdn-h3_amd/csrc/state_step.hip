@@ -64,10 +64,13 @@ __device__ __forceinline__ f32x4_t load4(const float *p, int c, int dim) {
     return x;
   }
 }
-template <bool VEC>
+template <bool VEC, bool STREAM>
 __device__ __forceinline__ void store4(float *p, int c, int dim, f32x4_t x) {
   if constexpr (VEC) {
-    if (c < dim) *reinterpret_cast<f32x4_t *>(p + c) = x;
+    f32x4_t *at = reinterpret_cast<f32x4_t *>(p + c);
+    if (c >= dim) return;
+    if (STREAM) __builtin_nontemporal_store(x, at);
+    else *at = x;
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -93,10 +96,11 @@ __device__ __forceinline__ f32x4_t load4(const uint16_t *p, int c, int dim) {
 
 // MODE 0: any layout and head dim, number by number; 1: 16-byte columns; 2: the same, and the head dim is the lanes' 16 E.
 // A workgroup takes 16 G rows of one request's state of one head: a wavefront 4 G of them, 16 lanes a row, E columns a lane.
-// HBM is the bound: 64 requests x 40 heads x 128 (335 MB) take 58.6 us, 5.7 TB/s, where a large copy reaches 4.8; one request
-// 4.5 us, a launch and two chains of loads. 32 rows a workgroup (16: 74 us, 64: 69, 128: 79, one request 4.2, 5.3, 7.2). States of
-// more than 64 channels are read past the caches (65.1 us without; of 64 channels 23.1 without and 25.1 with); written so too
-// they take 60.8.
+// HBM is the bound: 64 requests x 40 heads x 128 (335 MB) take 61.5 us, 5.5 TB/s, where a large copy reaches 4.8; one request
+// 4.5 us, a launch and two chains of loads. 32 rows a workgroup (with states in the caches 65 us, 16 rows 74, 64 rows 69, 128
+// rows 79; one request 4.5, 4.2, 5.3, 7.2). States of more than 64 channels pass the caches both ways: between two tokens lie the
+// other layers' states (70.7 us without, 67 read so, 68.6 written so; a state that is still in the caches 60.8, and 58.6 read
+// so; of 64 channels 25.3, and 23.1 without either if it is there).
 template <bool DELTA, int E, int G, int MODE>
 __global__ __launch_bounds__(256) void state_step_kernel(StepCall p) {
   constexpr int Q = E / 4;
@@ -172,7 +176,7 @@ __global__ __launch_bounds__(256) void state_step_kernel(StepCall p) {
     const int r = row0 + 4 * g + r4;
     if (r < dim)
 #pragma unroll
-      for (int c = 0; c < Q; ++c) store4<VEC>(state + (int64_t)r * dim, 64 * c + 4 * l16, dim, s[g][c]);
+      for (int c = 0; c < Q; ++c) store4<VEC, (E > 4)>(state + (int64_t)r * dim, 64 * c + 4 * l16, dim, s[g][c]);
   }
 }
 
