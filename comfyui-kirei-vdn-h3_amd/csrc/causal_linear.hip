@@ -6,6 +6,7 @@
 // Value head h reads query / key head h / (heads / qk_heads). Sequence b is the rows [cu[b], cu[b + 1]); its state
 // starts from initial[b] or zeros. With chunks of C = 64 tokens that begin with their sequence, row r of a chunk of n:
 //   o_r = scale (a^{r+1} S q_r + sum_{j <= r} a^{r-j} (q_r . k_j) v_j),   S' = a^n S + sum_j a^{n-1-j} v_j k_j^T
+#include <algorithm>
 #include <cmath>
 
 #include "common.h"
@@ -31,6 +32,7 @@ struct LinCall {
   float *carry;    // [ranges, heads, D, D]: the state at the end of a range, where its last sequence goes on
   int32_t *meta;   // [ranges]: tokens of a range that lies in one sequence begun before it, -1 for others
   int sequences, rows, heads, group, ranges;
+  int scanned;     // the states at the ranges' ends are whole, not only what each range adds
   float scale;
 };
 
@@ -115,6 +117,7 @@ __device__ __forceinline__ int v_swizzle(int r) {
 }
 
 typedef short lin_s16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 lin_bf16x2_t __attribute__((ext_vector_type(2)));
 // Four rows of one channel per lane: 16 lanes read 4 rows of 16 channels (lane i: 4 channels of row i / 4) and get their
 // transpose (lane i: channel i of the 4 rows).
 __device__ __forceinline__ u32x2_t lin_read_transposed(const uint16_t *p) {
@@ -128,14 +131,27 @@ struct Split2 {
 };
 __device__ __forceinline__ float lo_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// What a pair of bf16 numbers leaves of the numbers that they were rounded from: x - hi by one v_dot2_f32_bf16, exactly. The
+// factors (-1, 0) and (0, -1) come in registers: as a constant of the instruction (-1, 0) reads as (0, -1).
+__device__ __forceinline__ float minus_dot(uint32_t hi, uint32_t factors, float x) {
+  asm("" : "+s"(factors));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(lin_bf16x2_t, hi), __builtin_bit_cast(lin_bf16x2_t, factors), x, false);
+}
+__device__ __forceinline__ float rest_lo(uint32_t hi, float x) { return minus_dot(hi, 0x0000bf80u, x); }
+__device__ __forceinline__ float rest_hi(uint32_t hi, float x) { return minus_dot(hi, 0xbf800000u, x); }
 __device__ __forceinline__ Split2 split2(const float *x) {
   Split2 s;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     s.hi[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
-    s.lo[j] = pack_bf2(x[2 * j] - lo_half(s.hi[j]), x[2 * j + 1] - hi_half(s.hi[j]));
+    s.lo[j] = pack_bf2(rest_lo(s.hi[j], x[2 * j]), rest_hi(s.hi[j], x[2 * j + 1]));
   }
   return s;
+}
+// Whether one of eight bf16 numbers is an infinity or a NaN: only their |x| of 0x7f80 and more reach bit 15 with 0x80 more
+__device__ __forceinline__ bool has_wild(u32x4_t x) {
+  x = (x & 0x7fff7fffu) + 0x00800080u;
+  return ((x[0] | x[1] | x[2] | x[3]) & 0x80008000u) != 0;
 }
 
 // A workgroup of D / 16 wavefronts walks a range of a head's chunks; a wavefront carries 16 rows (dv) of the state in
@@ -148,9 +164,11 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
   constexpr int C = kLinC, KC = D / 8, NW = D / 16, THREADS = 64 * NW, TILE = C * D;
   constexpr int NS = D / 32;            // k-steps over dk
   constexpr int PT = NW == 8 ? 2 : 4;   // 16 x 16 tiles of P that a wavefront makes at most
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][TILE], Vs[2][TILE];
-  __shared__ __attribute__((aligned(16))) uint16_t Qs[CARRY ? 1 : 2][CARRY ? 8 : TILE];
-  __shared__ __attribute__((aligned(16))) u32x4_t Ps[CARRY ? 1 : 2][CARRY ? 1 : 8][64];  // hi / lo, (row tile, k-step), lane
+  // Tiles on their way two chunks ahead where LDS holds three of each (156 KB), else one (two workgroups a CU)
+  constexpr int RING = D == 128 && !CARRY ? 3 : 2, LOADS = (CARRY ? 2 : 3) * C * KC / THREADS;
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[RING][TILE], Vs[RING][TILE];
+  __shared__ __attribute__((aligned(16))) uint16_t Qs[CARRY ? 1 : RING][CARRY ? 8 : TILE];
+  __shared__ __attribute__((aligned(16))) u32x4_t Ps[CARRY ? 1 : 2][CARRY ? 1 : 6][64];  // hi / lo, (row tile, k-step), lane
   __shared__ int64_t sums[NW];
   __shared__ int found[4];
 
@@ -214,26 +232,56 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
   } else {
     if (range == 0) pass_empty(0);
     if (rg.count <= 0) return;
-    load_state(rg.at.row > rg.at.s0 ? p.carry + (range - 1) * state_step + state_at : initial_of(rg.at.b));
+    if (rg.at.row == rg.at.s0) {
+      load_state(initial_of(rg.at.b));
+    } else {
+      int w = range - 1;
+      load_state(p.carry + w * state_step + state_at);
+      // where nobody has: what the ranges in front add to it, back to the one in which the sequence begins
+      float fade = 1.f;
+      for (int tokens; !p.scanned && (tokens = p.meta[w]) >= 0;) {
+        fade *= decay_pow(log2a, tokens);
+        const float *r = p.carry + --w * state_step + state_at + (int64_t)dv * D + 4 * g;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          const f32x4_t x = *reinterpret_cast<const f32x4_t *>(r + 16 * t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][i] = fmaf(fade, x[i], s[t][i]);
+        }
+      }
+    }
   }
 
   // ---- tile loads, straight to LDS: thread chunk i fills position THREADS i + tid: row P / KC, slot P % KC ----------
   constexpr int CG = C * KC / THREADS;
   static_assert(CG == 2 && THREADS / KC % 16 == 0, "the swizzle is the same for a thread's rows");
-  const int kr0 = tid / KC, slot = tid % KC;
-  const uint32_t qk_chunk = (slot ^ qk_swizzle<D>(kr0)) * 8, v_chunk = (slot ^ v_swizzle<D>(kr0)) * 8;
+  const int kr0 = tid / KC, slot16 = tid % KC;
+  const uint32_t qk_chunk = (slot16 ^ qk_swizzle<D>(kr0)) * 8, v_chunk = (slot16 ^ v_swizzle<D>(kr0)) * 8;
   const uint16_t *kp = p.k.p + hk * p.k.head, *vp = p.v.p + h * p.v.head, *qp = p.q.p + hk * p.q.head;
   const uint32_t wave_lds = __builtin_amdgcn_readfirstlane(wave * 1024);
   // rows behind the chunk's last repeat it: their weights are zero and their outputs are not stored
-  auto load_tiles = [&](int row, int n, int buf) __device__ {
+  uint32_t k_off[CG], v_off[CG], q_off[CG];
 #pragma unroll
-    for (int i = 0; i < CG; ++i) {
-      const uint32_t r = min(kr0 + i * (THREADS / KC), n - 1), to = wave_lds + i * THREADS * 16;
-      global_to_lds16_sbase(kp + (int64_t)row * p.k.row, 2u * (r * (uint32_t)p.k.row + qk_chunk), lds_address(Ks[buf]) + to);
-      global_to_lds16_sbase(vp + (int64_t)row * p.v.row, 2u * (r * (uint32_t)p.v.row + v_chunk), lds_address(Vs[buf]) + to);
-      if constexpr (!CARRY)
-        global_to_lds16_sbase(qp + (int64_t)row * p.q.row, 2u * (r * (uint32_t)p.q.row + qk_chunk), lds_address(Qs[buf]) + to);
-    }
+  for (int i = 0; i < CG; ++i) {
+    const uint32_t r = kr0 + i * (THREADS / KC);
+    k_off[i] = 2u * (r * (uint32_t)p.k.row + qk_chunk);
+    v_off[i] = 2u * (r * (uint32_t)p.v.row + v_chunk);
+    q_off[i] = 2u * (r * (uint32_t)p.q.row + qk_chunk);
+  }
+  auto load_tile = [&](const uint16_t *base, int64_t stride, const uint32_t *whole, uint32_t part, int n, const uint16_t *tile) __device__ {
+    uint32_t off[CG];
+#pragma unroll
+    for (int i = 0; i < CG; ++i)
+      off[i] = n == C ? whole[i] : 2u * ((uint32_t)min(kr0 + i * (THREADS / KC), n - 1) * (uint32_t)stride + part);
+#pragma unroll
+    for (int i = 0; i < CG; ++i) global_to_lds16_sbase(base, off[i], lds_address(tile) + wave_lds + i * THREADS * 16);
+  };
+  auto load_tiles = [&](const LinPlace &place, int slot) __device__ {
+    const int n = min(C, place.s1 - place.row);
+    const int64_t row = place.row;
+    load_tile(kp + row * p.k.row, p.k.row, k_off, qk_chunk, n, Ks[slot]);
+    load_tile(vp + row * p.v.row, p.v.row, v_off, v_chunk, n, Vs[slot]);
+    if constexpr (!CARRY) load_tile(qp + row * p.q.row, p.q.row, q_off, qk_chunk, n, Qs[slot]);
   };
 
   // ---- what stays the same over a head's chunks ----------------------------------------------------------------------
@@ -258,31 +306,72 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
 #pragma unroll
     for (int x = 0; x < PT; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pw[x][i] = decay_pow(log2a, max(16 * (prt - pu - PS * x) + l16 - 4 * g - i, 0));
+      for (int i = 0; i < 4; ++i) pw[x][i] = p.scale * decay_pow(log2a, max(16 * (prt - pu - PS * x) + l16 - 4 * g - i, 0));
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt) row_weight[rt] = decay_pow(log2a, 16 * rt + l16 + 1);
+    for (int rt = 0; rt < 4; ++rt) row_weight[rt] = p.scale * decay_pow(log2a, 16 * rt + l16 + 1);
     // tiles of P behind the diagonal that share a k-step with one on it
-    for (int i = tid; i < 2 * 8 * 64; i += THREADS) (&Ps[0][0][0])[i] = u32x4_t{};
+    for (int i = tid; i < 2 * 6 * 64; i += THREADS) (&Ps[0][0][0])[i] = u32x4_t{};
   }
   float vw[16];  // a^{n-1-j} of the lane's tokens j of a chunk of n
   int vw_n = -1;
 
-  LinPlace at = rg.at;
-  int n = min(C, at.s1 - at.row), buf = 0;
-  load_tiles(at.row, n, 0);
-  for (int64_t left = rg.count; left > 0; --left, buf ^= 1) {
-    wait_vm_lds<0>();
-    bare_barrier();
-    // the next chunk
-    LinPlace next = at;
-    next.row = at.row + C;
-    const bool ends = next.row >= at.s1;
-    if (ends && (left > 1 || !CARRY)) {
-      const int b = pass_empty(at.b + 1);
-      if (left > 1) next = LinPlace{b, lin_bound(p, b), lin_bound(p, b + 1), lin_bound(p, b)};
+  // the next chunk of the range
+  auto after = [&](const LinPlace &place) __device__ {
+    if (place.row + C < place.s1) return LinPlace{place.b, place.s0, place.s1, place.row + C};
+    const int b = pass_empty(place.b + 1);
+    return LinPlace{b, lin_bound(p, b), lin_bound(p, b + 1), lin_bound(p, b)};
+  };
+  // P^T = scale K Q^T with the decays, as two bf16 numbers
+  auto make_p = [&](const uint16_t *kt, const uint16_t *qt) __device__ {
+#pragma unroll
+    for (int x = 0; x < PT; ++x) {
+      const int u = pu + PS * x;
+      if (u > prt) break;
+      f32x4_t c = {};
+#pragma unroll
+      for (int t = 0; t < NS; ++t) c = mfma_bf16_16x16x32(qk_frag(kt + 16 * u * D, t), qk_frag(qt + 16 * prt * D, t), c);
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // behind the diagonal nothing is taken, whatever the key holds
+        w[i] = u < prt || l16 >= 4 * g + i ? c[i] * pw[x][i] : 0.f;
+      }
+      const uint32_t h0 = pack_bf2(w[0], w[1]), h1 = pack_bf2(w[2], w[3]);
+      const uint32_t e0 = pack_bf2(rest_lo(h0, w[0]), rest_hi(h0, w[1])), e1 = pack_bf2(rest_lo(h1, w[2]), rest_hi(h1, w[3]));
+      const int f = prt < 2 ? prt : 2 * prt - 2 + (u >> 1);
+      reinterpret_cast<u32x2_t *>(&Ps[0][f][lane])[u & 1] = u32x2_t{h0, h1};
+      reinterpret_cast<u32x2_t *>(&Ps[1][f][lane])[u & 1] = u32x2_t{e0, e1};
     }
-    const int next_n = min(C, next.s1 - next.row);
-    if (left > 1) load_tiles(next.row, next_n, buf ^ 1);
+  };
+
+  LinPlace at = rg.at, next = at;
+  int slot = 0, o_row = 0, o_n = 0;
+  // outputs lie in the Q tile of their chunk, which no wavefront reads any more, until they are stored in whole rows
+  auto store_outputs = [&](const uint16_t *tile) __device__ {
+#pragma unroll
+    for (int i = 0; i < CG; ++i) {
+      const int r = kr0 + i * (THREADS / KC);
+      if (r < o_n) st16(p.out + (int64_t)(o_row + r) * p.o_row + h * p.o_head + qk_chunk, ld16(tile + (r * KC + slot16) * 8));
+    }
+  };
+  load_tiles(at, 0);
+  if (rg.count > 1) {
+    next = after(at);
+    if (RING == 3) load_tiles(next, 1);
+  }
+  for (int64_t left = rg.count; left > 0; --left) {
+    const int slot_next = slot + 1 == RING ? 0 : slot + 1, slot_last = slot == 0 ? RING - 1 : slot - 1;
+    // this chunk's tiles; the next one's, the newest that were asked for, may still be on their way
+    if (RING == 3 && left > 1) wait_vm_lds<LOADS>();
+    else wait_vm_lds<0>();
+    bare_barrier();
+    const int n = min(C, at.s1 - at.row);
+    const bool ends = at.row + C >= at.s1;
+    LinPlace later = next;  // the chunk after the next
+    if (left > 2) later = after(next);
+    if (RING == 2 && left > 1) load_tiles(next, slot_next);
+    if (RING == 3 && !CARRY) store_outputs(Qs[CARRY ? 0 : slot_last]);
+    if (!CARRY && ends && left == 1) pass_empty(at.b + 1);
 
     if (n != vw_n) {
       vw_n = n;
@@ -292,7 +381,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
         vw[x] = back < 0 ? 0.f : decay_pow(log2a, back);
       }
     }
-    const uint16_t *kt = Ks[buf], *vt = Vs[buf];
+    const uint16_t *kt = Ks[slot], *vt = Vs[slot];
     u32x4_t vf[2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -301,29 +390,9 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
     }
 
     if constexpr (!CARRY) {
-      const uint16_t *qt = Qs[buf];
-      // P^T = K Q^T with the decays, as two bf16 numbers
-#pragma unroll
-      for (int x = 0; x < PT; ++x) {
-        const int u = pu + PS * x;
-        if (u > prt) break;
-        f32x4_t c = {};
-#pragma unroll
-        for (int t = 0; t < NS; ++t)
-          c = mfma_bf16_16x16x32(qk_frag(kt + 16 * u * D, t), qk_frag(qt + 16 * prt * D, t), c);
-        float w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // behind the diagonal nothing is taken, whatever the key holds
-          w[i] = u < prt || l16 >= 4 * g + i ? c[i] * pw[x][i] : 0.f;
-        }
-        const uint32_t h0 = pack_bf2(w[0], w[1]), h1 = pack_bf2(w[2], w[3]);
-        const uint32_t e0 = pack_bf2(w[0] - lo_half(h0), w[1] - hi_half(h0)), e1 = pack_bf2(w[2] - lo_half(h1), w[3] - hi_half(h1));
-        const int f = 2 * prt + (u >> 1);
-        reinterpret_cast<u32x2_t *>(&Ps[0][f][lane])[u & 1] = u32x2_t{h0, h1};
-        reinterpret_cast<u32x2_t *>(&Ps[1][f][lane])[u & 1] = u32x2_t{e0, e1};
-      }
-      // O^T = S Q^T, rows by a^{r+1}
+      uint16_t *qt = Qs[slot];
+      make_p(kt, qt);
+      // O^T = S Q^T, rows by scale a^{r+1}
       f32x4_t o[4] = {};
 #pragma unroll
       for (int t = 0; t < NS; ++t) {
@@ -344,12 +413,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
         for (int i = 0; i < 4; ++i) o[rt][i] *= row_weight[rt];
       // a value that is no finite number would reach rows in front of it as 0 * inf: it is left out of the product, and its
       // channel ends there
-      uint32_t worst = 0;
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) worst = max(worst, max(vf[ks][j] & 0x7fffu, (vf[ks][j] >> 16) & 0x7fffu));
-      const bool careful = __any(worst >= 0x7f80u);
+      const bool careful = __any(has_wild(vf[0]) || has_wild(vf[1]));
       u32x4_t vc[2] = {vf[0], vf[1]};
       int bad = C;
       if (careful) {
@@ -372,8 +436,9 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       for (int rt = 0; rt < 4; ++rt)
 #pragma unroll
         for (int ks = 0; ks <= rt / 2; ++ks) {
-          o[rt] = mfma_bf16_16x16x32(as_bf16x8(vc[ks]), as_bf16x8(Ps[0][2 * rt + ks][lane]), o[rt]);
-          o[rt] = mfma_bf16_16x16x32(as_bf16x8(vc[ks]), as_bf16x8(Ps[1][2 * rt + ks][lane]), o[rt]);
+          const int f = rt < 2 ? rt : 2 * rt - 2 + ks;
+          o[rt] = mfma_bf16_16x16x32(as_bf16x8(vc[ks]), as_bf16x8(Ps[0][f][lane]), o[rt]);
+          o[rt] = mfma_bf16_16x16x32(as_bf16x8(vc[ks]), as_bf16x8(Ps[1][f][lane]), o[rt]);
         }
       if (careful) {
 #pragma unroll
@@ -384,13 +449,23 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
             if (16 * rt + l16 >= from) o[rt][i] = __builtin_nanf("");
         }
       }
-      uint16_t *op = p.out + (int64_t)at.row * p.o_row + h * p.o_head + 16 * wave + 4 * g;
+      if constexpr (RING == 3) {
+        // chunk c of row r at slot c ^ swizzle(r), as Q's
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        const int r = 16 * rt + l16;
-        if (r < n)
-          *reinterpret_cast<u32x2_t *>(op + r * p.o_row) =
-              u32x2_t{pack_bf2(o[rt][0] * p.scale, o[rt][1] * p.scale), pack_bf2(o[rt][2] * p.scale, o[rt][3] * p.scale)};
+        for (int rt = 0; rt < 4; ++rt)
+          *reinterpret_cast<u32x2_t *>(qt + (16 * rt + l16) * D + ((2 * wave + (g >> 1)) ^ qk_swizzle<D>(l16)) * 8 + 4 * (g & 1)) =
+              u32x2_t{pack_bf2(o[rt][0], o[rt][1]), pack_bf2(o[rt][2], o[rt][3])};
+        o_row = at.row;
+        o_n = n;
+        if (left > 2) load_tiles(later, slot_last);
+      } else {
+        uint16_t *op = p.out + (int64_t)at.row * p.o_row + h * p.o_head + 16 * wave + 4 * g;
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) {
+          const int r = 16 * rt + l16;
+          if (r < n)
+            *reinterpret_cast<u32x2_t *>(op + r * p.o_row) = u32x2_t{pack_bf2(o[rt][0], o[rt][1]), pack_bf2(o[rt][2], o[rt][3])};
+        }
       }
     }
 
@@ -407,9 +482,9 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       for (int j = 0; j < 4; ++j) {
         const float x0 = lo_half(vf[ks][j]) * vw[8 * ks + 2 * j], x1 = hi_half(vf[ks][j]) * vw[8 * ks + 2 * j + 1];
         w0[j] = pack_bf2(x0, x1);
-        const float y0 = x0 - lo_half(w0[j]), y1 = x1 - hi_half(w0[j]);
+        const float y0 = rest_lo(w0[j], x0), y1 = rest_hi(w0[j], x1);
         w1[j] = pack_bf2(y0, y1);
-        w2[j] = pack_bf2(y0 - lo_half(w1[j]), y1 - hi_half(w1[j]));
+        w2[j] = pack_bf2(rest_lo(w1[j], y0), rest_hi(w1[j], y1));
       }
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
@@ -426,7 +501,13 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       if (left > 1) load_state(initial_of(next.b));
     }
     at = next;
-    n = next_n;
+    next = later;
+    slot = slot_next;
+  }
+  if constexpr (RING == 3 && !CARRY) {
+    wait_vm_lds<63>();
+    bare_barrier();
+    store_outputs(Qs[slot == 0 ? RING - 1 : slot - 1]);
   }
   if (CARRY) store_state(p.carry + range * state_step + state_at);
 }
@@ -458,7 +539,7 @@ int launch_causal_linear(const LinCall &p, hipStream_t s) {
     hipLaunchKernelGGL((causal_linear_kernel<D, true>), dim3(p.ranges * p.heads), dim3(D * 4), 0, s, p);
     int rc = check_launch("causal_linear");
     if (rc) return rc;
-    if (p.ranges > 2) {
+    if (p.scanned) {
       hipLaunchKernelGGL(carry_scan_kernel, dim3((unsigned)(((int64_t)p.heads * D * D / 4 + 255) / 256)), dim3(256), 0, s, p, D * D);
       rc = check_launch("causal_linear");
       if (rc) return rc;
@@ -467,6 +548,13 @@ int launch_causal_linear(const LinCall &p, hipStream_t s) {
   hipLaunchKernelGGL((causal_linear_kernel<D, false>), dim3(p.ranges * p.heads), dim3(D * 4), 0, s, p);
   return check_launch("causal_linear");
 }
+
+// Up to so many ranges each adds up what those in front of it left, its workgroups for themselves; more take a launch of their
+// own for it (9 ranges of 56 heads x 64: 85.4 us and 89.5, 4 of 40 x 128: 30.4 and 32.1).
+constexpr int kAddedRanges = 16;
+
+// Chunks of a call, at most: the sequences' lengths are on the device.
+int64_t most_chunks(int rows, int sequences) { return rows / kLinC + std::min(rows, sequences); }
 
 int check_lin_operand(const void *p, int64_t row, int64_t head, const char *name) {
   VDNH3_HOST_CHECK(p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && head % 8 == 0 && row >= 0 &&
@@ -481,9 +569,10 @@ int check_lin_operand(const void *p, int64_t row, int64_t head, const char *name
 
 extern "C" int vdnh3_causal_linear_ranges(int rows, int sequences, int heads, int head_dim) {
   if (rows <= 0 || sequences <= 0 || heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  const int64_t chunks = (int64_t)rows / vdnh3::kLinC + 1, slots = head_dim == 128 ? 256 : 512;
-  const int64_t ranges = slots / heads;
-  return (int)(ranges < 1 ? 1 : ranges > chunks / 4 ? (chunks / 4 > 1 ? chunks / 4 : 1) : ranges);
+  // One round of workgroups, two chunks of each or more: 512 tokens x 40 heads x 128 take 30.4 us in 4 ranges (3 33.4, 6 34.7),
+  // 3,939 of 7 sequences 84 in 6 (4 112, 12 95), 40,688 650 (4 835, 12 652, 1 2,300).
+  const int64_t slots = head_dim == 128 ? 256 : 512;  // workgroups that run at once
+  return (int)std::max<int64_t>(1, std::min(slots / heads, vdnh3::most_chunks(rows, sequences) / 2));
 }
 
 extern "C" size_t vdnh3_causal_linear_workspace_bytes(int ranges, int heads, int head_dim) {
@@ -525,7 +614,7 @@ extern "C" int vdnh3_causal_linear_packed(const uint16_t *q, int64_t q_row, int6
   const LinCall p{{q, q_row, q_head}, {k, k_row, k_head}, {v, v_row, v_head}, out, o_row, o_head, log_decay, cu_seqlens,
                   initial_state, final_state, carry,
                   reinterpret_cast<int32_t *>(carry + (ranges > 1 ? (int64_t)ranges * heads * head_dim * head_dim : 0)),
-                  sequences, rows, heads, heads / qk_heads, ranges, scale};
+                  sequences, rows, heads, heads / qk_heads, ranges, ranges > kAddedRanges, scale};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return head_dim == 128 ? launch_causal_linear<128>(p, s) : launch_causal_linear<64>(p, s);
 }
