@@ -177,7 +177,8 @@ def test_c_entry_points_refuse_before_any_launch(built_lib):
     for bad in [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(decay=None), dict(pool=None), dict(layout=False),
                 dict(slots=0), dict(batch=0), dict(new=0), dict(heads=0), dict(qk_heads=0), dict(dim=0), dict(dim=129), dict(heads=5),
                 dict(batch=1 << 31), dict(new=1 << 40), dict(slot=4096), dict(state_head=4095), dict(slot=0), dict(state_head=0),
-                dict(slot=4 * 4096 - 1), dict(batch=1 << 30, heads=1 << 10), dict(heads=1 << 30, qk_heads=1, state_head=4096, slot=1 << 60)]:
+                dict(slot=4 * 4096 - 1), dict(batch=1 << 30, heads=1 << 10),
+                dict(heads=1 << 30, qk_heads=1, state_head=4096, slot=1 << 60)]:
         for delta in (False, True):
             sizes = dict(bad)
             if sizes.get("slots") == 0:
