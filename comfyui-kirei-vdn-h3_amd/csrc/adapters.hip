@@ -171,8 +171,8 @@ constexpr int kTurnRow = 68, kTurn = 16 * kTurnRow;
 // out = y + B h of the rows of one adapter in a block, a wavefront's 64 of each STEP columns of the workgroup's span.
 // C[column][row] tiles whose columns are ordered so that a pair of tiles gives a lane eight neighbours: row m of tile t is
 // column 32 (t / 2) + 8 (m / 4) + 4 (t % 2) + m % 4. They turn in LDS so that y and out are read and written in runs of 128
-// bytes of a row, eight rows at a time: 833 MB take 150 us that way, and 197 as 64 bytes of 16 rows, as the tiles lie. KS: the ranks in 32s, kept as operands over the columns; 0: 16 ranks;
-// -1: any number of 32s, read again for each 64 columns.
+// bytes of a row, eight rows at a time: 833 MB take 150 us that way, and 197 as 64 bytes of 16 rows, as the tiles lie.
+// KS: the ranks in 32s, kept as operands over the columns; 0: 16 ranks; -1: any number of 32s, read again for each 64 columns.
 // STEP: the columns of the workgroup's wavefronts.
 template <int MT, int KS, int STEP, bool LISTED>
 __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, const int *list, int count, int adapter, int col0,
@@ -391,9 +391,9 @@ AdapterCut adapter_cut(int rows, int out_width, int adapters, int rank) {
 }
 
 int check_adapter_rows(const void *p, int64_t row, int width, const char *name, bool read) {
-  VDNH3_HOST_CHECK(p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && (row >= width || (read && row == 0)),
-                   VDNH3_ERR_INVALID, "adapter_add: %s must be 16-byte aligned with a row stride of a multiple of 8 that covers "
-                   "the width", name);
+  VDNH3_HOST_CHECK(p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && row >= (read ? 0 : width),
+                   VDNH3_ERR_INVALID, "adapter_add: %s must be 16-byte aligned with a row stride of a multiple of 8, rows of out "
+                   "apart", name);
   return VDNH3_OK;
 }
 

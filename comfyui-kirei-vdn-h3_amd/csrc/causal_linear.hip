@@ -592,6 +592,10 @@ extern "C" int vdnh3_causal_linear_packed(const uint16_t *q, int64_t q_row, int6
   VDNH3_HOST_CHECK(rows > 0 && sequences > 0 && heads > 0 && qk_heads > 0 && heads % qk_heads == 0, VDNH3_ERR_INVALID,
                    "causal_linear: rows, sequences and heads must be positive and heads a multiple of qk_heads, got %d rows, "
                    "%d sequences, %d / %d heads", rows, sequences, heads, qk_heads);
+  // one row, or one head, has no stride, whatever a caller passes for it
+  if (rows == 1) q_row = k_row = v_row = o_row = 0;
+  if (qk_heads == 1) q_head = k_head = 0;
+  if (heads == 1) v_head = o_head = 0;
   int rc = check_lin_operand(q, q_row, q_head, "q");
   if (!rc) rc = check_lin_operand(k, k_row, k_head, "k");
   if (!rc) rc = check_lin_operand(v, v_row, v_head, "v");

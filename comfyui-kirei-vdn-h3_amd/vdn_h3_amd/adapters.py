@@ -60,7 +60,7 @@ class LowRankAdapters:
     """The adapters of one projection ``[out, width]``: ``down`` ``[n, rank, width]`` (A) and ``up`` ``[n, out, rank]`` (B), bf16 on
     the GPU, and ``scales``, ``n`` numbers (a tensor or a sequence; ``None``: ones), kept in fp32.
 
-    Widths are multiples of 8, ranks at most 1024. The object keeps both in the kernels' order, copied once (a later change of the
+    Widths are multiples of 8, ranks at most 1024. The object keeps copies, A and B in the kernels' order (a later change of the
     tensors is not seen), and has to outlive graphs that were captured with it. ``from_pairs`` takes adapters of different
     ranks.
     """
@@ -79,12 +79,12 @@ class LowRankAdapters:
             raise ValueError(f"ranks up to 1024 are supported, got {self.rank}")
         _lib.forward_only("LowRankAdapters", down, up, scales)
         if scales is not None:
-            scales = torch.as_tensor(scales, dtype=torch.float32, device=down.device).reshape(-1).contiguous()
+            scales = torch.as_tensor(scales, dtype=torch.float32, device=down.device).detach().reshape(-1).clone()
             if scales.numel() != self.count:
                 raise ValueError(f"scales must be {self.count} numbers, got {scales.numel()}")
         self.device = _lib.require_device(down, up, scales)
         self.down, self.up = _layouts(down.detach(), up.detach())
-        self.scales = None if scales is None else scales.detach()
+        self.scales = scales
 
     @classmethod
     def from_pairs(cls, pairs, scales=None) -> "LowRankAdapters":

@@ -158,3 +158,25 @@ def test_replays_take_another_index(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, handle.add(y, x, index))
+
+
+def test_layouts_of_rows_and_kept_scales(device):
+    """Rows that overlap or lie far apart (past 32 bits), one row with any stride; the object keeps the scales that it was given."""
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    (x, y, down, up, scales), g = _case(70, 256, 128, 3, 40, device)
+    index = torch.randint(-1, 3, (70,), generator=g, dtype=torch.int32).to(device)
+    handle = LowRankAdapters(down, up, scales)
+    want = handle.add(y, x, index)
+    scales.zero_()
+    assert torch.equal(handle.add(y, x, index), want)
+    sliding = x.flatten().as_strided((70, 256), (8, 1))
+    assert torch.equal(handle.add(y, sliding, index), handle.add(y, sliding.contiguous(), index))
+    room = torch.empty(70 * 2 ** 25 + 256, dtype=BF, device=device)
+    far_x, far_y = room.as_strided((70, 256), (2 ** 25, 1)), room.as_strided((70, 128), (2 ** 25, 1), 512)
+    far_x.copy_(x)
+    far_y.copy_(y)
+    assert torch.equal(handle.add(far_y, far_x, index), want) and handle.add(far_y, far_x, index, out=far_y) is far_y
+    assert torch.equal(far_y, want) and torch.equal(far_x, x)
+    one = x.flatten()[:300].as_strided((1, 256), (3, 1))
+    assert torch.equal(handle.add(y[:1].as_strided((1, 128), (1, 1)), one, index[:1]), handle.add(y[:1], one.clone(), index[:1]))

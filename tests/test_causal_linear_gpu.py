@@ -217,3 +217,32 @@ def test_replays_take_other_lengths(device):
         torch.cuda.synchronize()
         want, end = causal_linear_packed(q, k, v, decay, cu, 0.2, initial_state=initial, output_final_state=True)
         assert torch.equal(out[:bounds[-1]], want[:bounds[-1]]) and torch.equal(final, end)
+
+
+def test_strides_of_single_rows_and_heads_and_past_32_bits(device):
+    """A single row or head has no stride, whatever its tensor says; offsets and states past 2^31 elements."""
+    from vdn_h3_amd.causal_linear import causal_linear_packed
+
+    for heads in (1, 3):
+        q, k, v, decay, initial = _case(1, heads, 1, 64, 3, device, 1)
+        want = causal_linear_packed(q, k, v, decay, [0, 1], 0.1, initial_state=initial, output_final_state=True)
+        odd = [t.flatten().as_strided(t.shape, (5, 64 if t.shape[1] > 1 else 3, 1)) for t in (q, k, v)]
+        out = torch.zeros(heads * 64, dtype=BF, device=device).as_strided((1, heads, 64), (7, 64 if heads > 1 else 1, 1))
+        got = causal_linear_packed(*odd, decay, [0, 1], 0.1, initial_state=initial, output_final_state=True, out=out)
+        assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+    q, k, v, decay, _ = _case(300, 2, 2, 64, 4, device)
+    want = causal_linear_packed(q, k, v, decay, [0, 130, 300], 0.1, output_final_state=True)
+    room = torch.empty(300 * 2 ** 23, dtype=BF, device=device)
+    far = [room.as_strided((300, 2, 64), (2 ** 23, 64 * (i + 1), 1), 1024 * i) for i in range(4)]
+    for t, x in zip(far, (q, k, v)):
+        t.copy_(x)
+    got = causal_linear_packed(*far[:3], decay, [0, 130, 300], 0.1, output_final_state=True, out=far[3])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # 70,000 sequences of a token each over 2 heads x 128: 2.3e9 numbers of states
+    q, k, v, decay, _ = _case(1, 2, 2, 128, 5, device)
+    cu = torch.zeros(70001, dtype=torch.int32, device=device)
+    cu[-1] = 1
+    del room, far, got
+    final = causal_linear_packed(q, k, v, decay, cu, 0.1, output_final_state=True)[1]
+    one = causal_linear_packed(q, k, v, decay, [0, 1], 0.1, output_final_state=True)[1]
+    assert torch.equal(final[-1], one[0]) and not final[69998].any() and not final[:5].any()

@@ -202,7 +202,7 @@ def test_c_entry_points_refuse_before_any_launch(built_lib):
 
     need = lib.vdnh3_adapter_workspace_bytes(200, 40)
     assert need == 200 * 64 * 4 and lib.vdnh3_adapter_workspace_bytes(64, 64) == 0 and lib.vdnh3_adapter_workspace_bytes(0, 8) == 0
-    for bad in [dict(y=None), dict(y=p + 8), dict(y_row=60), dict(y_row=8), dict(x=p + 2), dict(x_row=64), dict(down=None),
+    for bad in [dict(y=None), dict(y=p + 8), dict(y_row=60), dict(y_row=-64), dict(x=p + 2), dict(x_row=-8), dict(down=None),
                 dict(down=p + 8), dict(up=p + 8), dict(index=None), dict(out=None), dict(out=p + 16, out_row=0), dict(out_row=128),
                 dict(rows=0), dict(width=0), dict(width=124), dict(out_width=60), dict(n=0), dict(rank=0), dict(rank=1025),
                 dict(work=None), dict(work=p + 8), dict(rank=40, size=need - 1)]:

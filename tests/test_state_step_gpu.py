@@ -186,3 +186,19 @@ def test_replays_take_other_slots_and_states(device, delta):
         torch.cuda.synchronize()
         want = _step(delta, q, k, v, gates, mirror, slots=slots)
         assert torch.equal(torch.nan_to_num(out, 9.0), torch.nan_to_num(want, 9.0)) and torch.equal(pool, mirror)
+
+
+@pytest.mark.parametrize("delta", [False, True])
+def test_pools_past_32_bits(device, delta):
+    """States at 2^31 elements and more, between slots and between heads."""
+    count = 66000
+    q, k, v, gates, _, _ = _case(2, 1, 2, 2, 2, 128, device, delta)
+    whole = torch.empty(2, count, 128, 128, device=device)
+    for pool in (whole.view(count, 2, 128, 128), whole.transpose(0, 1)):
+        small = torch.randn(2, 2, 128, 128, device=device)
+        pool[0], pool[count - 1] = small[0], small[1]
+        pool[count - 2] = 5.0
+        slots = torch.tensor([0, count - 1], dtype=torch.int64, device=device)
+        got = _step(delta, q, k, v, gates, pool, slots=slots)
+        assert torch.equal(got, _step(delta, q, k, v, gates, small))
+        assert torch.equal(pool[0], small[0]) and torch.equal(pool[count - 1], small[1]) and (pool[count - 2] == 5.0).all()
