@@ -102,18 +102,14 @@ __device__ __forceinline__ LinRange lin_range(const LinCall &p, int range, int64
                                     __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3])}};
 }
 
-// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Q and K: the same chunk of the 16 rows of a fragment read
-// lies in 16 different 16-byte bank groups, and 32 bytes of the 8 rows that half a wavefront reads transposed in 8 different
-// 32-byte ones. V: only the latter.
+// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Four neighbouring chunks of four neighbouring rows (transposed
+// reads) lie in 16 different 16-byte bank groups; so do the chunks 4 t + g of the rows that one turn of a 16-byte fragment read
+// takes, rows 0 to 3 and 12 to 15 of one g with rows 4 to 11 of the next (8 cycles a wavefront with r / 4 for 0, 2, 3, 1: 6).
 template <int D>
-__device__ __forceinline__ int qk_swizzle(int r) {
-  if constexpr (D == 128) return ((r & 7) << 1) | ((r >> 3) & 1);
-  else return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
-}
-template <int D>
-__device__ __forceinline__ int v_swizzle(int r) {
-  if constexpr (D == 128) return 2 * (r & 7);
-  else return 2 * ((r >> 1) & 3);
+__device__ __forceinline__ int swizzle(int r) {
+  const int four = ((r ^ (r >> 1)) & 4) >> 1 | ((r >> 3) & 1);  // 0, 2, 3, 1 for r / 4 = 0, 1, 2, 3
+  if constexpr (D == 128) return ((r & 3) << 2) | four;
+  else return (((r >> 1) & 1) << 2) | four;
 }
 
 typedef short lin_s16x4_t __attribute__((ext_vector_type(4)));
@@ -139,13 +135,22 @@ __device__ __forceinline__ float minus_dot(uint32_t hi, uint32_t factors, float 
 }
 __device__ __forceinline__ float rest_lo(uint32_t hi, float x) { return minus_dot(hi, 0x0000bf80u, x); }
 __device__ __forceinline__ float rest_hi(uint32_t hi, float x) { return minus_dot(hi, 0xbf800000u, x); }
+// The same of eight numbers that stay where they are: the compiler has a form of the instruction only that overwrites x, and
+// copies x for it. A dot product's result may be read by other instructions after three more: s_nop 2.
 __device__ __forceinline__ Split2 split2(const float *x) {
   Split2 s;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    s.hi[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
-    s.lo[j] = pack_bf2(rest_lo(s.hi[j], x[2 * j]), rest_hi(s.hi[j], x[2 * j + 1]));
-  }
+  for (int j = 0; j < 4; ++j) s.hi[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
+  float r[8];
+  asm("v_dot2_f32_bf16 %0, %8, %20, %12\n\tv_dot2_f32_bf16 %1, %8, %21, %13\n\t"
+      "v_dot2_f32_bf16 %2, %9, %20, %14\n\tv_dot2_f32_bf16 %3, %9, %21, %15\n\t"
+      "v_dot2_f32_bf16 %4, %10, %20, %16\n\tv_dot2_f32_bf16 %5, %10, %21, %17\n\t"
+      "v_dot2_f32_bf16 %6, %11, %20, %18\n\tv_dot2_f32_bf16 %7, %11, %21, %19\n\ts_nop 2"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+      : "v"(s.hi[0]), "v"(s.hi[1]), "v"(s.hi[2]), "v"(s.hi[3]), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]),
+        "v"(x[6]), "v"(x[7]), "s"(0x0000bf80u), "s"(0xbf800000u));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s.lo[j] = pack_bf2(r[2 * j], r[2 * j + 1]);
   return s;
 }
 // Whether one of eight bf16 numbers is an infinity or a NaN: only their |x| of 0x7f80 and more reach bit 15 with 0x80 more
@@ -155,9 +160,8 @@ __device__ __forceinline__ bool has_wild(u32x4_t x) {
 }
 
 // A workgroup of D / 16 wavefronts walks a range of a head's chunks; a wavefront carries 16 rows (dv) of the state in
-// accumulators, as C[dk][dv] tiles: a lane has dk = 16 t + 4 g + i of its dv, and two tiles are the operand of S q as they lie,
-// with k = 8 g + j standing for dk = 32 s + 16 (j / 4) + 4 g + j % 4; Q and K are read in that order too. Outputs are computed
-// transposed, O^T[dv][row].
+// accumulators, as C[dk][dv] tiles: row 4 g + i of tile t is dk = 32 (t / 2) + 8 g + 4 (t % 2) + i, so that two tiles are the
+// operand of S q as they lie, a lane with eight neighbouring dk of its dv. Outputs are computed transposed, O^T[dv][row].
 // CARRY: only the state at the range's end, where the last sequence goes on behind it.
 template <int D, bool CARRY>
 __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
@@ -186,14 +190,17 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       for (int t = 0; t < D / 16; ++t) s[t] = f32x4_t{};
       return;
     }
-    const float *r = from + (int64_t)dv * D + 4 * g;
+    const float *r = from + (int64_t)dv * D + 8 * g;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) s[t] = *reinterpret_cast<const f32x4_t *>(r + 16 * t);
+    for (int t = 0; t < D / 16; ++t) s[t] = *reinterpret_cast<const f32x4_t *>(r + 16 * t - 12 * (t % 2));
+    // here, once a sequence: left to the loop, the wait for them is one for every load and store of each chunk
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) asm volatile("" : "+v"(s[t]));
   };
   auto store_state = [&](float *to) __device__ {
-    float *r = to + (int64_t)dv * D + 4 * g;
+    float *r = to + (int64_t)dv * D + 8 * g;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t *>(r + 16 * t) = s[t];
+    for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4_t *>(r + 16 * t - 12 * (t % 2)) = s[t];
   };
   const int64_t state_at = (int64_t)h * D * D, state_step = (int64_t)p.heads * D * D;
   auto initial_of = [&](int b) __device__ { return p.initial ? p.initial + b * state_step + state_at : nullptr; };
@@ -239,12 +246,12 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       load_state(p.carry + w * state_step + state_at);
       // where nobody has: what the ranges in front add to it, back to the one in which the sequence begins
       float fade = 1.f;
-      for (int tokens; !p.scanned && (tokens = p.meta[w]) >= 0;) {
+      for (int tokens; w > 0 && !p.scanned && (tokens = p.meta[w]) >= 0;) {
         fade *= decay_pow(log2a, tokens);
-        const float *r = p.carry + --w * state_step + state_at + (int64_t)dv * D + 4 * g;
+        const float *r = p.carry + --w * state_step + state_at + (int64_t)dv * D + 8 * g;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
-          const f32x4_t x = *reinterpret_cast<const f32x4_t *>(r + 16 * t);
+          const f32x4_t x = *reinterpret_cast<const f32x4_t *>(r + 16 * t - 12 * (t % 2));
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][i] = fmaf(fade, x[i], s[t][i]);
         }
@@ -256,7 +263,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
   constexpr int CG = C * KC / THREADS;
   static_assert(CG == 2 && THREADS / KC % 16 == 0, "the swizzle is the same for a thread's rows");
   const int kr0 = tid / KC, slot16 = tid % KC;
-  const uint32_t qk_chunk = (slot16 ^ qk_swizzle<D>(kr0)) * 8, v_chunk = (slot16 ^ v_swizzle<D>(kr0)) * 8;
+  const uint32_t chunk = (slot16 ^ swizzle<D>(kr0)) * 8;
   const uint16_t *kp = p.k.p + hk * p.k.head, *vp = p.v.p + h * p.v.head, *qp = p.q.p + hk * p.q.head;
   const uint32_t wave_lds = __builtin_amdgcn_readfirstlane(wave * 1024);
   // rows behind the chunk's last repeat it: their weights are zero and their outputs are not stored
@@ -264,40 +271,38 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
 #pragma unroll
   for (int i = 0; i < CG; ++i) {
     const uint32_t r = kr0 + i * (THREADS / KC);
-    k_off[i] = 2u * (r * (uint32_t)p.k.row + qk_chunk);
-    v_off[i] = 2u * (r * (uint32_t)p.v.row + v_chunk);
-    q_off[i] = 2u * (r * (uint32_t)p.q.row + qk_chunk);
+    k_off[i] = 2u * (r * (uint32_t)p.k.row + chunk);
+    v_off[i] = 2u * (r * (uint32_t)p.v.row + chunk);
+    q_off[i] = 2u * (r * (uint32_t)p.q.row + chunk);
   }
-  auto load_tile = [&](const uint16_t *base, int64_t stride, const uint32_t *whole, uint32_t part, int n, const uint16_t *tile) __device__ {
+  auto load_tile = [&](const uint16_t *base, int64_t stride, const uint32_t *whole, int n, const uint16_t *tile) __device__ {
     uint32_t off[CG];
 #pragma unroll
     for (int i = 0; i < CG; ++i)
-      off[i] = n == C ? whole[i] : 2u * ((uint32_t)min(kr0 + i * (THREADS / KC), n - 1) * (uint32_t)stride + part);
+      off[i] = n == C ? whole[i] : 2u * ((uint32_t)min(kr0 + i * (THREADS / KC), n - 1) * (uint32_t)stride + chunk);
 #pragma unroll
     for (int i = 0; i < CG; ++i) global_to_lds16_sbase(base, off[i], lds_address(tile) + wave_lds + i * THREADS * 16);
   };
   auto load_tiles = [&](const LinPlace &place, int slot) __device__ {
     const int n = min(C, place.s1 - place.row);
     const int64_t row = place.row;
-    load_tile(kp + row * p.k.row, p.k.row, k_off, qk_chunk, n, Ks[slot]);
-    load_tile(vp + row * p.v.row, p.v.row, v_off, v_chunk, n, Vs[slot]);
-    if constexpr (!CARRY) load_tile(qp + row * p.q.row, p.q.row, q_off, qk_chunk, n, Qs[slot]);
+    load_tile(kp + row * p.k.row, p.k.row, k_off, n, Ks[slot]);
+    load_tile(vp + row * p.v.row, p.v.row, v_off, n, Vs[slot]);
+    if constexpr (!CARRY) load_tile(qp + row * p.q.row, p.q.row, q_off, n, Qs[slot]);
   };
 
   // ---- what stays the same over a head's chunks ----------------------------------------------------------------------
-  // fragment of row l16 of a 16-row tile of Q or K by 16 dk: 8 bytes; transposed reads of K by dk tiles, and of V
-  int qk_at[D / 16], kt_at[D / 16];
+  // fragments of row l16 of a 16-row tile of Q or K by 32 dk; transposed reads of K by a pair of dk tiles, and of V
+  int qk_at[NS], kt_at[NS];
   const int tr = 4 * g + (l16 >> 2);
+  auto tile_at = [&](int r, int c) __device__ { return r * D + (c ^ swizzle<D>(r)) * 8; };
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) {
-    qk_at[t] = l16 * D + ((2 * t + (g >> 1)) ^ qk_swizzle<D>(l16)) * 8 + 4 * (g & 1);
-    kt_at[t] = tr * D + ((2 * t + ((l16 >> 1) & 1)) ^ qk_swizzle<D>(tr)) * 8 + 4 * (l16 & 1);
+  for (int t = 0; t < NS; ++t) {
+    qk_at[t] = tile_at(l16, 4 * t + g);
+    kt_at[t] = tile_at(tr, 4 * t + (l16 & 3));
   }
-  auto qk_frag = [&](const uint16_t *tile, int t) __device__ {
-    const u32x2_t a = *reinterpret_cast<const u32x2_t *>(tile + qk_at[2 * t]), b = *reinterpret_cast<const u32x2_t *>(tile + qk_at[2 * t + 1]);
-    return as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
-  };
-  const int vt_at = tr * D + ((2 * wave + ((l16 >> 1) & 1)) ^ v_swizzle<D>(tr)) * 8 + 4 * (l16 & 1);
+  auto qk_frag = [&](const uint16_t *tile, int t) __device__ { return as_bf16x8(ld16(tile + qk_at[t])); };
+  const int vt_at = tile_at(tr, 2 * wave + ((l16 >> 1) & 1)) + 4 * (l16 & 1);
   // the wavefront's tiles of P^T: row tile prt, token tiles pu, pu + PS, ... up to the diagonal
   constexpr int PS = NW / 4;
   const int prt = wave / PS, pu = wave % PS;
@@ -344,6 +349,8 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
     }
   };
 
+  // the wavefronts of a SIMD (w and w + 4) at different steps, one at the matrix core and one at the vector unit
+  if (!CARRY && NW == 8 && wave >= 4) __builtin_amdgcn_s_setprio(1);
   LinPlace at = rg.at, next = at;
   int slot = 0, o_row = 0, o_n = 0;
   // outputs lie in the Q tile of their chunk, which no wavefront reads any more, until they are stored in whole rows
@@ -351,7 +358,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
 #pragma unroll
     for (int i = 0; i < CG; ++i) {
       const int r = kr0 + i * (THREADS / KC);
-      if (r < o_n) st16(p.out + (int64_t)(o_row + r) * p.o_row + h * p.o_head + qk_chunk, ld16(tile + (r * KC + slot16) * 8));
+      if (r < o_n) st16(p.out + (int64_t)(o_row + r) * p.o_row + h * p.o_head + chunk, ld16(tile + (r * KC + slot16) * 8));
     }
   };
   load_tiles(at, 0);
@@ -453,7 +460,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
         // chunk c of row r at slot c ^ swizzle(r), as Q's
 #pragma unroll
         for (int rt = 0; rt < 4; ++rt)
-          *reinterpret_cast<u32x2_t *>(qt + (16 * rt + l16) * D + ((2 * wave + (g >> 1)) ^ qk_swizzle<D>(l16)) * 8 + 4 * (g & 1)) =
+          *reinterpret_cast<u32x2_t *>(qt + 16 * rt * D + tile_at(l16, 2 * wave + (g >> 1)) + 4 * (g & 1)) =
               u32x2_t{pack_bf2(o[rt][0], o[rt][1]), pack_bf2(o[rt][2], o[rt][3])};
         o_row = at.row;
         o_n = n;
@@ -477,24 +484,29 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
       for (int i = 0; i < 4; ++i) s[t][i] *= all;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      u32x4_t w0, w1, w2;
+      u32x4_t w[3];
+      bf16x8_t kf[D / 16];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float x0 = lo_half(vf[ks][j]) * vw[8 * ks + 2 * j], x1 = hi_half(vf[ks][j]) * vw[8 * ks + 2 * j + 1];
-        w0[j] = pack_bf2(x0, x1);
-        const float y0 = rest_lo(w0[j], x0), y1 = rest_hi(w0[j], x1);
-        w1[j] = pack_bf2(y0, y1);
-        w2[j] = pack_bf2(rest_lo(w1[j], y0), rest_hi(w1[j], y1));
+        w[0][j] = pack_bf2(x0, x1);
+        const float y0 = rest_lo(w[0][j], x0), y1 = rest_hi(w[0][j], x1);
+        w[1][j] = pack_bf2(y0, y1);
+        w[2][j] = pack_bf2(rest_lo(w[1][j], y0), rest_hi(w[1][j], y1));
       }
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        const uint16_t *kr = kt + 32 * ks * D + kt_at[t];
+        const uint16_t *kr = kt + 32 * ks * D + kt_at[t / 2] + 4 * (t % 2);
         const u32x2_t a = lin_read_transposed(kr), b = lin_read_transposed(kr + 16 * D);
-        const bf16x8_t kf = as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
-        s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w2), s[t]);
-        s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w1), s[t]);
-        s[t] = mfma_bf16_16x16x32(kf, as_bf16x8(w0), s[t]);
+        kf[t] = as_bf16x8(u32x4_t{a[0], a[1], b[0], b[1]});
       }
+      // four tiles in turn: a product waits for the last one into the same tile
+#pragma unroll
+      for (int t = 0; t < D / 16; t += 4)
+#pragma unroll
+        for (int e = 2; e >= 0; --e)
+#pragma unroll
+          for (int u = t; u < t + 4; ++u) s[u] = mfma_bf16_16x16x32(kf[u], as_bf16x8(w[e]), s[u]);
     }
     if (!CARRY && ends) {
       if (p.final_state) store_state(p.final_state + at.b * state_step + state_at);
