@@ -184,7 +184,8 @@ __device__ __forceinline__ void expand_rows(const AdapterCall &p, int row0, cons
   for (int i = 0; i < 2 * MT; ++i) row[i] = row0 + list[8 * i + r8];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    hp[m] = h + (LISTED ? 16 * m + l16 : (int64_t)row0 + list[16 * m + l16]) * p.ranks * 2 + (KS ? 16 * g : 16 * (g / 2) + 4 * (g % 2));
+    hp[m] = h + (LISTED ? 16 * m + l16 : (int64_t)row0 + list[16 * m + l16]) * p.ranks * 2 +
+            (KS ? 16 * g : 16 * (g / 2) + 4 * (g % 2));
   }
   constexpr int KEPT = KS > 0 ? KS : 1;
   u32x4_t hi[KEPT][MT], lo[KEPT][MT];  // 16 ranks: the first halves
@@ -303,7 +304,8 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, i
   int *list = lists[wave];
   const int mine = adapter_of(p, row0, kExpandRows);
   uint64_t left = __ballot(mine >= 0);
-  if (p.copy) copy_rows<256>(p, row0, __ballot(mine < 0 && lane < kExpandRows && row0 + lane < p.rows), list, share, shares, col0, col_end);
+  if (p.copy)
+    copy_rows<256>(p, row0, __ballot(mine < 0 && lane < kExpandRows && row0 + lane < p.rows), list, share, shares, col0, col_end);
   for (int n = 0; left; ++n) {
     const int adapter = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
     const uint64_t rows = __ballot(mine == adapter);
@@ -439,14 +441,18 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (needed == 0) {
     p.shares = std::min({rows, adapters, 16});
-    const int wide = (out_width + 511) / 512, span = 512 * ((wide * p.shares + 255) / 256), few_spans = (out_width + span - 1) / span;
-    auto few = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(few_spans * p.shares), dim3(64 * kShrinkWaves), 0, s, p, few_spans, span); };
+    const int wide = (out_width + 511) / 512, span = 512 * ((wide * p.shares + 255) / 256), spans = (out_width + span - 1) / span;
+    auto few = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(spans * p.shares), dim3(64 * kShrinkWaves), 0, s, p, spans, span);
+    };
     if (c.ranks == 16) few(adapter_few_rows_kernel<1, 0>);
     else if (c.ranks == 32) few(adapter_few_rows_kernel<2, 1>);
     else few(adapter_few_rows_kernel<4, 2>);
     return check_launch("adapter_add");
   }
-  auto shrink = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.shrink), dim3(64 * kShrinkWaves), 0, s, p, c.groups); };
+  auto shrink = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)c.shrink), dim3(64 * kShrinkWaves), 0, s, p, c.groups);
+  };
   auto by_ranks = [&](auto rows16) {
     constexpr int MT = decltype(rows16)::value;
     if (c.rank_tiles == 1) shrink(adapter_shrink_kernel<MT, 1>);
@@ -460,7 +466,9 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   rc = check_launch("adapter_add");
   if (rc) return rc;
   const int spans = (out_width + c.span - 1) / c.span;
-  auto expand = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)c.expand), dim3(256), 0, s, p, spans, c.span, c.expand_shares); };
+  auto expand = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)c.expand), dim3(256), 0, s, p, spans, c.span, c.expand_shares);
+  };
   if (c.ranks == 16) expand(adapter_expand_kernel<0>);
   else if (c.ranks == 32) expand(adapter_expand_kernel<1>);
   else if (c.ranks == 64) expand(adapter_expand_kernel<2>);

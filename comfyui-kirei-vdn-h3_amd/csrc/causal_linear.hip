@@ -6,6 +6,15 @@
 // Value head h reads query / key head h / (heads / qk_heads). Sequence b is the rows [cu[b], cu[b + 1]); its state
 // starts from initial[b] or zeros. With chunks of C = 64 tokens that begin with their sequence, row r of a chunk of n:
 //   o_r = scale (a^{r+1} S q_r + sum_{j <= r} a^{r-j} (q_r . k_j) v_j),   S' = a^n S + sum_j a^{n-1-j} v_j k_j^T
+//
+// All three are bf16 MFMA with fp32 sums. Against rounding, S and the scores meet their products as two bf16 numbers (2^-17; one
+// would add 2^-9 of them to the outputs' own 2^-9), the weighted values as three: the states keep 24 bits.
+// Chunks of a sequence follow one another, so a head's chunks are cut into ranges that run beside each other, a workgroup a CU: a
+// first pass makes the state that each range adds, and the second starts from them. It reads K and V twice.
+// 40,688 tokens x 40 heads x 128 take 610 us: the first pass 185 (its loads alone 141, its arithmetic alone 150), the second 425
+// (loads and stores alone 330, arithmetic alone 345: 3.25 us a chunk, of which a SIMD's matrix core is busy 1.4 and its vector unit
+// 1.7, each wavefront now in one, now in the other). 3,939 tokens of 7 sequences take 80 us, 512 of one 29, 77 13.7 (a launch, a
+// start of three loads one after another, two chunks).
 #include <algorithm>
 #include <cmath>
 
@@ -102,8 +111,8 @@ __device__ __forceinline__ LinRange lin_range(const LinCall &p, int range, int64
                                     __builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3])}};
 }
 
-// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Four neighbouring chunks of four neighbouring rows (transposed
-// reads) lie in 16 different 16-byte bank groups; so do the chunks 4 t + g of the rows that one turn of a 16-byte fragment read
+// LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Four neighbouring chunks of four neighbouring rows
+// (transposed reads) lie in 16 different 16-byte bank groups; so do the chunks 4 t + g of the rows that one turn of a 16-byte fragment read
 // takes, rows 0 to 3 and 12 to 15 of one g with rows 4 to 11 of the next (8 cycles a wavefront with r / 4 for 0, 2, 3, 1: 6).
 template <int D>
 __device__ __forceinline__ int swizzle(int r) {
@@ -113,7 +122,6 @@ __device__ __forceinline__ int swizzle(int r) {
 }
 
 typedef short lin_s16x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 lin_bf16x2_t __attribute__((ext_vector_type(2)));
 // Four rows of one channel per lane: 16 lanes read 4 rows of 16 channels (lane i: 4 channels of row i / 4) and get their
 // transpose (lane i: channel i of the 4 rows).
 __device__ __forceinline__ u32x2_t lin_read_transposed(const uint16_t *p) {
@@ -121,36 +129,22 @@ __device__ __forceinline__ u32x2_t lin_read_transposed(const uint16_t *p) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)));
 }
 
-// x as bf16 numbers that add up to it: hi + lo hold 16 bits of it, hi + mid + lo all 24.
+__device__ __forceinline__ float lo_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// What the halves of a pair of bf16 numbers leave of the number that they were rounded from, exactly
+__device__ __forceinline__ float rest_lo(uint32_t hi, float x) { return x - lo_half(hi); }
+__device__ __forceinline__ float rest_hi(uint32_t hi, float x) { return x - hi_half(hi); }
+// x as two bf16 numbers each that hold 16 bits of it
 struct Split2 {
   u32x4_t hi, lo;
 };
-__device__ __forceinline__ float lo_half(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float hi_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// What a pair of bf16 numbers leaves of the numbers that they were rounded from: x - hi by one v_dot2_f32_bf16, exactly. The
-// factors (-1, 0) and (0, -1) come in registers: as a constant of the instruction (-1, 0) reads as (0, -1).
-__device__ __forceinline__ float minus_dot(uint32_t hi, uint32_t factors, float x) {
-  asm("" : "+s"(factors));
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(lin_bf16x2_t, hi), __builtin_bit_cast(lin_bf16x2_t, factors), x, false);
-}
-__device__ __forceinline__ float rest_lo(uint32_t hi, float x) { return minus_dot(hi, 0x0000bf80u, x); }
-__device__ __forceinline__ float rest_hi(uint32_t hi, float x) { return minus_dot(hi, 0xbf800000u, x); }
-// The same of eight numbers that stay where they are: the compiler has a form of the instruction only that overwrites x, and
-// copies x for it. A dot product's result may be read by other instructions after three more: s_nop 2.
 __device__ __forceinline__ Split2 split2(const float *x) {
   Split2 s;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) s.hi[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
-  float r[8];
-  asm("v_dot2_f32_bf16 %0, %8, %20, %12\n\tv_dot2_f32_bf16 %1, %8, %21, %13\n\t"
-      "v_dot2_f32_bf16 %2, %9, %20, %14\n\tv_dot2_f32_bf16 %3, %9, %21, %15\n\t"
-      "v_dot2_f32_bf16 %4, %10, %20, %16\n\tv_dot2_f32_bf16 %5, %10, %21, %17\n\t"
-      "v_dot2_f32_bf16 %6, %11, %20, %18\n\tv_dot2_f32_bf16 %7, %11, %21, %19\n\ts_nop 2"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-      : "v"(s.hi[0]), "v"(s.hi[1]), "v"(s.hi[2]), "v"(s.hi[3]), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]),
-        "v"(x[6]), "v"(x[7]), "s"(0x0000bf80u), "s"(0xbf800000u));
-#pragma unroll
-  for (int j = 0; j < 4; ++j) s.lo[j] = pack_bf2(r[2 * j], r[2 * j + 1]);
+  for (int j = 0; j < 4; ++j) {
+    s.hi[j] = pack_bf2(x[2 * j], x[2 * j + 1]);
+    s.lo[j] = pack_bf2(rest_lo(s.hi[j], x[2 * j]), rest_hi(s.hi[j], x[2 * j + 1]));
+  }
   return s;
 }
 // Whether one of eight bf16 numbers is an infinity or a NaN: only their |x| of 0x7f80 and more reach bit 15 with 0x80 more
@@ -168,7 +162,8 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
   constexpr int C = kLinC, KC = D / 8, NW = D / 16, THREADS = 64 * NW, TILE = C * D;
   constexpr int NS = D / 32;            // k-steps over dk
   constexpr int PT = NW == 8 ? 2 : 4;   // 16 x 16 tiles of P that a wavefront makes at most
-  // Tiles on their way two chunks ahead where LDS holds three of each (156 KB), else one (two workgroups a CU)
+  // Tiles on their way two chunks ahead where LDS holds three of each (156 KB; one ahead 625 us for 610), else one (two
+  // workgroups a CU). The first pass gains nothing by a third.
   constexpr int RING = D == 128 && !CARRY ? 3 : 2, LOADS = (CARRY ? 2 : 3) * C * KC / THREADS;
   __shared__ __attribute__((aligned(16))) uint16_t Ks[RING][TILE], Vs[RING][TILE];
   __shared__ __attribute__((aligned(16))) uint16_t Qs[CARRY ? 1 : RING][CARRY ? 8 : TILE];
@@ -349,7 +344,7 @@ __global__ __launch_bounds__(D * 4, 1) void causal_linear_kernel(LinCall p) {
     }
   };
 
-  // the wavefronts of a SIMD (w and w + 4) at different steps, one at the matrix core and one at the vector unit
+  // the wavefronts of a SIMD (w and w + 4) at different steps, one at the matrix core and one at the vector unit (606 us, 610)
   if (!CARRY && NW == 8 && wave >= 4) __builtin_amdgcn_s_setprio(1);
   LinPlace at = rg.at, next = at;
   int slot = 0, o_row = 0, o_n = 0;
@@ -552,7 +547,8 @@ int launch_causal_linear(const LinCall &p, hipStream_t s) {
     int rc = check_launch("causal_linear");
     if (rc) return rc;
     if (p.scanned) {
-      hipLaunchKernelGGL(carry_scan_kernel, dim3((unsigned)(((int64_t)p.heads * D * D / 4 + 255) / 256)), dim3(256), 0, s, p, D * D);
+      const int64_t groups = ((int64_t)p.heads * D * D / 4 + 255) / 256;
+      hipLaunchKernelGGL(carry_scan_kernel, dim3((unsigned)groups), dim3(256), 0, s, p, D * D);
       rc = check_launch("causal_linear");
       if (rc) return rc;
     }
@@ -562,7 +558,8 @@ int launch_causal_linear(const LinCall &p, hipStream_t s) {
 }
 
 // Up to so many ranges each adds up what those in front of it left, its workgroups for themselves; more take a launch of their
-// own for it (9 ranges of 56 heads x 64: 85.4 us and 89.5, 4 of 40 x 128: 30.4 and 32.1).
+// own for it (9 ranges of 56 heads x 64: 83 us and 86, 4 of 40 x 128 28.8 and 30.1, 6 of 7 sequences 80 and 84; 32 of 8 heads 87
+// and 57).
 constexpr int kAddedRanges = 16;
 
 // Chunks of a call, at most: the sequences' lengths are on the device.
@@ -581,8 +578,8 @@ int check_lin_operand(const void *p, int64_t row, int64_t head, const char *name
 
 extern "C" int vdnh3_causal_linear_ranges(int rows, int sequences, int heads, int head_dim) {
   if (rows <= 0 || sequences <= 0 || heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  // One round of workgroups, two chunks of each or more: 512 tokens x 40 heads x 128 take 30.4 us in 4 ranges (3 33.4, 6 34.7),
-  // 3,939 of 7 sequences 84 in 6 (4 112, 12 95), 40,688 650 (4 835, 12 652, 1 2,300).
+  // One round of workgroups, two chunks of each or more: 512 tokens x 40 heads x 128 take 29 us in 4 ranges (1 33, 3 31, 6 33),
+  // 3,939 of 7 sequences 80 in 6 (5 90, 12 91, 1 247), 40,688 610 (4 780, 12 620, 1 2,070); 8,000 x 56 x 64 87 in 9 (4 124, 18 101).
   const int64_t slots = head_dim == 128 ? 256 : 512;  // workgroups that run at once
   return (int)std::max<int64_t>(1, std::min(slots / heads, vdnh3::most_chunks(rows, sequences) / 2));
 }
@@ -617,7 +614,8 @@ extern "C" int vdnh3_causal_linear_packed(const uint16_t *q, int64_t q_row, int6
   VDNH3_HOST_CHECK(reinterpret_cast<uintptr_t>(initial_state) % 16 == 0 && reinterpret_cast<uintptr_t>(final_state) % 16 == 0,
                    VDNH3_ERR_INVALID, "causal_linear: states must be 16-byte aligned");
   VDNH3_HOST_CHECK(std::isfinite(scale), VDNH3_ERR_INVALID, "causal_linear: scale must be finite");
-  VDNH3_HOST_CHECK(ranges >= 1 && ranges <= (1 << 20), VDNH3_ERR_INVALID, "causal_linear: ranges must be positive, got %d", ranges);
+  VDNH3_HOST_CHECK(ranges >= 1 && ranges <= (1 << 20), VDNH3_ERR_INVALID, "causal_linear: ranges must be positive, got %d",
+                   ranges);
   VDNH3_HOST_CHECK(ranges == 1 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
                                    workspace_bytes >= vdnh3_causal_linear_workspace_bytes(ranges, heads, head_dim)),
                    VDNH3_ERR_INVALID, "causal_linear: %d ranges need a 16-byte aligned workspace of %zu bytes", ranges,

@@ -118,7 +118,8 @@ __global__ __launch_bounds__(256) void state_step_kernel(StepCall p) {
   for (int g = 0; g < G; ++g) {
     const int r = row0 + 4 * g + r4;
 #pragma unroll
-    for (int c = 0; c < Q; ++c) s[g][c] = live && r < dim ? load4<VEC, (E > 4)>(state + (int64_t)r * dim, 64 * c + 4 * l16, dim) : f32x4_t{};
+    for (int c = 0; c < Q; ++c)
+      s[g][c] = live && r < dim ? load4<VEC, (E > 4)>(state + (int64_t)r * dim, 64 * c + 4 * l16, dim) : f32x4_t{};
   }
   // one request a slot: the first that names it has it, whatever order the workgroups run in
   bool taken = false;

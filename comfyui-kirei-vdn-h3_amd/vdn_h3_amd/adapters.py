@@ -99,8 +99,8 @@ class LowRankAdapters:
                    torch.stack([pad(b, (0, rank - b.shape[1])) for _, b in pairs]), scales)
 
     def add(self, y: torch.Tensor, x: torch.Tensor, index: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
-        """``y`` ``[T, out]`` with each row's adapter applied to ``x`` ``[T, width]`` added, both bf16: a new tensor, or ``out``, which
-        may be ``y`` itself (but not overlap it, or x, otherwise).
+        """``y`` ``[T, out]`` with each row's adapter applied to ``x`` ``[T, width]`` added, both bf16: a new tensor, or ``out``,
+        which may be ``y`` itself (but not overlap it, or x, otherwise).
 
         ``index`` (``[T]`` integers on the GPU) names a row's adapter; a number outside ``[0, n)`` (-1 by custom) names none, and
         the row keeps ``y``. The sum is rounded once; ``A x`` is fp32. Rows of one adapter are fastest next to each other.

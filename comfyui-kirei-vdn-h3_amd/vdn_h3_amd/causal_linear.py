@@ -57,8 +57,8 @@ def _cut(rows: int, sequences: int, heads: int, dim: int) -> tuple[int, int]:
 def causal_linear_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, log_decay: torch.Tensor, cu_seqlens,
                          scale: float, *, initial_state: torch.Tensor | None = None, output_final_state: bool = False,
                          out: torch.Tensor | None = None):
-    """``(o [T, H, D] bf16, final states [B, H, D, D] fp32 or None)`` of packed sequences: q and k ``[T, H_qk, D]``, v ``[T, H, D]``,
-    all bf16, ``log_decay`` ``[H]`` (0 keeps everything, -inf nothing).
+    """``(o [T, H, D] bf16, final states [B, H, D, D] fp32 or None)`` of packed sequences: q and k ``[T, H_qk, D]``, v
+    ``[T, H, D]``, all bf16, ``log_decay`` ``[H]`` (0 keeps everything, -inf nothing).
 
     Sequence ``b`` is the rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` as in ``causal_softmax_packed``; its state starts from
     ``initial_state[b]`` (``[B, H, D, D]`` fp32, dv rows, dk columns) or zeros. An empty sequence's final state is its initial
