@@ -204,6 +204,9 @@ class HipLinear(torch.nn.Module):
         if adapters is not None:
             if accumulate:
                 raise ValueError("adapters are added to the projection's own output: not with accumulate")
+            if (adapters.width, adapters.out_width) != (self.in_features, self.out_features) or adapter_index is None:
+                raise ValueError(f"adapters of {adapters.width} -> {adapters.out_width}, and an index of them, beside a projection of "
+                                 f"{self.in_features} -> {self.out_features}")
             if x.dtype != torch.bfloat16:
                 x = x.to(torch.bfloat16)
             y = self.forward(x, out=out)

@@ -180,3 +180,18 @@ def test_layouts_of_rows_and_kept_scales(device):
     assert torch.equal(far_y, want) and torch.equal(far_x, x)
     one = x.flatten()[:300].as_strided((1, 256), (3, 1))
     assert torch.equal(handle.add(y[:1].as_strided((1, 128), (1, 1)), one, index[:1]), handle.add(y[:1], one.clone(), index[:1]))
+
+
+def test_a_projection_refuses_adapters_of_another(device):
+    """Before anything is written."""
+    from vdn_h3_amd.adapters import LowRankAdapters
+    from vdn_h3_amd.linear import HipLinear
+
+    (x, _, down, up, scales), _ = _case(9, 256, 128, 3, 16, device)
+    layer, out = HipLinear(torch.zeros(128, 256, dtype=BF, device=device)), torch.full((9, 128), 7.0, dtype=BF, device=device)
+    index = torch.zeros(9, dtype=torch.int32, device=device)
+    for handle, at in ((LowRankAdapters(down[..., :128], up), index), (LowRankAdapters(down, up[:, :64]), index),
+                       (LowRankAdapters(down, up), None)):
+        with pytest.raises(ValueError):
+            layer(x, out=out, adapters=handle, adapter_index=at)
+    assert (out == 7.0).all()

@@ -188,3 +188,32 @@ def test_on_another_stream(device, delta):
             results.append([layer.tokens(_inputs(device, 3, n, WIDTH, seed=n), index, pool, slots, False) for n in (1, 2)] + [pool])
         stream.synchronize()
     assert all(torch.equal(torch.nan_to_num(a, 7.0), torch.nan_to_num(b, 7.0)) for a, b in zip(*results))
+
+
+def test_calls_of_two_streams_at_once(device):
+    """Prompts, tokens and adapters of two streams in turn, without a wait between them: the results of one after another."""
+    layers = [_Layer(device, False), _Layer(device, True)]
+    pools = [_started(device, layer) for layer in layers]
+    prompts = [_inputs(device, 900 + 64 * i, WIDTH, seed=i) for i in range(2)]
+    tokens = [_inputs(device, 3, 1, WIDTH, seed=50 + i) for i in range(2)]
+    rows = [torch.arange(x.shape[0], device=device, dtype=torch.int32) % 4 - 1 for x in prompts]
+
+    def turn(i, pool):
+        y = layers[i].prompts(prompts[i], [0, prompts[i].shape[0]], rows[i], pool, [1], False)
+        return y, layers[i].tokens(tokens[i], pools[i][1], pool, pools[i][2], False)
+
+    want = []
+    for i in range(2):
+        pool = pools[i][0].clone()
+        want.append([turn(i, pool) for _ in range(4)] + [pool])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(turn(i, pools[i][0]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(torch.nan_to_num(pools[i][0], 7.0), torch.nan_to_num(want[i][-1], 7.0))
+        assert all(torch.equal(a, b) for x, y in zip(got[i], want[i]) for a, b in zip(x, y))
