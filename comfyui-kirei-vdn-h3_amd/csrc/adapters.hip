@@ -367,12 +367,14 @@ constexpr int kRows32 = 8192, kRows64 = 16384;
 // 15,360 columns 6.3 us (all adapters in one workgroup 98, in 16 8.1), 256 of them 13.7 (18, 15); 40,688 rows x 5,120 columns
 // 183 us in six spans, 191 in three; 9,000 x 15,360 111 and 125.
 constexpr int kShrinkGroups = 512, kExpandShares = 1024, kExpandGroups = 8192;
+constexpr int kMostWidth = 1 << 30;  // the kernels step over columns in 32 bits
 
 struct AdapterCut {
   int ranks, row_tiles, rank_tiles, groups, shares, span, expand_shares;
   int64_t shrink, expand;  // workgroups
 };
-AdapterCut adapter_cut(int rows, int out_width, int adapters, int rank) {
+// In 64 bits: rows are any 32-bit number
+AdapterCut adapter_cut(int64_t rows, int64_t out_width, int adapters, int rank) {
   AdapterCut c;
   c.ranks = kept_ranks(rank);
   c.row_tiles = rows >= kRows64 ? 4 : rows >= kRows32 ? 2 : 1;
@@ -380,7 +382,7 @@ AdapterCut adapter_cut(int rows, int out_width, int adapters, int rank) {
   c.rank_tiles = 1;
   while (c.rank_tiles < most && 16 * c.rank_tiles < c.ranks) c.rank_tiles *= 2;
   c.groups = (c.ranks + 16 * c.rank_tiles - 1) / (16 * c.rank_tiles);
-  const int64_t blocks = (rows + 16 * c.row_tiles - 1) / (16 * c.row_tiles), of = std::min(rows, adapters);
+  const int64_t blocks = (rows + 16 * c.row_tiles - 1) / (16 * c.row_tiles), of = std::min<int64_t>(rows, adapters);
   c.shares = (int)std::max<int64_t>(1, std::min({of, (int64_t)16 * c.row_tiles, kShrinkGroups / (blocks * c.groups)}));
   c.shrink = blocks * c.groups * c.shares;
   // columns of an expanding workgroup: fewer than all where that leaves too few workgroups
@@ -416,9 +418,9 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   VDNH3_HOST_CHECK(rows > 0 && width > 0 && out_width > 0 && adapters > 0 && rank > 0, VDNH3_ERR_INVALID,
                    "adapter_add: rows, widths, adapters and rank must be positive, got %d rows, %d -> %d, %d of rank %d", rows, width,
                    out_width, adapters, rank);
-  VDNH3_HOST_CHECK(width % 8 == 0 && out_width % 8 == 0 && rank <= 1024, VDNH3_ERR_INVALID,
-                   "adapter_add: widths must be multiples of 8 and the rank at most 1024, got %d -> %d, rank %d", width, out_width,
-                   rank);
+  VDNH3_HOST_CHECK(width % 8 == 0 && out_width % 8 == 0 && width <= kMostWidth && out_width <= kMostWidth && rank <= 1024,
+                   VDNH3_ERR_INVALID, "adapter_add: widths must be multiples of 8, at most 2^30, and the rank at most 1024, got "
+                   "%d -> %d, rank %d", width, out_width, rank);
   VDNH3_HOST_CHECK(index != nullptr, VDNH3_ERR_INVALID, "adapter_add: an index is needed");
   if (rows == 1) y_row = out_row = out_width, x_row = width;  // one row has no stride, whatever a caller passes for it
   int rc = check_adapter_rows(x, x_row, width, "x", true);

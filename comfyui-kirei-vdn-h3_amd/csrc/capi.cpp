@@ -32,7 +32,7 @@ int check_launch(const char *what) {
 }
 
 int check_grid(int64_t workgroups, int threads, const char *what) {
-  if (workgroups * threads > (int64_t)UINT32_MAX)
+  if (workgroups < 0 || workgroups > (int64_t)UINT32_MAX / threads)
     return set_error(VDNH3_ERR_INVALID, "%s: %lld workgroups are too many for one launch", what, (long long)workgroups);
   return VDNH3_OK;
 }

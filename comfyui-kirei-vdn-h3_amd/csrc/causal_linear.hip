@@ -563,7 +563,7 @@ int launch_causal_linear(const LinCall &p, hipStream_t s) {
 constexpr int kAddedRanges = 16;
 
 // Chunks of a call, at most: the sequences' lengths are on the device.
-int64_t most_chunks(int rows, int sequences) { return rows / kLinC + std::min(rows, sequences); }
+int64_t most_chunks(int64_t rows, int64_t sequences) { return rows / kLinC + std::min(rows, sequences); }
 
 int check_lin_operand(const void *p, int64_t row, int64_t head, const char *name) {
   VDNH3_HOST_CHECK(p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % 8 == 0 && head % 8 == 0 && row >= 0 &&

@@ -60,7 +60,7 @@ class LowRankAdapters:
     """The adapters of one projection ``[out, width]``: ``down`` ``[n, rank, width]`` (A) and ``up`` ``[n, out, rank]`` (B), bf16 on
     the GPU, and ``scales``, ``n`` numbers (a tensor or a sequence; ``None``: ones), kept in fp32.
 
-    Widths are multiples of 8, ranks at most 1024. The object keeps copies, A and B in the kernels' order (a later change of the
+    Widths are multiples of 8 (at most 2**30), ranks at most 1024. The object keeps copies, A and B in the kernels' order (a later change of the
     tensors is not seen), and has to outlive graphs that were captured with it. ``from_pairs`` takes adapters of different
     ranks.
     """
@@ -73,8 +73,8 @@ class LowRankAdapters:
             raise TypeError(f"LowRankAdapters computes in bf16; got {down.dtype}/{up.dtype}")
         self.count, self.rank, self.width = (int(n) for n in down.shape)
         self.out_width = int(up.shape[1])
-        if self.width % 8 or self.out_width % 8:
-            raise ValueError(f"the projection's widths must be multiples of 8, got {self.width} -> {self.out_width}")
+        if self.width % 8 or self.out_width % 8 or max(self.width, self.out_width) > 2 ** 30:
+            raise ValueError(f"the projection's widths must be multiples of 8, at most 2**30, got {self.width} -> {self.out_width}")
         if self.rank > 1024:
             raise ValueError(f"ranks up to 1024 are supported, got {self.rank}")
         _lib.forward_only("LowRankAdapters", down, up, scales)

@@ -601,7 +601,7 @@ int vdnh3_gated_delta_step(const uint16_t *q, const uint16_t *k, const uint16_t 
 
 /* out[t] = bf16(y[t] + scales[i] B_i (A_i x[t])), i = index[t]: the low-rank adapters of many requests, A_i [rank, width] and
  * B_i [out_width, rank], beside a projection's output y [rows, out_width]. scales null: ones. An index outside [0, adapters) names
- * no adapter: out[t] = y[t]. out may be y. Widths are multiples of 8, the rank is at most 1024; rows of x and y may overlap.
+ * no adapter: out[t] = y[t]. out may be y. Widths are multiples of 8, at most 2^30, the rank at most 1024. Rows of x and y may overlap.
  * A and B lie in the order of the wavefronts' operands, zeros behind their own numbers, with R = 16 ranks for ranks up to 16,
  * else the rank rounded up to 32:
  *   down [adapters][width / 64, rounded up][R / 16][2][4][16][8] bf16: the element [i][s][t][k][g][m][j] is

@@ -224,3 +224,26 @@ def test_ranges_of_a_call(built_lib):
     assert lib.vdnh3_causal_linear_ranges(8000, 1, 1000, 128) == 1
     for bad in [(0, 1, 1, 64), (1, 0, 1, 64), (1, 1, 0, 64), (1, 1, 1, 80)]:
         assert lib.vdnh3_causal_linear_ranges(*bad) == 0
+
+
+def test_sizes_at_the_end_of_32_bits_are_refused(built_lib):
+    """Block counts of the largest rows and widths that a call can name: a status, not a launch of a count that wrapped around."""
+    from vdn_h3_amd import _lib
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    lib, p = _lib.lib(), 1 << 20  # an address that is never read
+
+    def add(rows=200, width=128, out_width=64, n=2, rank=8):
+        return lib.vdnh3_adapter_add(p, out_width, p, width, p, p, None, p, p, out_width, rows, width, out_width, n, rank, p, 1 << 62,
+                                     None)
+
+    top = (1 << 31) - 1
+    for bad in [dict(rows=top), dict(rows=top - 62), dict(rows=top, rank=1024), dict(out_width=top - 7), dict(width=top - 7),
+                dict(rows=1, out_width=top - 7), dict(rows=top, out_width=top - 7, n=top)]:
+        assert add(**bad) == _lib.VDNH3_ERR_INVALID, bad
+        assert "adapter_add" in _lib.last_error()
+    assert lib.vdnh3_causal_linear_ranges(top, top, 1, 64) == 512  # chunks counted past 32 bits
+    one = _z(1)
+    for width, out in ((2 ** 30 + 8, 8), (8, 2 ** 30 + 8)):
+        with pytest.raises(ValueError, match="widths"):
+            LowRankAdapters(one.expand(1, 1, width), one.expand(1, out, 1))
