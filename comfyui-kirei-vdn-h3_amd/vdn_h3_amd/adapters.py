@@ -18,6 +18,7 @@ import torch
 from . import _lib
 
 _INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+_NAME = "LowRankAdapters.add"
 
 
 @lru_cache(maxsize=4096)
@@ -31,7 +32,7 @@ def _add_plan(xs, xt, xd, ys, yt, yd, ins, it, ind, width: int, out_width: int, 
         raise TypeError(f"LowRankAdapters.add computes in bf16; got {yd}/{xd}")
     if tuple(ins) != (rows,) or ind not in _INTEGERS:
         raise ValueError(f"index must be a tensor of {rows} integers, one per row")
-    _lib.int32_sizes("LowRankAdapters.add", rows)
+    _lib.int32_sizes(_NAME, rows)
 
     def whole(t):
         return t[1] == 1 and (rows < 2 or t[0] % 8 == 0)
@@ -105,18 +106,27 @@ class LowRankAdapters:
         ``index`` (``[T]`` integers on the GPU) names a row's adapter; a number outside ``[0, n)`` (-1 by custom) names none, and
         the row keeps ``y``. The sum is rounded once; ``A x`` is fp32. Rows of one adapter are fastest next to each other.
         """
-        name = "LowRankAdapters.add"
+        return self.apply(self.checked(y, x, index, out), y, x, index, out)
+
+    def checked(self, y: torch.Tensor, x: torch.Tensor, index: torch.Tensor, out: torch.Tensor | None) -> tuple:
+        """What ``apply`` needs to know of a call, after every check of its arguments, before anything is written."""
         if not isinstance(index, torch.Tensor):
             raise ValueError(f"index must be a tensor of integers, one per row, got {type(index).__name__}")
         rows, size, as_they_lie = _add_plan(x.shape, x.stride(), x.dtype, y.shape, y.stride(), y.dtype, index.shape, index.stride(),
                                             index.dtype, self.width, self.out_width, self.rank)
-        _lib.forward_only(name, y, x, out)
+        _lib.forward_only(_NAME, y, x, out)
         device = _lib.require_device(self.down, y, x, index, out)
+        if out is not None and (
+                out is not y and (tuple(out.shape) != (rows, self.out_width) or out.dtype != torch.bfloat16) or
+                not _lib.in_place(out) or (rows > 1 and out.stride(0) < self.out_width)):
+            raise ValueError(f"out must be a bf16 [{rows}, {self.out_width}] tensor with 16-byte aligned rows that do not overlap")
+        return rows, size, as_they_lie, device
+
+    def apply(self, plan: tuple, y: torch.Tensor, x: torch.Tensor, index: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+        """``add`` of arguments that ``checked`` gave a plan for."""
+        rows, size, as_they_lie, device = plan
         if out is None:
             out = torch.empty(rows, self.out_width, dtype=torch.bfloat16, device=device)
-        elif out is not y and (tuple(out.shape) != (rows, self.out_width) or out.dtype != torch.bfloat16) or \
-                not _lib.in_place(out) or (rows > 1 and out.stride(0) < self.out_width):
-            raise ValueError(f"out must be a bf16 [{rows}, {self.out_width}] tensor with 16-byte aligned rows that do not overlap")
         if rows == 0:
             return out
         if not as_they_lie or x.data_ptr() % 16 or y.data_ptr() % 16:
@@ -125,7 +135,7 @@ class LowRankAdapters:
                 index = index.clamp(-1, self.count)  # outside stays outside in 32 bits
             index = index.to(torch.int32).contiguous()
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _lib.launch(name, _lib.lib().vdnh3_adapter_add, device,
+        _lib.launch(_NAME, _lib.lib().vdnh3_adapter_add, device,
                     y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), self.down.data_ptr(), self.up.data_ptr(),
                     _lib.ptr(self.scales), index.data_ptr(), out.data_ptr(), out.stride(0), rows, self.width, self.out_width,
                     self.count, self.rank, _lib.ptr(workspace), size)

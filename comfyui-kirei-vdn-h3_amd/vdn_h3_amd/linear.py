@@ -201,6 +201,8 @@ class HipLinear(torch.nn.Module):
                 adapter_index: torch.Tensor | None = None):
         """The projection of ``x``; with ``adapters`` (``adapters.LowRankAdapters``) each row's low-rank adapter
         (``adapter_index``) is applied to the bf16 ``x`` and added to the projection's bf16 output, in place."""
+        if x.ndim != 2 or x.shape[1] != self.in_features:
+            raise ValueError(f"expected [rows, {self.in_features}] input, got {tuple(x.shape)}")
         if adapters is not None:
             if accumulate:
                 raise ValueError("adapters are added to the projection's own output: not with accumulate")
@@ -209,12 +211,13 @@ class HipLinear(torch.nn.Module):
                                  f"{self.in_features} -> {self.out_features}")
             if x.dtype != torch.bfloat16:
                 x = x.to(torch.bfloat16)
-            y = self.forward(x, out=out)
-            return adapters.add(y, x, adapter_index, out=y)
+            if out is None:
+                out = torch.empty(x.shape[0], self.out_features, dtype=torch.bfloat16, device=x.device)
+            plan = adapters.checked(out, x, adapter_index, out)  # before the projection writes
+            self.forward(x, out=out)
+            return adapters.apply(plan, out, x, adapter_index, out)
         if adapter_index is not None:
             raise ValueError("adapter_index without adapters")
-        if x.ndim != 2 or x.shape[1] != self.in_features:
-            raise ValueError(f"expected [rows, {self.in_features}] input, got {tuple(x.shape)}")
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
         if self.precision == "bf16":

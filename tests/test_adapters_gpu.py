@@ -195,3 +195,31 @@ def test_a_projection_refuses_adapters_of_another(device):
         with pytest.raises(ValueError):
             layer(x, out=out, adapters=handle, adapter_index=at)
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("precision", ["bf16", "int8", "fp8"])
+def test_a_projection_refuses_operands_of_its_adapters(device, precision):
+    """An index or an output that the adapters do not take: before anything is written."""
+    from vdn_h3_amd.adapters import LowRankAdapters
+    from vdn_h3_amd.linear import HipLinear
+
+    (x, _, down, up, scales), _ = _case(9, 256, 128, 3, 16, device)
+    layer, handle = HipLinear(torch.zeros(128, 256, dtype=BF, device=device), precision), LowRankAdapters(down, up, scales)
+    room = torch.full((9 * 200,), 7.0, device=device)
+    good, wide = room.to(BF)[:9 * 128].view(9, 128), room.to(BF)
+    index = torch.zeros(9, dtype=torch.int32, device=device)
+    at = dict(x=x, out=good, adapter_index=index)
+    for error, change in [(ValueError, dict(adapter_index=index[:8])), (ValueError, dict(adapter_index=index[:, None])),
+                          (ValueError, dict(adapter_index=index.float())), (ValueError, dict(adapter_index=[0] * 9)),
+                          (RuntimeError, dict(adapter_index=index.cpu())), (TypeError, dict(out=room[:9 * 128].view(9, 128))),
+                          (ValueError, dict(out=wide[1:1 + 9 * 128].view(9, 128))),
+                          (ValueError, dict(out=wide.as_strided((9, 128), (132, 1)))),
+                          (ValueError, dict(out=wide.as_strided((9, 128), (64, 1)))), (ValueError, dict(out=good[:8])),
+                          (ValueError, dict(x=x[:8])), (ValueError, dict(x=x[:, :128]))]:
+        with pytest.raises(error):
+            layer(adapters=handle, **(at | change))
+        assert (change.get("out", good) == 7.0).all() and (good == 7.0).all(), change
+    with pytest.raises(RuntimeError, match="forward-only"):
+        layer(adapters=handle, **(at | dict(out=good.clone().requires_grad_())))
+    assert layer(adapters=handle, **at) is good
+    assert torch.equal(good, layer(x, adapters=handle, adapter_index=index))
