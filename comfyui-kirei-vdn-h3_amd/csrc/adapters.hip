@@ -32,7 +32,7 @@ struct AdapterCall {
   const float *scales;
   const int32_t *index;
   uint16_t *h;  // [rows, ranks, in eights: 8 first numbers, 8 second ones]: s A x as two bf16 numbers
-  int rows, width, out_width, adapters, ranks, shares, copy;  // ranks: 16, or the rank rounded up to 32
+  int rows, width, out_width, adapters, rank, ranks, shares, copy;  // ranks: 16, or the rank rounded up to 32
 };
 
 // Between what lanes of a wavefront write to LDS and what others of them read: its LDS operations run in order, but the compiler
@@ -58,6 +58,12 @@ __device__ __forceinline__ void list_rows(uint64_t mask, int *list) {
   wave_sync();
 }
 
+// What the first bf16 number of x, `hi` as fp32 bits, leaves of it: nothing of an infinity, where inf - inf is a NaN
+__device__ __forceinline__ float rest(float x, uint32_t hi) {
+  const float d = x - __uint_as_float(hi);
+  return d == d ? d : 0.f;
+}
+
 // s A x of the rows of one adapter in a block, in two bf16 numbers, 2^-17 of it: one would add 1.1e-3 of the product to the
 // result's own 1.7e-3 of rounding. The wavefronts take steps of 64 channels in turn and add their sums up in LDS.
 // C[rank][row] tiles: a lane has four ranks of a row.
@@ -81,10 +87,10 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
   __syncthreads();  // the sums of another adapter have been read
   for (int step = wave; step < steps; step += W) {
     u32x4_t a[2][NT], x[2 * MT];
-    // channels behind the width: A holds zeros for them, x is read again
-    const int c = min(64 * step + 8 * c8, p.width - 8);
+    // channels behind the width: A holds zeros for them, and x, read again, becomes zeros (0 * inf would be a NaN)
+    const int c = 64 * step + 8 * c8;
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) x[i] = ld16(xp[i] + c);
+    for (int i = 0; i < 2 * MT; ++i) x[i] = ld16(xp[i] + min(c, p.width - 8));
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -92,6 +98,9 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
     wave_sync();
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) stage[(8 * i + r8) * 8 + (c8 ^ r8)] = x[i];
+    if (64 * step + 64 > p.width && c >= p.width)
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) stage[(8 * i + r8) * 8 + (c8 ^ r8)] = u32x4_t{};
     wave_sync();
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -119,9 +128,12 @@ __device__ __forceinline__ void shrink_rows(const AdapterCall &p, int row0, cons
     const int i = k * W + wave, m = i % MT, r = rank0 + 16 * (i / MT) + 4 * g;
     if (16 * m + l16 >= count || r >= p.ranks) continue;
     all *= scale;
+    if (p.rank < p.ranks)  // ranks that the adapters do not have, whatever x holds
+#pragma unroll
+      for (int j = 0; j < 4; ++j) all[j] = r + j < p.rank ? all[j] : 0.f;
     const u32x2_t hi = {pack_bf2(all[0], all[1]), pack_bf2(all[2], all[3])};
-    const u32x2_t lo = {pack_bf2(all[0] - __uint_as_float(hi[0] << 16), all[1] - __uint_as_float(hi[0] & 0xffff0000u)),
-                        pack_bf2(all[2] - __uint_as_float(hi[1] << 16), all[3] - __uint_as_float(hi[1] & 0xffff0000u))};
+    const u32x2_t lo = {pack_bf2(rest(all[0], hi[0] << 16), rest(all[1], hi[0] & 0xffff0000u)),
+                        pack_bf2(rest(all[2], hi[1] << 16), rest(all[3], hi[1] & 0xffff0000u))};
     const int64_t row = LISTED ? 16 * m + l16 : row0 + list[16 * m + l16];
     uint16_t *to = h + (row * p.ranks + (r & ~7)) * 2 + (r & 4);
     *reinterpret_cast<u32x2_t *>(to) = hi;
@@ -439,7 +451,7 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   if (!rc) rc = check_grid(c.expand, 256, "adapter_add");
   if (rc) return rc;
   AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<uint16_t *>(workspace), rows, width,
-                out_width, adapters, c.ranks, c.shares, out != y};
+                out_width, adapters, rank, c.ranks, c.shares, out != y};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (needed == 0) {
     p.shares = std::min({rows, adapters, 16});

@@ -89,7 +89,8 @@ class LowRankAdapters:
 
     @classmethod
     def from_pairs(cls, pairs, scales=None) -> "LowRankAdapters":
-        """From ``(down [rank_i, width], up [out, rank_i])`` of each adapter; smaller ranks are filled up with zeros."""
+        """From ``(down [rank_i, width], up [out, rank_i])`` of each adapter; smaller ranks are filled up with zeros
+        (which are a NaN times an infinite x)."""
         pairs = list(pairs)
         if not pairs or any(a.ndim != 2 or b.ndim != 2 or a.shape[0] != b.shape[1] or a.shape[1] != pairs[0][0].shape[1] or
                             b.shape[0] != pairs[0][1].shape[0] for a, b in pairs):
@@ -105,6 +106,8 @@ class LowRankAdapters:
 
         ``index`` (``[T]`` integers on the GPU) names a row's adapter; a number outside ``[0, n)`` (-1 by custom) names none, and
         the row keeps ``y``. The sum is rounded once; ``A x`` is fp32. Rows of one adapter are fastest next to each other.
+        A number that is not finite stays in its row: infinities of A and x come out as by the formula, those of B as no finite
+        numbers.
         """
         return self.apply(self.checked(y, x, index, out), y, x, index, out)
 
