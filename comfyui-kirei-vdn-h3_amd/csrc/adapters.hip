@@ -23,7 +23,7 @@ namespace {
 constexpr int kListRows = 64;    // the most rows of a block
 constexpr int kExpandRows = 32;  // 64 leave one wavefront a SIMD: 286 us for 40,688 rows x 5,120 of rank 64 instead of 183
 constexpr int kShrinkWaves = 8;
-constexpr int kFewRows = 64, kFewRanks = 64;  // up to which one launch makes both products
+constexpr int kFewRows = 64, kFewRanks = 64;  // up to which one launch can make both products
 
 struct AdapterCall {
   const uint16_t *x, *y, *down, *up;
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, i
 // Both products in one launch for few rows: every workgroup of a span of columns makes s A x of its adapters' rows anew, in LDS.
 // Spans of 512 columns or more, as many workgroups as one round of the CUs: one row x 5,120 -> 15,360 of rank 16 takes 5.9 us
 // (two launches 7.7, and 4 us more of the host's), 64 rows of 16 adapters 11.0 in spans of 1,024 (512 16.7, 2,048 12.6, two
-// launches 13.9), but 64 rows of one adapter of rank 32 x 5,120 -> 5,120 14.5 (9.9).
+// launches 13.9). Where it is taken: one_launch.
 template <int NT, int KS>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_few_rows_kernel(AdapterCall p, int spans, int span) {
   constexpr int STEP = 64 * kShrinkWaves;
@@ -371,6 +371,18 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_few_rows_kernel(Ada
 
 // The ranks that are kept: 16, or a multiple of 32; zeros behind the adapter's own.
 int kept_ranks(int rank) { return rank <= 16 ? 16 : (rank + 31) / 32 * 32; }
+
+// Whether the one launch for few rows is the faster form. Its workgroups, a span of columns and every `shares`-th registered adapter
+// each, make A x anew, so it loses where many rows of wide x fall to few adapters; the host knows the registered ones, not those
+// that rows name. Kernel times, one launch / two, for rows x width -> columns of rank 32: one adapter 16 x 5,120 -> 5,120 7.2 / 8.9
+// us, 32 9.2 / 9.5, 48 13.8 / 9.6, 64 15.5 / 9.7; 16 x 13,824 -> 5,120 15.9 / 16.8, 24 20.0 / 17.2; 64 x 1,024 -> 1,024 8.2 / 7.0, of which
+// two take 4 us more of the host's; 64 x 5,120 of four adapters 9.8 / 9.3 with rows of each, 14.8 / 9.6 if all name one; 64 x 5,120 ->
+// 15,360 of 16 adapters 12.9 / 15.2 and 20.3 / 11.8.
+constexpr int kFewRowsAlways = 16;
+constexpr int64_t kFewChannels = 32 * 5120;
+bool one_launch(int64_t rows, int64_t width, int64_t adapters) {
+  return rows <= kFewRowsAlways || rows * width <= kFewChannels * std::min(rows, adapters);
+}
 
 // Rows of a shrinking workgroup: 16 until there are workgroups enough without, since A is read for each (3,939 rows of rank 32:
 // 15.2 us with 16, 21 with 32, 35 with 64; 9,000 of rank 128: 59 with 16, 48 with 32; 40,688 of rank 64: 117, 85, 84).
@@ -422,6 +434,13 @@ extern "C" size_t vdnh3_adapter_workspace_bytes(int rows, int rank) {
   return (size_t)rows * vdnh3::kept_ranks(rank) * 4;
 }
 
+extern "C" size_t vdnh3_adapter_workspace_wanted(int rows, int width, int adapters, int rank) {
+  if (rows <= 0 || width <= 0 || adapters <= 0 || rank <= 0 || rank > 1024) return 0;
+  const size_t needed = vdnh3_adapter_workspace_bytes(rows, rank);
+  if (needed || vdnh3::one_launch(rows, width, adapters)) return needed;
+  return (size_t)rows * vdnh3::kept_ranks(rank) * 4;
+}
+
 extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_t *x, int64_t x_row, const uint16_t *down,
                                  const uint16_t *up, const float *scales, const int32_t *index, uint16_t *out, int64_t out_row,
                                  int rows, int width, int out_width, int adapters, int rank, void *workspace,
@@ -453,7 +472,9 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
   AdapterCall p{x, y, down, up, out, x_row, y_row, out_row, scales, index, static_cast<uint16_t *>(workspace), rows, width,
                 out_width, adapters, rank, c.ranks, c.shares, out != y};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (needed == 0) {
+  const size_t wanted = vdnh3_adapter_workspace_wanted(rows, width, adapters, rank);
+  const bool room = workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && workspace_bytes >= wanted;
+  if (needed == 0 && (wanted == 0 || !room)) {
     p.shares = std::min({rows, adapters, 16});
     const int wide = (out_width + 511) / 512, span = 512 * ((wide * p.shares + 255) / 256), spans = (out_width + span - 1) / span;
     auto few = [&](auto kernel) {

@@ -41,4 +41,4 @@ int check_grid(int64_t workgroups, int threads, const char *what) {
 
 extern "C" const char *vdnh3_last_error(void) { return g_last_error.c_str(); }
 
-extern "C" int vdnh3_abi_version(void) { return 104; }
+extern "C" int vdnh3_abi_version(void) { return 105; }

@@ -130,6 +130,7 @@ SIGNATURES = {
     "vdnh3_causal_linear_step": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_float, _vp]),
     "vdnh3_gated_delta_step": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vdnh3_adapter_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "vdnh3_adapter_workspace_wanted": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
     "vdnh3_adapter_add": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_int, _c_int, _c_int, _c_int,
                                    _c_int, _vp, _c_size, _vp]),
     "vdnh3_head_gate": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int, _vp]),

@@ -22,7 +22,7 @@ _NAME = "LowRankAdapters.add"
 
 
 @lru_cache(maxsize=4096)
-def _add_plan(xs, xt, xd, ys, yt, yd, ins, it, ind, width: int, out_width: int, rank: int) -> tuple[int, int, bool]:
+def _add_plan(xs, xt, xd, ys, yt, yd, ins, it, ind, width: int, out_width: int, count: int, rank: int) -> tuple[int, int, bool]:
     """What the layouts of a call say, checked once for each set of them: ``(rows, workspace bytes, whether no operand has to be
     copied but for an address off 16 bytes)``."""
     rows = xs[0] if len(xs) == 2 else -1
@@ -38,7 +38,7 @@ def _add_plan(xs, xt, xd, ys, yt, yd, ins, it, ind, width: int, out_width: int, 
         return t[1] == 1 and (rows < 2 or t[0] % 8 == 0)
 
     as_they_lie = whole(xt) and whole(yt) and ind == torch.int32 and (rows < 2 or it[0] == 1)
-    return rows, _lib.lib().vdnh3_adapter_workspace_bytes(rows, rank) if rows else 0, as_they_lie
+    return rows, _lib.lib().vdnh3_adapter_workspace_wanted(rows, width, count, rank), as_they_lie
 
 
 def _layouts(down: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -116,7 +116,7 @@ class LowRankAdapters:
         if not isinstance(index, torch.Tensor):
             raise ValueError(f"index must be a tensor of integers, one per row, got {type(index).__name__}")
         rows, size, as_they_lie = _add_plan(x.shape, x.stride(), x.dtype, y.shape, y.stride(), y.dtype, index.shape, index.stride(),
-                                            index.dtype, self.width, self.out_width, self.rank)
+                                            index.dtype, self.width, self.out_width, self.count, self.rank)
         _lib.forward_only(_NAME, y, x, out)
         device = _lib.require_device(self.down, y, x, index, out)
         if out is not None and (

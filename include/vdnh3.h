@@ -610,8 +610,10 @@ int vdnh3_gated_delta_step(const uint16_t *q, const uint16_t *k, const uint16_t 
  *        B_i[32 p + 8 (m / 4) + 4 t + m % 4][32 k + 8 g + j]; for R = 16 [adapters][out_width / 32][4][16][2][4]: [i][p][g][m][t][j]
  *        is B_i[32 p + 8 (m / 4) + 4 t + m % 4][4 g + j].
  * workspace (vdnh3_adapter_workspace_bytes, 16-byte aligned) holds scales[i] A_i x[t] as two bf16
- * numbers each (0 bytes where a call of few rows needs none). */
+ * numbers each (0 bytes where a call of few rows needs none). vdnh3_adapter_workspace_wanted gives the bytes with which a call is
+ * fastest: a call of few rows that needs none takes two launches where they are faster and it has them, one otherwise. */
 size_t vdnh3_adapter_workspace_bytes(int rows, int rank);
+size_t vdnh3_adapter_workspace_wanted(int rows, int width, int adapters, int rank);
 int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_t *x, int64_t x_row, const uint16_t *down,
                       const uint16_t *up, const float *scales, const int32_t *index, uint16_t *out, int64_t out_row, int rows,
                       int width, int out_width, int adapters, int rank, void *workspace, size_t workspace_bytes, void *stream);

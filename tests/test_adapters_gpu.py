@@ -248,3 +248,26 @@ def test_infinities_of_x(device, rows, width, rank):
     assert touched.sum() >= 4 and torch.equal(got[~touched], plain[~touched])
     assert torch.equal(got[touched].isnan(), want[touched].isnan()) and not got[touched].isfinite().any()
     assert torch.equal(torch.nan_to_num(got[touched].double(), 0.0, 1.0, -1.0), torch.nan_to_num(want[touched], 0.0, 1.0, -1.0))
+
+
+@pytest.mark.parametrize("rows,width,n,rank", [(33, 5120, 1, 16), (64, 5120, 1, 32), (64, 13824, 4, 64), (24, 13824, 1, 8)])
+def test_one_launch_and_two_are_equal(device, rows, width, n, rank):
+    """Calls of few rows with the workspace that they want, without one and with one off 16 bytes: the same bits."""
+    from vdn_h3_amd import _lib
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    (x, y, down, up, scales), g = _case(rows, width, 264, n, rank, device)
+    handle, lib = LowRankAdapters(down, up, scales), _lib.lib()
+    index = torch.randint(-1, n, (rows,), generator=g, dtype=torch.int32).to(device)
+    size = lib.vdnh3_adapter_workspace_wanted(rows, width, n, rank)
+    assert size > 0 and lib.vdnh3_adapter_workspace_bytes(rows, rank) == 0
+    got = handle.add(y, x, index)
+    _check(got, x, y, down, up, scales, index)
+    work = torch.zeros(size + 16, dtype=torch.uint8, device=device)
+    for at, room, used in ((None, 0, False), (work.data_ptr(), size - 1, False), (work.data_ptr() + 8, size, False),
+                           (work.data_ptr(), size, True)):
+        out = torch.full_like(y, 7.0)
+        _lib.check(lib.vdnh3_adapter_add(y.data_ptr(), 264, x.data_ptr(), width, handle.down.data_ptr(), handle.up.data_ptr(),
+                                         handle.scales.data_ptr(), index.data_ptr(), out.data_ptr(), 264, rows, width, 264, n, rank,
+                                         at, room, _lib.stream_handle(device)), "add")
+        assert torch.equal(out, got) and work.any().item() == used

@@ -247,3 +247,22 @@ def test_sizes_at_the_end_of_32_bits_are_refused(built_lib):
     for width, out in ((2 ** 30 + 8, 8), (8, 2 ** 30 + 8)):
         with pytest.raises(ValueError, match="widths"):
             LowRankAdapters(one.expand(1, 1, width), one.expand(1, out, 1))
+
+
+def test_launches_of_the_adapters(built_lib):
+    """The workspace that a call wants says which form it takes: one launch (none) for few rows, two where many rows of wide x fall
+    to few adapters."""
+    from vdn_h3_amd import _lib
+
+    lib = _lib.lib()
+    want = lib.vdnh3_adapter_workspace_wanted
+    for rows, width, adapters in ((1, 5120, 1), (16, 2 ** 20, 1), (32, 5120, 1), (64, 2560, 1), (64, 5120, 2), (64, 5120, 16),
+                                  (64, 13824, 16), (17, 9600, 1), (33, 5120, 2 ** 31 - 1)):
+        assert want(rows, width, adapters, 64) == 0, (rows, width, adapters)
+    for rows, width, adapters in ((33, 5120, 1), (64, 5120, 1), (64, 2568, 1), (24, 13824, 1), (48, 13824, 4), (64, 5128, 2),
+                                  (64, 2 ** 30, 64)):
+        assert want(rows, width, adapters, 8) == rows * 16 * 4 and want(rows, width, adapters, 40) == rows * 64 * 4
+    for rows, rank in ((65, 8), (200, 40), (1, 65), (64, 1024)):  # what a call needs, it wants
+        assert want(rows, 64, 3, rank) == lib.vdnh3_adapter_workspace_bytes(rows, rank) > 0
+    for bad in ((0, 64, 1, 8), (8, 0, 1, 8), (8, 64, 0, 8), (8, 64, 1, 0), (8, 64, 1, 1025)):
+        assert want(*bad) == 0
