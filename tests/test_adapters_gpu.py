@@ -271,3 +271,28 @@ def test_one_launch_and_two_are_equal(device, rows, width, n, rank):
                                          handle.scales.data_ptr(), index.data_ptr(), out.data_ptr(), 264, rows, width, 264, n, rank,
                                          at, room, _lib.stream_handle(device)), "add")
         assert torch.equal(out, got) and work.any().item() == used
+
+
+TALL = [  # rows, width, out, adapters, rank: blocks of 32 and 64 rows with every number of rank tiles, several steps of columns
+    (9000, 64, 72, 3, 8), (9000, 72, 40, 3, 24), (9000, 64, 64, 4, 64), (9000, 136, 72, 2, 136), (17000, 64, 72, 3, 8),
+    (17000, 72, 64, 3, 64), (17000, 64, 40, 2, 136), (64, 72, 8712, 16, 16), (63, 64, 8712, 17, 40), (64, 64, 8712, 16, 24),
+    (16001, 64, 4104, 3, 8), (16001, 64, 4104, 2, 32), (16001, 64, 4104, 2, 40), (16001, 64, 4104, 2, 136)]
+
+
+@pytest.mark.parametrize("rows,width,out,n,rank", TALL)
+def test_blocks_and_steps_against_float64(device, rows, width, out, n, rank):
+    from vdn_h3_amd.adapters import LowRankAdapters
+
+    print(f"case adapters {rows} x {width} -> {out}, {n} of rank {rank}", flush=True)
+    (x, y, down, up, scales), g = _case(rows, width, out, n, rank, device)
+    handle = LowRankAdapters(down, up, scales)
+    any_order = torch.randint(-1, n + 1, (rows,), generator=g, dtype=torch.int32)
+    few = torch.where(torch.rand(rows, generator=g) < 0.3, any_order, -1)  # fewer than 16 rows of each in a block
+    half = torch.where(torch.arange(rows) % 64 < 20, any_order, n - 1)  # up to 64 of the last, few of the others
+    runs = torch.randint(-1, n, (rows,), generator=g, dtype=torch.int32).sort()[0]
+    for index in (any_order, few, half, runs):
+        index = index.to(torch.int32).to(device)
+        got = handle.add(y, x, index)
+        _check(got, x, y, down, up, scales, index)
+        again = y.clone()
+        assert handle.add(again, x, index, out=again) is again and torch.equal(again, got)
