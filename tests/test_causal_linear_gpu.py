@@ -246,3 +246,30 @@ def test_strides_of_single_rows_and_heads_and_past_32_bits(device):
     final = causal_linear_packed(q, k, v, decay, cu, 0.1, output_final_state=True)[1]
     one = causal_linear_packed(q, k, v, decay, [0, 1], 0.1, output_final_state=True)[1]
     assert torch.equal(final[-1], one[0]) and not final[69998].any() and not final[:5].any()
+
+
+@pytest.mark.parametrize("lengths,heads,dim", [([700], 2, 128), ([130, 0, 1, 333, 64, 65], 3, 64), ([0, 64, 64, 0], 2, 128),
+                                               ([1], 2, 64), ([1300, 700], 1, 64)])
+def test_what_a_workspace_held_takes_no_part(device, lengths, heads, dim):
+    """Every number of ranges, with token counts of another call where the ranges' own go: a count that the first pass left out
+    would add a state that is none, or one of NaNs."""
+    from vdn_h3_amd import _lib
+
+    lib, bounds = _lib.lib(), _bounds(lengths)
+    q, k, v, decay, initial = _case(bounds[-1], heads, heads, dim, 5, device, len(lengths))
+    cu, want = torch.tensor(bounds, dtype=torch.int32, device=device), _want(q, k, v, decay, bounds, 0.3, initial)
+    for ranges in (2, 3, 4, 7, 12, 17, 18, 40):
+        results = []
+        for tokens, state in ((-1, torch.nan), (64, torch.nan), (0, 1.0), (640, 1e30)):
+            print(f"ranges {ranges} over {tokens} {state}", flush=True)
+            size = lib.vdnh3_causal_linear_workspace_bytes(ranges, heads, dim)
+            work = torch.full((size // 4,), state, device=device)
+            work.view(torch.int32)[-ranges:] = tokens
+            out, final = torch.zeros_like(v), torch.zeros(len(lengths), heads, dim, dim, device=device)
+            _lib.check(lib.vdnh3_causal_linear_packed(
+                q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], out.data_ptr(),
+                *out.stride()[:2], decay.data_ptr(), cu.data_ptr(), initial.data_ptr(), final.data_ptr(), len(lengths), bounds[-1],
+                heads, heads, dim, 0.3, ranges, work.data_ptr(), size, _lib.stream_handle(device)), "packed")
+            results.append((out, final))
+        _check(results[0], want, dim, max(lengths))
+        assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
