@@ -217,3 +217,49 @@ def test_calls_of_two_streams_at_once(device):
     for i in range(2):
         assert torch.equal(torch.nan_to_num(pools[i][0], 7.0), torch.nan_to_num(want[i][-1], 7.0))
         assert all(torch.equal(a, b) for x, y in zip(got[i], want[i]) for a, b in zip(x, y))
+
+
+def _leave_in_memory(value):
+    """Memory of every size that an allocation is cut from, freed with ``value`` (None: normal numbers) in it."""
+    blocks = [torch.empty(1 << n, device="cuda") for n in (26, 24, 22, 20, 18, 16, 12) for _ in range(4)]
+    for t in blocks:
+        t.normal_() if value is None else t.fill_(value)
+
+
+def test_calls_repeat_bit_for_bit(device):
+    """Every operator on the same inputs, whatever its outputs and workspaces held before and whatever ran in between."""
+    from vdn_h3_amd.adapters import LowRankAdapters
+    from vdn_h3_amd.causal_linear import causal_linear_packed, causal_linear_step
+    from vdn_h3_amd.gdn import gated_delta_step
+    from vdn_h3_amd.linear import HipLinear
+
+    g = torch.Generator().manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    calls = []
+    for bounds, heads, dim in (([0, 1135], 20, 64), ([0, 77, 78, 78, 1000, 1500], 8, 128), ([0, 6000], 4, 128), ([0, 30], 8, 128)):
+        q, k, v = (rand(bounds[-1], n, dim).to(BF).to(device) for n in (heads // 4, heads // 4, heads))
+        decay, initial = -torch.rand(heads, generator=g).to(device), rand(len(bounds) - 1, heads, dim, dim).to(device)
+        calls.append(lambda a=(q, k, v, decay, bounds, 0.1), s=initial: causal_linear_packed(
+            *a, initial_state=s, output_final_state=True))
+    for batch, new, dim in ((9, 1, 128), (5, 4, 64), (3, 2, 80)):
+        q, k, v = (rand(batch, new, n, dim).to(BF).to(device) for n in (4, 4, 8))
+        pool, beta = rand(batch, 8, dim, dim).to(device), torch.rand(batch, new, 8, generator=g).to(device)
+
+        def steps(a=(q, k / 8, v), pool=pool, beta=beta):
+            pools = pool.clone(), pool.clone()
+            return causal_linear_step(*a, -beta[0, 0], pools[0], 0.1), gated_delta_step(*a, beta, -beta, pools[1]), *pools
+
+        calls.append(steps)
+    for rows, width, out, n, rank in ((1, 640, 5120, 2, 16), (64, 5120, 256, 1, 32), (60, 640, 512, 9, 64), (700, 256, 384, 3, 40),
+                                      (9000, 64, 128, 3, 8)):
+        layer = HipLinear((rand(out, width) * width ** -0.5).to(BF).to(device))
+        handle = LowRankAdapters(rand(n, rank, width).to(BF).to(device), rand(n, out, rank).to(BF).to(device))
+        x, index = rand(rows, width).to(BF).to(device), torch.randint(-1, n, (rows,), generator=g, dtype=torch.int32).to(device)
+        calls.append(lambda layer=layer, x=x, h=handle, i=index: (layer(x, adapters=h, adapter_index=i),))
+    want = [call() for call in calls]
+    for value in (torch.nan, None, 0.0, None):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        _leave_in_memory(value)
+        got = [call() for call in calls]
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
