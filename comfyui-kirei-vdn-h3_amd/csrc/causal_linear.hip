@@ -112,8 +112,9 @@ __device__ __forceinline__ LinRange lin_range(const LinCall &p, int range, int64
 }
 
 // LDS slots: chunk c (16 bytes) of row r lies at slot c ^ swizzle(r). Four neighbouring chunks of four neighbouring rows
-// (transposed reads) lie in 16 different 16-byte bank groups; so do the chunks 4 t + g of the rows that one turn of a 16-byte fragment read
-// takes, rows 0 to 3 and 12 to 15 of one g with rows 4 to 11 of the next (8 cycles a wavefront with r / 4 for 0, 2, 3, 1: 6).
+// (transposed reads) lie in 16 different 16-byte bank groups; so do the chunks 4 t + g of the rows that one turn of a 16-byte
+// fragment read takes, rows 0 to 3 and 12 to 15 of one g with rows 4 to 11 of the next (8 cycles a wavefront with r / 4 for 0, 2,
+// 3, 1: 6).
 template <int D>
 __device__ __forceinline__ int swizzle(int r) {
   const int four = ((r ^ (r >> 1)) & 4) >> 1 | ((r >> 3) & 1);  // 0, 2, 3, 1 for r / 4 = 0, 1, 2, 3
@@ -579,7 +580,8 @@ int check_lin_operand(const void *p, int64_t row, int64_t head, const char *name
 extern "C" int vdnh3_causal_linear_ranges(int rows, int sequences, int heads, int head_dim) {
   if (rows <= 0 || sequences <= 0 || heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
   // One round of workgroups, two chunks of each or more: 512 tokens x 40 heads x 128 take 29 us in 4 ranges (1 33, 3 31, 6 33),
-  // 3,939 of 7 sequences 80 in 6 (5 90, 12 91, 1 247), 40,688 610 (4 780, 12 620, 1 2,070); 8,000 x 56 x 64 87 in 9 (4 124, 18 101).
+  // 3,939 of 7 sequences 80 in 6 (5 90, 12 91, 1 247), 40,688 610 (4 780, 12 620, 1 2,070); 8,000 x 56 x 64 87 in 9 (4 124, 18
+  // 101).
   const int64_t slots = head_dim == 128 ? 256 : 512;  // workgroups that run at once
   return (int)std::max<int64_t>(1, std::min(slots / heads, vdnh3::most_chunks(rows, sequences) / 2));
 }

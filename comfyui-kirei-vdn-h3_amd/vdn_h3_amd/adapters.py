@@ -16,8 +16,8 @@ from functools import lru_cache
 import torch
 
 from . import _lib
+from .causal import _INTEGERS
 
-_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 _NAME = "LowRankAdapters.add"
 
 
@@ -61,9 +61,9 @@ class LowRankAdapters:
     """The adapters of one projection ``[out, width]``: ``down`` ``[n, rank, width]`` (A) and ``up`` ``[n, out, rank]`` (B), bf16 on
     the GPU, and ``scales``, ``n`` numbers (a tensor or a sequence; ``None``: ones), kept in fp32.
 
-    Widths are multiples of 8 (at most 2**30), ranks at most 1024. The object keeps copies, A and B in the kernels' order (a later change of the
-    tensors is not seen), and has to outlive graphs that were captured with it. ``from_pairs`` takes adapters of different
-    ranks.
+    Widths are multiples of 8 (at most 2**30), ranks at most 1024. The object keeps copies, A and B in the kernels' order (a later
+    change of the tensors is not seen), and has to outlive graphs that were captured with it. ``from_pairs`` takes adapters of
+    different ranks.
     """
 
     def __init__(self, down: torch.Tensor, up: torch.Tensor, scales=None):
@@ -75,7 +75,8 @@ class LowRankAdapters:
         self.count, self.rank, self.width = (int(n) for n in down.shape)
         self.out_width = int(up.shape[1])
         if self.width % 8 or self.out_width % 8 or max(self.width, self.out_width) > 2 ** 30:
-            raise ValueError(f"the projection's widths must be multiples of 8, at most 2**30, got {self.width} -> {self.out_width}")
+            raise ValueError(f"the projection's widths must be multiples of 8, at most 2**30, got {self.width} -> "
+                             f"{self.out_width}")
         if self.rank > 1024:
             raise ValueError(f"ranks up to 1024 are supported, got {self.rank}")
         _lib.forward_only("LowRankAdapters", down, up, scales)
@@ -83,7 +84,7 @@ class LowRankAdapters:
             scales = torch.as_tensor(scales, dtype=torch.float32, device=down.device).detach().reshape(-1).clone()
             if scales.numel() != self.count:
                 raise ValueError(f"scales must be {self.count} numbers, got {scales.numel()}")
-        self.device = _lib.require_device(down, up, scales)
+        _lib.require_device(down, up, scales)
         self.down, self.up = _layouts(down.detach(), up.detach())
         self.scales = scales
 

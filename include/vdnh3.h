@@ -601,14 +601,15 @@ int vdnh3_gated_delta_step(const uint16_t *q, const uint16_t *k, const uint16_t 
 
 /* out[t] = bf16(y[t] + scales[i] B_i (A_i x[t])), i = index[t]: the low-rank adapters of many requests, A_i [rank, width] and
  * B_i [out_width, rank], beside a projection's output y [rows, out_width]. scales null: ones. An index outside [0, adapters) names
- * no adapter: out[t] = y[t]. out may be y. Widths are multiples of 8, at most 2^30, the rank at most 1024. Rows of x and y may overlap.
+ * no adapter: out[t] = y[t]. out may be y. Widths are multiples of 8, at most 2^30, the rank at most 1024. Rows of x and y may
+ * overlap.
  * A and B lie in the order of the wavefronts' operands, zeros behind their own numbers, with R = 16 ranks for ranks up to 16,
  * else the rank rounded up to 32:
  *   down [adapters][width / 64, rounded up][R / 16][2][4][16][8] bf16: the element [i][s][t][k][g][m][j] is
  *        A_i[16 t + m][64 s + 32 k + 8 g + j];
  *   up   [adapters][out_width / 32, rounded up][R / 32][2][4][16][8]: [i][p][k][t][g][m][j] is
- *        B_i[32 p + 8 (m / 4) + 4 t + m % 4][32 k + 8 g + j]; for R = 16 [adapters][out_width / 32][4][16][2][4]: [i][p][g][m][t][j]
- *        is B_i[32 p + 8 (m / 4) + 4 t + m % 4][4 g + j].
+ *        B_i[32 p + 8 (m / 4) + 4 t + m % 4][32 k + 8 g + j]; for R = 16 [adapters][out_width / 32][4][16][2][4]:
+ *        [i][p][g][m][t][j] is B_i[32 p + 8 (m / 4) + 4 t + m % 4][4 g + j].
  * workspace (vdnh3_adapter_workspace_bytes, 16-byte aligned) holds scales[i] A_i x[t] as two bf16
  * numbers each (0 bytes where a call of few rows needs none). vdnh3_adapter_workspace_wanted gives the bytes with which a call is
  * fastest: a call of few rows that needs none takes two launches where they are faster and it has them, one otherwise. */

@@ -239,8 +239,9 @@ def test_infinities_of_x(device, rows, width, rank):
     index = (torch.arange(rows, device=device, dtype=torch.int32) % 4) - 1
     plain = LowRankAdapters(down, up, scales).add(y, x, index)
     bad = x.clone()
-    for row, (channel, value) in enumerate([(0, torch.inf), (width - 1, torch.inf), (width // 2, -torch.inf), (width - 8, -torch.inf),
-                                            (width - 3, torch.nan), (5, torch.inf)]):
+    places = [(0, torch.inf), (width - 1, torch.inf), (width // 2, -torch.inf), (width - 8, -torch.inf), (width - 3, torch.nan),
+              (5, torch.inf)]
+    for row, (channel, value) in enumerate(places):
         bad[3 * row + 1, channel] = value
     got = LowRankAdapters(down, up, scales).add(y, bad, index)
     want, _ = ro.adapters(y, bad, down, up, scales, index)

@@ -234,8 +234,8 @@ def test_sizes_at_the_end_of_32_bits_are_refused(built_lib):
     lib, p = _lib.lib(), 1 << 20  # an address that is never read
 
     def add(rows=200, width=128, out_width=64, n=2, rank=8):
-        return lib.vdnh3_adapter_add(p, out_width, p, width, p, p, None, p, p, out_width, rows, width, out_width, n, rank, p, 1 << 62,
-                                     None)
+        return lib.vdnh3_adapter_add(p, out_width, p, width, p, p, None, p, p, out_width, rows, width, out_width, n, rank, p,
+                                     1 << 62, None)
 
     top = (1 << 31) - 1
     for bad in [dict(rows=top), dict(rows=top - 62), dict(rows=top, rank=1024), dict(out_width=top - 7), dict(width=top - 7),
