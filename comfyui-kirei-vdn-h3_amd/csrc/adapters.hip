@@ -3,15 +3,17 @@
 //   out_t = bf16(y_t + s_i B_i (A_i x_t)),  i = index[t]     A_i: [rank, width], B_i: [out_width, rank], s_i fp32
 //
 // y is the projection's output for all rows; a row whose index names no adapter keeps it. h = A x is held in fp32, summed over
-// the parts of the width that different workgroups take; s h meets B as two bf16 numbers (16 bits of it), and the sum with y is
-// rounded once. Rows are taken in blocks of 64 neighbours; a block finds the adapters in it by ballots and takes their rows
-// together, so the rows of one request share each fragment of its adapter, in whatever order requests lie.
+// the parts of the width that a workgroup's wavefronts take; s h meets B as two bf16 numbers (16 bits of it), and the sum with y
+// is rounded once. Rows are taken in blocks of 16 to 64 neighbours; a block finds the adapters in it by ballots and takes their
+// rows together, so the rows of one request share each fragment of its adapter, in whatever order requests lie.
 //
 // A and B are kept in the order in which the wavefronts read them, a kilobyte of neighbours per load: fragments of 16 ranks x 32
 // channels of A (strided rows of A took 18 us of 31 at 3,939 rows x 5,120 of rank 32) and of 32 columns x 32 (16) ranks of B.
-// x, y and out move in runs of 128 bytes of a row. HBM bounds both passes where there are many rows: 40,688 rows x 5,120 -> 5,120
-// of rank 64 take 84 us (x, 5.0 TB/s) and 183 us (y and out, 4.6 TB/s), a copy's rate; one row x 5,120 -> 15,360 of rank 16
-// 5.9 us in one launch, a chain of loads.
+// x, y and out move in runs of 128 bytes of a row. 40,688 rows x 5,120 -> 5,120 of rank 64, each row with an adapter, take 304 us:
+// the first product alone 105 (x, 4.0 TB/s; behind the second, whose last outputs are still on their way to HBM, 127), the second
+// alone 192 (y and out, 4.3 TB/s, where a large copy reaches 4.8). Rows that name no adapter are copied: 257 us with a third of
+// them, 209 with two. Adapters that change from row to row take 531. One row x 5,120 -> 15,360 of rank 16: 6.0 us in one launch, a
+// chain of loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -21,7 +23,7 @@ namespace vdnh3 {
 namespace {
 
 constexpr int kListRows = 64;    // the most rows of a block
-constexpr int kExpandRows = 32;  // 64 leave one wavefront a SIMD: 286 us for 40,688 rows x 5,120 of rank 64 instead of 183
+constexpr int kExpandRows = 32;  // 64 leave one wavefront a SIMD: 40,688 rows x 5,120 of rank 64 take 700 us instead of 304
 constexpr int kShrinkWaves = 8;
 constexpr int kFewRows = 64, kFewRanks = 64;  // up to which one launch can make both products
 
@@ -331,8 +333,8 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_kernel(AdapterCall p, i
 }
 
 // Both products in one launch for few rows: every workgroup of a span of columns makes s A x of its adapters' rows anew, in LDS.
-// Spans of 512 columns or more, as many workgroups as one round of the CUs: one row x 5,120 -> 15,360 of rank 16 takes 5.9 us
-// (two launches 7.7, and 4 us more of the host's), 64 rows of 16 adapters 11.0 in spans of 1,024 (512 16.7, 2,048 12.6, two
+// Spans of 512 columns or more, as many workgroups as one round of the CUs: one row x 5,120 -> 15,360 of rank 16 takes 6.0 us
+// (two launches 7.7, and 4 us more of the host's), 64 rows of 16 adapters 11.1 in spans of 1,024 (512 16.7, 2,048 12.6, two
 // launches 13.9). Where it is taken: one_launch.
 template <int NT, int KS>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_few_rows_kernel(AdapterCall p, int spans, int span) {
@@ -372,12 +374,12 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_few_rows_kernel(Ada
 // The ranks that are kept: 16, or a multiple of 32; zeros behind the adapter's own.
 int kept_ranks(int rank) { return rank <= 16 ? 16 : (rank + 31) / 32 * 32; }
 
-// Whether the one launch for few rows is the faster form. Its workgroups, a span of columns and every `shares`-th registered adapter
-// each, make A x anew, so it loses where many rows of wide x fall to few adapters; the host knows the registered ones, not those
-// that rows name. Kernel times, one launch / two, for rows x width -> columns of rank 32: one adapter 16 x 5,120 -> 5,120 7.2 / 8.9
-// us, 32 9.2 / 9.5, 48 13.8 / 9.6, 64 15.5 / 9.7; 16 x 13,824 -> 5,120 15.9 / 16.8, 24 20.0 / 17.2; 64 x 1,024 -> 1,024 8.2 / 7.0, of which
-// two take 4 us more of the host's; 64 x 5,120 of four adapters 9.8 / 9.3 with rows of each, 14.8 / 9.6 if all name one; 64 x 5,120 ->
-// 15,360 of 16 adapters 12.9 / 15.2 and 20.3 / 11.8.
+// Whether the one launch for few rows is the faster form. Its workgroups, a span of columns and every `shares`-th registered
+// adapter each, make A x anew, so it loses where many rows of wide x fall to few adapters; the host knows the registered ones,
+// not those that rows name. Kernel times in us, one launch / two (which are 4 us more of the host's), for rows x width -> columns
+// of rank 32: one adapter 16 x 5,120 -> 5,120 7.2 / 8.9, 32 9.2 / 9.5, 48 13.8 / 9.6, 64 15.5 / 9.7; 16 x 13,824 -> 5,120
+// 15.9 / 16.8, 24 20.0 / 17.2; 64 x 1,024 -> 1,024 8.2 / 7.0; of four adapters 64 x 5,120 -> 5,120 9.8 / 9.3 with rows of each,
+// 14.8 / 9.6 if all name one; of 16 64 x 5,120 -> 15,360 12.9 / 15.2 and 20.3 / 11.8.
 constexpr int kFewRowsAlways = 16;
 constexpr int64_t kFewChannels = 32 * 5120;
 bool one_launch(int64_t rows, int64_t width, int64_t adapters) {
@@ -385,11 +387,12 @@ bool one_launch(int64_t rows, int64_t width, int64_t adapters) {
 }
 
 // Rows of a shrinking workgroup: 16 until there are workgroups enough without, since A is read for each (3,939 rows of rank 32:
-// 15.2 us with 16, 21 with 32, 35 with 64; 9,000 of rank 128: 59 with 16, 48 with 32; 40,688 of rank 64: 117, 85, 84).
+// 15.2 us with 16, 21 with 32, 35 with 64; 9,000 of rank 128: 59 with 16, 48 with 32; 40,688 of rank 64, both products: 336, 307,
+// 304, and 760, 583, 531 with adapters that change from row to row).
 constexpr int kRows32 = 8192, kRows64 = 16384;
 // Adapters of a block go to workgroups of their own, and its columns, until there are about this many: 64 rows of 16 adapters x
-// 15,360 columns 6.3 us (all adapters in one workgroup 98, in 16 8.1), 256 of them 13.7 (18, 15); 40,688 rows x 5,120 columns
-// 183 us in six spans, 191 in three; 9,000 x 15,360 111 and 125.
+// 15,360 columns 6.3 us (all adapters in one workgroup 98, in 16 8.1), 256 of them 13.7 (18, 15); 40,688 rows x 5,120 columns,
+// both products, 304 us in six spans, 313 in three; 9,000 x 15,360 111 and 125.
 constexpr int kShrinkGroups = 512, kExpandShares = 1024, kExpandGroups = 8192;
 constexpr int kMostWidth = 1 << 30;  // the kernels step over columns in 32 bits
 
@@ -447,8 +450,8 @@ extern "C" int vdnh3_adapter_add(const uint16_t *y, int64_t y_row, const uint16_
                                  size_t workspace_bytes, void *stream) {
   using namespace vdnh3;
   VDNH3_HOST_CHECK(rows > 0 && width > 0 && out_width > 0 && adapters > 0 && rank > 0, VDNH3_ERR_INVALID,
-                   "adapter_add: rows, widths, adapters and rank must be positive, got %d rows, %d -> %d, %d of rank %d", rows, width,
-                   out_width, adapters, rank);
+                   "adapter_add: rows, widths, adapters and rank must be positive, got %d rows, %d -> %d, %d of rank %d", rows,
+                   width, out_width, adapters, rank);
   VDNH3_HOST_CHECK(width % 8 == 0 && out_width % 8 == 0 && width <= kMostWidth && out_width <= kMostWidth && rank <= 1024,
                    VDNH3_ERR_INVALID, "adapter_add: widths must be multiples of 8, at most 2^30, and the rank at most 1024, got "
                    "%d -> %d, rank %d", width, out_width, rank);

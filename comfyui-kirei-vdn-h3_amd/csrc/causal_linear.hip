@@ -11,10 +11,10 @@
 // would add 2^-9 of them to the outputs' own 2^-9), the weighted values as three: the states keep 24 bits.
 // Chunks of a sequence follow one another, so a head's chunks are cut into ranges that run beside each other, a workgroup a CU: a
 // first pass makes the state that each range adds, and the second starts from them. It reads K and V twice.
-// 40,688 tokens x 40 heads x 128 take 610 us: the first pass 185 (its loads alone 141, its arithmetic alone 150), the second 425
-// (loads and stores alone 330, arithmetic alone 345: 3.25 us a chunk, of which a SIMD's matrix core is busy 1.4 and its vector unit
-// 1.7, each wavefront now in one, now in the other, at 2.0 GHz). 3,939 tokens of 7 sequences take 80 us, 512 of one 29, 77 13.7 (a launch, a
-// start of three loads one after another, two chunks).
+// 40,688 tokens x 40 heads x 128 take 610 to 625 us: the first pass 185 (its loads alone 141, its arithmetic alone 150), the second
+// 425 (loads and stores alone 330, arithmetic alone 345): 106 chunks of 4.0 us, by the counters 7,830 cycles at 2.0 GHz, of which a
+// SIMD's matrix core is busy 3,105 and its vector unit 4,096, each wavefront now in one, now in the other. 3,939 tokens of 7
+// sequences take 80 us, 512 of one 29, 77 13.7 (a launch, a start of three loads one after another, two chunks).
 #include <algorithm>
 #include <cmath>
 
