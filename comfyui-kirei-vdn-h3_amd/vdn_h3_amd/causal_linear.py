@@ -62,10 +62,10 @@ def causal_linear_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Te
 
     Sequence ``b`` is the rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` as in ``causal_softmax_packed``; its state starts from
     ``initial_state[b]`` (``[B, H, D, D]`` fp32, dv rows, dk columns) or zeros. An empty sequence's final state is its initial
-    one. Rows outside every sequence are not written. A value that is no finite number ends its channel: from its token on that
-    channel's outputs and states are none either, rows in front of it are as without it. A token behind a row takes no part in
-    it, whatever it holds. ``out`` must not overlap the inputs. Head dims 64 and 128 run natively, others up to 128 with zero
-    channels added. Rows are at most 2**23 elements apart.
+    one. Rows outside every sequence are not written. A value (or a number of an initial state's row) that is no finite number
+    ends its channel: from its token on that channel's outputs and states are none either, rows in front of it are as without it.
+    A token behind a row takes no part in it, whatever it holds. ``out`` must not overlap the inputs. Head dims 64 and 128 run
+    natively, others up to 128 with zero channels added. Rows are at most 2**23 elements apart.
     """
     name = "causal_linear_packed"
     if query.ndim != 3 or query.shape != key.shape or value.ndim != 3 or query.shape[0] != value.shape[0] or \

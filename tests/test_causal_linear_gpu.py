@@ -273,3 +273,19 @@ def test_what_a_workspace_held_takes_no_part(device, lengths, heads, dim):
             results.append((out, final))
         _check(results[0], want, dim, max(lengths))
         assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
+
+
+@pytest.mark.parametrize("dim", [128, 64, 40])
+def test_a_state_that_is_no_number_ends_its_channel(device, dim):
+    from vdn_h3_amd.causal_linear import causal_linear_packed
+
+    q, k, v, decay, initial = _case(700, 2, 2, dim, 8, device, 3)
+    bounds = [0, 300, 300, 700]
+    want, end = causal_linear_packed(q, k, v, decay, bounds, 0.2, initial_state=initial, output_final_state=True)
+    for value in (torch.nan, torch.inf):
+        bad = initial.clone()
+        bad[2, 1, 5, 7] = bad[1, 0, 3, 0] = value
+        o, s = causal_linear_packed(q, k, v, decay, bounds, 0.2, initial_state=bad, output_final_state=True)
+        assert not o[300:, 1, 5].isfinite().any() and not s[2, 1, 5, 7].isfinite() and not s[1, 0, 3, 0].isfinite()
+        o[300:, 1, 5], s[2, 1, 5], s[1, 0, 3, 0] = want[300:, 1, 5], end[2, 1, 5], end[1, 0, 3, 0]
+        assert torch.equal(o, want) and torch.equal(s, end)
